@@ -489,6 +489,158 @@ int mlq_argmax_workspace(int64_t n, size_t* bytes);
 int mlq_greedy_next(const float* logits, int vocab, int32_t* token_dev, int32_t* pos_dev,
                     void* ws, size_t ws_bytes, mlq_stream_t stream);
 
+/* ---------------------------------------------------------------------- */
+/* Many sequences: a paged key-value cache                                 */
+/* ---------------------------------------------------------------------- */
+/* No counterpart in the reference, whose cache holds one sequence. A step
+ * over a batch of sequences is mlq_paged_plan (pages, positions and slots of
+ * the new tokens), then per layer mlq_qk_norm_rope and
+ * mlq_paged_attention_decode or _prefill. Activations are fp32. Every array
+ * is on the device unless noted; sizes come from the host, so a step can be
+ * captured in a graph and replayed while lengths, pages and tokens change on
+ * the device. What the device arrays hold is checked there: a length or page
+ * that is out of range gives NaN outputs or writes nothing, never a wild
+ * access. */
+enum mlq_kv_type { MLQ_KV_F32 = 0, MLQ_KV_F16 = 1, MLQ_KV_BF16 = 2 };
+
+/* keys and values: [n_layers][n_pages][n_kv_heads][page_size][head_dim] each,
+ * 16-byte aligned; token t of a sequence is token t % page_size of the page
+ * that its block table names at t / page_size. page_size: a power of two,
+ * 16 .. 4096; head_dim: a multiple of 8 up to 256 (MLQ_ERR_UNSUPPORTED
+ * otherwise). */
+typedef struct mlq_paged_cache {
+  void* keys;
+  void* values;
+  int32_t type;                      /* enum mlq_kv_type */
+  int32_t n_layers, n_pages, page_size, n_kv_heads, head_dim;
+} mlq_paged_cache;
+/* Bytes of each of the two arrays (keys and values are not read). */
+int mlq_paged_cache_bytes(const mlq_paged_cache* c, size_t* bytes);
+
+/* The device arrays of a batch. Row r is a new token: rows row_start[i] ..
+ * row_start[i + 1] - 1 belong to sequence i and are its last tokens, in
+ * order. */
+typedef struct mlq_paged_batch {
+  int32_t n_seqs, max_pages, max_rows;
+  int32_t* block_table;              /* [n_seqs][max_pages] page of each page_size tokens */
+  int32_t* lengths;                  /* [n_seqs] tokens in the cache, new rows included */
+  int32_t* row_start;                /* [n_seqs + 1] */
+  int32_t* positions;                /* [max_rows], -1: no row */
+  int64_t* slots;                    /* [max_rows] page * page_size + offset, -1: no row */
+  int32_t* status;                   /* [1] enum mlq_plan_status */
+} mlq_paged_batch;
+
+enum mlq_plan_status {
+  MLQ_PLAN_OK = 0,
+  MLQ_PLAN_BAD_COUNT = 1, /* a length, count or n_free out of range */
+  MLQ_PLAN_ROWS = 2,      /* more new tokens than max_rows */
+  MLQ_PLAN_PAGES = 3      /* fewer free pages than needed: end sequences, then plan again */
+};
+
+/* One step of the batch: n_new[i] >= 0 tokens join sequence i behind its
+ * lengths[i], n_new[i] = -1 ends it (length 0, its pages return to the free
+ * pages). free_pages [n_pages] is a stack with *n_free entries: pages of ended
+ * sequences are pushed in order of sequence and position, then the pages that
+ * the new tokens need are popped in that order into block_table, whose
+ * other entries stay. Writes b->lengths, b->row_start, positions and slots of
+ * every new token (-1 up to max_rows behind the last), *n_free_out and
+ * b->status. With another status than MLQ_PLAN_OK nothing is allocated,
+ * released or counted and there are no rows. b->lengths may be `lengths`
+ * and n_free_out may be n_free (a loop's state); no other arrays overlap.
+ * Entries of block_table are not checked here. page_size as in
+ * mlq_paged_cache. */
+int mlq_paged_plan(const mlq_paged_batch* b, int page_size, int n_pages, const int32_t* lengths,
+                   const int32_t* n_new, int32_t* free_pages, const int32_t* n_free,
+                   int32_t* n_free_out, mlq_stream_t stream);
+
+/* How rotation frequencies f_i = theta^(-2i/rot_dim) are stretched for
+ * contexts longer than trained ones:
+ *  NONE;
+ *  LINEAR: f_i / factor;
+ *  PARTS (YaRN): pairs that turn more than beta_fast times in original_len
+ *   positions keep f_i, pairs that turn fewer than beta_slow times get
+ *   f_i / factor, between them a ramp linear in the pair's index between the
+ *   two indices where those counts fall (rounded outwards); the rotated
+ *   values are scaled by 0.1 ln(factor) + 1. */
+enum mlq_rope_scaling { MLQ_ROPE_SCALE_NONE = 0, MLQ_ROPE_SCALE_LINEAR = 1, MLQ_ROPE_SCALE_PARTS = 2 };
+/* Host only: freqs [rot_dim / 2] (host, radians per position) and *magnitude
+ * for mlq_rotary. factor >= 1 is read by LINEAR and PARTS; original_len > 0 and
+ * beta_fast > beta_slow > 0 by PARTS. */
+int mlq_rope_frequencies(double theta, int rot_dim, int scaling, double factor, int original_len,
+                         double beta_fast, double beta_slow, double* freqs, float* magnitude);
+
+/* What a model does to each query and key head. */
+typedef struct mlq_rotary {
+  int32_t head_dim;                  /* a multiple of 8, up to 256 */
+  int32_t rot_dim;                   /* even, 0 .. head_dim: the head's first rot_dim elements turn */
+  int32_t rope_type;                 /* enum mlq_rope_type: pairs (2i, 2i+1) or (i, i + rot_dim/2) */
+  float magnitude;                   /* of the turned elements, 1 for none */
+  float eps;                         /* of the norms */
+  const double* freqs;               /* [rot_dim / 2] (device); may be NULL when rot_dim is 0 */
+  const float* q_norm;               /* [head_dim] or NULL: no norm */
+  const float* k_norm;
+} mlq_rotary;
+
+/* For each row r with positions[r] >= 0: q_out[r] and k_out[r] = the heads of
+ * q[r] and k[r], each x * w / sqrt(mean(x^2) + eps) (mlq_rmsnorm's rule) and
+ * turned by positions[r] * freqs (angles in 64 bits: exact at far positions),
+ * and, with a cache, k and v stored (rounded to its type, past fp16's range
+ * to infinities) at slots[r] of `layer` unless that is outside the cache. Rows with a negative position
+ * are left as they were. Row strides in floats, multiples of 4; heads lie
+ * side by side; 16-byte aligned float pointers. q_out may be q, k_out k (same
+ * strides then; no other overlap). k_out may be NULL with a cache; without
+ * one (c NULL) k_out is needed and v, slots and layer are not read.
+ * Distinct rows need distinct slots. rows = 0 does nothing. */
+int mlq_qk_norm_rope(const mlq_rotary* r, int rows, const int32_t* positions, int n_heads,
+                     int n_kv_heads, const float* q, int64_t q_stride, const float* k,
+                     int64_t k_stride, const float* v, int64_t v_stride, float* q_out,
+                     int64_t q_out_stride, float* k_out, int64_t k_out_stride,
+                     const mlq_paged_cache* c, int layer, const int64_t* slots,
+                     mlq_stream_t stream);
+
+/* How a score s = q . k becomes the softmax's input for a query at position p
+ * and a key at position t <= p: s * scale, then softcap * tanh(that /
+ * softcap) if softcap > 0, then + slopes[head] * (t - p) if slopes is given;
+ * keys with t <= p - window are not seen if window > 0. */
+typedef struct mlq_attention_rule {
+  float scale;                       /* 0: 1 / sqrt(head_dim) */
+  float softcap;                     /* 0: none */
+  int32_t window;                    /* 0: none */
+  const float* slopes;               /* [n_heads] (device) or NULL */
+} mlq_attention_rule;
+
+/* Workspace of mlq_paged_attention_decode for any lengths up to max_len and
+ * any rule. */
+int mlq_paged_attention_workspace(const mlq_paged_cache* c, int n_heads, int n_seqs, int max_len,
+                                  size_t* bytes);
+/* One new token of each sequence: for every sequence with a row (b->row_start
+ * NULL: row i of sequence i), out of its last row = attention of q's last row
+ * at position lengths[i] - 1 over the sequence's pages, query head h reading
+ * kv head h / (n_heads / n_kv_heads). The new tokens' keys and values are in
+ * the cache already. A length of 0 gives zeros; a length above max_len or
+ * the block table, or a page outside the cache, NaN. q and out: rows of
+ * n_heads * head_dim floats at strides in floats (multiples of 4, pointers
+ * 16-byte aligned); b's block_table, lengths and row_start are read. max_len
+ * bounds the lengths (grid and workspace; at most max_pages * page_size).
+ * Keys behind a sequence's end are not read into results, whatever the pages
+ * hold there. Sums and softmax in fp32; fp16 and bf16 caches multiply on
+ * 16-bit matrix instructions with q and the weights split into exact parts.
+ * NaN / inf among the seen keys and values give NaN / inf outputs. ws:
+ * 256-byte aligned, scratch, may be NULL when its size is 0; calls that
+ * share one (two captured graphs, too) must be ordered. */
+int mlq_paged_attention_decode(const mlq_paged_cache* c, int layer, const mlq_paged_batch* b,
+                               const mlq_attention_rule* rule, int n_heads, const float* q,
+                               int64_t q_stride, float* out, int64_t out_stride, int max_len,
+                               void* ws, size_t ws_bytes, mlq_stream_t stream);
+/* Every new row of every sequence (prompts, or pieces of them behind what is
+ * cached): row j of n new ones of sequence i is at position lengths[i] - n + j
+ * and sees the keys up to it. Same rule, layouts and checks; no workspace.
+ * b->max_rows bounds row_start[n_seqs] (rows past it are not computed). */
+int mlq_paged_attention_prefill(const mlq_paged_cache* c, int layer, const mlq_paged_batch* b,
+                                const mlq_attention_rule* rule, int n_heads, const float* q,
+                                int64_t q_stride, float* out, int64_t out_stride,
+                                mlq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

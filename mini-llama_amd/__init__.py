@@ -106,12 +106,46 @@ class MlqModel(ctypes.Structure):
                 ("lm_head", MlqWeight), ("layers", ctypes.POINTER(MlqLayer))]
 
 
+class MlqPagedCache(ctypes.Structure):
+    """struct mlq_paged_cache (include/mlq.h)."""
+    _fields_ = [("keys", ctypes.c_void_p), ("values", ctypes.c_void_p), ("type", ctypes.c_int32),
+                ("n_layers", ctypes.c_int32), ("n_pages", ctypes.c_int32),
+                ("page_size", ctypes.c_int32), ("n_kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32)]
+
+
+class MlqPagedBatch(ctypes.Structure):
+    """struct mlq_paged_batch (include/mlq.h)."""
+    _fields_ = [("n_seqs", ctypes.c_int32), ("max_pages", ctypes.c_int32),
+                ("max_rows", ctypes.c_int32), ("block_table", ctypes.c_void_p),
+                ("lengths", ctypes.c_void_p), ("row_start", ctypes.c_void_p),
+                ("positions", ctypes.c_void_p), ("slots", ctypes.c_void_p),
+                ("status", ctypes.c_void_p)]
+
+
+class MlqRotary(ctypes.Structure):
+    """struct mlq_rotary (include/mlq.h)."""
+    _fields_ = [("head_dim", ctypes.c_int32), ("rot_dim", ctypes.c_int32),
+                ("rope_type", ctypes.c_int32), ("magnitude", ctypes.c_float),
+                ("eps", ctypes.c_float), ("freqs", ctypes.c_void_p),
+                ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p)]
+
+
+class MlqAttentionRule(ctypes.Structure):
+    """struct mlq_attention_rule (include/mlq.h)."""
+    _fields_ = [("scale", ctypes.c_float), ("softcap", ctypes.c_float),
+                ("window", ctypes.c_int32), ("slopes", ctypes.c_void_p)]
+
+
 # Every symbol declared in include/mlq.h, with its ctypes signature.
 _P, _I, _Z = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t
 _WP = ctypes.POINTER(MlqWeight)
 _I64, _F = ctypes.c_int64, ctypes.c_float
 _KVP = ctypes.POINTER(MlqKvCache)
 _MP = ctypes.POINTER(MlqModel)
+_D = ctypes.c_double
+_PCP, _PBP = ctypes.POINTER(MlqPagedCache), ctypes.POINTER(MlqPagedBatch)
+_RTP, _ARP = ctypes.POINTER(MlqRotary), ctypes.POINTER(MlqAttentionRule)
 SIGNATURES = {
     "mlq_status_string": ([_I], ctypes.c_char_p),
     "mlq_last_hip_error": ([], _I),
@@ -166,6 +200,16 @@ SIGNATURES = {
     "mlq_prefill": ([_MP, _KVP, _P, _I, _I, _P, _P, _Z, _P], _I),
     "mlq_argmax_workspace": ([_I64, ctypes.POINTER(_Z)], _I),
     "mlq_greedy_next": ([_P, _I, _P, _P, _P, _Z, _P], _I),
+    "mlq_paged_cache_bytes": ([_PCP, ctypes.POINTER(_Z)], _I),
+    "mlq_paged_plan": ([_PBP, _I, _I, _P, _P, _P, _P, _P, _P], _I),
+    "mlq_rope_frequencies": ([_D, _I, _I, _D, _I, _D, _D, ctypes.POINTER(_D),
+                              ctypes.POINTER(_F)], _I),
+    "mlq_qk_norm_rope": ([_RTP, _I, _P, _I, _I, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I64,
+                          _PCP, _I, _P, _P], _I),
+    "mlq_paged_attention_workspace": ([_PCP, _I, _I, _I, ctypes.POINTER(_Z)], _I),
+    "mlq_paged_attention_decode": ([_PCP, _I, _PBP, _ARP, _I, _P, _I64, _P, _I64, _I, _P, _Z, _P],
+                                   _I),
+    "mlq_paged_attention_prefill": ([_PCP, _I, _PBP, _ARP, _I, _P, _I64, _P, _I64, _P], _I),
 }
 
 _LIB = None

@@ -1,0 +1,351 @@
+// The paged cache's bookkeeping and what writes it: the plan of a step (block
+// tables, positions, slots) and the per-head norm + rotation of queries and
+// keys with the cache write.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "device_common.h"
+#include "paged.h"
+
+namespace mlq {
+namespace {
+
+// ---- the plan -----------------------------------------------------------------
+// held = ceil(L / P) pages of a sequence, need = ceil((L + a) / P) - held new
+// ones; releases are pushed on the stack at the prefix sum of their counts,
+// needs popped at theirs, so the result is that of a loop over sequences. One
+// workgroup walks the sequences in tiles of a thread each (the scans are all
+// there is to do; 300 sequences fit one tile); pages and rows of a tile are
+// then spread over all threads, each finding its sequence by a search in the
+// tile's prefix sums.
+constexpr int kPlanThreads = 1024;
+// Row arrays up to this size are written by the scanning workgroup itself,
+// larger ones by a second launch over the whole chip.
+constexpr int kPlanInlineRows = 4096;
+
+// Inclusive prefix sum over the workgroup; every thread gets its own and the
+// total. `lds`: one int per wave.
+__device__ __forceinline__ int block_scan(int v, int* lds, int* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int u = __shfl_up(v, o);
+    if (lane >= o) v += u;
+  }
+  __syncthreads();  // (an earlier scan's readers are done with lds)
+  if (lane == 63) lds[wave] = v;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanThreads / 64; ++w) {
+    const int t = lds[w];
+    before += w < wave ? t : 0;
+    all += t;
+  }
+  *total = all;
+  return v + before;
+}
+
+__device__ __forceinline__ int64_t block_sum64(int64_t v, int64_t* lds) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  int64_t all = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanThreads / 64; ++w) all += lds[w];
+  return all;
+}
+
+// Last i with start[i] <= r; start[0] <= r. The one that r falls into: an
+// empty sequence starts where the next one does.
+__device__ __forceinline__ int find_start(const int* start, int n, int r) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (start[mid] <= r) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+struct PlanSeq {
+  int len, add, held, need, freed;
+  bool bad;
+};
+__device__ __forceinline__ PlanSeq plan_seq(const PlanArgs& a, int i) {
+  PlanSeq s = {};
+  if (i >= a.n_seqs) return s;
+  const int64_t cap = (int64_t)a.max_pages << a.page_shift;
+  const int len = a.lengths[i], n = a.n_new[i];
+  if (n < -1 || len < 0 || (int64_t)len + max(n, 0) > cap) {
+    s.bad = true;
+    return s;
+  }
+  const int up = (1 << a.page_shift) - 1;  // (sums below stay under 2^31: cap does)
+  s.len = len;
+  s.add = max(n, 0);
+  s.held = (int)(((int64_t)len + up) >> a.page_shift);
+  s.freed = n < 0 ? s.held : 0;
+  s.need = n < 0 ? 0 : (int)(((int64_t)len + n + up) >> a.page_shift) - s.held;
+  return s;
+}
+
+__global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a, int inline_rows) {
+  __shared__ int scan_lds[kPlanThreads / 64];
+  __shared__ int64_t sum_lds[kPlanThreads / 64];
+  __shared__ int first[kPlanThreads], rows[kPlanThreads], held[kPlanThreads], lens[kPlanThreads];
+  const int tid = threadIdx.x;
+  const int free0 = *a.n_free;
+
+  int64_t add = 0, need = 0, freed = 0, bad = 0;
+  for (int i0 = 0; i0 < a.n_seqs; i0 += kPlanThreads) {
+    const PlanSeq s = plan_seq(a, i0 + tid);
+    add += s.add;
+    need += s.need;
+    freed += s.freed;
+    bad += s.bad;
+  }
+  add = block_sum64(add, sum_lds);
+  need = block_sum64(need, sum_lds);
+  freed = block_sum64(freed, sum_lds);
+  bad = block_sum64(bad, sum_lds);
+  const int64_t avail = free0 + freed;
+  int status = MLQ_PLAN_OK;
+  if (bad != 0 || free0 < 0 || avail > a.n_pages) status = MLQ_PLAN_BAD_COUNT;
+  else if (add > a.max_rows) status = MLQ_PLAN_ROWS;
+  else if (need > avail) status = MLQ_PLAN_PAGES;
+  const bool ok = status == MLQ_PLAN_OK;
+
+  if (ok && freed > 0) {
+    int base = free0;
+    for (int i0 = 0; i0 < a.n_seqs; i0 += kPlanThreads) {
+      const PlanSeq s = plan_seq(a, i0 + tid);
+      int total;
+      const int end = block_scan(s.freed, scan_lds, &total);
+      first[tid] = end - s.freed;
+      __syncthreads();
+      for (int r = tid; r < total; r += kPlanThreads) {
+        const int i = find_start(first, kPlanThreads, r);
+        a.free_pages[base + r] = a.block_table[(size_t)(i0 + i) * a.max_pages + (r - first[i])];
+      }
+      base += total;
+      __syncthreads();
+    }
+  }
+  int popped = 0, row0 = 0;
+  for (int i0 = 0; i0 < a.n_seqs; i0 += kPlanThreads) {
+    const int seq = i0 + tid;
+    const PlanSeq s = plan_seq(a, seq);
+    int needs = 0, adds = 0;
+    if (ok) {
+      const int need_end = block_scan(s.need, scan_lds, &needs);
+      const int add_end = block_scan(s.add, scan_lds, &adds);
+      first[tid] = need_end - s.need;
+      rows[tid] = add_end - s.add;
+      held[tid] = s.held;
+      lens[tid] = s.len;
+    }
+    if (seq < a.n_seqs) {
+      a.row_start[seq] = ok ? row0 + rows[tid] : 0;
+      a.lengths_out[seq] = ok ? (s.freed > 0 || a.n_new[seq] < 0 ? 0 : s.len + s.add) : a.lengths[seq];
+    }
+    __syncthreads();
+    for (int r = tid; r < needs; r += kPlanThreads) {
+      const int i = find_start(first, kPlanThreads, r);
+      a.block_table[(size_t)(i0 + i) * a.max_pages + held[i] + (r - first[i])] =
+          a.free_pages[avail - 1 - (popped + r)];
+    }
+    __syncthreads();
+    if (inline_rows) {
+      for (int r = tid; r < adds; r += kPlanThreads) {
+        const int i = find_start(rows, kPlanThreads, r);
+        const int pos = lens[i] + (r - rows[i]);
+        const int page = a.block_table[(size_t)(i0 + i) * a.max_pages + (pos >> a.page_shift)];
+        a.positions[row0 + r] = pos;
+        a.slots[row0 + r] = ((int64_t)page << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
+      }
+    }
+    popped += needs;
+    row0 += adds;
+    __syncthreads();
+  }
+  if (inline_rows)
+    for (int r = row0 + tid; r < a.max_rows; r += kPlanThreads) {
+      a.positions[r] = -1;
+      a.slots[r] = -1;
+    }
+  if (tid == 0) {
+    a.row_start[a.n_seqs] = row0;
+    *a.n_free_out = ok ? (int)(avail - need) : free0;
+    *a.status = status;
+  }
+}
+
+// A thread per row, from what plan_kernel wrote.
+__global__ __launch_bounds__(256) void plan_rows_kernel(PlanArgs a) {
+  const int r = blockIdx.x * 256 + threadIdx.x;
+  if (r >= a.max_rows) return;
+  int pos = -1;
+  int64_t slot = -1;
+  if (r < a.row_start[a.n_seqs]) {
+    const int i = find_start(a.row_start, a.n_seqs, r);
+    pos = a.lengths_out[i] - (a.row_start[i + 1] - r);
+    const int page = a.block_table[(size_t)i * a.max_pages + (pos >> a.page_shift)];
+    slot = ((int64_t)page << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
+  }
+  a.positions[r] = pos;
+  a.slots[r] = slot;
+}
+
+// ---- norm, rotation and cache write ---------------------------------------------
+// A head lies in LG lanes of 4 elements (LG a power of two >= head_dim / 4), so
+// its mean square is a sum over lanes and pairs are in a lane (interleaved)
+// or rot / 8 lanes apart. The row's angles are computed once per workgroup,
+// in 64 bits up to the quarter turn: pos * f in 32 bits would be off by
+// 2^-24 pos radians.
+constexpr int kRotaryThreads = 256, kRotaryMaxHalf = 128;
+
+__device__ __forceinline__ void store_kv(void* base, int type, int64_t at, float4 x) {
+  typedef float v4 __attribute__((ext_vector_type(4)));
+  typedef _Float16 hv4 __attribute__((ext_vector_type(4)));
+  typedef __bf16 bv4 __attribute__((ext_vector_type(4)));
+  const v4 f = {x.x, x.y, x.z, x.w};
+  if (type == MLQ_KV_F32) *(v4*)((float*)base + at) = f;
+  else if (type == MLQ_KV_F16) *(hv4*)((_Float16*)base + at) = __builtin_convertvector(f, hv4);
+  else *(bv4*)((__bf16*)base + at) = __builtin_convertvector(f, bv4);
+}
+
+template <int LG>
+__global__ __launch_bounds__(kRotaryThreads) void qk_norm_rope_kernel(RotaryArgs a) {
+  __shared__ float2 turn[kRotaryMaxHalf];  // cos, sin, times the magnitude
+  const int row = blockIdx.x;
+  const int pos = a.positions[row];
+  if (pos < 0) return;
+  const int half = a.rot >> 1;
+  if ((int)threadIdx.x < half) {
+    // quarter turns: pos * f * 2 / pi = n + x, x in [-1/2, 1/2]
+    const double t = (double)pos * a.freqs[threadIdx.x] * 0.63661977236758134308;
+    const double n = rint(t);
+    float s, c;
+    sincospif(0.5f * (float)(t - n), &s, &c);
+    const int quarter = (int)((int64_t)n & 3);
+    const float c1 = quarter & 1 ? -s : c, s1 = quarter & 1 ? c : s;
+    const float m = quarter & 2 ? -a.magnitude : a.magnitude;
+    turn[threadIdx.x] = float2{m * c1, m * s1};
+  }
+  __syncthreads();
+  const int l = threadIdx.x % LG, d = 4 * l;
+  const bool in = d < a.hd;
+  const int n_kv_out = a.keys != nullptr ? 2 * a.n_kv : a.n_kv;
+  int64_t slot = -1;
+  if (a.keys != nullptr) {
+    slot = a.slots[row];
+    if (slot >= a.n_slots) slot = -1;
+  }
+  const int64_t page = slot >> a.page_shift, off = slot & (((int64_t)1 << a.page_shift) - 1);
+  const bool quads = (half & 3) == 0;
+  const int groups = kRotaryThreads / LG * gridDim.y;
+  for (int h = blockIdx.y * (kRotaryThreads / LG) + threadIdx.x / LG; h < a.n_heads + n_kv_out;
+       h += groups) {
+    const bool is_q = h < a.n_heads, is_v = h >= a.n_heads + a.n_kv;
+    const int kh = h - a.n_heads - (is_v ? a.n_kv : 0);  // kv head of k and v
+    const float* src = is_q ? a.q + row * a.q_stride + (int64_t)h * a.hd
+                            : (is_v ? a.v + row * a.v_stride : a.k + row * a.k_stride) +
+                                  (int64_t)kh * a.hd;
+    float4 x = in ? *(const float4*)(src + d) : float4{0.0f, 0.0f, 0.0f, 0.0f};
+    const int64_t at = ((page * a.n_kv + kh) << a.page_shift) * a.hd + off * a.hd + d;
+    if (is_v) {
+      if (in && slot >= 0) store_kv(a.values, a.type, at, x);
+      continue;
+    }
+    const float* w = is_q ? a.q_norm : a.k_norm;
+    float inv = 1.0f;
+    if (w != nullptr) {
+      const float ss = row_sum<LG>(x.x * x.x + x.y * x.y + (x.z * x.z + x.w * x.w));
+      inv = 1.0f / sqrtf(ss / (float)a.hd + a.eps);
+      const float4 g = in ? *(const float4*)(w + d) : float4{0.0f, 0.0f, 0.0f, 0.0f};
+      x = float4{x.x * g.x * inv, x.y * g.y * inv, x.z * g.z * inv, x.w * g.w * inv};
+    }
+    if (a.rot > 0) {
+      if (a.neox) {
+        float p[4], v[4] = {x.x, x.y, x.z, x.w};
+        if (quads) {  // the partner is the same component of another lane
+          const int other = d < half ? l + (half >> 2) : l - (half >> 2);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) p[c] = __shfl(v[c], other, LG);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int e = d + c < half ? d + c + half : d + c - half;
+            p[c] = 0.0f;
+            if (d + c < a.rot) p[c] = w != nullptr ? src[e] * w[e] * inv : src[e];
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (d + c < a.rot) {
+            const float2 t = turn[d + c < half ? d + c : d + c - half];
+            v[c] = d + c < half ? v[c] * t.x - p[c] * t.y : v[c] * t.x + p[c] * t.y;
+          }
+        x = float4{v[0], v[1], v[2], v[3]};
+      } else {
+        if (d < a.rot) {
+          const float2 t = turn[2 * l];
+          const float y = x.x * t.x - x.y * t.y;
+          x.y = x.x * t.y + x.y * t.x;
+          x.x = y;
+        }
+        if (d + 2 < a.rot) {
+          const float2 t = turn[2 * l + 1];
+          const float y = x.z * t.x - x.w * t.y;
+          x.w = x.z * t.y + x.w * t.x;
+          x.z = y;
+        }
+      }
+    }
+    if (!in) continue;
+    if (is_q) {
+      *(float4*)(a.q_out + row * a.q_out_stride + (int64_t)h * a.hd + d) = x;
+    } else {
+      if (a.k_out != nullptr)
+        *(float4*)(a.k_out + row * a.k_out_stride + (int64_t)kh * a.hd + d) = x;
+      if (slot >= 0) store_kv(a.keys, a.type, at, x);
+    }
+  }
+}
+
+template <int LG>
+void rotary_launch(const RotaryArgs& a, hipStream_t stream) {
+  const int heads = a.n_heads + (a.keys != nullptr ? 2 : 1) * a.n_kv;
+  const int per = kRotaryThreads / LG;
+  // few rows: a row's heads over several workgroups, each with its own angles
+  const int most = (heads + per - 1) / per;
+  const int split = std::min(most, std::max(1, 2 * device_cus() / a.rows));
+  hipLaunchKernelGGL(qk_norm_rope_kernel<LG>, dim3(a.rows, split), dim3(kRotaryThreads), 0,
+                     stream, a);
+}
+
+}  // namespace
+
+hipError_t launch_paged_plan(const PlanArgs& a, hipStream_t stream) {
+  const bool rows = a.max_rows <= kPlanInlineRows;
+  hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, a, rows ? 1 : 0);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || rows) return e;
+  hipLaunchKernelGGL(plan_rows_kernel, dim3((a.max_rows + 255) / 256), dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_qk_norm_rope(const RotaryArgs& a, hipStream_t stream) {
+  if (a.hd <= 32) rotary_launch<8>(a, stream);
+  else if (a.hd <= 64) rotary_launch<16>(a, stream);
+  else if (a.hd <= 128) rotary_launch<32>(a, stream);
+  else rotary_launch<64>(a, stream);
+  return hipGetLastError();
+}
+
+}  // namespace mlq
