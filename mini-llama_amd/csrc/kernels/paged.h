@@ -62,12 +62,13 @@ struct PagedAttnArgs {
   float scale, softcap;
   int window;
   const float* slopes;
-  // decode: `splits` parts of a sequence's keys of `part_len` keys each
-  int splits, part_len;
-  float* part;
+  // decode: about part_target parts of equal length over all sequences and kv
+  // heads, at most max_items; `part`: the workspace, null when every sequence
+  // is one part
+  int part_target, max_items;
+  void* part;
 };
-// Plans the split (a.splits, a.part_len) for a.max_len keys; the workspace it
-// needs.
+// Sets part_target and max_items for lengths up to a.max_len; the workspace.
 size_t plan_paged_decode(PagedAttnArgs& a);
 hipError_t launch_paged_decode(const PagedAttnArgs& a, hipStream_t stream);
 hipError_t launch_paged_prefill(const PagedAttnArgs& a, hipStream_t stream);

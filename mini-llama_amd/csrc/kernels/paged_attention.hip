@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "device_common.h"
 #include "paged.h"
@@ -105,16 +106,617 @@ hipError_t rows_launch(const PagedAttnArgs& a, int rows, int decode, hipStream_t
   return hipGetLastError();
 }
 
+
+// ---- decode ------------------------------------------------------------------------
+// One query row of each sequence; out = softmax(rule(K q)) V with one pass over
+// the keys and a running maximum. The reads of K and V bound it, so the grid
+// is made of parts of equal length over all sequences (a sequence's keys are
+// cut into parts of part_len keys, part_len from the sum of the lengths, which
+// only the device knows: every workgroup scans the lengths), and a part's
+// workgroup joins its four waves in LDS. Sequences of more than one part leave
+// partials (maximum, sum, accumulator) that a second launch joins in order.
+//
+// A wave takes tiles of kKeys keys and the up to 16 query heads of one kv head
+// through two products, both with the heads as columns:
+//   S^T = K Q^T   A: lane = key lane % 16, 8 (fp32: 4) dims of quarter lane / 16
+//   O^T = V^T P^T A: lane = HD / 16 dims of chunk lane % 16, keys of the quarter
+// K and V go from the cache to the A operands as they lie (V by byte permutes:
+// 8 keys x 1 dim a register quad); the D layout of S^T (4 keys of quarter
+// lane / 16, head lane % 16) is the B layout of P^T, so a tile needs no LDS and
+// the maximum of a head two lane swaps. 16-bit caches multiply on 16-bit
+// instructions at full precision: q and P are split into parts that add up to
+// fp32's 24 bits (bf16: three of 8) or 22 (fp16: two of 11, under a power of
+// two: q's largest element at 2^14, the largest weight at 2^15, so what falls
+// below fp16's subnormals is 2^-39 of those), the cache's values are exact.
+// fp32 caches take the fp32 instructions, whose rate is no bound here either.
+constexpr int kDecWaves = 4, kDecThreads = 64 * kDecWaves;
+constexpr int kDecMaxSeqs = 4096;  // sequences of a launch: their prefix sums lie in LDS
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+
+template <typename T>
+struct KvTraits;
+template <>
+struct KvTraits<float> {
+  static constexpr int kKeys = 16;   // of a tile
+  static constexpr int kParts = 1;   // of q and of the weights
+  static constexpr float kLift = 0.0f;
+};
+template <>
+struct KvTraits<_Float16> {
+  static constexpr int kKeys = 32, kParts = 2;
+  static constexpr float kLift = 15.0f;  // weights are 2^15 times their size
+  typedef h8_t vec;
+  typedef h2_t pair;
+  static __device__ __forceinline__ f4 mfma(vec a, vec b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct KvTraits<__bf16> {
+  static constexpr int kKeys = 32, kParts = 3;
+  static constexpr float kLift = 0.0f;
+  typedef bf8 vec;
+  typedef bf2 pair;
+  static __device__ __forceinline__ f4 mfma(vec a, vec b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+};
+
+// a, b = the sum of p's parts, each rounded to nearest: two values of a vec.
+template <typename T>
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t (&p)[KvTraits<T>::kParts]) {
+  f2_t x = {a, b};
+#pragma unroll
+  for (int i = 0; i < KvTraits<T>::kParts; ++i) {
+    const auto h = __builtin_convertvector(x, typename KvTraits<T>::pair);
+    p[i] = __builtin_bit_cast(uint32_t, h);
+    if (i + 1 < KvTraits<T>::kParts) {
+      x.x -= (float)h.x;
+      x.y -= (float)h.y;
+    }
+  }
+}
+
+// What a row of the batch is to a kernel: its place in q and out and its
+// number of keys; row < 0: no row. A length that the table or the caller's
+// bound does not hold is `bad`.
+struct DecodeRow {
+  int row, len;
+  bool bad;
+};
+__device__ __forceinline__ DecodeRow decode_row(const PagedAttnArgs& a, int seq) {
+  DecodeRow r;
+  r.row = seq;
+  if (a.row_start != nullptr) {
+    r.row = a.row_start[seq + 1] - 1;
+    if (r.row < a.row_start[seq] || r.row >= a.max_rows) r.row = -1;
+  }
+  const int len = a.lengths[seq];
+  r.bad = len > a.max_len;
+  r.len = r.bad ? 0 : max(len, 0);
+  return r;
+}
+__device__ __forceinline__ int first_key(const PagedAttnArgs& a, int len) {
+  return a.window > 0 ? max(0, len - a.window) : 0;
+}
+
+// The softmax's input in base 2 for a product s: without cap and slopes
+// s * sl2.
+struct ScoreRule {
+  float sl2;         // scale * log2 e, divided by the power of two that q carries
+  float cap_in, cap_out;  // cap_out tanh(s * cap_in); cap_out 0: no cap
+  float slope2;      // slope * log2 e
+};
+__device__ __forceinline__ ScoreRule score_rule(const PagedAttnArgs& a, int head, int q_exp) {
+  constexpr float kLog2e = 1.44269504088896341f;
+  ScoreRule r;
+  r.sl2 = ldexp_f(a.scale * kLog2e, -q_exp);
+  r.cap_in = a.softcap > 0.0f ? ldexp_f(a.scale / a.softcap, -q_exp) : 0.0f;
+  r.cap_out = a.softcap * kLog2e;
+  r.slope2 = a.slopes != nullptr ? a.slopes[head] * kLog2e : 0.0f;
+  return r;
+}
+
+// Workgroup-wide exclusive prefix sum over kDecThreads values.
+__device__ __forceinline__ int dec_scan(int v, int* lds, int* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int u = __shfl_up(x, o);
+    if (lane >= o) x += u;
+  }
+  __syncthreads();
+  if (lane == 63) lds[wave] = x;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kDecWaves; ++w) {
+    before += w < wave ? lds[w] : 0;
+    all += lds[w];
+  }
+  *total = all;
+  return x - v + before;
+}
+
+// Partials of an item (a part of one sequence's keys for up to `tg` heads of
+// a kv head): maxima and sums [tg] each, accumulators [tg][hd].
+struct DecodePartials {
+  int* first_item;  // [n_seqs] of the sequence, over n_tiles
+  int* parts;       // [n_seqs] 1 and less: out is written already
+  float* m;
+  float* l;
+  float* acc;
+};
+__host__ __device__ inline size_t dec_align(size_t b) { return (b + 255) & ~(size_t)255; }
+__host__ __device__ inline DecodePartials decode_partials(void* ws, int n_seqs, int items, int tg) {
+  DecodePartials p;
+  char* c = (char*)ws;
+  p.first_item = (int*)c;
+  p.parts = p.first_item + n_seqs;
+  c += dec_align((size_t)n_seqs * 8);
+  p.m = (float*)c;
+  p.l = p.m + (size_t)items * tg;
+  c += dec_align((size_t)items * tg * 8);
+  p.acc = (float*)c;
+  return p;
+}
+
+template <typename T, int HD, bool FULL>
+__global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_kernel(PagedAttnArgs a) {
+  using Tr = KvTraits<T>;
+  constexpr bool F32 = sizeof(T) == 4;
+  constexpr int KT = Tr::kKeys, NS = KT / 16;  // keys, runs of 16 keys
+  constexpr int NP = Tr::kParts;
+  constexpr int KS = F32 ? HD / 16 : HD / 32;  // 16-byte pieces of a K row per lane
+  constexpr int VD = HD / 16;                  // dims of V (and of the output) per lane
+  constexpr int VW = VD * (int)sizeof(T) / 4;  // their words
+  constexpr int RD = VD < 8 ? VD : 8;          // output dims per lane merged at a time
+  constexpr int OS = 16 * RD + 4;
+  constexpr int kUnit = kDecWaves * KT;
+  __shared__ int base[kDecMaxSeqs + 1];
+  __shared__ int scan_lds[kDecWaves];
+  __shared__ int64_t total_lds[kDecWaves];
+  __shared__ __align__(16) float merge[kDecWaves][16][OS];
+  __shared__ float wm[kDecWaves][16], wl[kDecWaves][16];
+  __shared__ int any_bad;
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int ai = lane & 15, ak = lane >> 4;
+  const int head_tiles = (a.group + 15) / 16, n_tiles = a.n_kv * head_tiles;
+
+  // ---- the parts of every sequence
+  int64_t keys = 0;
+  for (int i = tid; i < a.n_seqs; i += kDecThreads) {
+    const DecodeRow r = decode_row(a, i);
+    if (r.row >= 0) keys += r.len - first_key(a, r.len);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) keys += __shfl_xor(keys, o);
+  if (lane == 0) total_lds[wave] = keys;
+  if (tid == 0) any_bad = 0;
+  __syncthreads();
+  keys = 0;
+#pragma unroll
+  for (int w = 0; w < kDecWaves; ++w) keys += total_lds[w];
+  const int64_t want = (keys * n_tiles + a.part_target - 1) / a.part_target;
+  const int part_len = (int)min((want / kUnit + (want % kUnit != 0)) * kUnit, (int64_t)1 << 30);
+  const int plen = max(part_len, kUnit);
+  int parts = 0;
+  for (int i0 = 0; i0 < a.n_seqs; i0 += kDecThreads) {
+    const int i = i0 + tid;
+    int n = 0;
+    if (i < a.n_seqs) {
+      const DecodeRow r = decode_row(a, i);
+      const int range = r.len - first_key(a, r.len);
+      if (r.row >= 0) n = max(1, range / plen + (range % plen != 0));
+    }
+    int total;
+    const int at = dec_scan(n, scan_lds, &total);
+    if (i < a.n_seqs) base[i] = parts + at;
+    parts += total;
+  }
+  if (tid == 0) base[a.n_seqs] = parts;
+  __syncthreads();
+  const DecodePartials pp = decode_partials(a.part, a.n_seqs, a.max_items, min(a.group, 16));
+  if (blockIdx.x == 0 && pp.first_item != nullptr)
+    for (int i = tid; i < a.n_seqs; i += kDecThreads) {
+      pp.first_item[i] = base[i];
+      pp.parts[i] = base[i + 1] - base[i];
+    }
+  const int item = blockIdx.x;
+  const int pi = item / n_tiles, tile = item - pi * n_tiles;
+  if (pi >= parts) return;
+  int seq = 0;
+  {
+    int hi = a.n_seqs;
+    while (hi - seq > 1) {
+      const int mid = (seq + hi) >> 1;
+      if (base[mid] <= pi) seq = mid;
+      else hi = mid;
+    }
+  }
+  seq = __builtin_amdgcn_readfirstlane(seq);
+  const int part = pi - base[seq], n_parts = base[seq + 1] - base[seq];
+  const DecodeRow dr = decode_row(a, seq);
+  const int kvh = tile / head_tiles, g0 = (tile - kvh * head_tiles) * 16;
+  const int G = min(16, a.group - g0), head0 = kvh * a.group + g0;
+  const int key_begin = first_key(a, dr.len), pos = dr.len - 1;
+  // tiles start at multiples of their size: a run of 16 keys lies in one page
+  const int lo = (key_begin & ~(KT - 1)) + part * plen;
+  const int hi = part == n_parts - 1 ? dr.len : lo + plen;
+
+  // ---- q
+  const bool has_head = ai < G;
+  const float* qp = a.q + dr.row * a.q_stride + (int64_t)(head0 + (has_head ? ai : 0)) * a.hd;
+  auto q_at = [&](int d) __attribute__((always_inline)) {
+    return has_head && (FULL || d < a.hd) ? *(const f4*)(qp + d) : f4{0.0f, 0.0f, 0.0f, 0.0f};
+  };
+  f4 qf[F32 ? KS : 1];
+  typedef typename std::conditional<F32, f4, bf8>::type raw8;  // (16 bytes of either)
+  raw8 qv[F32 ? 1 : NP][F32 ? 1 : KS];
+  int q_exp = 0;
+  if constexpr (F32) {
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[s] = q_at(16 * s + 4 * ak);
+  } else {
+    f4 x[KS][2];
+    float big = 0.0f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        x[s][j] = q_at(32 * s + 8 * ak + 4 * j);
+        big = fmaxf(fmaxf(big, fmaxf(fabsf(x[s][j].x), fabsf(x[s][j].y))),
+                    fmaxf(fabsf(x[s][j].z), fabsf(x[s][j].w)));
+      }
+    if constexpr (Tr::kLift != 0.0f) q_exp = pow2_scale_exp(xor32_max(xor16_max(big)));
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      uint32_t w[NP][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float u = x[s][j >> 1][2 * (j & 1)], v = x[s][j >> 1][2 * (j & 1) + 1];
+        if constexpr (Tr::kLift != 0.0f) {
+          u = ldexp_f(u, q_exp);
+          v = ldexp_f(v, q_exp);
+        }
+        uint32_t p[NP];
+        split_pair<T>(u, v, p);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) w[i][j] = p[i];
+      }
+#pragma unroll
+      for (int i = 0; i < NP; ++i)
+        qv[i][s] = __builtin_bit_cast(raw8, u32x4_t{w[i][0], w[i][1], w[i][2], w[i][3]});
+    }
+  }
+  const ScoreRule rule = score_rule(a, head0 + (has_head ? ai : 0), q_exp);
+  const bool plain = a.softcap <= 0.0f && a.slopes == nullptr;
+
+  // ---- the keys
+  const int mask = (1 << a.page_shift) - 1;
+  bool bad = dr.bad;
+  const int32_t* table = a.block_table + (size_t)seq * a.max_pages;
+  // The rows of the run of 16 keys at k, or of the sequence's last run.
+  auto row_of = [&](int k) __attribute__((always_inline)) {
+    const int kk = min(k, pos);
+    int page = __builtin_amdgcn_readfirstlane(table[kk >> a.page_shift]);
+    const bool out = page < 0 || page >= a.n_pages;
+    bad |= out;
+    page = out ? 0 : page;
+    return (((int64_t)page * a.n_kv + kvh) << a.page_shift) + (kk & mask & ~15);
+  };
+  u32x4_t kr[NS][KS];
+  uint32_t vr[F32 ? 4 : 8][VW];
+  int64_t rows[NS];
+  auto load_k = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < NS; ++u) {
+      const char* p = (const char*)a.keys + rows[u] * a.hd * sizeof(T) + (size_t)ai * a.hd * sizeof(T);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const int d = F32 ? 16 * s + 4 * ak : 32 * s + 8 * ak;
+        if (FULL || d < a.hd) kr[u][s] = *(const u32x4_t*)(p + (size_t)d * sizeof(T));
+        else kr[u][s] = u32x4_t{0, 0, 0, 0};
+      }
+    }
+  };
+  // this lane's keys of quarter ak: 4 ak + r of each run
+  auto load_v = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < 4 * NS; ++e) {
+      const char* p = (const char*)a.values +
+                      (rows[e >> 2] + 4 * ak + (e & 3)) * a.hd * (int64_t)sizeof(T);
+#pragma unroll
+      for (int w = 0; w < VW; w += (VW < 4 ? 2 : 4)) {
+        const int d = VD * ai + w * 4 / (int)sizeof(T);
+        if constexpr (VW < 4) {
+          const u32x2_t x = FULL || d < a.hd ? *(const u32x2_t*)(p + (size_t)d * sizeof(T)) : u32x2_t{0, 0};
+          vr[e][w] = x.x;
+          vr[e][w + 1] = x.y;
+        } else {
+          const u32x4_t x = FULL || d < a.hd ? *(const u32x4_t*)(p + (size_t)d * sizeof(T)) : u32x4_t{0, 0, 0, 0};
+          vr[e][w] = x.x;
+          vr[e][w + 1] = x.y;
+          vr[e][w + 2] = x.z;
+          vr[e][w + 3] = x.w;
+        }
+      }
+    }
+  };
+
+  float m = -INFINITY, l = 0.0f;  // of head ai; l of this quarter's keys
+  f4 acc[VD];                     // dims VD (4 ak + r) + c of head ai in acc[c][r]
+#pragma unroll
+  for (int c = 0; c < VD; ++c) acc[c] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+  int k0 = lo + wave * KT;
+  if (k0 < hi) {
+#pragma unroll
+    for (int u = 0; u < NS; ++u) rows[u] = row_of(k0 + 16 * u);
+    load_k();
+  }
+  for (; k0 < hi; k0 += kUnit) {
+    load_v();
+    f4 s[NS];
+    if constexpr (F32) {
+      // eight chains added as a tree: few roundings on the way to a score
+      f4 c8[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) c8[i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int st = 0; st < KS; ++st)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          f4& c = c8[4 * (st & 1) + i];
+          c = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f4, kr[0][st])[i], qf[st][i], c, 0, 0, 0);
+        }
+      s[0] = ((c8[0] + c8[1]) + (c8[2] + c8[3])) + ((c8[4] + c8[5]) + (c8[6] + c8[7]));
+    } else {
+#pragma unroll
+      for (int u = 0; u < NS; ++u) s[u] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+      // the small parts first: their roundings are below the score's
+#pragma unroll
+      for (int i = NP - 1; i >= 0; --i)
+#pragma unroll
+        for (int st = 0; st < KS; ++st)
+#pragma unroll
+          for (int u = 0; u < NS; ++u)
+            s[u] = Tr::mfma(__builtin_bit_cast(typename Tr::vec, kr[u][st]),
+                            __builtin_bit_cast(typename Tr::vec, qv[i][st]), s[u]);
+    }
+    const bool edge = k0 < key_begin || k0 + KT > hi;
+    float p[4 * NS];
+    float mx = -INFINITY;
+    if (plain) {
+#pragma unroll
+      for (int e = 0; e < 4 * NS; ++e) p[e] = s[e >> 2][e & 3] * rule.sl2;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4 * NS; ++e) {
+        float x = s[e >> 2][e & 3];
+        x = a.softcap > 0.0f ? rule.cap_out * tanhf(x * rule.cap_in) : x * rule.sl2;
+        p[e] = x + rule.slope2 * (float)(k0 + 16 * (e >> 2) + 4 * ak + (e & 3) - pos);
+      }
+    }
+    if (edge) {
+#pragma unroll
+      for (int e = 0; e < 4 * NS; ++e) {
+        const int k = k0 + 16 * (e >> 2) + 4 * ak + (e & 3);
+        if (k < key_begin || k >= hi) {
+          p[e] = -INFINITY;
+          // (what lies there may be anything, and 0 * inf is not 0)
+#pragma unroll
+          for (int w = 0; w < VW; ++w) vr[e][w] = 0;
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4 * NS; ++e) mx = fmaxf(mx, p[e]);
+    mx = fmaxf(m, xor32_max(xor16_max(mx)));
+    const float ref = (mx == -INFINITY ? 0.0f : mx) - Tr::kLift;
+    const float al = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mx);
+    m = mx;
+    if (__any(al != 1.0f)) {
+      l *= al;
+#pragma unroll
+      for (int c = 0; c < VD; ++c) acc[c] *= al;
+    }
+    if (plain && !edge) {
+      // (scaled and shifted with one rounding)
+#pragma unroll
+      for (int e = 0; e < 4 * NS; ++e)
+        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e >> 2][e & 3], rule.sl2, -ref));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4 * NS; ++e) p[e] = __builtin_amdgcn_exp2f(p[e] - ref);
+    }
+    if constexpr (NS == 1) l += (p[0] + p[1]) + (p[2] + p[3]);
+    else l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+
+    if (k0 + kUnit < hi) {
+#pragma unroll
+      for (int u = 0; u < NS; ++u) rows[u] = row_of(k0 + kUnit + 16 * u);
+      load_k();
+    }
+    if constexpr (F32) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int c = 0; c < VD; ++c)
+          acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, vr[e][c]), p[e], acc[c], 0, 0, 0);
+    } else {
+      uint32_t w[NP][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t q[NP];
+        split_pair<T>(p[2 * j], p[2 * j + 1], q);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) w[i][j] = q[i];
+      }
+#pragma unroll
+      for (int c = 0; c < VD; ++c) {
+        // dim c of the eight keys: the low or the high half of a word of each
+        const uint32_t sel = c & 1 ? 0x07060302u : 0x05040100u;
+        u32x4_t v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          v[j] = __builtin_amdgcn_perm(vr[2 * j + 1][c >> 1], vr[2 * j][c >> 1], sel);
+#pragma unroll
+        for (int i = NP - 1; i >= 0; --i)
+          acc[c] = Tr::mfma(__builtin_bit_cast(typename Tr::vec, v),
+                            __builtin_bit_cast(typename Tr::vec, u32x4_t{w[i][0], w[i][1], w[i][2], w[i][3]}),
+                            acc[c]);
+      }
+    }
+  }
+  l = xor32_sum(xor16_sum(l));
+
+  // ---- the waves joined in their order
+  if (bad) any_bad = 1;
+  if (ak == 0) {
+    wm[wave][ai] = m;
+    wl[wave][ai] = l;
+  }
+  const int TG = min(a.group, 16);
+  float* out = a.out + dr.row * a.out_stride + (int64_t)head0 * a.hd;
+#pragma unroll
+  for (int c0 = 0; c0 < VD; c0 += RD) {
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int c = 0; c < RD; c += 4)
+        *(f4*)&merge[wave][ai][RD * (4 * ak + r) + c] =
+            f4{acc[c0 + c][r], acc[c0 + c + 1][r], acc[c0 + c + 2][r], acc[c0 + c + 3][r]};
+    __syncthreads();
+    for (int e = tid; e < G * 16 * RD; e += kDecThreads) {
+      const int g = e / (16 * RD), x = e % (16 * RD);
+      const int d = VD * (x / RD) + c0 + x % RD;
+      if (!FULL && d >= a.hd) continue;
+      float mx = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kDecWaves; ++w) mx = fmaxf(mx, wm[w][g]);
+      float sum = 0.0f, o = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kDecWaves; ++w) {
+        // (a wave without keys holds zeros)
+        const float f = wm[w][g] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(wm[w][g] - mx);
+        sum += wl[w][g] * f;
+        o += merge[w][g][x] * f;
+      }
+      if (any_bad) sum = __builtin_nanf("");
+      if (n_parts == 1) {
+        out[(int64_t)g * a.hd + d] = dr.len > 0 || any_bad ? o / sum : 0.0f;
+      } else {
+        const size_t at = (size_t)item * TG + g;
+        if (d == 0) {
+          pp.m[at] = mx;
+          pp.l[at] = sum;
+        }
+        pp.acc[at * a.hd + d] = o;
+      }
+    }
+  }
+}
+
+// The parts of a sequence joined in their order, for one query head: wave w
+// takes parts w, w + 4, .., then the waves are joined.
+__global__ __launch_bounds__(kDecThreads) void paged_combine_kernel(PagedAttnArgs a) {
+  __shared__ float wl[kDecWaves], wo[kDecWaves][256];
+  const int seq = blockIdx.x, head = blockIdx.y;
+  const int TG = min(a.group, 16), head_tiles = (a.group + 15) / 16, n_tiles = a.n_kv * head_tiles;
+  const DecodePartials pp = decode_partials(a.part, a.n_seqs, a.max_items, TG);
+  const int parts = pp.parts[seq];
+  if (parts <= 1) return;
+  const int first = pp.first_item[seq];
+  const int kvh = head / a.group, g = head - kvh * a.group;
+  const int tile = kvh * head_tiles + g / 16;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  auto at = [&](int p) { return ((size_t)(first + p) * n_tiles + tile) * TG + g % 16; };
+  float mx = -INFINITY;
+  for (int p = lane; p < parts; p += 64) mx = fmaxf(mx, pp.m[at(p)]);
+  mx = wave_max(mx);
+  float l = 0.0f, acc[4] = {};
+#pragma unroll 4
+  for (int p = wave; p < parts; p += kDecWaves) {
+    const float pm = pp.m[at(p)];
+    const float f = pm == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(pm - mx);
+    l += pp.l[at(p)] * f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (lane + 64 * j < a.hd) acc[j] += pp.acc[at(p) * a.hd + lane + 64 * j] * f;
+  }
+  if (lane == 0) wl[wave] = l;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) wo[wave][lane + 64 * j] = acc[j];
+  __syncthreads();
+  const DecodeRow dr = decode_row(a, seq);
+  float* out = a.out + dr.row * a.out_stride + (int64_t)head * a.hd;
+  const int d = threadIdx.x;
+  if (d < a.hd) {
+    const float sum = (wl[0] + wl[1]) + (wl[2] + wl[3]);
+    out[d] = ((wo[0][d] + wo[1][d]) + (wo[2][d] + wo[3][d])) / sum;
+  }
+}
+
+template <typename T, int HD>
+void decode_launch(const PagedAttnArgs& a, int grid, hipStream_t stream) {
+  if (a.hd == HD)
+    hipLaunchKernelGGL((paged_decode_kernel<T, HD, true>), dim3(grid), dim3(kDecThreads), 0, stream, a);
+  else
+    hipLaunchKernelGGL((paged_decode_kernel<T, HD, false>), dim3(grid), dim3(kDecThreads), 0, stream, a);
+}
+template <typename T>
+void decode_launch_hd(const PagedAttnArgs& a, int grid, hipStream_t stream) {
+  if (a.hd <= 64) decode_launch<T, 64>(a, grid, stream);
+  else if (a.hd <= 128) decode_launch<T, 128>(a, grid, stream);
+  else decode_launch<T, 256>(a, grid, stream);
+}
+
 }  // namespace
 
 size_t plan_paged_decode(PagedAttnArgs& a) {
-  a.splits = 1;
-  a.part_len = a.max_len;
-  return 0;
+  const int head_tiles = (a.group + 15) / 16;
+  const int64_t seqs = std::min(a.n_seqs, kDecMaxSeqs), tiles = (int64_t)a.n_kv * head_tiles;
+  const int unit = kDecWaves * (a.type == MLQ_KV_F32 ? 16 : 32);
+  a.part_target = 4 * device_cus();
+  // a sequence has at most one part more than its share of the target, and one per unit
+  a.max_items = (int)std::min(seqs * tiles * ((a.max_len + unit - 1) / unit + 1),
+                              a.part_target + 2 * seqs * tiles);
+  if (a.max_len <= unit) return 0;  // every sequence is one part
+  const size_t tg = std::min(a.group, 16);
+  return dec_align((size_t)seqs * 8) + dec_align((size_t)a.max_items * tg * 8) +
+         (size_t)a.max_items * tg * a.hd * sizeof(float);
 }
 
-hipError_t launch_paged_decode(const PagedAttnArgs& a, hipStream_t stream) {
-  return rows_launch(a, a.n_seqs, 1, stream);
+hipError_t launch_paged_decode(const PagedAttnArgs& all, hipStream_t stream) {
+  for (int s0 = 0; s0 < all.n_seqs; s0 += kDecMaxSeqs) {
+    PagedAttnArgs a = all;
+    a.n_seqs = std::min(kDecMaxSeqs, all.n_seqs - s0);
+    a.block_table += (size_t)s0 * a.max_pages;
+    a.lengths += s0;
+    if (a.row_start != nullptr) {
+      a.row_start += s0;
+    } else {
+      a.q += (int64_t)s0 * a.q_stride;
+      a.out += (int64_t)s0 * a.out_stride;
+    }
+    if (a.type == MLQ_KV_F32) decode_launch_hd<float>(a, a.max_items, stream);
+    else if (a.type == MLQ_KV_F16) decode_launch_hd<_Float16>(a, a.max_items, stream);
+    else decode_launch_hd<__bf16>(a, a.max_items, stream);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    if (a.part == nullptr) continue;
+    hipLaunchKernelGGL(paged_combine_kernel, dim3(a.n_seqs, a.n_kv * a.group), dim3(kDecThreads), 0,
+                       stream, a);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 hipError_t launch_paged_prefill(const PagedAttnArgs& a, hipStream_t stream) {
