@@ -13,52 +13,40 @@
 namespace mlq {
 namespace {
 
-// One wave per (row, query head): a lane scores a key of a tile of 64 against
-// q in LDS, then takes head dims lane, lane + 64, .. of the output.
+// One row of one query head by one wave, in plain fp32: a lane scores a key of
+// a tile of 64 against q in LDS, then takes head dims lane, lane + 64, .. of
+// the output. What the matrix kernels hand to it: rows that could see a value
+// or page that those do not carry. `lds`: kSlowFloats of the wave's own.
+constexpr int kSlowFloats = 256 + 64 + 128;
 template <typename T>
-__global__ __launch_bounds__(64) void paged_rows_kernel(PagedAttnArgs a, int decode) {
-  __shared__ __align__(16) float qs[256];
-  __shared__ float ps[64];
-  __shared__ int64_t at[64];
-  const int lane = threadIdx.x, head = blockIdx.y, kvh = head / a.group;
-  int seq, row, pos;
-  if (decode) {
-    seq = blockIdx.x;
-    row = seq;
-    if (a.row_start != nullptr) {
-      row = a.row_start[seq + 1] - 1;
-      if (row < a.row_start[seq]) return;
-    }
-    pos = a.lengths[seq] - 1;
-  } else {
-    row = blockIdx.x;
-    if (row >= a.row_start[a.n_seqs]) return;
-    int lo = 0, hi = a.n_seqs;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (a.row_start[mid] <= row) lo = mid;
-      else hi = mid;
-    }
-    seq = lo;
-    pos = a.lengths[seq] - (a.row_start[seq + 1] - row);
-  }
-  if (row < 0 || row >= a.max_rows) return;
+__device__ void slow_row(const PagedAttnArgs& a, int seq, int row, int pos, int head, float* lds) {
+  float* qs = lds;
+  float* ps = lds + 256;
+  int64_t* at = (int64_t*)(lds + 320);
+  const int lane = threadIdx.x & 63, kvh = head / a.group;
+  auto sync = [] {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  };
   const int len = pos + 1;
   const float* q = a.q + row * a.q_stride + (int64_t)head * a.hd;
+  sync();
   for (int d = lane; d < a.hd; d += 64) qs[d] = q[d];
-  __syncthreads();
+  sync();
   float m = -INFINITY, l = 0.0f, acc[4] = {};
   const float slope = a.slopes != nullptr ? a.slopes[head] : 0.0f;
-  bool bad = len > a.max_len || a.lengths[seq] > a.max_len;
+  bool bad = false;
   const int first = a.window > 0 ? max(0, len - a.window) : 0;
-  for (int t0 = first; t0 < len && !bad; t0 += 64) {
+  for (int t0 = first; t0 < len; t0 += 64) {
     const int t = t0 + lane;
     float s = -INFINITY;
     int64_t base = 0;
     if (t < len) {
       const int page = a.block_table[(size_t)seq * a.max_pages + (t >> a.page_shift)];
-      if (page < 0 || page >= a.n_pages) bad = true;
-      else {
+      if (page < 0 || page >= a.n_pages) {
+        bad = true;
+      } else {
         base = ((((int64_t)page * a.n_kv + kvh) << a.page_shift) + (t & ((1 << a.page_shift) - 1))) * a.hd;
         const T* k = (const T*)a.keys + base;
         s = 0.0f;
@@ -76,10 +64,10 @@ __global__ __launch_bounds__(64) void paged_rows_kernel(PagedAttnArgs a, int dec
     const float p = t < len ? expf(s - ref) : 0.0f;
     l = l * al + wave_sum(p);
     m = mx;
-    __syncthreads();
+    sync();
     ps[lane] = p;
     at[lane] = base;
-    __syncthreads();
+    sync();
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[j] *= al;
     for (int i = 0; i < min(64, len - t0); ++i) {
@@ -90,22 +78,11 @@ __global__ __launch_bounds__(64) void paged_rows_kernel(PagedAttnArgs a, int dec
     }
   }
   float* out = a.out + row * a.out_stride + (int64_t)head * a.hd;
+#pragma unroll
   for (int j = 0; j < 4; ++j)
     if (lane + 64 * j < a.hd)
       out[lane + 64 * j] = bad ? __builtin_nanf("") : len > 0 ? acc[j] / l : 0.0f;
 }
-
-hipError_t rows_launch(const PagedAttnArgs& a, int rows, int decode, hipStream_t stream) {
-  const dim3 grid(rows, a.n_kv * a.group);
-  if (a.type == MLQ_KV_F32)
-    hipLaunchKernelGGL(paged_rows_kernel<float>, grid, dim3(64), 0, stream, a, decode);
-  else if (a.type == MLQ_KV_F16)
-    hipLaunchKernelGGL(paged_rows_kernel<_Float16>, grid, dim3(64), 0, stream, a, decode);
-  else
-    hipLaunchKernelGGL(paged_rows_kernel<__bf16>, grid, dim3(64), 0, stream, a, decode);
-  return hipGetLastError();
-}
-
 
 // ---- decode ------------------------------------------------------------------------
 // One query row of each sequence; out = softmax(rule(K q)) V with one pass over
@@ -678,6 +655,443 @@ void decode_launch_hd(const PagedAttnArgs& a, int grid, hipStream_t stream) {
   else decode_launch<T, 256>(a, grid, stream);
 }
 
+// ---- prefill -----------------------------------------------------------------------
+// Causal attention of every new row of every sequence. Bound by the matrix
+// instructions. A workgroup owns 128 consecutive (row, query head) pairs of one
+// sequence and kv head (pairs r * group + h: no padding whatever the group), a
+// wave 32 of them as the columns of both products, S^T = K Q^T and
+// O^T = V^T P^T on 32 x 32 x 16 instructions. A lane then holds 16 keys of one
+// column: the softmax is in registers but for one lane swap, and P^T is the
+// second product's B operand as it stands, V^T lying in LDS in the order in
+// which the first product leaves the keys. q and the weights are split into
+// parts as in the decode kernel; fp32 caches into three bf16 parts too, of whose
+// nine part products the six largest are taken (the others are below 2^-25 of
+// the product). Tiles of 32 keys pass through LDS: K's next tile is in flight
+// during the output's products, V's during the scores'.
+// A value that a masked weight of 0 does not silence (infinite or NaN), or that
+// the split does not carry, and a page outside the cache send the workgroup's
+// rows to slow_row.
+constexpr int kPreCols = 128, kPreKeys = 32, kPreThreads = 256;
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+
+template <typename T>
+struct PreTraits : KvTraits<T> {
+  typedef T mat;
+  static constexpr int kCacheParts = 1;
+  static __device__ __forceinline__ f16v mfma32(h8_t a, h8_t b, f16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f16v mfma32(bf8 a, bf8 b, f16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct PreTraits<float> : KvTraits<__bf16> {
+  typedef __bf16 mat;
+  static constexpr int kCacheParts = 3;
+  static __device__ __forceinline__ f16v mfma32(bf8 a, bf8 b, f16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+
+template <typename T, int HD>
+struct PreTile {
+  static constexpr int NK = PreTraits<T>::kCacheParts;
+  uint16_t k[NK][kPreKeys][HD + 8];   // [key][dim]
+  uint16_t v[NK][HD][kPreKeys + 8];   // [dim][key slot], see v_slot
+  int count[kPreThreads / 64];
+};
+
+// Where the 8-slot unit of a dim's row lies: a wave writes a few dims of four
+// keys a lane, so neighbouring lanes are some rows apart; turning the units by
+// the dim spreads them over the banks.
+__device__ __forceinline__ int v_slot(int unit, int dim) { return (unit ^ ((dim >> 4) & 3)) * 8; }
+
+// RULE: scores are capped or biased (a variant of its own: its values spill
+// beside the others').
+template <typename T, int HD, bool FULL, bool RULE>
+__global__ __launch_bounds__(kPreThreads, HD <= 128 ? 2 : 1) void paged_prefill_kernel(PagedAttnArgs a) {
+  using Tr = PreTraits<T>;
+  using M = typename Tr::mat;
+  using vec = typename Tr::vec;
+  constexpr bool F32 = sizeof(T) == 4;
+  constexpr int NP = Tr::kParts, NK = Tr::kCacheParts;
+  constexpr int KT = HD / 16;        // 16-dim steps of the scores
+  constexpr int VB = HD / 32;        // 32-dim blocks of the output
+  constexpr int KW = HD / 8 * (int)sizeof(T) / 4;   // words of K per thread: HD / 8 dims of a key
+  constexpr int VDT = HD / 32;       // dims of V per thread, of 4 keys
+  constexpr int VWT = VDT * (int)sizeof(T) / 4;     // their words a key (fp16 / bf16, HD 64: 1)
+  extern __shared__ __align__(16) uint8_t pre_smem[];
+  PreTile<T, HD>& tl = *(PreTile<T, HD>*)pre_smem;
+  int* const count_lds = tl.count;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const int G = a.group;
+  const int kvh = blockIdx.x % a.n_kv;
+  const int tile = (int)(gridDim.x / a.n_kv) - 1 - (int)(blockIdx.x / a.n_kv);
+
+  // Sequence i owns the tiles from row_start[i] * G / 128 + i on: at least as
+  // many as it needs, found without a sum over the sequences before it.
+  auto first_tile = [&](int i) { return (int)((int64_t)a.row_start[i] * G / kPreCols) + i; };
+  int before = 0;
+  for (int i = tid; i < a.n_seqs; i += kPreThreads) before += first_tile(i) <= tile;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o);
+  if (lane == 0) count_lds[wave] = before;
+  __syncthreads();
+  const int seq = __builtin_amdgcn_readfirstlane(count_lds[0] + count_lds[1] + count_lds[2] + count_lds[3]) - 1;
+  if (seq < 0) return;
+  const int row0 = a.row_start[seq], row1 = min(a.row_start[seq + 1], a.max_rows);
+  const int64_t pairs = (int64_t)(row1 - row0) * G;
+  const int64_t c0 = (int64_t)(tile - first_tile(seq)) * kPreCols;
+  if (row0 < 0 || c0 < 0 || c0 >= pairs) return;
+  const int len = a.lengths[seq];
+  const int pos0 = len - (a.row_start[seq + 1] - row0);  // of the sequence's first row
+  // this lane's column
+  const int64_t cc = c0 + wave * 32 + col;
+  const bool live = cc < pairs;
+  const int jr = (int)((live ? cc : pairs - 1) / G), qh = (int)((live ? cc : pairs - 1) - (int64_t)jr * G);
+  const int row = row0 + jr, qpos = pos0 + jr, head = kvh * G + qh;
+  float* out = a.out + row * a.out_stride + (int64_t)head * a.hd;
+  // the workgroup's first and last key, the wave's first and last row
+  const int ja = (int)(c0 / G), jb = (int)((min(c0 + kPreCols, pairs) - 1) / G);
+  const int kmax = pos0 + jb;
+  const int key0 = a.window > 0 ? max(0, pos0 + ja + 1 - a.window) : 0;
+  const int wave_first = __builtin_amdgcn_readfirstlane(__shfl(qpos, 0));
+  const int wave_last = __builtin_amdgcn_readfirstlane(__shfl(qpos, 63));
+  if (len > a.max_len || kmax < 0) {  // (kmax < 0: nothing to see)
+    if (live)
+      for (int d = 4 * half; d < a.hd; d += 8) {
+        const float x = len > a.max_len ? __builtin_nanf("") : 0.0f;
+        *(f4*)(out + d) = f4{x, x, x, x};
+      }
+    return;
+  }
+
+  // ---- q
+  int q_exp = 0;
+  vec q[NP][KT];
+  bool odd = false;  // something that the matrix products do not carry
+  {
+    const float* qp = a.q + row * a.q_stride + (int64_t)head * a.hd + 8 * half;
+    auto q_at = [&](int s, int u) __attribute__((always_inline)) {
+      return live && (FULL || 16 * s + 8 * half < a.hd) ? *(const f4*)(qp + 16 * s + 4 * u)
+                                                          : f4{0.0f, 0.0f, 0.0f, 0.0f};
+    };
+    if constexpr (Tr::kLift != 0.0f) {
+      float big = 0.0f;
+#pragma unroll
+      for (int s = 0; s < KT; ++s)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const f4 x = q_at(s, u);
+          big = fmaxf(fmaxf(big, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
+        }
+      q_exp = pow2_scale_exp(xor32_max(big));
+    }
+#pragma unroll
+    for (int s = 0; s < KT; ++s) {
+      uint32_t w[NP][4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        f4 x = q_at(s, u);
+        if constexpr (Tr::kLift != 0.0f)
+          x = f4{ldexp_f(x.x, q_exp), ldexp_f(x.y, q_exp), ldexp_f(x.z, q_exp), ldexp_f(x.w, q_exp)};
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint32_t p[NP];
+          split_pair<M>(x[2 * j], x[2 * j + 1], p);
+#pragma unroll
+          for (int i = 0; i < NP; ++i) w[i][2 * u + j] = p[i];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NP; ++i)
+        q[i][s] = __builtin_bit_cast(vec, u32x4_t{w[i][0], w[i][1], w[i][2], w[i][3]});
+    }
+  }
+  const ScoreRule rule = score_rule(a, head, q_exp);
+
+  // ---- staging: a wave's keys lie in one run of 16 (and so in one page)
+  const int32_t* table = a.block_table + (size_t)seq * a.max_pages;
+  const int mask = (1 << a.page_shift) - 1;
+  auto run_of = [&](int k0) __attribute__((always_inline)) {
+    const int kk = min(k0 + 16 * (wave >> 1), kmax);
+    int page = __builtin_amdgcn_readfirstlane(table[kk >> a.page_shift]);
+    const bool outside = page < 0 || page >= a.n_pages;
+    odd |= outside;
+    page = outside ? 0 : page;
+    return (((int64_t)page * a.n_kv + kvh) << a.page_shift) + (kk & mask & ~15);
+  };
+  const int kkey = tid >> 3, kd = (tid & 7) * (16 / (int)sizeof(T));  // K: dims kd + 8 threads' pieces
+  const int vkg = tid >> 5, vd = (tid & 31) * VDT;                    // V: keys 4 vkg .. + 3
+  uint32_t kw[KW], vw[4][VWT];
+  float largest = 0.0f;
+  us2 largest16 = {0, 0};
+  auto load_k = [&](int64_t run) __attribute__((always_inline)) {
+    const char* p = (const char*)a.keys + (run + (kkey & 15)) * a.hd * (int64_t)sizeof(T);
+#pragma unroll
+    for (int w = 0; w < KW; w += 4) {
+      const int d = kd + w * 32 / (int)sizeof(T);
+      const u32x4_t x = FULL || d < a.hd ? *(const u32x4_t*)(p + (size_t)d * sizeof(T)) : u32x4_t{0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) kw[w + i] = x[i];
+    }
+  };
+  auto load_v = [&](int64_t run) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const char* p = (const char*)a.values +
+                      ((run + 4 * (vkg & 3) + e) * a.hd + vd) * (int64_t)sizeof(T);
+      if constexpr (VWT >= 4) {
+#pragma unroll
+        for (int w = 0; w < VWT; w += 4) {
+          const bool in = FULL || vd + w * 4 / (int)sizeof(T) < a.hd;
+          const u32x4_t x = in ? *(const u32x4_t*)(p + 4 * w) : u32x4_t{0, 0, 0, 0};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) vw[e][w + i] = x[i];
+        }
+      } else if constexpr (VWT == 2) {
+        const u32x2_t x = FULL || vd < a.hd ? *(const u32x2_t*)p : u32x2_t{0, 0};
+        vw[e][0] = x.x;
+        vw[e][1] = x.y;
+      } else {
+        vw[e][0] = FULL || vd < a.hd ? *(const uint32_t*)p : 0u;
+      }
+    }
+  };
+  auto note = [&](uint32_t w) __attribute__((always_inline)) {
+    if constexpr (F32)
+      largest = __builtin_elementwise_maximum(largest, fabsf(__builtin_bit_cast(float, w)));
+    else
+      largest16 = __builtin_elementwise_max(largest16, __builtin_bit_cast(us2, w & 0x7fff7fffu));
+  };
+  auto put_k = [&](int k0) __attribute__((always_inline)) {
+    if constexpr (F32) {
+      if (k0 + kkey > kmax) {  // (what lies there may be anything)
+#pragma unroll
+        for (int w = 0; w < KW; ++w) kw[w] = 0;
+      }
+#pragma unroll
+      for (int w = 0; w < KW; w += 4) {
+        uint32_t x[3], y[3];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) note(kw[w + i]);
+        split_pair<__bf16>(__builtin_bit_cast(float, kw[w]), __builtin_bit_cast(float, kw[w + 1]), x);
+        split_pair<__bf16>(__builtin_bit_cast(float, kw[w + 2]), __builtin_bit_cast(float, kw[w + 3]), y);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) *(u32x2_t*)&tl.k[i][kkey][kd + w * 8] = u32x2_t{x[i], y[i]};
+      }
+    } else {
+#pragma unroll
+      for (int w = 0; w < KW; w += 4)
+        *(u32x4_t*)&tl.k[0][kkey][kd + w * 16] = u32x4_t{kw[w], kw[w + 1], kw[w + 2], kw[w + 3]};
+    }
+  };
+  auto put_v = [&](int k0) __attribute__((always_inline)) {
+    if (k0 + kPreKeys - 1 > kmax) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (k0 + 4 * vkg + e > kmax) {
+#pragma unroll
+          for (int w = 0; w < VWT; ++w) vw[e][w] = 0;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int w = 0; w < VWT; ++w) note(vw[e][w]);
+    // the key group's slots in its run of 16: keys 0-3, 8-11 | 4-7, 12-15
+    const int unit = 2 * (vkg >> 2) + (vkg & 1), sub = 4 * ((vkg >> 1) & 1);
+#pragma unroll
+    for (int j = 0; j < VDT; ++j) {
+      const int at = v_slot(unit, vd + j) + sub;
+      if constexpr (F32) {
+        uint32_t x[3], y[3];
+        split_pair<__bf16>(__builtin_bit_cast(float, vw[0][j]), __builtin_bit_cast(float, vw[1][j]), x);
+        split_pair<__bf16>(__builtin_bit_cast(float, vw[2][j]), __builtin_bit_cast(float, vw[3][j]), y);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) *(u32x2_t*)&tl.v[i][vd + j][at] = u32x2_t{x[i], y[i]};
+      } else {
+        const uint32_t sel = j & 1 ? 0x07060302u : 0x05040100u;
+        *(u32x2_t*)&tl.v[0][vd + j][at] =
+            u32x2_t{__builtin_amdgcn_perm(vw[1][j >> 1], vw[0][j >> 1], sel),
+                    __builtin_amdgcn_perm(vw[3][j >> 1], vw[2][j >> 1], sel)};
+      }
+    }
+  };
+
+  f16v acc[VB];
+#pragma unroll
+  for (int b = 0; b < VB; ++b) acc[b] = (f16v){};
+  float m = -INFINITY, l = 0.0f;  // of the column; l of this half's keys
+  int k0 = key0 & ~(kPreKeys - 1);
+  int64_t run = run_of(k0);
+  load_k(run);
+  for (; k0 <= kmax; k0 += kPreKeys) {
+    put_k(k0);  // (the last tile's K is done with since its second barrier)
+    load_v(run);
+    __syncthreads();
+    f16v s = {}, s1 = {};
+    // the small part products of all dims first: few roundings at a score's own size
+#pragma unroll
+    for (int i = 0; i < KT; ++i) {
+      vec kk[NK];
+#pragma unroll
+      for (int x = 0; x < NK; ++x) kk[x] = *(const vec*)&tl.k[x][col][16 * i + 8 * half];
+#pragma unroll
+      for (int sum = NP - 1; sum > 0; --sum)
+#pragma unroll
+        for (int x = NK - 1; x >= 0; --x)
+          if (sum - x >= 0 && sum - x < NP) s = Tr::mfma32(kk[x], q[sum - x][i], s);
+    }
+#pragma unroll
+    for (int i = 0; i < KT; ++i) {
+      const vec kh = *(const vec*)&tl.k[0][col][16 * i + 8 * half];
+      f16v& c = i % 2 == 0 ? s : s1;
+      c = Tr::mfma32(kh, q[0][i], c);
+    }
+    s += s1;
+    put_v(k0);
+    if (k0 + kPreKeys <= kmax) {
+      run = run_of(k0 + kPreKeys);
+      load_k(run);
+    }
+    __syncthreads();
+    // lane: keys 8 (i / 4) + 4 half + i % 4 of its column
+    const bool edge = k0 + kPreKeys - 1 > wave_first || (a.window > 0 && k0 <= wave_last - a.window);
+    float sl = rule.sl2;  // what is left to multiply
+    if (RULE || edge) {
+      sl = 1.0f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int k = k0 + 8 * (i >> 2) + 4 * half + (i & 3);
+        s[i] = RULE && a.softcap > 0.0f ? rule.cap_out * tanhf(s[i] * rule.cap_in) : s[i] * rule.sl2;
+        if constexpr (RULE) s[i] += rule.slope2 * (float)(k - qpos);
+        if (k > qpos || (a.window > 0 && k <= qpos - a.window)) s[i] = -INFINITY;
+      }
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[i] * sl);
+    mx = fmaxf(m, xor32_max(mx));
+    // rows with nothing visible yet keep m = -inf and weight 0
+    const float ref = (mx == -INFINITY ? 0.0f : mx) - Tr::kLift;
+    const float alpha = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mx);
+    if (__any(alpha != 1.0f)) {
+#pragma unroll
+      for (int b = 0; b < VB; ++b) acc[b] *= alpha;
+      l *= alpha;
+    }
+    m = mx;
+    // (scaled and shifted with one rounding)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], sl, -ref));
+    l += (((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]))) +
+         (((s[8] + s[9]) + (s[10] + s[11])) + ((s[12] + s[13]) + (s[14] + s[15])));
+    vec p[NP][2];  // 16 keys each
+    {
+      uint32_t w[NP][8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        uint32_t x[NP];
+        split_pair<M>(s[2 * j], s[2 * j + 1], x);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) w[i][j] = x[i];
+      }
+#pragma unroll
+      for (int i = 0; i < NP; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          p[i][u] = __builtin_bit_cast(vec, u32x4_t{w[i][4 * u], w[i][4 * u + 1], w[i][4 * u + 2], w[i][4 * u + 3]});
+    }
+    // a tile's sum from zero, its small products first: one rounding a tile at
+    // the output's own size
+#pragma unroll
+    for (int b = 0; b < VB; ++b) {
+      f16v o = {};
+      vec vh[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int at = v_slot(2 * u + half, 32 * b + col);
+        vec vv[NK];
+#pragma unroll
+        for (int x = 0; x < NK; ++x) vv[x] = *(const vec*)&tl.v[x][32 * b + col][at];
+        vh[u] = vv[0];
+#pragma unroll
+        for (int sum = NP - 1; sum > 0; --sum)
+#pragma unroll
+          for (int x = NK - 1; x >= 0; --x)
+            if (sum - x >= 0 && sum - x < NP) o = Tr::mfma32(vv[x], p[sum - x][u], o);
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) o = Tr::mfma32(vh[u], p[0][u], o);
+      acc[b] += o;
+    }
+  }
+  // (2^127: the rounding to bf16 may pass fp32's range)
+  if constexpr (F32) {
+    odd |= !(largest < 0x1p127f);
+  } else {
+    constexpr unsigned short inf = std::is_same<T, __bf16>::value ? 0x7f80 : 0x7c00;
+    odd |= largest16.x >= inf || largest16.y >= inf;
+  }
+  __syncthreads();  // every wave is done with the tile
+  if (lane == 0) count_lds[wave] = 0;
+  __builtin_amdgcn_wave_barrier();
+  if (__any(odd) && lane == 0) count_lds[wave] = 1;
+  __syncthreads();
+  if ((count_lds[0] | count_lds[1] | count_lds[2] | count_lds[3]) != 0) {
+    for (int c = 0; c < 32; ++c) {
+      const int64_t p = c0 + wave * 32 + c;
+      if (p >= pairs) break;
+      const int j = (int)(p / G);
+      slow_row<T>(a, seq, row0 + j, pos0 + j, kvh * G + (int)(p - (int64_t)j * G),
+                  (float*)pre_smem + wave * kSlowFloats);
+    }
+    return;
+  }
+  const float sum = xor32_sum(l);
+  if (!live) return;
+  const float f = qpos < 0 ? 1.0f : sum;  // (a row before the first key: zeros)
+#pragma unroll
+  for (int b = 0; b < VB; ++b)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int d = 32 * b + 8 * i + 4 * half;
+      if (FULL || d < a.hd)
+        *(f4*)(out + d) = f4{acc[b][4 * i] / f, acc[b][4 * i + 1] / f, acc[b][4 * i + 2] / f, acc[b][4 * i + 3] / f};
+    }
+}
+
+template <typename T, int HD, bool FULL, bool RULE>
+hipError_t prefill_launch(const PagedAttnArgs& a, hipStream_t stream) {
+  constexpr size_t tile = sizeof(PreTile<T, HD>), slow = 4 * kSlowFloats * sizeof(float);
+  constexpr size_t lds = tile > slow ? tile : slow;
+  const auto kernel = paged_prefill_kernel<T, HD, FULL, RULE>;
+  const hipError_t e = allow_dynamic_lds((const void*)kernel, lds);
+  if (e != hipSuccess) return e;
+  const int64_t grid = ((int64_t)a.max_rows * a.group / kPreCols + a.n_seqs) * a.n_kv;
+  if (grid > INT32_MAX) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(kPreThreads), lds, stream, a);
+  return hipGetLastError();
+}
+template <typename T, int HD>
+hipError_t prefill_launch_hd(const PagedAttnArgs& a, hipStream_t stream) {
+  const bool rule = a.softcap > 0.0f || a.slopes != nullptr;
+  if (a.hd == HD)
+    return rule ? prefill_launch<T, HD, true, true>(a, stream) : prefill_launch<T, HD, true, false>(a, stream);
+  return rule ? prefill_launch<T, HD, false, true>(a, stream) : prefill_launch<T, HD, false, false>(a, stream);
+}
+template <typename T>
+hipError_t prefill_launch_type(const PagedAttnArgs& a, hipStream_t stream) {
+  if (a.hd <= 64) return prefill_launch_hd<T, 64>(a, stream);
+  if (a.hd <= 128) return prefill_launch_hd<T, 128>(a, stream);
+  return prefill_launch_hd<T, 256>(a, stream);
+}
+
 }  // namespace
 
 size_t plan_paged_decode(PagedAttnArgs& a) {
@@ -720,7 +1134,9 @@ hipError_t launch_paged_decode(const PagedAttnArgs& all, hipStream_t stream) {
 }
 
 hipError_t launch_paged_prefill(const PagedAttnArgs& a, hipStream_t stream) {
-  return rows_launch(a, a.max_rows, 0, stream);
+  if (a.type == MLQ_KV_F32) return prefill_launch_type<float>(a, stream);
+  if (a.type == MLQ_KV_F16) return prefill_launch_type<_Float16>(a, stream);
+  return prefill_launch_type<__bf16>(a, stream);
 }
 
 }  // namespace mlq
