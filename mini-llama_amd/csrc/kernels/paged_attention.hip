@@ -187,11 +187,12 @@ struct ScoreRule {
   float cap_in, cap_out;  // cap_out tanh(s * cap_in); cap_out 0: no cap
   float slope2;      // slope * log2 e
 };
-__device__ __forceinline__ ScoreRule score_rule(const PagedAttnArgs& a, int head, int q_exp) {
+__device__ __forceinline__ ScoreRule score_rule(const PagedAttnArgs& a, int head, int q_exp,
+                                                float scale) {
   constexpr float kLog2e = 1.44269504088896341f;
   ScoreRule r;
-  r.sl2 = ldexp_f(a.scale * kLog2e, -q_exp);
-  r.cap_in = a.softcap > 0.0f ? ldexp_f(a.scale / a.softcap, -q_exp) : 0.0f;
+  r.sl2 = ldexp_f(scale * kLog2e, -q_exp);
+  r.cap_in = a.softcap > 0.0f ? ldexp_f(scale / a.softcap, -q_exp) : 0.0f;
   r.cap_out = a.softcap * kLog2e;
   r.slope2 = a.slopes != nullptr ? a.slopes[head] * kLog2e : 0.0f;
   return r;
@@ -372,7 +373,7 @@ __global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_k
         qv[i][s] = __builtin_bit_cast(raw8, u32x4_t{w[i][0], w[i][1], w[i][2], w[i][3]});
     }
   }
-  const ScoreRule rule = score_rule(a, head0 + (has_head ? ai : 0), q_exp);
+  const ScoreRule rule = score_rule(a, head0 + (has_head ? ai : 0), q_exp, a.scale);
   const bool plain = a.softcap <= 0.0f && a.slopes == nullptr;
 
   // ---- the keys
@@ -673,7 +674,6 @@ void decode_launch_hd(const PagedAttnArgs& a, int grid, hipStream_t stream) {
 // rows to slow_row.
 constexpr int kPreCols = 128, kPreKeys = 32, kPreThreads = 256;
 typedef float f16v __attribute__((ext_vector_type(16)));
-typedef unsigned short us2 __attribute__((ext_vector_type(2)));
 
 template <typename T>
 struct PreTraits : KvTraits<T> {
@@ -700,6 +700,16 @@ struct PreTile {
   static constexpr int NK = PreTraits<T>::kCacheParts;
   uint16_t k[NK][kPreKeys][HD + 8];   // [key][dim]
   uint16_t v[NK][HD][kPreKeys + 8];   // [dim][key slot], see v_slot
+};
+template <typename T, int HD>
+struct PreLds {
+  // 16-bit caches: the next tile is written beside the one that is read, a
+  // barrier a tile; fp32's parts leave no room for it (two barriers)
+  static constexpr int kBuf = sizeof(T) == 4 ? 1 : 2;
+  // steps of q's last part per wave and lane (in registers they spill)
+  static constexpr int kQ = PreTraits<T>::kParts < 3 || HD < 128 ? 0 : sizeof(T) == 4 ? HD / 32 : HD / 16;
+  PreTile<T, HD> tile[kBuf];
+  u32x4_t q[kQ > 0 ? kQ : 1][kPreThreads];
   int count[kPreThreads / 64];
 };
 
@@ -722,9 +732,11 @@ __global__ __launch_bounds__(kPreThreads, HD <= 128 ? 2 : 1) void paged_prefill_
   constexpr int KW = HD / 8 * (int)sizeof(T) / 4;   // words of K per thread: HD / 8 dims of a key
   constexpr int VDT = HD / 32;       // dims of V per thread, of 4 keys
   constexpr int VWT = VDT * (int)sizeof(T) / 4;     // their words a key (fp16 / bf16, HD 64: 1)
+  constexpr float kSlack = Tr::kLift == 0.0f ? 8.0f : 0.0f;
   extern __shared__ __align__(16) uint8_t pre_smem[];
-  PreTile<T, HD>& tl = *(PreTile<T, HD>*)pre_smem;
-  int* const count_lds = tl.count;
+  PreLds<T, HD>& lds = *(PreLds<T, HD>*)pre_smem;
+  constexpr int BUF = PreLds<T, HD>::kBuf, QL = PreLds<T, HD>::kQ;
+  int* const count_lds = lds.count;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
@@ -773,13 +785,17 @@ __global__ __launch_bounds__(kPreThreads, HD <= 128 ? 2 : 1) void paged_prefill_
   // ---- q
   int q_exp = 0;
   vec q[NP][KT];
-  bool odd = false;  // something that the matrix products do not carry
+  bool odd = false;  // a page outside the cache
+  bool cut = false;  // this column is written already
   {
     const float* qp = a.q + row * a.q_stride + (int64_t)head * a.hd + 8 * half;
     auto q_at = [&](int s, int u) __attribute__((always_inline)) {
       return live && (FULL || 16 * s + 8 * half < a.hd) ? *(const f4*)(qp + 16 * s + 4 * u)
                                                           : f4{0.0f, 0.0f, 0.0f, 0.0f};
     };
+    // (q's sign turned where the scale is negative: the largest score is then
+    // the largest product)
+    const float turned = a.scale < 0.0f ? -1.0f : 1.0f;
     if constexpr (Tr::kLift != 0.0f) {
       float big = 0.0f;
 #pragma unroll
@@ -796,7 +812,7 @@ __global__ __launch_bounds__(kPreThreads, HD <= 128 ? 2 : 1) void paged_prefill_
       uint32_t w[NP][4];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        f4 x = q_at(s, u);
+        f4 x = q_at(s, u) * turned;
         if constexpr (Tr::kLift != 0.0f)
           x = f4{ldexp_f(x.x, q_exp), ldexp_f(x.y, q_exp), ldexp_f(x.z, q_exp), ldexp_f(x.w, q_exp)};
 #pragma unroll
@@ -810,32 +826,42 @@ __global__ __launch_bounds__(kPreThreads, HD <= 128 ? 2 : 1) void paged_prefill_
 #pragma unroll
       for (int i = 0; i < NP; ++i)
         q[i][s] = __builtin_bit_cast(vec, u32x4_t{w[i][0], w[i][1], w[i][2], w[i][3]});
+      if (s < QL) lds.q[s < QL ? s : 0][tid] = __builtin_bit_cast(u32x4_t, q[NP - 1][s]);  // (read by this lane only)
     }
   }
-  const ScoreRule rule = score_rule(a, head, q_exp);
+  auto q_part = [&](int i, int s) __attribute__((always_inline)) {
+    return i == NP - 1 && s < QL ? __builtin_bit_cast(vec, lds.q[s < QL ? s : 0][tid]) : q[i][s];
+  };
+  const ScoreRule rule = score_rule(a, head, q_exp, fabsf(a.scale));
 
   // ---- staging: a wave's keys lie in one run of 16 (and so in one page)
   const int32_t* table = a.block_table + (size_t)seq * a.max_pages;
-  const int mask = (1 << a.page_shift) - 1;
-  auto run_of = [&](int k0) __attribute__((always_inline)) {
+  const int mask = (1 << a.page_shift) - 1, row_bytes = a.hd * (int)sizeof(T);
+  // Asked for a tile ahead of the rows it names: a load that waits for it waits
+  // twice.
+  auto page_of = [&](int k0) __attribute__((always_inline)) {
+    return table[min(k0 + 16 * (wave >> 1), kmax) >> a.page_shift];
+  };
+  auto run_of = [&](int k0, int id) __attribute__((always_inline)) {
     const int kk = min(k0 + 16 * (wave >> 1), kmax);
-    int page = __builtin_amdgcn_readfirstlane(table[kk >> a.page_shift]);
+    int page = __builtin_amdgcn_readfirstlane(id);
     const bool outside = page < 0 || page >= a.n_pages;
     odd |= outside;
     page = outside ? 0 : page;
-    return (((int64_t)page * a.n_kv + kvh) << a.page_shift) + (kk & mask & ~15);
+    return ((((int64_t)page * a.n_kv + kvh) << a.page_shift) + (kk & mask & ~15)) * row_bytes;
   };
   const int kkey = tid >> 3, kd = (tid & 7) * (16 / (int)sizeof(T));  // K: dims kd + 8 threads' pieces
   const int vkg = tid >> 5, vd = (tid & 31) * VDT;                    // V: keys 4 vkg .. + 3
   uint32_t kw[KW], vw[4][VWT];
-  float largest = 0.0f;
-  us2 largest16 = {0, 0};
+  // (a run's start is uniform, a lane's place in it never changes)
+  const uint32_t k_at = (kkey & 15) * row_bytes + kd * (int)sizeof(T);
+  const uint32_t v_at = 4 * (vkg & 3) * row_bytes + vd * (int)sizeof(T);
   auto load_k = [&](int64_t run) __attribute__((always_inline)) {
-    const char* p = (const char*)a.keys + (run + (kkey & 15)) * a.hd * (int64_t)sizeof(T);
+    const char* p = (const char*)a.keys + run;
 #pragma unroll
     for (int w = 0; w < KW; w += 4) {
-      const int d = kd + w * 32 / (int)sizeof(T);
-      const u32x4_t x = FULL || d < a.hd ? *(const u32x4_t*)(p + (size_t)d * sizeof(T)) : u32x4_t{0, 0, 0, 0};
+      const bool in = FULL || kd + w * 32 / (int)sizeof(T) < a.hd;
+      const u32x4_t x = in ? *(const u32x4_t*)(p + k_at + w * 32) : u32x4_t{0, 0, 0, 0};
 #pragma unroll
       for (int i = 0; i < 4; ++i) kw[w + i] = x[i];
     }
@@ -843,42 +869,29 @@ __global__ __launch_bounds__(kPreThreads, HD <= 128 ? 2 : 1) void paged_prefill_
   auto load_v = [&](int64_t run) __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const char* p = (const char*)a.values +
-                      ((run + 4 * (vkg & 3) + e) * a.hd + vd) * (int64_t)sizeof(T);
+      const char* p = (const char*)a.values + run + e * row_bytes;
       if constexpr (VWT >= 4) {
 #pragma unroll
         for (int w = 0; w < VWT; w += 4) {
           const bool in = FULL || vd + w * 4 / (int)sizeof(T) < a.hd;
-          const u32x4_t x = in ? *(const u32x4_t*)(p + 4 * w) : u32x4_t{0, 0, 0, 0};
+          const u32x4_t x = in ? *(const u32x4_t*)(p + v_at + 4 * w) : u32x4_t{0, 0, 0, 0};
 #pragma unroll
           for (int i = 0; i < 4; ++i) vw[e][w + i] = x[i];
         }
       } else if constexpr (VWT == 2) {
-        const u32x2_t x = FULL || vd < a.hd ? *(const u32x2_t*)p : u32x2_t{0, 0};
+        const u32x2_t x = FULL || vd < a.hd ? *(const u32x2_t*)(p + v_at) : u32x2_t{0, 0};
         vw[e][0] = x.x;
         vw[e][1] = x.y;
       } else {
-        vw[e][0] = FULL || vd < a.hd ? *(const uint32_t*)p : 0u;
+        vw[e][0] = FULL || vd < a.hd ? *(const uint32_t*)(p + v_at) : 0u;
       }
     }
   };
-  auto note = [&](uint32_t w) __attribute__((always_inline)) {
-    if constexpr (F32)
-      largest = __builtin_elementwise_maximum(largest, fabsf(__builtin_bit_cast(float, w)));
-    else
-      largest16 = __builtin_elementwise_max(largest16, __builtin_bit_cast(us2, w & 0x7fff7fffu));
-  };
-  auto put_k = [&](int k0) __attribute__((always_inline)) {
+  auto put_k = [&](PreTile<T, HD>& tl) __attribute__((always_inline)) {
     if constexpr (F32) {
-      if (k0 + kkey > kmax) {  // (what lies there may be anything)
-#pragma unroll
-        for (int w = 0; w < KW; ++w) kw[w] = 0;
-      }
 #pragma unroll
       for (int w = 0; w < KW; w += 4) {
         uint32_t x[3], y[3];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) note(kw[w + i]);
         split_pair<__bf16>(__builtin_bit_cast(float, kw[w]), __builtin_bit_cast(float, kw[w + 1]), x);
         split_pair<__bf16>(__builtin_bit_cast(float, kw[w + 2]), __builtin_bit_cast(float, kw[w + 3]), y);
 #pragma unroll
@@ -890,7 +903,7 @@ __global__ __launch_bounds__(kPreThreads, HD <= 128 ? 2 : 1) void paged_prefill_
         *(u32x4_t*)&tl.k[0][kkey][kd + w * 16] = u32x4_t{kw[w], kw[w + 1], kw[w + 2], kw[w + 3]};
     }
   };
-  auto put_v = [&](int k0) __attribute__((always_inline)) {
+  auto put_v = [&](PreTile<T, HD>& tl, int k0) __attribute__((always_inline)) {
     if (k0 + kPreKeys - 1 > kmax) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -899,10 +912,6 @@ __global__ __launch_bounds__(kPreThreads, HD <= 128 ? 2 : 1) void paged_prefill_
           for (int w = 0; w < VWT; ++w) vw[e][w] = 0;
         }
     }
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-#pragma unroll
-      for (int w = 0; w < VWT; ++w) note(vw[e][w]);
     // the key group's slots in its run of 16: keys 0-3, 8-11 | 4-7, 12-15
     const int unit = 2 * (vkg >> 2) + (vkg & 1), sub = 4 * ((vkg >> 1) & 1);
 #pragma unroll
@@ -928,16 +937,38 @@ __global__ __launch_bounds__(kPreThreads, HD <= 128 ? 2 : 1) void paged_prefill_
   for (int b = 0; b < VB; ++b) acc[b] = (f16v){};
   float m = -INFINITY, l = 0.0f;  // of the column; l of this half's keys
   int k0 = key0 & ~(kPreKeys - 1);
-  int64_t run = run_of(k0);
+  int64_t run = run_of(k0, page_of(k0));
   load_k(run);
-  for (; k0 <= kmax; k0 += kPreKeys) {
-    put_k(k0);  // (the last tile's K is done with since its second barrier)
+  int next_page = page_of(k0 + kPreKeys);
+  auto next = [&](int k) __attribute__((always_inline)) {
+    run = run_of(k, next_page);
+    next_page = page_of(k + kPreKeys);
+  };
+  if constexpr (BUF == 2) {
     load_v(run);
+    put_k(lds.tile[0]);
+    put_v(lds.tile[0], k0);
     __syncthreads();
+  }
+  for (int cur = 0; k0 <= kmax; k0 += kPreKeys, cur ^= BUF - 1) {
+    PreTile<T, HD>& tl = lds.tile[cur];
+    const bool more = k0 + kPreKeys <= kmax;
+    if constexpr (BUF == 2) {
+      if (more) {
+        next(k0 + kPreKeys);
+        load_k(run);
+        load_v(run);
+      }
+    } else {
+      put_k(tl);  // (the last tile's K is done with since its second barrier)
+      load_v(run);
+      __syncthreads();
+    }
     f16v s = {}, s1 = {};
     // the small part products of all dims first: few roundings at a score's own size
 #pragma unroll
     for (int i = 0; i < KT; ++i) {
+      f16v& c = i % 2 == 0 ? s : s1;
       vec kk[NK];
 #pragma unroll
       for (int x = 0; x < NK; ++x) kk[x] = *(const vec*)&tl.k[x][col][16 * i + 8 * half];
@@ -945,21 +976,22 @@ __global__ __launch_bounds__(kPreThreads, HD <= 128 ? 2 : 1) void paged_prefill_
       for (int sum = NP - 1; sum > 0; --sum)
 #pragma unroll
         for (int x = NK - 1; x >= 0; --x)
-          if (sum - x >= 0 && sum - x < NP) s = Tr::mfma32(kk[x], q[sum - x][i], s);
+          if (sum - x >= 0 && sum - x < NP) c = Tr::mfma32(kk[x], q_part(sum - x, i), c);
     }
 #pragma unroll
     for (int i = 0; i < KT; ++i) {
-      const vec kh = *(const vec*)&tl.k[0][col][16 * i + 8 * half];
       f16v& c = i % 2 == 0 ? s : s1;
-      c = Tr::mfma32(kh, q[0][i], c);
+      c = Tr::mfma32(*(const vec*)&tl.k[0][col][16 * i + 8 * half], q[0][i], c);
     }
     s += s1;
-    put_v(k0);
-    if (k0 + kPreKeys <= kmax) {
-      run = run_of(k0 + kPreKeys);
-      load_k(run);
+    if constexpr (BUF == 1) {
+      put_v(tl, k0);
+      if (more) {
+        next(k0 + kPreKeys);
+        load_k(run);
+      }
+      __syncthreads();
     }
-    __syncthreads();
     // lane: keys 8 (i / 4) + 4 half + i % 4 of its column
     const bool edge = k0 + kPreKeys - 1 > wave_first || (a.window > 0 && k0 <= wave_last - a.window);
     float sl = rule.sl2;  // what is left to multiply
@@ -973,19 +1005,22 @@ __global__ __launch_bounds__(kPreThreads, HD <= 128 ? 2 : 1) void paged_prefill_
         if (k > qpos || (a.window > 0 && k <= qpos - a.window)) s[i] = -INFINITY;
       }
     }
-    float mx = -INFINITY;
+    float mx = s[0];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[i] * sl);
-    mx = fmaxf(m, xor32_max(mx));
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+    mx = fmaxf(m, xor32_max(mx) * sl);
+    // The reference of the weights follows the maximum only where it is 2^kSlack
+    // behind (bf16 parts hold any size): less to rescale.
+    if constexpr (kSlack > 0.0f) mx = mx > m + kSlack ? mx : m;
     // rows with nothing visible yet keep m = -inf and weight 0
     const float ref = (mx == -INFINITY ? 0.0f : mx) - Tr::kLift;
-    const float alpha = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mx);
-    if (__any(alpha != 1.0f)) {
+    if (__any(mx != m)) {
+      const float alpha = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mx);
 #pragma unroll
       for (int b = 0; b < VB; ++b) acc[b] *= alpha;
       l *= alpha;
+      m = mx;
     }
-    m = mx;
     // (scaled and shifted with one rounding)
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], sl, -ref));
@@ -1007,54 +1042,55 @@ __global__ __launch_bounds__(kPreThreads, HD <= 128 ? 2 : 1) void paged_prefill_
         for (int u = 0; u < 2; ++u)
           p[i][u] = __builtin_bit_cast(vec, u32x4_t{w[i][4 * u], w[i][4 * u + 1], w[i][4 * u + 2], w[i][4 * u + 3]});
     }
-    // a tile's sum from zero, its small products first: one rounding a tile at
-    // the output's own size
 #pragma unroll
-    for (int b = 0; b < VB; ++b) {
-      f16v o = {};
-      vec vh[2];
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+      for (int b = 0; b < VB; ++b) {
         const int at = v_slot(2 * u + half, 32 * b + col);
         vec vv[NK];
 #pragma unroll
         for (int x = 0; x < NK; ++x) vv[x] = *(const vec*)&tl.v[x][32 * b + col][at];
-        vh[u] = vv[0];
 #pragma unroll
-        for (int sum = NP - 1; sum > 0; --sum)
+        for (int sum = NP - 1; sum >= 0; --sum)
 #pragma unroll
           for (int x = NK - 1; x >= 0; --x)
-            if (sum - x >= 0 && sum - x < NP) o = Tr::mfma32(vv[x], p[sum - x][u], o);
+            if (sum - x >= 0 && sum - x < NP) acc[b] = Tr::mfma32(vv[x], p[sum - x][u], acc[b]);
       }
-#pragma unroll
-      for (int u = 0; u < 2; ++u) o = Tr::mfma32(vh[u], p[0][u], o);
-      acc[b] += o;
+    if constexpr (BUF == 2) {
+      if (more) {
+        put_k(lds.tile[cur ^ 1]);
+        put_v(lds.tile[cur ^ 1], k0 + kPreKeys);
+        __syncthreads();
+      }
     }
   }
-  // (2^127: the rounding to bf16 may pass fp32's range)
-  if constexpr (F32) {
-    odd |= !(largest < 0x1p127f);
-  } else {
-    constexpr unsigned short inf = std::is_same<T, __bf16>::value ? 0x7f80 : 0x7c00;
-    odd |= largest16.x >= inf || largest16.y >= inf;
-  }
+  const float sum = xor32_sum(l);
+  // Infinities and NaN end up in the output, also those that a weight of 0 was
+  // to silence: columns that hold any, and all of a workgroup that met a page
+  // outside the cache, are computed again.
+  float zeros = sum * 0.0f;
+#pragma unroll
+  for (int b = 0; b < VB; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) zeros = __builtin_fmaf(acc[b][i], 0.0f, zeros);
   __syncthreads();  // every wave is done with the tile
   if (lane == 0) count_lds[wave] = 0;
   __builtin_amdgcn_wave_barrier();
   if (__any(odd) && lane == 0) count_lds[wave] = 1;
   __syncthreads();
-  if ((count_lds[0] | count_lds[1] | count_lds[2] | count_lds[3]) != 0) {
-    for (int c = 0; c < 32; ++c) {
-      const int64_t p = c0 + wave * 32 + c;
-      if (p >= pairs) break;
-      const int j = (int)(p / G);
-      slow_row<T>(a, seq, row0 + j, pos0 + j, kvh * G + (int)(p - (int64_t)j * G),
-                  (float*)pre_smem + wave * kSlowFloats);
-    }
-    return;
+  const bool again = (count_lds[0] | count_lds[1] | count_lds[2] | count_lds[3]) != 0;
+  uint64_t redo = __ballot(live && (again || !(zeros == 0.0f)));
+  redo = (redo | redo >> 32) & 0xffffffffu;
+  while (redo != 0) {
+    const int c = __builtin_ctzll(redo);
+    redo &= redo - 1;
+    const int64_t p = c0 + wave * 32 + c;
+    const int j = (int)(p / G);
+    slow_row<T>(a, seq, row0 + j, pos0 + j, kvh * G + (int)(p - (int64_t)j * G),
+                (float*)pre_smem + wave * kSlowFloats);
+    if (c == col) cut = true;
   }
-  const float sum = xor32_sum(l);
-  if (!live) return;
+  if (!live || cut) return;
   const float f = qpos < 0 ? 1.0f : sum;  // (a row before the first key: zeros)
 #pragma unroll
   for (int b = 0; b < VB; ++b)
@@ -1068,8 +1104,8 @@ __global__ __launch_bounds__(kPreThreads, HD <= 128 ? 2 : 1) void paged_prefill_
 
 template <typename T, int HD, bool FULL, bool RULE>
 hipError_t prefill_launch(const PagedAttnArgs& a, hipStream_t stream) {
-  constexpr size_t tile = sizeof(PreTile<T, HD>), slow = 4 * kSlowFloats * sizeof(float);
-  constexpr size_t lds = tile > slow ? tile : slow;
+  constexpr size_t lds = sizeof(PreLds<T, HD>);
+  static_assert(sizeof(PreTile<T, HD>) >= kPreThreads / 64 * kSlowFloats * sizeof(float), "slow_row's");
   const auto kernel = paged_prefill_kernel<T, HD, FULL, RULE>;
   const hipError_t e = allow_dynamic_lds((const void*)kernel, lds);
   if (e != hipSuccess) return e;
