@@ -718,6 +718,100 @@ struct PreLds {
 // the dim spreads them over the banks.
 __device__ __forceinline__ int v_slot(int unit, int dim) { return (unit ^ ((dim >> 4) & 3)) * 8; }
 
+// Which tile of which sequence a workgroup takes (seq < 0: none).
+struct PreWork {
+  int seq, tile;
+};
+__device__ __forceinline__ int wave_sum_int(int b) {
+  b += __builtin_amdgcn_update_dpp(0, b, kDppXor1, 0xF, 0xF, false);
+  b += __builtin_amdgcn_update_dpp(0, b, kDppXor2, 0xF, 0xF, false);
+  b += __builtin_amdgcn_update_dpp(0, b, kDppHalfMirror, 0xF, 0xF, false);
+  b += __builtin_amdgcn_update_dpp(0, b, kDppMirror, 0xF, 0xF, false);
+  return (__builtin_amdgcn_readlane(b, 0) + __builtin_amdgcn_readlane(b, 16)) +
+         (__builtin_amdgcn_readlane(b, 32) + __builtin_amdgcn_readlane(b, 48));
+}
+__device__ __forceinline__ int wave_max_int(int b) {
+  b = max(b, __builtin_amdgcn_update_dpp(0, b, kDppXor1, 0xF, 0xF, false));
+  b = max(b, __builtin_amdgcn_update_dpp(0, b, kDppXor2, 0xF, 0xF, false));
+  b = max(b, __builtin_amdgcn_update_dpp(0, b, kDppHalfMirror, 0xF, 0xF, false));
+  b = max(b, __builtin_amdgcn_update_dpp(0, b, kDppMirror, 0xF, 0xF, false));
+  return max(max(__builtin_amdgcn_readlane(b, 0), __builtin_amdgcn_readlane(b, 16)),
+             max(__builtin_amdgcn_readlane(b, 32), __builtin_amdgcn_readlane(b, 48)));
+}
+__device__ __forceinline__ int seq_tiles(const PagedAttnArgs& a, int i) {
+  const int s0 = a.row_start[i], s1 = min(a.row_start[i + 1], a.max_rows);
+  return s0 < 0 || s1 <= s0 ? 0 : (int)(((int64_t)(s1 - s0) * a.group + kPreCols - 1) / kPreCols);
+}
+// The x-th tile when those with the most keys come first, so that no long one
+// starts last: a tile's level is how many tiles' rows its last key lies before
+// the longest sequence's end, a sequence has one tile a level, and the level
+// of x is found by a search over the count of tiles before it. Every wave does
+// that for itself, kPreSeqsPerLane sequences a lane.
+constexpr int kPreSeqsPerLane = 4;
+__device__ __forceinline__ PreWork longest_first(const PagedAttnArgs& a, int x) {
+  const int lane = threadIdx.x & 63;
+  int tiles[kPreSeqsPerLane], level[kPreSeqsPerLane], longest = 0, total = 0, end = 0;
+#pragma unroll
+  for (int n = 0; n < kPreSeqsPerLane; ++n) {
+    const int i = lane + 64 * n;
+    tiles[n] = 0;
+    level[n] = 0;
+    if (i < a.n_seqs) {
+      tiles[n] = seq_tiles(a, i);
+      level[n] = min(max(a.lengths[i], 0), a.max_len);
+      if (tiles[n] > 0) longest = max(longest, level[n]);
+    }
+    total += tiles[n];
+  }
+  longest = wave_max_int(longest);
+#pragma unroll
+  for (int n = 0; n < kPreSeqsPerLane; ++n) {
+    level[n] = (int)((int64_t)(longest - min(level[n], longest)) * a.group / kPreCols);
+    if (tiles[n] > 0) end = max(end, level[n] + tiles[n]);
+  }
+  if (x >= wave_sum_int(total)) return {-1, 0};
+  auto before = [&](int at) {
+    int c = 0;
+#pragma unroll
+    for (int n = 0; n < kPreSeqsPerLane; ++n) c += min(max(at - level[n], 0), tiles[n]);
+    return wave_sum_int(c);
+  };
+  int lo = 0, hi = wave_max_int(end);  // before(lo) <= x < before(hi)
+  while (hi - lo > 1) {
+    const int mid = lo + ((hi - lo) >> 1);
+    if (before(mid) <= x) lo = mid;
+    else hi = mid;
+  }
+  int rank = x - before(lo);
+  PreWork w = {-1, 0};
+#pragma unroll
+  for (int n = 0; n < kPreSeqsPerLane; ++n) {
+    uint64_t has = __ballot(tiles[n] > 0 && lo >= level[n] && lo < level[n] + tiles[n]);
+    const int count = __builtin_popcountll(has);
+    if (w.seq < 0 && rank < count) {
+      for (int r = 0; r < rank; ++r) has &= has - 1;
+      const int from = __builtin_ctzll(has);
+      w.seq = from + 64 * n;
+      w.tile = __builtin_amdgcn_readlane(tiles[n], from) - 1 - (lo - __builtin_amdgcn_readlane(level[n], from));
+    }
+    rank -= count;
+  }
+  return w;
+}
+// For many sequences: sequence i owns the tiles from row_start[i] * G / 128 + i
+// on, at least as many as it needs, found without a sum over the sequences
+// before it.
+__device__ __forceinline__ PreWork by_row(const PagedAttnArgs& a, int x, int* lds) {
+  auto first_tile = [&](int i) { return (int)((int64_t)a.row_start[i] * a.group / kPreCols) + i; };
+  int before = 0;
+  for (int i = threadIdx.x; i < a.n_seqs; i += kPreThreads) before += first_tile(i) <= x;
+  before = wave_sum_int(before);
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = before;
+  __syncthreads();
+  const int seq = __builtin_amdgcn_readfirstlane(lds[0] + lds[1] + lds[2] + lds[3]) - 1;
+  return {seq, seq < 0 ? 0 : x - first_tile(seq)};
+}
+
 // RULE: scores are capped or biased (a variant of its own: its values spill
 // beside the others').
 template <typename T, int HD, bool FULL, bool RULE>
@@ -742,22 +836,13 @@ __global__ __launch_bounds__(kPreThreads, HD <= 128 ? 2 : 1) void paged_prefill_
   const int col = lane & 31, half = lane >> 5;
   const int G = a.group;
   const int kvh = blockIdx.x % a.n_kv;
-  const int tile = (int)(gridDim.x / a.n_kv) - 1 - (int)(blockIdx.x / a.n_kv);
-
-  // Sequence i owns the tiles from row_start[i] * G / 128 + i on: at least as
-  // many as it needs, found without a sum over the sequences before it.
-  auto first_tile = [&](int i) { return (int)((int64_t)a.row_start[i] * G / kPreCols) + i; };
-  int before = 0;
-  for (int i = tid; i < a.n_seqs; i += kPreThreads) before += first_tile(i) <= tile;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o);
-  if (lane == 0) count_lds[wave] = before;
-  __syncthreads();
-  const int seq = __builtin_amdgcn_readfirstlane(count_lds[0] + count_lds[1] + count_lds[2] + count_lds[3]) - 1;
+  const PreWork work = a.n_seqs <= 64 * kPreSeqsPerLane ? longest_first(a, (int)(blockIdx.x / a.n_kv))
+                                                        : by_row(a, (int)(blockIdx.x / a.n_kv), count_lds);
+  const int seq = work.seq;
   if (seq < 0) return;
   const int row0 = a.row_start[seq], row1 = min(a.row_start[seq + 1], a.max_rows);
   const int64_t pairs = (int64_t)(row1 - row0) * G;
-  const int64_t c0 = (int64_t)(tile - first_tile(seq)) * kPreCols;
+  const int64_t c0 = (int64_t)work.tile * kPreCols;
   if (row0 < 0 || c0 < 0 || c0 >= pairs) return;
   const int len = a.lengths[seq];
   const int pos0 = len - (a.row_start[seq + 1] - row0);  // of the sequence's first row
