@@ -16,48 +16,39 @@ namespace {
 // held = ceil(L / P) pages of a sequence, need = ceil((L + a) / P) - held new
 // ones; releases are pushed on the stack at the prefix sum of their counts,
 // needs popped at theirs, so the result is that of a loop over sequences. One
-// workgroup walks the sequences in tiles of a thread each (the scans are all
-// there is to do; 300 sequences fit one tile); pages and rows of a tile are
-// then spread over all threads, each finding its sequence by a search in the
-// tile's prefix sums.
-constexpr int kPlanThreads = 1024;
+// workgroup walks the sequences in tiles of a thread each. Latency is all of it:
+// the prefix sums run in registers with one barrier a tile, a thread writes a
+// few pages and rows of its sequence itself and the wave many of them, and a
+// row takes its page from the stack or the table as they were, not from what
+// was just written. 48 sequences, a
+// token each: 4.1 us, of them about 2 for the launch.
 // Row arrays up to this size are written by the scanning workgroup itself,
-// larger ones by a second launch over the whole chip.
+// larger ones by a second launch over the whole chip (4096 rows: 5.5 us against
+// 4.4 + 2.9).
 constexpr int kPlanInlineRows = 4096;
+constexpr int kPlanOwn = 8;  // pages or rows of a sequence that its own thread writes
 
-// Inclusive prefix sum over the workgroup; every thread gets its own and the
-// total. `lds`: one int per wave.
-__device__ __forceinline__ int block_scan(int v, int* lds, int* total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int u = __shfl_up(v, o);
-    if (lane >= o) v += u;
-  }
-  __syncthreads();  // (an earlier scan's readers are done with lds)
-  if (lane == 63) lds[wave] = v;
-  __syncthreads();
-  int before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < kPlanThreads / 64; ++w) {
-    const int t = lds[w];
-    before += w < wave ? t : 0;
-    all += t;
-  }
-  *total = all;
-  return v + before;
+template <int CTRL>
+__device__ __forceinline__ int64_t dpp64(int64_t v) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, 0xF, 0xF, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, 0xF, 0xF, false);
+  return (int64_t)((uint64_t)hi << 32 | lo);
 }
-
-__device__ __forceinline__ int64_t block_sum64(int64_t v, int64_t* lds) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-  __syncthreads();
-  int64_t all = 0;
-#pragma unroll
-  for (int w = 0; w < kPlanThreads / 64; ++w) all += lds[w];
-  return all;
+__device__ __forceinline__ int64_t readlane64(int64_t v, int lane) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane);
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+// Inclusive prefix sum over the wave: within the rows of 16 lanes by shifts
+// (0x110 + n: from n lanes below, 0 where there is none), then the rows before.
+__device__ __forceinline__ int64_t wave_scan64(int64_t v) {
+  v += dpp64<0x111>(v);
+  v += dpp64<0x112>(v);
+  v += dpp64<0x114>(v);
+  v += dpp64<0x118>(v);
+  const int row = (threadIdx.x & 63) >> 4;
+  const int64_t a = readlane64(v, 15), b = a + readlane64(v, 31), c = b + readlane64(v, 47);
+  return v + (row == 0 ? 0 : row == 1 ? a : row == 2 ? b : c);
 }
 
 // Last i with start[i] <= r; start[0] <= r. The one that r falls into: an
@@ -74,7 +65,7 @@ __device__ __forceinline__ int find_start(const int* start, int n, int r) {
 
 struct PlanSeq {
   int len, add, held, need, freed;
-  bool bad;
+  bool bad, ended;
 };
 __device__ __forceinline__ PlanSeq plan_seq(const PlanArgs& a, int i) {
   PlanSeq s = {};
@@ -85,102 +76,146 @@ __device__ __forceinline__ PlanSeq plan_seq(const PlanArgs& a, int i) {
     s.bad = true;
     return s;
   }
-  const int up = (1 << a.page_shift) - 1;  // (sums below stay under 2^31: cap does)
+  const int up = (1 << a.page_shift) - 1;
   s.len = len;
   s.add = max(n, 0);
+  s.ended = n < 0;
   s.held = (int)(((int64_t)len + up) >> a.page_shift);
   s.freed = n < 0 ? s.held : 0;
   s.need = n < 0 ? 0 : (int)(((int64_t)len + n + up) >> a.page_shift) - s.held;
   return s;
 }
 
-__global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a, int inline_rows) {
-  __shared__ int scan_lds[kPlanThreads / 64];
-  __shared__ int64_t sum_lds[kPlanThreads / 64];
-  __shared__ int first[kPlanThreads], rows[kPlanThreads], held[kPlanThreads], lens[kPlanThreads];
-  const int tid = threadIdx.x;
-  const int free0 = *a.n_free;
+// Sums of rows, needed and released pages: before a thread's sequence, or of
+// all. 64 bits: bad counts may add up to anything.
+struct PlanSums {
+  int64_t add, need, freed;
+  int bad;
+};
 
-  int64_t add = 0, need = 0, freed = 0, bad = 0;
-  for (int i0 = 0; i0 < a.n_seqs; i0 += kPlanThreads) {
-    const PlanSeq s = plan_seq(a, i0 + tid);
-    add += s.add;
-    need += s.need;
-    freed += s.freed;
-    bad += s.bad;
+// A tile's prefix sums (exclusive) and totals; `lds`: a PlanSums per wave.
+template <int T>
+__device__ __forceinline__ PlanSums plan_scan(const PlanSeq& s, PlanSums* lds, PlanSums* total) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t add = wave_scan64(s.add), need = wave_scan64(s.need), freed = wave_scan64(s.freed);
+  const bool bad = __any(s.bad);
+  __syncthreads();  // (an earlier scan's readers are done with lds)
+  if ((threadIdx.x & 63) == 63) lds[wave] = {add, need, freed, bad};
+  __syncthreads();
+  // every wave scans the waves' sums, a lane each
+  const int lane = threadIdx.x & 63;
+  const PlanSums mine = lane < T / 64 ? lds[lane] : PlanSums{0, 0, 0, 0};
+  const int64_t adds = wave_scan64(mine.add), needs = wave_scan64(mine.need),
+                freeds = wave_scan64(mine.freed);
+  *total = {readlane64(adds, 63), readlane64(needs, 63), readlane64(freeds, 63), __any(mine.bad)};
+  PlanSums before = {add - s.add, need - s.need, freed - s.freed, 0};
+  if (wave > 0) {
+    before.add += readlane64(adds, wave - 1);
+    before.need += readlane64(needs, wave - 1);
+    before.freed += readlane64(freeds, wave - 1);
   }
-  add = block_sum64(add, sum_lds);
-  need = block_sum64(need, sum_lds);
-  freed = block_sum64(freed, sum_lds);
-  bad = block_sum64(bad, sum_lds);
-  const int64_t avail = free0 + freed;
+  return before;
+}
+
+template <int T>
+__global__ __launch_bounds__(T) void plan_kernel(PlanArgs a, int inline_rows) {
+  __shared__ PlanSums scan_lds[T / 64];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int free0 = *a.n_free;
+  const PlanSeq s0 = plan_seq(a, tid);
+
+  PlanSums all, tile0;
+  const PlanSums before0 = plan_scan<T>(s0, scan_lds, &tile0);
+  all = tile0;
+  for (int i0 = T; i0 < a.n_seqs; i0 += T) {
+    PlanSums t;
+    plan_scan<T>(plan_seq(a, i0 + tid), scan_lds, &t);
+    all.add += t.add;
+    all.need += t.need;
+    all.freed += t.freed;
+    all.bad |= t.bad;
+  }
+  const int64_t avail = free0 + all.freed;
   int status = MLQ_PLAN_OK;
-  if (bad != 0 || free0 < 0 || avail > a.n_pages) status = MLQ_PLAN_BAD_COUNT;
-  else if (add > a.max_rows) status = MLQ_PLAN_ROWS;
-  else if (need > avail) status = MLQ_PLAN_PAGES;
+  if (all.bad != 0 || free0 < 0 || avail > a.n_pages) status = MLQ_PLAN_BAD_COUNT;
+  else if (all.add > a.max_rows) status = MLQ_PLAN_ROWS;
+  else if (all.need > avail) status = MLQ_PLAN_PAGES;
   const bool ok = status == MLQ_PLAN_OK;
 
-  if (ok && freed > 0) {
-    int base = free0;
-    for (int i0 = 0; i0 < a.n_seqs; i0 += kPlanThreads) {
-      const PlanSeq s = plan_seq(a, i0 + tid);
-      int total;
-      const int end = block_scan(s.freed, scan_lds, &total);
-      first[tid] = end - s.freed;
-      __syncthreads();
-      for (int r = tid; r < total; r += kPlanThreads) {
-        const int i = find_start(first, kPlanThreads, r);
-        a.free_pages[base + r] = a.block_table[(size_t)(i0 + i) * a.max_pages + (r - first[i])];
-      }
-      base += total;
-      __syncthreads();
+  const int64_t width = a.max_pages;
+  // f(i, k, n) for the n items of each lane's i: a few by the lane itself, many
+  // by the whole wave, lane after lane.
+  auto each = [&](int n, auto item) __attribute__((always_inline)) {
+    if (n <= kPlanOwn)
+      for (int k = 0; k < n; ++k) item(k, -1);
+    uint64_t many = __ballot(n > kPlanOwn);
+    while (many != 0) {
+      const int from = __builtin_ctzll(many);
+      many &= many - 1;
+      const int count = __builtin_amdgcn_readlane(n, from);
+      for (int k = lane; k < count; k += 64) item(k, from);
     }
+  };
+  // a lane's value, or that of the lane whose items the wave does
+  auto of = [](int v, int from) __attribute__((always_inline)) {
+    return from < 0 ? v : __builtin_amdgcn_readlane(v, from < 0 ? 0 : from);
+  };
+  if (ok && all.freed > 0) {
+    int base = free0;
+    for (int i0 = 0; i0 < a.n_seqs; i0 += T) {
+      PlanSeq s = s0;
+      PlanSums total = tile0, before = before0;
+      if (i0 > 0) {
+        s = plan_seq(a, i0 + tid);
+        before = plan_scan<T>(s, scan_lds, &total);
+      }
+      const int seq = i0 + tid, at = base + (int)before.freed;
+      each(s.freed, [&](int k, int from) {
+        a.free_pages[of(at, from) + k] = a.block_table[of(seq, from) * width + k];
+      });
+      base += (int)total.freed;
+    }
+    __syncthreads();
   }
+  const int page_mask = (1 << a.page_shift) - 1;
   int popped = 0, row0 = 0;
-  for (int i0 = 0; i0 < a.n_seqs; i0 += kPlanThreads) {
+  for (int i0 = 0; i0 < a.n_seqs; i0 += T) {
     const int seq = i0 + tid;
-    const PlanSeq s = plan_seq(a, seq);
-    int needs = 0, adds = 0;
-    if (ok) {
-      const int need_end = block_scan(s.need, scan_lds, &needs);
-      const int add_end = block_scan(s.add, scan_lds, &adds);
-      first[tid] = need_end - s.need;
-      rows[tid] = add_end - s.add;
-      held[tid] = s.held;
-      lens[tid] = s.len;
+    PlanSeq s = s0;
+    PlanSums total = tile0, before = before0;
+    if (i0 > 0) {
+      s = plan_seq(a, seq);
+      before = plan_scan<T>(s, scan_lds, &total);
     }
     if (seq < a.n_seqs) {
-      a.row_start[seq] = ok ? row0 + rows[tid] : 0;
-      a.lengths_out[seq] = ok ? (s.freed > 0 || a.n_new[seq] < 0 ? 0 : s.len + s.add) : a.lengths[seq];
+      a.row_start[seq] = ok ? row0 + (int)before.add : 0;
+      a.lengths_out[seq] = ok ? (s.ended ? 0 : s.len + s.add) : a.lengths[seq];
     }
-    __syncthreads();
-    for (int r = tid; r < needs; r += kPlanThreads) {
-      const int i = find_start(first, kPlanThreads, r);
-      a.block_table[(size_t)(i0 + i) * a.max_pages + held[i] + (r - first[i])] =
-          a.free_pages[avail - 1 - (popped + r)];
-    }
-    __syncthreads();
-    if (inline_rows) {
-      for (int r = tid; r < adds; r += kPlanThreads) {
-        const int i = find_start(rows, kPlanThreads, r);
-        const int pos = lens[i] + (r - rows[i]);
-        const int page = a.block_table[(size_t)(i0 + i) * a.max_pages + (pos >> a.page_shift)];
-        a.positions[row0 + r] = pos;
-        a.slots[row0 + r] = ((int64_t)page << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
-      }
-    }
-    popped += needs;
-    row0 += adds;
-    __syncthreads();
+    if (!ok) continue;
+    const int rank = popped + (int)before.need, row = row0 + (int)before.add;
+    auto pop = [&](int r) { return a.free_pages[avail - 1 - r]; };
+    each(s.need, [&](int k, int from) {
+      a.block_table[of(seq, from) * width + of(s.held, from) + k] = pop(of(rank, from) + k);
+    });
+    if (inline_rows)
+      each(s.add, [&](int k, int from) {
+        const int pos = of(s.len, from) + k, j = pos >> a.page_shift, held = of(s.held, from);
+        const int page = j < held ? a.block_table[of(seq, from) * width + j] : pop(of(rank, from) + j - held);
+        const int r = of(row, from) + k;
+        a.positions[r] = pos;
+        a.slots[r] = ((int64_t)page << a.page_shift) + (pos & page_mask);
+      });
+    popped += (int)total.need;
+    row0 += (int)total.add;
   }
   if (inline_rows)
-    for (int r = row0 + tid; r < a.max_rows; r += kPlanThreads) {
+    for (int r = row0 + tid; r < a.max_rows; r += T) {
       a.positions[r] = -1;
       a.slots[r] = -1;
     }
   if (tid == 0) {
     a.row_start[a.n_seqs] = row0;
-    *a.n_free_out = ok ? (int)(avail - need) : free0;
+    *a.n_free_out = ok ? (int)(avail - all.need) : free0;
     *a.status = status;
   }
 }
@@ -333,7 +368,12 @@ void rotary_launch(const RotaryArgs& a, hipStream_t stream) {
 
 hipError_t launch_paged_plan(const PlanArgs& a, hipStream_t stream) {
   const bool rows = a.max_rows <= kPlanInlineRows;
-  hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, a, rows ? 1 : 0);
+  // (a workgroup of the sequences' size: a barrier of four waves costs less
+  // than one of sixteen)
+  if (a.n_seqs <= 256 && a.max_rows <= 1024)
+    hipLaunchKernelGGL(plan_kernel<256>, dim3(1), dim3(256), 0, stream, a, rows ? 1 : 0);
+  else
+    hipLaunchKernelGGL(plan_kernel<1024>, dim3(1), dim3(1024), 0, stream, a, rows ? 1 : 0);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || rows) return e;
   hipLaunchKernelGGL(plan_rows_kernel, dim3((a.max_rows + 255) / 256), dim3(256), 0, stream, a);
