@@ -9,6 +9,7 @@
 
 #include "device_common.h"
 #include "paged.h"
+#include "paged_device.h"
 
 namespace mlq {
 namespace {
@@ -107,6 +108,7 @@ __device__ void slow_row(const PagedAttnArgs& a, int seq, int row, int pos, int 
 // below fp16's subnormals is 2^-39 of those), the cache's values are exact.
 // fp32 caches take the fp32 instructions, whose rate is no bound here either.
 constexpr int kDecWaves = 4, kDecThreads = 64 * kDecWaves;
+constexpr int kDecSeqsPerLane = 1;  // up to 64 sequences each wave plans for itself
 constexpr int kDecMaxSeqs = 4096;  // sequences of a launch: their prefix sums lie in LDS
 
 typedef float f4 __attribute__((ext_vector_type(4)));
@@ -198,28 +200,6 @@ __device__ __forceinline__ ScoreRule score_rule(const PagedAttnArgs& a, int head
   return r;
 }
 
-// Workgroup-wide exclusive prefix sum over kDecThreads values.
-__device__ __forceinline__ int dec_scan(int v, int* lds, int* total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int x = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int u = __shfl_up(x, o);
-    if (lane >= o) x += u;
-  }
-  __syncthreads();
-  if (lane == 63) lds[wave] = x;
-  __syncthreads();
-  int before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < kDecWaves; ++w) {
-    before += w < wave ? lds[w] : 0;
-    all += lds[w];
-  }
-  *total = all;
-  return x - v + before;
-}
-
 // Partials of an item (a part of one sequence's keys for up to `tg` heads of
 // a kv head): maxima and sums [tg] each, accumulators [tg][hd].
 struct DecodePartials {
@@ -260,7 +240,7 @@ __global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_k
   __shared__ int64_t total_lds[kDecWaves];
   __shared__ __align__(16) float merge[kDecWaves][16][OS];
   __shared__ float wm[kDecWaves][16], wl[kDecWaves][16];
-  __shared__ int any_bad;
+  __shared__ int wave_bad[kDecWaves];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -268,59 +248,117 @@ __global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_k
   const int head_tiles = (a.group + 15) / 16, n_tiles = a.n_kv * head_tiles;
 
   // ---- the parts of every sequence
-  int64_t keys = 0;
-  for (int i = tid; i < a.n_seqs; i += kDecThreads) {
-    const DecodeRow r = decode_row(a, i);
-    if (r.row >= 0) keys += r.len - first_key(a, r.len);
-  }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) keys += __shfl_xor(keys, o);
-  if (lane == 0) total_lds[wave] = keys;
-  if (tid == 0) any_bad = 0;
-  __syncthreads();
-  keys = 0;
-#pragma unroll
-  for (int w = 0; w < kDecWaves; ++w) keys += total_lds[w];
-  const int64_t want = (keys * n_tiles + a.part_target - 1) / a.part_target;
-  const int part_len = (int)min((want / kUnit + (want % kUnit != 0)) * kUnit, (int64_t)1 << 30);
-  const int plen = max(part_len, kUnit);
-  int parts = 0;
-  for (int i0 = 0; i0 < a.n_seqs; i0 += kDecThreads) {
-    const int i = i0 + tid;
-    int n = 0;
-    if (i < a.n_seqs) {
-      const DecodeRow r = decode_row(a, i);
-      const int range = r.len - first_key(a, r.len);
-      if (r.row >= 0) n = max(1, range / plen + (range % plen != 0));
-    }
-    int total;
-    const int at = dec_scan(n, scan_lds, &total);
-    if (i < a.n_seqs) base[i] = parts + at;
-    parts += total;
-  }
-  if (tid == 0) base[a.n_seqs] = parts;
-  __syncthreads();
   const DecodePartials pp = decode_partials(a.part, a.n_seqs, a.max_items, min(a.group, 16));
-  if (blockIdx.x == 0 && pp.first_item != nullptr)
-    for (int i = tid; i < a.n_seqs; i += kDecThreads) {
-      pp.first_item[i] = base[i];
-      pp.parts[i] = base[i + 1] - base[i];
-    }
   const int item = blockIdx.x;
   const int pi = item / n_tiles, tile = item - pi * n_tiles;
-  if (pi >= parts) return;
-  int seq = 0;
-  {
+  auto part_of = [&](int64_t keys) {  // a part's length: whole tiles of the four waves
+    const int64_t want = (keys * n_tiles + a.part_target - 1) / a.part_target;
+    return (int)min(max((want + kUnit - 1) / kUnit, (int64_t)1) * kUnit, (int64_t)1 << 30);
+  };
+  auto parts_of = [&](const DecodeRow& r, int plen) {
+    const int range = r.len - first_key(a, r.len);
+    return r.row < 0 ? 0 : max(1, range / plen + (range % plen != 0));
+  };
+  int seq = 0, part = 0, n_parts = 1, plen;
+  DecodeRow dr;
+  if (a.n_seqs <= 64 * kDecSeqsPerLane) {
+    // neighbouring sequences in a lane, in every wave for itself: no barriers
+    constexpr int NL = kDecSeqsPerLane;
+    DecodeRow r[NL];
+    int n[NL], sum = 0;
+#pragma unroll
+    for (int j = 0; j < NL; ++j) {
+      r[j] = {-1, 0, false};
+      if (NL * lane + j < a.n_seqs) r[j] = decode_row(a, NL * lane + j);
+    }
+    int64_t total = 0;
+#pragma unroll
+    for (int j = 0; j < NL; ++j) {
+      if (r[j].row >= 0) total += r[j].len - first_key(a, r[j].len);
+    }
+    plen = part_of(wave_last64(wave_scan64(total)));
+#pragma unroll
+    for (int j = 0; j < NL; ++j) {
+      n[j] = parts_of(r[j], plen);
+      sum += n[j];
+    }
+    const int end = (int)wave_scan64(sum);
+    if (item == 0 && wave == 0 && pp.first_item != nullptr) {
+      int at = end - sum;
+#pragma unroll
+      for (int j = 0; j < NL; ++j) {
+        if (NL * lane + j < a.n_seqs) {
+          pp.first_item[NL * lane + j] = at;
+          pp.parts[NL * lane + j] = n[j];
+        }
+        at += n[j];
+      }
+    }
+    const uint64_t behind = __ballot(end > pi);  // (lanes past the last sequence hold the total)
+    if (behind == 0) return;
+    const int from = __builtin_ctzll(behind);
+    int at = __builtin_amdgcn_readlane(end - sum, from);
+    bool found = false;
+#pragma unroll
+    for (int j = 0; j < NL; ++j) {
+      const int count = __builtin_amdgcn_readlane(n[j], from);
+      if (!found && pi < at + count) {
+        found = true;
+        seq = NL * from + j;
+        part = pi - at;
+        n_parts = count;
+        dr = {__builtin_amdgcn_readlane(r[j].row, from), __builtin_amdgcn_readlane(r[j].len, from),
+              __builtin_amdgcn_readlane((int)r[j].bad, from) != 0};
+      }
+      at += count;
+    }
+  } else {
+    int64_t keys = 0;
+    for (int i = tid; i < a.n_seqs; i += kDecThreads) {
+      const DecodeRow r = decode_row(a, i);
+      if (r.row >= 0) keys += r.len - first_key(a, r.len);
+    }
+    keys = wave_last64(wave_scan64(keys));
+    if (lane == 0) total_lds[wave] = keys;
+    __syncthreads();
+    plen = part_of((total_lds[0] + total_lds[1]) + (total_lds[2] + total_lds[3]));
+    int parts = 0;
+    for (int i0 = 0; i0 < a.n_seqs; i0 += kDecThreads) {
+      const int i = i0 + tid;
+      const int n = i < a.n_seqs ? parts_of(decode_row(a, i), plen) : 0;
+      const int end = (int)wave_scan64(n);
+      __syncthreads();  // (an earlier tile's readers are done with scan_lds)
+      if (lane == 63) scan_lds[wave] = end;
+      __syncthreads();
+      int before = 0, all = 0;
+#pragma unroll
+      for (int w = 0; w < kDecWaves; ++w) {
+        before += w < wave ? scan_lds[w] : 0;
+        all += scan_lds[w];
+      }
+      if (i < a.n_seqs) base[i] = parts + before + end - n;
+      parts += all;
+    }
+    if (tid == 0) base[a.n_seqs] = parts;
+    __syncthreads();
+    if (item == 0 && pp.first_item != nullptr)
+      for (int i = tid; i < a.n_seqs; i += kDecThreads) {
+        pp.first_item[i] = base[i];
+        pp.parts[i] = base[i + 1] - base[i];
+      }
+    if (pi >= parts) return;
+    seq = 0;
     int hi = a.n_seqs;
     while (hi - seq > 1) {
       const int mid = (seq + hi) >> 1;
       if (base[mid] <= pi) seq = mid;
       else hi = mid;
     }
+    seq = __builtin_amdgcn_readfirstlane(seq);
+    part = pi - base[seq];
+    n_parts = base[seq + 1] - base[seq];
+    dr = decode_row(a, seq);
   }
-  seq = __builtin_amdgcn_readfirstlane(seq);
-  const int part = pi - base[seq], n_parts = base[seq + 1] - base[seq];
-  const DecodeRow dr = decode_row(a, seq);
   const int kvh = tile / head_tiles, g0 = (tile - kvh * head_tiles) * 16;
   const int G = min(16, a.group - g0), head0 = kvh * a.group + g0;
   const int key_begin = first_key(a, dr.len), pos = dr.len - 1;
@@ -399,7 +437,7 @@ __global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_k
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         const int d = F32 ? 16 * s + 4 * ak : 32 * s + 8 * ak;
-        if (FULL || d < a.hd) kr[u][s] = *(const u32x4_t*)(p + (size_t)d * sizeof(T));
+        if (FULL || d < a.hd) kr[u][s] = __builtin_nontemporal_load((const u32x4_t*)(p + (size_t)d * sizeof(T)));
         else kr[u][s] = u32x4_t{0, 0, 0, 0};
       }
     }
@@ -414,11 +452,11 @@ __global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_k
       for (int w = 0; w < VW; w += (VW < 4 ? 2 : 4)) {
         const int d = VD * ai + w * 4 / (int)sizeof(T);
         if constexpr (VW < 4) {
-          const u32x2_t x = FULL || d < a.hd ? *(const u32x2_t*)(p + (size_t)d * sizeof(T)) : u32x2_t{0, 0};
+          const u32x2_t x = FULL || d < a.hd ? __builtin_nontemporal_load((const u32x2_t*)(p + (size_t)d * sizeof(T))) : u32x2_t{0, 0};
           vr[e][w] = x.x;
           vr[e][w + 1] = x.y;
         } else {
-          const u32x4_t x = FULL || d < a.hd ? *(const u32x4_t*)(p + (size_t)d * sizeof(T)) : u32x4_t{0, 0, 0, 0};
+          const u32x4_t x = FULL || d < a.hd ? __builtin_nontemporal_load((const u32x4_t*)(p + (size_t)d * sizeof(T))) : u32x4_t{0, 0, 0, 0};
           vr[e][w] = x.x;
           vr[e][w + 1] = x.y;
           vr[e][w + 2] = x.z;
@@ -555,7 +593,7 @@ __global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_k
   l = xor32_sum(xor16_sum(l));
 
   // ---- the waves joined in their order
-  if (bad) any_bad = 1;
+  if (lane == 0) wave_bad[wave] = bad;
   if (ak == 0) {
     wm[wave][ai] = m;
     wl[wave][ai] = l;
@@ -587,6 +625,7 @@ __global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_k
         sum += wl[w][g] * f;
         o += merge[w][g][x] * f;
       }
+      const bool any_bad = (wave_bad[0] | wave_bad[1] | wave_bad[2] | wave_bad[3]) != 0;
       if (any_bad) sum = __builtin_nanf("");
       if (n_parts == 1) {
         out[(int64_t)g * a.hd + d] = dr.len > 0 || any_bad ? o / sum : 0.0f;
@@ -602,44 +641,72 @@ __global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_k
   }
 }
 
-// The parts of a sequence joined in their order, for one query head: wave w
-// takes parts w, w + 4, .., then the waves are joined.
+// The parts of a sequence joined for one query head: wave w takes parts 4 i + w,
+// kJoin at a time with every load asked for at once (places past the last
+// part read the last one and weigh 0), then the waves are joined in order.
+// KD: head dims per lane.
+constexpr int kJoin = 4;
+template <int KD>
 __global__ __launch_bounds__(kDecThreads) void paged_combine_kernel(PagedAttnArgs a) {
-  __shared__ float wl[kDecWaves], wo[kDecWaves][256];
+  __shared__ float wm[kDecWaves], wl[kDecWaves], wo[kDecWaves][64 * KD];
   const int seq = blockIdx.x, head = blockIdx.y;
   const int TG = min(a.group, 16), head_tiles = (a.group + 15) / 16, n_tiles = a.n_kv * head_tiles;
   const DecodePartials pp = decode_partials(a.part, a.n_seqs, a.max_items, TG);
-  const int parts = pp.parts[seq];
+  const int parts = pp.parts[seq], first = pp.first_item[seq];
   if (parts <= 1) return;
-  const int first = pp.first_item[seq];
   const int kvh = head / a.group, g = head - kvh * a.group;
   const int tile = kvh * head_tiles + g / 16;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  auto at = [&](int p) { return ((size_t)(first + p) * n_tiles + tile) * TG + g % 16; };
-  float mx = -INFINITY;
-  for (int p = lane; p < parts; p += 64) mx = fmaxf(mx, pp.m[at(p)]);
-  mx = wave_max(mx);
-  float l = 0.0f, acc[4] = {};
-#pragma unroll 4
-  for (int p = wave; p < parts; p += kDecWaves) {
-    const float pm = pp.m[at(p)];
-    const float f = pm == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(pm - mx);
-    l += pp.l[at(p)] * f;
+  float m = -INFINITY, l = 0.0f, acc[KD] = {};
+  for (int p0 = wave; p0 < parts; p0 += kDecWaves * kJoin) {
+    float pm[kJoin], pl[kJoin], pa[kJoin][KD];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (lane + 64 * j < a.hd) acc[j] += pp.acc[at(p) * a.hd + lane + 64 * j] * f;
+    for (int i = 0; i < kJoin; ++i) {
+      const size_t at = ((size_t)(first + min(p0 + kDecWaves * i, parts - 1)) * n_tiles + tile) * TG + g % 16;
+      pm[i] = pp.m[at];
+      pl[i] = pp.l[at];
+#pragma unroll
+      for (int j = 0; j < KD; ++j) pa[i][j] = pp.acc[at * a.hd + min(lane + 64 * j, a.hd - 1)];
+    }
+    float mx = m;
+#pragma unroll
+    for (int i = 0; i < kJoin; ++i) {
+      if (p0 + kDecWaves * i >= parts) pm[i] = -INFINITY;
+      mx = fmaxf(mx, pm[i]);
+    }
+    const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mx);
+    m = mx;
+    l *= f;
+#pragma unroll
+    for (int j = 0; j < KD; ++j) acc[j] *= f;
+#pragma unroll
+    for (int i = 0; i < kJoin; ++i) {
+      if (p0 + kDecWaves * i >= parts) break;  // (a part past the last, NaN or not, stays out)
+      const float w = pm[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(pm[i] - mx);
+      l += pl[i] * w;
+#pragma unroll
+      for (int j = 0; j < KD; ++j) acc[j] += pa[i][j] * w;
+    }
   }
-  if (lane == 0) wl[wave] = l;
+  if (lane == 0) {
+    wm[wave] = m;
+    wl[wave] = l;
+  }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) wo[wave][lane + 64 * j] = acc[j];
+  for (int j = 0; j < KD; ++j) wo[wave][lane + 64 * j] = acc[j];
   __syncthreads();
-  const DecodeRow dr = decode_row(a, seq);
-  float* out = a.out + dr.row * a.out_stride + (int64_t)head * a.hd;
   const int d = threadIdx.x;
-  if (d < a.hd) {
-    const float sum = (wl[0] + wl[1]) + (wl[2] + wl[3]);
-    out[d] = ((wo[0][d] + wo[1][d]) + (wo[2][d] + wo[3][d])) / sum;
+  if (d >= a.hd) return;
+  float mx = -INFINITY, sum = 0.0f, o = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kDecWaves; ++w) mx = fmaxf(mx, wm[w]);
+#pragma unroll
+  for (int w = 0; w < kDecWaves; ++w) {
+    const float f = wm[w] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(wm[w] - mx);
+    sum += wl[w] * f;
+    o += wo[w][d] * f;
   }
+  a.out[decode_row(a, seq).row * a.out_stride + (int64_t)head * a.hd + d] = o / sum;
 }
 
 template <typename T, int HD>
@@ -1247,8 +1314,13 @@ hipError_t launch_paged_decode(const PagedAttnArgs& all, hipStream_t stream) {
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     if (a.part == nullptr) continue;
-    hipLaunchKernelGGL(paged_combine_kernel, dim3(a.n_seqs, a.n_kv * a.group), dim3(kDecThreads), 0,
-                       stream, a);
+    const dim3 grid(a.n_seqs, a.n_kv * a.group);
+    if (a.hd <= 64)
+      hipLaunchKernelGGL(paged_combine_kernel<1>, grid, dim3(kDecThreads), 0, stream, a);
+    else if (a.hd <= 128)
+      hipLaunchKernelGGL(paged_combine_kernel<2>, grid, dim3(kDecThreads), 0, stream, a);
+    else
+      hipLaunchKernelGGL(paged_combine_kernel<4>, grid, dim3(kDecThreads), 0, stream, a);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   return hipSuccess;
