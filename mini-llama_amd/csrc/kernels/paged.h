@@ -44,6 +44,7 @@ struct RotaryArgs {
   int type, page_shift;
   int64_t n_slots;
   const int64_t* slots;
+  int stream;    // set by the launcher: q_out written past the caches
 };
 hipError_t launch_qk_norm_rope(const RotaryArgs& a, hipStream_t stream);
 
@@ -62,13 +63,12 @@ struct PagedAttnArgs {
   float scale, softcap;
   int window;
   const float* slopes;
-  // decode: about part_target parts of equal length over all sequences and kv
-  // heads, at most max_items; `part`: the workspace, null when every sequence
-  // is one part
-  int part_target, max_items;
+  // decode: launches of launch_seqs sequences, at most `ranges` workgroups;
+  // `part`: the workspace, null when every sequence is one piece
+  int launch_seqs, ranges;
   void* part;
 };
-// Sets part_target and max_items for lengths up to a.max_len; the workspace.
+// Sets launch_seqs and ranges for lengths up to a.max_len; the workspace.
 size_t plan_paged_decode(PagedAttnArgs& a);
 hipError_t launch_paged_decode(const PagedAttnArgs& a, hipStream_t stream);
 hipError_t launch_paged_prefill(const PagedAttnArgs& a, hipStream_t stream);

@@ -88,11 +88,14 @@ __device__ void slow_row(const PagedAttnArgs& a, int seq, int row, int pos, int 
 // ---- decode ------------------------------------------------------------------------
 // One query row of each sequence; out = softmax(rule(K q)) V with one pass over
 // the keys and a running maximum. The reads of K and V bound it, so the grid
-// is made of parts of equal length over all sequences (a sequence's keys are
-// cut into parts of part_len keys, part_len from the sum of the lengths, which
-// only the device knows: every workgroup scans the lengths), and a part's
-// workgroup joins its four waves in LDS. Sequences of more than one part leave
-// partials (maximum, sum, accumulator) that a second launch joins in order.
+// is as many workgroups as the chip holds, each with the same number of tiles:
+// the key tiles of every sequence and kv head, one behind the other, are cut
+// into equal ranges (their number is only known on the device: every workgroup
+// scans the lengths). A range runs over the ends of short sequences and stops
+// inside long ones: what it has of those it leaves as a partial (maximum, sum,
+// accumulator), at most one at either end, and a second launch joins them in
+// order. Sequences are padded to four tiles, one for each wave, so the
+// smallest ranges, of four tiles, hold one piece each.
 //
 // A wave takes tiles of kKeys keys and the up to 16 query heads of one kv head
 // through two products, both with the heads as columns:
@@ -108,7 +111,17 @@ __device__ void slow_row(const PagedAttnArgs& a, int seq, int row, int pos, int 
 // below fp16's subnormals is 2^-39 of those), the cache's values are exact.
 // fp32 caches take the fp32 instructions, whose rate is no bound here either.
 constexpr int kDecWaves = 4, kDecThreads = 64 * kDecWaves;
-constexpr int kDecSeqsPerLane = 1;  // up to 64 sequences each wave plans for itself
+// Ranges per CU: the workgroups that a CU holds (registers: 3, 2 and 1 waves a
+// SIMD at head dims up to 64, 128 and 256), so that all run at once. us with
+// another number: 64 sequences of up to 8000, 28 heads on 4 of 128, bf16, 1 / 2 /
+// 4 / 8 a CU: - / 69.6 / 73.7 / 82.4 (a workgroup for each part of one sequence:
+// 71.2); 20 of up to 20000, 16 on 1 of 256: 49 with 1, 64 with 2. At head dim 64
+// pieces are over soon, and where a range holds two and more of them, twice the
+// ranges let one workgroup's start hide behind another's work (180 of up to 2500,
+// 16 heads of 64, fp32: 3 a CU 161, 6 141; 30 of up to 9000, 40 on 8: 46 and 48).
+constexpr int dec_per_cu(int hd, int64_t pieces, int cus) {
+  return hd <= 64 ? (pieces >= 6 * (int64_t)cus ? 6 : 3) : hd <= 128 ? 2 : 1;
+}
 constexpr int kDecMaxSeqs = 4096;  // sequences of a launch: their prefix sums lie in LDS
 
 typedef float f4 __attribute__((ext_vector_type(4)));
@@ -200,25 +213,31 @@ __device__ __forceinline__ ScoreRule score_rule(const PagedAttnArgs& a, int head
   return r;
 }
 
-// Partials of an item (a part of one sequence's keys for up to `tg` heads of
-// a kv head): maxima and sums [tg] each, accumulators [tg][hd].
+// The cut: range w holds tiles w * range .. of all of them; sequence i's lie
+// from first[i] * n_tiles on, count[i] (a multiple of 4; 0: no row) for each of
+// the n_tiles kv heads (or runs of 16 heads of one). Partials: a range's first
+// and last piece, up to `tg` heads each: maxima and sums [tg], accumulators
+// [tg][hd].
 struct DecodePartials {
-  int* first_item;  // [n_seqs] of the sequence, over n_tiles
-  int* parts;       // [n_seqs] 1 and less: out is written already
+  int64_t* range;
+  int* first;
+  int* count;
   float* m;
   float* l;
   float* acc;
 };
 __host__ __device__ inline size_t dec_align(size_t b) { return (b + 255) & ~(size_t)255; }
-__host__ __device__ inline DecodePartials decode_partials(void* ws, int n_seqs, int items, int tg) {
+__host__ __device__ inline size_t dec_header(int n_seqs) { return dec_align(8 + (size_t)n_seqs * 8); }
+__host__ __device__ inline DecodePartials decode_partials(void* ws, int n_seqs, int ranges, int tg) {
   DecodePartials p;
   char* c = (char*)ws;
-  p.first_item = (int*)c;
-  p.parts = p.first_item + n_seqs;
-  c += dec_align((size_t)n_seqs * 8);
+  p.range = (int64_t*)c;
+  p.first = (int*)(c + 8);
+  p.count = p.first + n_seqs;
+  c += dec_header(n_seqs);
   p.m = (float*)c;
-  p.l = p.m + (size_t)items * tg;
-  c += dec_align((size_t)items * tg * 8);
+  p.l = p.m + (size_t)2 * ranges * tg;
+  c += dec_align((size_t)2 * ranges * tg * 8);
   p.acc = (float*)c;
   return p;
 }
@@ -237,7 +256,6 @@ __global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_k
   constexpr int kUnit = kDecWaves * KT;
   __shared__ int base[kDecMaxSeqs + 1];
   __shared__ int scan_lds[kDecWaves];
-  __shared__ int64_t total_lds[kDecWaves];
   __shared__ __align__(16) float merge[kDecWaves][16][OS];
   __shared__ float wm[kDecWaves][16], wl[kDecWaves][16];
   __shared__ int wave_bad[kDecWaves];
@@ -245,89 +263,30 @@ __global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_k
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int ai = lane & 15, ak = lane >> 4;
-  const int head_tiles = (a.group + 15) / 16, n_tiles = a.n_kv * head_tiles;
+  const int head_tiles = (a.group + 15) / 16, n_tiles = a.n_kv * head_tiles, TG = min(a.group, 16);
+  const DecodePartials pp = decode_partials(a.part, a.n_seqs, a.ranges, TG);
 
-  // ---- the parts of every sequence
-  const DecodePartials pp = decode_partials(a.part, a.n_seqs, a.max_items, min(a.group, 16));
-  const int item = blockIdx.x;
-  const int pi = item / n_tiles, tile = item - pi * n_tiles;
-  auto part_of = [&](int64_t keys) {  // a part's length: whole tiles of the four waves
-    const int64_t want = (keys * n_tiles + a.part_target - 1) / a.part_target;
-    return (int)min(max((want + kUnit - 1) / kUnit, (int64_t)1) * kUnit, (int64_t)1 << 30);
+  // ---- the ranges
+  auto tiles_of = [&](const DecodeRow& r) {
+    if (r.row < 0) return 0;
+    const int tiles = (r.len - (first_key(a, r.len) & ~(KT - 1)) + KT - 1) / KT;
+    return max((tiles + kDecWaves - 1) / kDecWaves, 1) * kDecWaves;
   };
-  auto parts_of = [&](const DecodeRow& r, int plen) {
-    const int range = r.len - first_key(a, r.len);
-    return r.row < 0 ? 0 : max(1, range / plen + (range % plen != 0));
-  };
-  int seq = 0, part = 0, n_parts = 1, plen;
-  DecodeRow dr;
-  if (a.n_seqs <= 64 * kDecSeqsPerLane) {
-    // neighbouring sequences in a lane, in every wave for itself: no barriers
-    constexpr int NL = kDecSeqsPerLane;
-    DecodeRow r[NL];
-    int n[NL], sum = 0;
-#pragma unroll
-    for (int j = 0; j < NL; ++j) {
-      r[j] = {-1, 0, false};
-      if (NL * lane + j < a.n_seqs) r[j] = decode_row(a, NL * lane + j);
-    }
-    int64_t total = 0;
-#pragma unroll
-    for (int j = 0; j < NL; ++j) {
-      if (r[j].row >= 0) total += r[j].len - first_key(a, r[j].len);
-    }
-    plen = part_of(wave_last64(wave_scan64(total)));
-#pragma unroll
-    for (int j = 0; j < NL; ++j) {
-      n[j] = parts_of(r[j], plen);
-      sum += n[j];
-    }
-    const int end = (int)wave_scan64(sum);
-    if (item == 0 && wave == 0 && pp.first_item != nullptr) {
-      int at = end - sum;
-#pragma unroll
-      for (int j = 0; j < NL; ++j) {
-        if (NL * lane + j < a.n_seqs) {
-          pp.first_item[NL * lane + j] = at;
-          pp.parts[NL * lane + j] = n[j];
-        }
-        at += n[j];
-      }
-    }
-    const uint64_t behind = __ballot(end > pi);  // (lanes past the last sequence hold the total)
-    if (behind == 0) return;
-    const int from = __builtin_ctzll(behind);
-    int at = __builtin_amdgcn_readlane(end - sum, from);
-    bool found = false;
-#pragma unroll
-    for (int j = 0; j < NL; ++j) {
-      const int count = __builtin_amdgcn_readlane(n[j], from);
-      if (!found && pi < at + count) {
-        found = true;
-        seq = NL * from + j;
-        part = pi - at;
-        n_parts = count;
-        dr = {__builtin_amdgcn_readlane(r[j].row, from), __builtin_amdgcn_readlane(r[j].len, from),
-              __builtin_amdgcn_readlane((int)r[j].bad, from) != 0};
-      }
-      at += count;
-    }
+  const bool few = a.n_seqs <= 64;  // a sequence a lane, in every wave for itself: no barriers
+  DecodeRow mine = {-1, 0, false};
+  int total, my_first = 0, my_count = 0;
+  if (few) {
+    if (lane < a.n_seqs) mine = decode_row(a, lane);
+    my_count = tiles_of(mine);
+    my_first = (int)wave_scan64(my_count) - my_count;
+    total = __builtin_amdgcn_readlane(my_first + my_count, 63);
   } else {
-    int64_t keys = 0;
-    for (int i = tid; i < a.n_seqs; i += kDecThreads) {
-      const DecodeRow r = decode_row(a, i);
-      if (r.row >= 0) keys += r.len - first_key(a, r.len);
-    }
-    keys = wave_last64(wave_scan64(keys));
-    if (lane == 0) total_lds[wave] = keys;
-    __syncthreads();
-    plen = part_of((total_lds[0] + total_lds[1]) + (total_lds[2] + total_lds[3]));
-    int parts = 0;
+    total = 0;
     for (int i0 = 0; i0 < a.n_seqs; i0 += kDecThreads) {
       const int i = i0 + tid;
-      const int n = i < a.n_seqs ? parts_of(decode_row(a, i), plen) : 0;
+      const int n = i < a.n_seqs ? tiles_of(decode_row(a, i)) : 0;
       const int end = (int)wave_scan64(n);
-      __syncthreads();  // (an earlier tile's readers are done with scan_lds)
+      __syncthreads();  // (an earlier round's readers are done with scan_lds)
       if (lane == 63) scan_lds[wave] = end;
       __syncthreads();
       int before = 0, all = 0;
@@ -336,35 +295,61 @@ __global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_k
         before += w < wave ? scan_lds[w] : 0;
         all += scan_lds[w];
       }
-      if (i < a.n_seqs) base[i] = parts + before + end - n;
-      parts += all;
+      if (i < a.n_seqs) base[i] = total + before + end - n;
+      total += all;
     }
-    if (tid == 0) base[a.n_seqs] = parts;
+    if (tid == 0) base[a.n_seqs] = total;
     __syncthreads();
-    if (item == 0 && pp.first_item != nullptr)
-      for (int i = tid; i < a.n_seqs; i += kDecThreads) {
-        pp.first_item[i] = base[i];
-        pp.parts[i] = base[i + 1] - base[i];
-      }
-    if (pi >= parts) return;
-    seq = 0;
-    int hi = a.n_seqs;
-    while (hi - seq > 1) {
-      const int mid = (seq + hi) >> 1;
-      if (base[mid] <= pi) seq = mid;
-      else hi = mid;
-    }
-    seq = __builtin_amdgcn_readfirstlane(seq);
-    part = pi - base[seq];
-    n_parts = base[seq + 1] - base[seq];
-    dr = decode_row(a, seq);
   }
+  const int64_t all = (int64_t)total * n_tiles;
+  const int64_t range = max((all + (int64_t)a.ranges * kDecWaves - 1) / ((int64_t)a.ranges * kDecWaves), (int64_t)1) * kDecWaves;
+  if (blockIdx.x == 0 && a.part != nullptr) {
+    if (tid == 0) *pp.range = range;
+    for (int i = tid; i < a.n_seqs; i += kDecThreads) {
+      pp.first[i] = few ? my_first : base[i];
+      pp.count[i] = few ? my_count : base[i + 1] - base[i];
+    }
+  }
+  int64_t u = blockIdx.x * range;
+  const int64_t uend = min(u + range, all);
+  if (u >= uend) return;
+  int seq = 0, first, count;  // of the piece's sequence
+  {
+    const int at = (int)(u / n_tiles);
+    if (few) {
+      seq = __builtin_ctzll(__ballot(my_first + my_count > at));
+    } else {
+      int hi = a.n_seqs;
+      while (hi - seq > 1) {
+        const int mid = (seq + hi) >> 1;
+        if (base[mid] <= at) seq = mid;
+        else hi = mid;
+      }
+      seq = __builtin_amdgcn_readfirstlane(seq);
+    }
+  }
+  auto take = [&]() __attribute__((always_inline)) {
+    first = few ? __builtin_amdgcn_readlane(my_first, seq) : __builtin_amdgcn_readfirstlane(base[seq]);
+    count = few ? __builtin_amdgcn_readlane(my_count, seq) : __builtin_amdgcn_readfirstlane(base[seq + 1]) - first;
+  };
+  take();
+  int tile = (int)((u - (int64_t)first * n_tiles) / count);
+  int k_at = (int)(u - (int64_t)first * n_tiles - (int64_t)tile * count);
+
+  // ---- the range's pieces
+  while (true) {
+  const DecodeRow dr = few ? DecodeRow{__builtin_amdgcn_readlane(mine.row, seq), __builtin_amdgcn_readlane(mine.len, seq),
+                                       __builtin_amdgcn_readlane((int)mine.bad, seq) != 0}
+                           : decode_row(a, seq);
+  const int piece = (int)min((int64_t)(count - k_at), uend - u);
+  const bool whole = piece == count;
+  const int slot = 2 * (int)blockIdx.x + (k_at == 0);
   const int kvh = tile / head_tiles, g0 = (tile - kvh * head_tiles) * 16;
   const int G = min(16, a.group - g0), head0 = kvh * a.group + g0;
   const int key_begin = first_key(a, dr.len), pos = dr.len - 1;
   // tiles start at multiples of their size: a run of 16 keys lies in one page
-  const int lo = (key_begin & ~(KT - 1)) + part * plen;
-  const int hi = part == n_parts - 1 ? dr.len : lo + plen;
+  const int lo = (key_begin & ~(KT - 1)) + k_at * KT;
+  const int hi = min((int64_t)lo + (int64_t)piece * KT, (int64_t)dr.len);
 
   // ---- q
   const bool has_head = ai < G;
@@ -593,12 +578,12 @@ __global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_k
   l = xor32_sum(xor16_sum(l));
 
   // ---- the waves joined in their order
+  __syncthreads();  // (the last piece's readers are done with the LDS)
   if (lane == 0) wave_bad[wave] = bad;
   if (ak == 0) {
     wm[wave][ai] = m;
     wl[wave][ai] = l;
   }
-  const int TG = min(a.group, 16);
   float* out = a.out + dr.row * a.out_stride + (int64_t)head0 * a.hd;
 #pragma unroll
   for (int c0 = 0; c0 < VD; c0 += RD) {
@@ -627,10 +612,10 @@ __global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_k
       }
       const bool any_bad = (wave_bad[0] | wave_bad[1] | wave_bad[2] | wave_bad[3]) != 0;
       if (any_bad) sum = __builtin_nanf("");
-      if (n_parts == 1) {
+      if (whole) {
         out[(int64_t)g * a.hd + d] = dr.len > 0 || any_bad ? o / sum : 0.0f;
       } else {
-        const size_t at = (size_t)item * TG + g;
+        const size_t at = (size_t)slot * TG + g;
         if (d == 0) {
           pp.m[at] = mx;
           pp.l[at] = sum;
@@ -639,30 +624,48 @@ __global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_k
       }
     }
   }
+  u += piece;
+  if (u >= uend) return;
+  k_at = 0;
+  if (++tile == n_tiles) {
+    tile = 0;
+    if (few) seq = __builtin_ctzll(__ballot(my_count > 0) & ~((2ull << seq) - 1));
+    else
+      do ++seq;
+      while (base[seq + 1] == base[seq]);
+    take();
+  }
+  }
 }
 
-// The parts of a sequence joined for one query head: wave w takes parts 4 i + w,
-// kJoin at a time with every load asked for at once (places past the last
-// part read the last one and weigh 0), then the waves are joined in order.
-// KD: head dims per lane.
+// The pieces of a sequence joined for one query head: wave w takes pieces
+// 4 i + w, kJoin at a time with every load asked for at once (places past the
+// last piece read the last one and weigh 0), then the waves are joined in
+// order. KD: head dims per lane.
 constexpr int kJoin = 4;
 template <int KD>
 __global__ __launch_bounds__(kDecThreads) void paged_combine_kernel(PagedAttnArgs a) {
   __shared__ float wm[kDecWaves], wl[kDecWaves], wo[kDecWaves][64 * KD];
   const int seq = blockIdx.x, head = blockIdx.y;
   const int TG = min(a.group, 16), head_tiles = (a.group + 15) / 16, n_tiles = a.n_kv * head_tiles;
-  const DecodePartials pp = decode_partials(a.part, a.n_seqs, a.max_items, TG);
-  const int parts = pp.parts[seq], first = pp.first_item[seq];
-  if (parts <= 1) return;
+  const DecodePartials pp = decode_partials(a.part, a.n_seqs, a.ranges, TG);
+  const int count = pp.count[seq], first_tile = pp.first[seq];
+  const int64_t range = *pp.range;
+  if (count <= 0) return;
   const int kvh = head / a.group, g = head - kvh * a.group;
   const int tile = kvh * head_tiles + g / 16;
+  const int64_t start = (int64_t)first_tile * n_tiles + (int64_t)tile * count;
+  const int w0 = (int)(start / range), parts = (int)((start + count - 1) / range) - w0 + 1;
+  if (parts <= 1) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   float m = -INFINITY, l = 0.0f, acc[KD] = {};
   for (int p0 = wave; p0 < parts; p0 += kDecWaves * kJoin) {
     float pm[kJoin], pl[kJoin], pa[kJoin][KD];
 #pragma unroll
     for (int i = 0; i < kJoin; ++i) {
-      const size_t at = ((size_t)(first + min(p0 + kDecWaves * i, parts - 1)) * n_tiles + tile) * TG + g % 16;
+      const int w = w0 + min(p0 + kDecWaves * i, parts - 1);
+      // (the sequence begins in its first range: that range's last piece)
+      const size_t at = (size_t)(2 * w + (w == w0)) * TG + g % 16;
       pm[i] = pp.m[at];
       pl[i] = pp.l[at];
 #pragma unroll
@@ -1283,23 +1286,23 @@ hipError_t prefill_launch_type(const PagedAttnArgs& a, hipStream_t stream) {
 }  // namespace
 
 size_t plan_paged_decode(PagedAttnArgs& a) {
-  const int head_tiles = (a.group + 15) / 16;
-  const int64_t seqs = std::min(a.n_seqs, kDecMaxSeqs), tiles = (int64_t)a.n_kv * head_tiles;
-  const int unit = kDecWaves * (a.type == MLQ_KV_F32 ? 16 : 32);
-  a.part_target = 4 * device_cus();
-  // a sequence has at most one part more than its share of the target, and one per unit
-  a.max_items = (int)std::min(seqs * tiles * ((a.max_len + unit - 1) / unit + 1),
-                              a.part_target + 2 * seqs * tiles);
-  if (a.max_len <= unit) return 0;  // every sequence is one part
+  const int64_t n_tiles = (int64_t)a.n_kv * ((a.group + 15) / 16);
+  const int keys = a.type == MLQ_KV_F32 ? 16 : 32, unit = kDecWaves * keys;
+  const int64_t units = (a.max_len + (int64_t)unit - 1) / unit;  // of a sequence
+  const int cus = device_cus();
+  // sequences of a launch: their prefix sums lie in LDS and fit 32 bits
+  a.launch_seqs = (int)std::min((int64_t)std::min(a.n_seqs, kDecMaxSeqs), std::max(((int64_t)1 << 28) / units, (int64_t)1));
+  a.ranges = (int)std::min(a.launch_seqs * n_tiles * units, (int64_t)dec_per_cu(a.hd, a.launch_seqs * n_tiles, cus) * cus);
+  if (units <= 1) return 0;  // every sequence is one piece
   const size_t tg = std::min(a.group, 16);
-  return dec_align((size_t)seqs * 8) + dec_align((size_t)a.max_items * tg * 8) +
-         (size_t)a.max_items * tg * a.hd * sizeof(float);
+  return dec_header(std::min(a.n_seqs, kDecMaxSeqs)) + dec_align((size_t)2 * a.ranges * tg * 8) +
+         (size_t)2 * a.ranges * tg * a.hd * sizeof(float);
 }
 
 hipError_t launch_paged_decode(const PagedAttnArgs& all, hipStream_t stream) {
-  for (int s0 = 0; s0 < all.n_seqs; s0 += kDecMaxSeqs) {
+  for (int s0 = 0; s0 < all.n_seqs; s0 += all.launch_seqs) {
     PagedAttnArgs a = all;
-    a.n_seqs = std::min(kDecMaxSeqs, all.n_seqs - s0);
+    a.n_seqs = std::min(all.launch_seqs, all.n_seqs - s0);
     a.block_table += (size_t)s0 * a.max_pages;
     a.lengths += s0;
     if (a.row_start != nullptr) {
@@ -1308,9 +1311,9 @@ hipError_t launch_paged_decode(const PagedAttnArgs& all, hipStream_t stream) {
       a.q += (int64_t)s0 * a.q_stride;
       a.out += (int64_t)s0 * a.out_stride;
     }
-    if (a.type == MLQ_KV_F32) decode_launch_hd<float>(a, a.max_items, stream);
-    else if (a.type == MLQ_KV_F16) decode_launch_hd<_Float16>(a, a.max_items, stream);
-    else decode_launch_hd<__bf16>(a, a.max_items, stream);
+    if (a.type == MLQ_KV_F32) decode_launch_hd<float>(a, a.ranges, stream);
+    else if (a.type == MLQ_KV_F16) decode_launch_hd<_Float16>(a, a.ranges, stream);
+    else decode_launch_hd<__bf16>(a, a.ranges, stream);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     if (a.part == nullptr) continue;

@@ -221,6 +221,11 @@ __global__ __launch_bounds__(256) void plan_rows_kernel(PlanArgs a) {
 // in 64 bits up to the quarter turn: pos * f in 32 bits would be off by
 // 2^-24 pos radians.
 constexpr int kRotaryThreads = 256, kRotaryMaxHalf = 128;
+// Queries past half of the last-level cache's 256 MB are written past the
+// caches: what reads them finds them gone anyway (8000 rows, 64 heads on 8 of
+// 128, bf16: 129 -> 122 us, 5.1 TB/s; the inputs are read through the caches,
+// where the projection may have left them: 701 rows 8.2 us, else 9.4).
+constexpr int64_t kRotaryStreamBytes = (int64_t)128 << 20;
 
 __device__ __forceinline__ void store_kv(void* base, int type, int64_t at, float4 x) {
   typedef float v4 __attribute__((ext_vector_type(4)));
@@ -322,7 +327,9 @@ __global__ __launch_bounds__(kRotaryThreads) void qk_norm_rope_kernel(RotaryArgs
     }
     if (!in) continue;
     if (is_q) {
-      *(float4*)(a.q_out + row * a.q_out_stride + (int64_t)h * a.hd + d) = x;
+      float* to = a.q_out + row * a.q_out_stride + (int64_t)h * a.hd + d;
+      if (a.stream) __builtin_nontemporal_store(f4_t{x.x, x.y, x.z, x.w}, (f4_t*)to);
+      else *(float4*)to = x;
     } else {
       if (a.k_out != nullptr)
         *(float4*)(a.k_out + row * a.k_out_stride + (int64_t)kh * a.hd + d) = x;
@@ -332,12 +339,13 @@ __global__ __launch_bounds__(kRotaryThreads) void qk_norm_rope_kernel(RotaryArgs
 }
 
 template <int LG>
-void rotary_launch(const RotaryArgs& a, hipStream_t stream) {
+void rotary_launch(RotaryArgs a, hipStream_t stream) {
   const int heads = a.n_heads + (a.keys != nullptr ? 2 : 1) * a.n_kv;
   const int per = kRotaryThreads / LG;
   // few rows: a row's heads over several workgroups, each with its own angles
   const int most = (heads + per - 1) / per;
   const int split = std::min(most, std::max(1, 2 * device_cus() / a.rows));
+  a.stream = (int64_t)a.rows * a.n_heads * a.hd * 4 > kRotaryStreamBytes;
   hipLaunchKernelGGL(qk_norm_rope_kernel<LG>, dim3(a.rows, split), dim3(kRotaryThreads), 0,
                      stream, a);
 }

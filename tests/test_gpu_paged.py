@@ -337,6 +337,21 @@ def test_decode_result_does_not_depend_on_the_bound(paged, seqs):
         assert torch.all(out[p.rows:] == 9.0)
 
 
+@pytest.mark.parametrize("row_start", [False, True])
+def test_decode_of_more_sequences_than_a_launch_takes(paged, row_start):
+    import torch
+    r = np.random.default_rng(8)
+    n = 4100
+    p = Problem(paged, "bf16", r.integers(0, 40, n), 4, 2, 64, 16, seed=19, new=(r.random(n) < 0.9).astype(int) if row_start else None)
+    if not row_start:
+        p.batch = paged.PagedBatch(p.batch.block_table, p.batch.lengths)
+    out = paged.attention_decode(p.cache, 0, p.batch, p.qd)
+    long = paged.attention_decode(p.cache, 0, p.batch, p.qd, max_len=p.table.shape[1] * 16)
+    torch.cuda.synchronize()
+    p.compare(out, p.want(rows=set(range(0, p.rows, 50)) | set(range(p.rows - 40, p.rows))))
+    assert torch.equal(out, long)
+
+
 def test_decode_rows_of_sequences_without_a_new_token(paged):
     """row_start names the rows: sequences that wait have none; of several new rows the last one is computed."""
     import torch
