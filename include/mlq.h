@@ -609,10 +609,12 @@ typedef struct mlq_attention_rule {
   const float* slopes;               /* [n_heads] (device) or NULL */
 } mlq_attention_rule;
 
-/* Workspace of mlq_paged_attention_decode for any lengths up to max_len and
- * any rule. */
-int mlq_paged_attention_workspace(const mlq_paged_cache* c, int n_heads, int n_seqs, int max_len,
-                                  size_t* bytes);
+/* Workspace of mlq_paged_attention_prefill for a batch of max_rows rows, with
+ * max_rows = 0 of mlq_paged_attention_decode, for any rule. Decode: also for
+ * any smaller max_len; prefill: for this max_rows, max_len and n_seqs (few rows
+ * share their keys over more workgroups). */
+int mlq_paged_attention_workspace(const mlq_paged_cache* c, int n_heads, int n_seqs, int max_rows,
+                                  int max_len, size_t* bytes);
 /* One new token of each sequence: for every sequence with a row (b->row_start
  * NULL: row i of sequence i), out of its last row = attention of q's last row
  * at position lengths[i] - 1 over the sequence's pages, query head h reading
@@ -634,12 +636,13 @@ int mlq_paged_attention_decode(const mlq_paged_cache* c, int layer, const mlq_pa
                                void* ws, size_t ws_bytes, mlq_stream_t stream);
 /* Every new row of every sequence (prompts, or pieces of them behind what is
  * cached): row j of n new ones of sequence i is at position lengths[i] - n + j
- * and sees the keys up to it. Same rule, layouts and checks; no workspace.
- * b->max_rows bounds row_start[n_seqs] (rows past it are not computed). */
+ * and sees the keys up to it. Same rule, layouts, checks and workspace
+ * contract. b->max_rows bounds row_start[n_seqs] (rows past it are not
+ * computed). */
 int mlq_paged_attention_prefill(const mlq_paged_cache* c, int layer, const mlq_paged_batch* b,
                                 const mlq_attention_rule* rule, int n_heads, const float* q,
-                                int64_t q_stride, float* out, int64_t out_stride,
-                                mlq_stream_t stream);
+                                int64_t q_stride, float* out, int64_t out_stride, int max_len,
+                                void* ws, size_t ws_bytes, mlq_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -206,10 +206,11 @@ SIGNATURES = {
                               ctypes.POINTER(_F)], _I),
     "mlq_qk_norm_rope": ([_RTP, _I, _P, _I, _I, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I64,
                           _PCP, _I, _P, _P], _I),
-    "mlq_paged_attention_workspace": ([_PCP, _I, _I, _I, ctypes.POINTER(_Z)], _I),
+    "mlq_paged_attention_workspace": ([_PCP, _I, _I, _I, _I, ctypes.POINTER(_Z)], _I),
     "mlq_paged_attention_decode": ([_PCP, _I, _PBP, _ARP, _I, _P, _I64, _P, _I64, _I, _P, _Z, _P],
                                    _I),
-    "mlq_paged_attention_prefill": ([_PCP, _I, _PBP, _ARP, _I, _P, _I64, _P, _I64, _P], _I),
+    "mlq_paged_attention_prefill": ([_PCP, _I, _PBP, _ARP, _I, _P, _I64, _P, _I64, _I, _P, _Z, _P],
+                                    _I),
 }
 
 _LIB = None

@@ -66,11 +66,15 @@ struct PagedAttnArgs {
   // decode: launches of launch_seqs sequences, at most `ranges` workgroups;
   // `part`: the workspace, null when every sequence is one piece
   int launch_seqs, ranges;
+  // prefill: workgroups that share a tile's keys
+  int splits;
   void* part;
 };
 // Sets launch_seqs and ranges for lengths up to a.max_len; the workspace.
 size_t plan_paged_decode(PagedAttnArgs& a);
 hipError_t launch_paged_decode(const PagedAttnArgs& a, hipStream_t stream);
+// Sets splits for a.max_rows rows and lengths up to a.max_len; the workspace.
+size_t plan_paged_prefill(PagedAttnArgs& a);
 hipError_t launch_paged_prefill(const PagedAttnArgs& a, hipStream_t stream);
 
 }  // namespace mlq

@@ -17,10 +17,11 @@ namespace {
 // One row of one query head by one wave, in plain fp32: a lane scores a key of
 // a tile of 64 against q in LDS, then takes head dims lane, lane + 64, .. of
 // the output. What the matrix kernels hand to it: rows that could see a value
-// or page that those do not carry. `lds`: kSlowFloats of the wave's own.
+// or page that those do not carry. Writes dims d0 .. d1 - 1; `lds`: kSlowFloats
+// of the wave's own.
 constexpr int kSlowFloats = 256 + 64 + 128;
 template <typename T>
-__device__ void slow_row(const PagedAttnArgs& a, int seq, int row, int pos, int head, float* lds) {
+__device__ void slow_row(const PagedAttnArgs& a, int seq, int row, int pos, int head, float* lds, int d0, int d1) {
   float* qs = lds;
   float* ps = lds + 256;
   int64_t* at = (int64_t*)(lds + 320);
@@ -81,7 +82,7 @@ __device__ void slow_row(const PagedAttnArgs& a, int seq, int row, int pos, int 
   float* out = a.out + row * a.out_stride + (int64_t)head * a.hd;
 #pragma unroll
   for (int j = 0; j < 4; ++j)
-    if (lane + 64 * j < a.hd)
+    if (lane + 64 * j >= d0 && lane + 64 * j < d1)
       out[lane + 64 * j] = bad ? __builtin_nanf("") : len > 0 ? acc[j] / l : 0.0f;
 }
 
@@ -817,7 +818,7 @@ __device__ __forceinline__ int seq_tiles(const PagedAttnArgs& a, int i) {
 // the longest sequence's end, a sequence has one tile a level, and the level
 // of x is found by a search over the count of tiles before it. Every wave does
 // that for itself, kPreSeqsPerLane sequences a lane.
-constexpr int kPreSeqsPerLane = 4;
+constexpr int kPreSeqsPerLane = 4, kPreSorted = 64 * kPreSeqsPerLane;
 __device__ __forceinline__ PreWork longest_first(const PagedAttnArgs& a, int x) {
   const int lane = threadIdx.x & 63;
   int tiles[kPreSeqsPerLane], level[kPreSeqsPerLane], longest = 0, total = 0, end = 0;
@@ -882,6 +883,54 @@ __device__ __forceinline__ PreWork by_row(const PagedAttnArgs& a, int x, int* ld
   return {seq, seq < 0 ? 0 : x - first_tile(seq)};
 }
 
+// A workgroup's tile of rows: its pairs, positions and the keys that they see.
+struct PreSpan {
+  int row0, pos0, len;  // of the sequence
+  int64_t pairs, c0;    // its pairs, the tile's first
+  int kfirst, kmax;     // first key (a multiple of kPreKeys) and last; kmax < 0: none
+  int tiles, each;      // key tiles, and of a workgroup when `splits` share them
+  bool live;
+};
+constexpr int kPreLeast = 4;  // key tiles of a workgroup, at least
+__device__ __forceinline__ PreSpan prefill_span(const PagedAttnArgs& a, const PreWork& w) {
+  PreSpan s = {};
+  if (w.seq < 0) return s;
+  s.row0 = a.row_start[w.seq];
+  const int end = a.row_start[w.seq + 1], row1 = min(end, a.max_rows);
+  s.pairs = (int64_t)(row1 - s.row0) * a.group;
+  s.c0 = (int64_t)w.tile * kPreCols;
+  if (s.row0 < 0 || s.c0 < 0 || s.c0 >= s.pairs) return s;
+  s.live = true;
+  s.len = a.lengths[w.seq];
+  s.pos0 = s.len - (end - s.row0);
+  const int ja = (int)(s.c0 / a.group), jb = (int)((min(s.c0 + kPreCols, s.pairs) - 1) / a.group);
+  s.kmax = s.pos0 + jb;
+  s.kfirst = (a.window > 0 ? max(0, s.pos0 + ja + 1 - a.window) : 0) & ~(kPreKeys - 1);
+  s.tiles = s.kmax < 0 ? 0 : (s.kmax - s.kfirst) / kPreKeys + 1;
+  s.each = max((s.tiles + a.splits - 1) / a.splits, kPreLeast);
+  return s;
+}
+
+// Partials of a tile of rows, kv head and split: maxima and sums [kPreCols],
+// accumulators [hd / 4][kPreCols][4]; before them what the join has to know of
+// each tile.
+struct PreJoin {
+  int parts;     // 1 and less: nothing to join
+  int cols, seq, row, pos, rem;  // of the first pair: its row, position and head of the group
+};
+struct PrePartial {
+  float* m;
+  float* l;
+  float* acc;
+};
+__host__ __device__ inline size_t prefill_partial_floats(int hd) { return (size_t)kPreCols * (hd + 2); }
+__host__ __device__ inline size_t prefill_header(int64_t blocks) { return dec_align((size_t)blocks * sizeof(PreJoin)); }
+__device__ __forceinline__ PrePartial prefill_partial(const PagedAttnArgs& a, int split) {
+  float* p = (float*)((char*)a.part + prefill_header(gridDim.x)) +
+             ((size_t)blockIdx.x * a.splits + split) * prefill_partial_floats(a.hd);
+  return {p, p + kPreCols, p + 2 * kPreCols};
+}
+
 // RULE: scores are capped or biased (a variant of its own: its values spill
 // beside the others').
 template <typename T, int HD, bool FULL, bool RULE>
@@ -906,36 +955,42 @@ __global__ __launch_bounds__(kPreThreads, HD <= 128 ? 2 : 1) void paged_prefill_
   const int col = lane & 31, half = lane >> 5;
   const int G = a.group;
   const int kvh = blockIdx.x % a.n_kv;
-  const PreWork work = a.n_seqs <= 64 * kPreSeqsPerLane ? longest_first(a, (int)(blockIdx.x / a.n_kv))
-                                                        : by_row(a, (int)(blockIdx.x / a.n_kv), count_lds);
-  const int seq = work.seq;
-  if (seq < 0) return;
-  const int row0 = a.row_start[seq], row1 = min(a.row_start[seq + 1], a.max_rows);
-  const int64_t pairs = (int64_t)(row1 - row0) * G;
-  const int64_t c0 = (int64_t)work.tile * kPreCols;
-  if (row0 < 0 || c0 < 0 || c0 >= pairs) return;
-  const int len = a.lengths[seq];
-  const int pos0 = len - (a.row_start[seq + 1] - row0);  // of the sequence's first row
+  const PreWork work = a.n_seqs <= kPreSorted ? longest_first(a, (int)(blockIdx.x / a.n_kv))
+                                              : by_row(a, (int)(blockIdx.x / a.n_kv), count_lds);
+  const PreSpan sp = prefill_span(a, work);
+  const int seq = work.seq, split = blockIdx.y;
+  if (split == 0 && a.part != nullptr && tid == 0) {
+    const int j = (int)(sp.c0 / G);
+    const bool join = sp.live && sp.len <= a.max_len && sp.tiles > sp.each;
+    ((PreJoin*)a.part)[blockIdx.x] = {join ? (sp.tiles + sp.each - 1) / sp.each : 0,
+                                      (int)min((int64_t)kPreCols, sp.pairs - sp.c0), seq, sp.row0 + j, sp.pos0 + j,
+                                      (int)(sp.c0 - (int64_t)j * G)};
+  }
+  if (!sp.live) return;
+  const int row0 = sp.row0, pos0 = sp.pos0, len = sp.len;
+  const int64_t pairs = sp.pairs, c0 = sp.c0;
   // this lane's column
   const int64_t cc = c0 + wave * 32 + col;
   const bool live = cc < pairs;
   const int jr = (int)((live ? cc : pairs - 1) / G), qh = (int)((live ? cc : pairs - 1) - (int64_t)jr * G);
   const int row = row0 + jr, qpos = pos0 + jr, head = kvh * G + qh;
   float* out = a.out + row * a.out_stride + (int64_t)head * a.hd;
-  // the workgroup's first and last key, the wave's first and last row
-  const int ja = (int)(c0 / G), jb = (int)((min(c0 + kPreCols, pairs) - 1) / G);
-  const int kmax = pos0 + jb;
-  const int key0 = a.window > 0 ? max(0, pos0 + ja + 1 - a.window) : 0;
+  // the workgroup's keys; the wave's first and last row
+  const bool parts = sp.tiles > sp.each;  // other workgroups have the tile's other keys
+  const int key0 = sp.kfirst + split * sp.each * kPreKeys;
+  const int kmax = min(sp.kmax, key0 + sp.each * kPreKeys - 1);
   const int wave_first = __builtin_amdgcn_readfirstlane(__shfl(qpos, 0));
   const int wave_last = __builtin_amdgcn_readfirstlane(__shfl(qpos, 63));
-  if (len > a.max_len || kmax < 0) {  // (kmax < 0: nothing to see)
-    if (live)
+  if (len > a.max_len || sp.kmax < 0) {  // (kmax < 0: nothing to see)
+    if (live && split == 0)
       for (int d = 4 * half; d < a.hd; d += 8) {
         const float x = len > a.max_len ? __builtin_nanf("") : 0.0f;
         *(f4*)(out + d) = f4{x, x, x, x};
       }
     return;
   }
+
+  if (key0 > kmax) return;
 
   // ---- q
   int q_exp = 0;
@@ -1091,7 +1146,7 @@ __global__ __launch_bounds__(kPreThreads, HD <= 128 ? 2 : 1) void paged_prefill_
 #pragma unroll
   for (int b = 0; b < VB; ++b) acc[b] = (f16v){};
   float m = -INFINITY, l = 0.0f;  // of the column; l of this half's keys
-  int k0 = key0 & ~(kPreKeys - 1);
+  int k0 = key0;
   int64_t run = run_of(k0, page_of(k0));
   load_k(run);
   int next_page = page_of(k0 + kPreKeys);
@@ -1220,6 +1275,30 @@ __global__ __launch_bounds__(kPreThreads, HD <= 128 ? 2 : 1) void paged_prefill_
     }
   }
   const float sum = xor32_sum(l);
+  if (parts) {
+    // (a page outside the cache shows up as a NaN sum in the join)
+    if (lane == 0) count_lds[wave] = 0;
+    __syncthreads();
+    if (__any(odd) && lane == 0) count_lds[wave] = 1;
+    __syncthreads();
+    const bool outside = (count_lds[0] | count_lds[1] | count_lds[2] | count_lds[3]) != 0;
+    const PrePartial pp = prefill_partial(a, split);
+    const int at = wave * 32 + col;
+    if (half == 0) {
+      pp.m[at] = m;
+      pp.l[at] = outside ? __builtin_nanf("") : sum;
+    }
+#pragma unroll
+    for (int b = 0; b < VB; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = 32 * b + 8 * i + 4 * half;
+        if (FULL || d < a.hd)
+          *(f4*)(pp.acc + ((size_t)(d >> 2) * kPreCols + at) * 4) =
+              f4{acc[b][4 * i], acc[b][4 * i + 1], acc[b][4 * i + 2], acc[b][4 * i + 3]};
+      }
+    return;
+  }
   // Infinities and NaN end up in the output, also those that a weight of 0 was
   // to silence: columns that hold any, and all of a workgroup that met a page
   // outside the cache, are computed again.
@@ -1242,7 +1321,7 @@ __global__ __launch_bounds__(kPreThreads, HD <= 128 ? 2 : 1) void paged_prefill_
     const int64_t p = c0 + wave * 32 + c;
     const int j = (int)(p / G);
     slow_row<T>(a, seq, row0 + j, pos0 + j, kvh * G + (int)(p - (int64_t)j * G),
-                (float*)pre_smem + wave * kSlowFloats);
+                (float*)pre_smem + wave * kSlowFloats, 0, a.hd);
     if (c == col) cut = true;
   }
   if (!live || cut) return;
@@ -1257,16 +1336,107 @@ __global__ __launch_bounds__(kPreThreads, HD <= 128 ? 2 : 1) void paged_prefill_
     }
 }
 
+// The splits of a tile of rows and kv head joined: a thread has one column and
+// two quads of dims, a workgroup 32 dims, four splits' loads are asked for at
+// once. Columns that are not finite go to slow_row, as in a workgroup that has
+// all keys.
+constexpr int kPreJoinThreads = 512, kPreJoinDims = 32, kPreMaxSplits = 32, kPreJoinAhead = 4;
+template <typename T>
+__global__ __launch_bounds__(kPreJoinThreads) void paged_prefill_join_kernel(PagedAttnArgs a) {
+  constexpr int kStep = kPreJoinThreads / kPreCols;  // quads of dims that the threads take at a time
+  constexpr int N = kPreJoinDims / 4 / kStep;        // per thread, of one column
+  __shared__ int redo[kPreCols];
+  __shared__ __align__(16) float slow[kPreJoinThreads / 64][kSlowFloats];
+  const PreJoin info = ((const PreJoin*)a.part)[blockIdx.x];
+  if (info.parts <= 1) return;
+  const int tid = threadIdx.x, kvh = blockIdx.x % a.n_kv, d0 = blockIdx.y * kPreJoinDims;
+  const int col = tid % kPreCols, q0 = d0 / 4 + tid / kPreCols, last = a.hd / 4 - 1;
+  if (tid < kPreCols) redo[tid] = 0;
+  __syncthreads();
+  const PrePartial first = prefill_partial(a, 0);
+  const size_t stride = prefill_partial_floats(a.hd);
+  float m = -INFINITY, l = 0.0f;
+  f4 o[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) o[n] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int i0 = 0; i0 < info.parts; i0 += kPreJoinAhead) {
+    float pm[kPreJoinAhead], pl[kPreJoinAhead];
+    f4 x[kPreJoinAhead][N];
+#pragma unroll
+    for (int i = 0; i < kPreJoinAhead; ++i) {
+      const size_t at = (size_t)min(i0 + i, info.parts - 1) * stride;
+      pm[i] = first.m[at + col];
+      pl[i] = first.l[at + col];
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        x[i][n] = *(const f4*)(first.acc + at + (size_t)min(q0 + kStep * n, last) * (4 * kPreCols) + 4 * col);
+    }
+    float mx = m;
+#pragma unroll
+    for (int i = 0; i < kPreJoinAhead; ++i)
+      if (i0 + i < info.parts) mx = fmaxf(mx, pm[i]);
+    const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mx);
+    m = mx;
+    l *= f;
+#pragma unroll
+    for (int n = 0; n < N; ++n) o[n] *= f;
+#pragma unroll
+    for (int i = 0; i < kPreJoinAhead; ++i) {
+      if (i0 + i >= info.parts) break;
+      const float w = pm[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(pm[i] - mx);
+      l += pl[i] * w;
+#pragma unroll
+      for (int n = 0; n < N; ++n) o[n] += x[i][n] * w;
+    }
+  }
+  auto place = [&](int c, int* row, int* pos, int* head) {
+    const int j = (info.rem + c) / a.group;
+    *row = info.row + j;
+    *pos = info.pos + j;
+    *head = kvh * a.group + info.rem + c - j * a.group;
+  };
+  int row, pos, head;
+  if (col < info.cols) {
+    place(col, &row, &pos, &head);
+    float* out = a.out + row * a.out_stride + (int64_t)head * a.hd;
+    const float f = pos < 0 ? 1.0f : l;  // (a row before the first key sees nothing: zeros)
+    float zeros = l * 0.0f;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const f4 z = o[n] * 0.0f;
+      zeros += (z.x + z.y) + (z.z + z.w);
+      if (q0 + kStep * n <= last) *(f4*)(out + 4 * (q0 + kStep * n)) = f4{o[n].x / f, o[n].y / f, o[n].z / f, o[n].w / f};
+    }
+    if (!(zeros == 0.0f)) redo[col] = 1;
+  }
+  __syncthreads();
+  for (int c = tid >> 6; c < info.cols; c += kPreJoinThreads / 64)
+    if (redo[c]) {
+      place(c, &row, &pos, &head);
+      slow_row<T>(a, info.seq, row, pos, head, slow[tid >> 6], d0, min(d0 + kPreJoinDims, a.hd));
+    }
+}
+
+// Tiles of rows that the grid has to hold: one more for each sequence than its
+// rows fill.
+int64_t prefill_tiles(const PagedAttnArgs& a) {
+  return (int64_t)a.max_rows * a.group / kPreCols + a.n_seqs;
+}
+
 template <typename T, int HD, bool FULL, bool RULE>
 hipError_t prefill_launch(const PagedAttnArgs& a, hipStream_t stream) {
   constexpr size_t lds = sizeof(PreLds<T, HD>);
   static_assert(sizeof(PreTile<T, HD>) >= kPreThreads / 64 * kSlowFloats * sizeof(float), "slow_row's");
   const auto kernel = paged_prefill_kernel<T, HD, FULL, RULE>;
-  const hipError_t e = allow_dynamic_lds((const void*)kernel, lds);
+  hipError_t e = allow_dynamic_lds((const void*)kernel, lds);
   if (e != hipSuccess) return e;
-  const int64_t grid = ((int64_t)a.max_rows * a.group / kPreCols + a.n_seqs) * a.n_kv;
+  const int64_t grid = prefill_tiles(a) * a.n_kv;
   if (grid > INT32_MAX) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(kPreThreads), lds, stream, a);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid, a.splits), dim3(kPreThreads), lds, stream, a);
+  e = hipGetLastError();
+  if (e != hipSuccess || a.splits == 1) return e;
+  hipLaunchKernelGGL(paged_prefill_join_kernel<T>,
+                     dim3((unsigned)grid, (a.hd + kPreJoinDims - 1) / kPreJoinDims), dim3(kPreJoinThreads), 0, stream, a);
   return hipGetLastError();
 }
 template <typename T, int HD>
@@ -1327,6 +1497,17 @@ hipError_t launch_paged_decode(const PagedAttnArgs& all, hipStream_t stream) {
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   return hipSuccess;
+}
+
+// Where the tiles of rows leave most of the chip idle, a tile's keys are shared
+// by several workgroups and joined.
+size_t plan_paged_prefill(PagedAttnArgs& a) {
+  const int64_t tiles = prefill_tiles(a) * a.n_kv, slots = (int64_t)(a.hd <= 128 ? 2 : 1) * device_cus();
+  const int64_t keys = ((int64_t)a.max_len + kPreKeys - 1) / kPreKeys;
+  a.splits = (int)std::max(std::min(std::min(slots / tiles, keys / kPreLeast), (int64_t)kPreMaxSplits), (int64_t)1);
+  if (a.n_seqs > kPreSorted) a.splits = 1;
+  if (a.splits == 1) return 0;
+  return prefill_header(tiles) + (size_t)tiles * a.splits * prefill_partial_floats(a.hd) * sizeof(float);
 }
 
 hipError_t launch_paged_prefill(const PagedAttnArgs& a, hipStream_t stream) {

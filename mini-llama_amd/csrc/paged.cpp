@@ -251,12 +251,12 @@ int mlq_qk_norm_rope(const mlq_rotary* r, int rows, const int32_t* positions, in
   return record_hip(launch_qk_norm_rope(a, (hipStream_t)stream));
 }
 
-int mlq_paged_attention_workspace(const mlq_paged_cache* c, int n_heads, int n_seqs, int max_len,
-                                  size_t* bytes) {
+int mlq_paged_attention_workspace(const mlq_paged_cache* c, int n_heads, int n_seqs, int max_rows,
+                                  int max_len, size_t* bytes) {
   const int rc = check_geometry(c);
   if (rc != MLQ_OK) return rc;
   if (bytes == nullptr) return MLQ_ERR_INVALID_ARG;
-  if (n_heads <= 0 || n_heads % c->n_kv_heads != 0 || n_seqs <= 0 || max_len <= 0)
+  if (n_heads <= 0 || n_heads % c->n_kv_heads != 0 || n_seqs <= 0 || max_rows < 0 || max_len <= 0)
     return MLQ_ERR_SHAPE;
   PagedAttnArgs a = {};
   a.type = c->type;
@@ -265,7 +265,8 @@ int mlq_paged_attention_workspace(const mlq_paged_cache* c, int n_heads, int n_s
   a.group = n_heads / c->n_kv_heads;
   a.n_seqs = n_seqs;
   a.max_len = max_len;
-  *bytes = plan_paged_decode(a);
+  a.max_rows = max_rows;
+  *bytes = max_rows == 0 ? plan_paged_decode(a) : plan_paged_prefill(a);
   return MLQ_OK;
 }
 
@@ -291,14 +292,19 @@ int mlq_paged_attention_decode(const mlq_paged_cache* c, int layer, const mlq_pa
 
 int mlq_paged_attention_prefill(const mlq_paged_cache* c, int layer, const mlq_paged_batch* b,
                                 const mlq_attention_rule* rule, int n_heads, const float* q,
-                                int64_t q_stride, float* out, int64_t out_stride,
-                                mlq_stream_t stream) {
+                                int64_t q_stride, float* out, int64_t out_stride, int max_len,
+                                void* ws, size_t ws_bytes, mlq_stream_t stream) {
   PagedAttnArgs a;
   const int rc = check_attention(c, layer, b, rule, n_heads, q, q_stride, out, out_stride, &a);
   if (rc != MLQ_OK) return rc;
   if (b->row_start == nullptr) return MLQ_ERR_INVALID_ARG;
-  if (b->max_rows <= 0) return MLQ_ERR_SHAPE;
-  a.max_len = b->max_pages * c->page_size;
+  if (b->max_rows <= 0 || max_len <= 0 || max_len > (int64_t)b->max_pages * c->page_size)
+    return MLQ_ERR_SHAPE;
+  a.max_len = max_len;
+  const size_t need = plan_paged_prefill(a);
+  if (((uintptr_t)ws & 255u) != 0) return MLQ_ERR_INVALID_ARG;
+  if (ws_bytes < need || (need > 0 && ws == nullptr)) return MLQ_ERR_BUFFER_TOO_SMALL;
+  a.part = need > 0 ? ws : nullptr;
   return record_hip(launch_paged_prefill(a, (hipStream_t)stream));
 }
 

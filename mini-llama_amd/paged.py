@@ -297,13 +297,15 @@ class AttentionRule:
         self.ref = ctypes.byref(self.struct)
 
 
-def attention_workspace_bytes(cache: PagedCache, n_heads: int, n_seqs: int, max_len: int) -> int:
-    """Workspace of attention_decode for any lengths up to max_len."""
-    key = (n_heads, n_seqs, max_len)
+def attention_workspace_bytes(cache: PagedCache, n_heads: int, n_seqs: int, max_len: int,
+                              rows: int = 0) -> int:
+    """Workspace of attention_decode for any lengths up to max_len, with rows
+    that of attention_prefill for so many rows."""
+    key = (n_heads, n_seqs, rows, max_len)
     need = cache._workspaces.get(key)
     if need is None:
         nbytes = ctypes.c_size_t()
-        _check(lib().mlq_paged_attention_workspace(cache.ref, n_heads, n_seqs, max_len,
+        _check(lib().mlq_paged_attention_workspace(cache.ref, n_heads, n_seqs, rows, max_len,
                                                    ctypes.byref(nbytes)),
                "mlq_paged_attention_workspace")
         need = nbytes.value
@@ -311,6 +313,20 @@ def attention_workspace_bytes(cache: PagedCache, n_heads: int, n_seqs: int, max_
             cache._workspaces.clear()
         cache._workspaces[key] = need
     return need
+
+
+def _workspace(cache, workspace, n_heads: int, n_seqs: int, max_len: int, rows: int):
+    """(tensor, address, bytes): the caller's workspace, or one of the call's
+    own, which the allocator reuses in the current stream's order."""
+    if workspace is None:
+        size = attention_workspace_bytes(cache, n_heads, n_seqs, max_len, rows)
+        if size == 0:
+            return None, None, 0
+        workspace = torch.empty(size, dtype=torch.uint8, device=cache.device)
+        return workspace, workspace.data_ptr(), size
+    if workspace.get_device() != cache.index or not workspace.is_contiguous():
+        raise ValueError("the workspace must be a contiguous tensor on the cache's device")
+    return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
 def _attention_args(cache, batch, q, out, rule):
@@ -352,16 +368,7 @@ def attention_decode(cache: PagedCache, layer: int, batch: PagedBatch, q, out=No
         raise ValueError("a row for each sequence is needed")
     if max_len is None:
         max_len = batch.max_pages * cache.page_size
-    wp, size = None, 0
-    if workspace is None:
-        size = attention_workspace_bytes(cache, heads, batch.n_seqs, max_len)
-        if size:
-            workspace = torch.empty(size, dtype=torch.uint8, device=cache.device)
-            wp = workspace.data_ptr()
-    else:
-        if workspace.get_device() != index or not workspace.is_contiguous():
-            raise ValueError("the workspace must be a contiguous tensor on the cache's device")
-        wp, size = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    workspace, wp, size = _workspace(cache, workspace, heads, batch.n_seqs, max_len, 0)
     if n:
         _check(lib().mlq_paged_attention_decode(cache.ref, layer, batch.bounded(n), ref, heads, qp, qs,
                                                 op, os, max_len, wp, size, _raw_stream(index)),
@@ -370,18 +377,26 @@ def attention_decode(cache: PagedCache, layer: int, batch: PagedBatch, q, out=No
 
 
 def attention_prefill(cache: PagedCache, layer: int, batch: PagedBatch, q, out=None,
-                      rule: AttentionRule | None = None, stream=None):
+                      rule: AttentionRule | None = None, max_len: int | None = None,
+                      workspace=None, stream=None):
     """out [rows, n_heads, head_dim]: causal attention of every new row of
-    every sequence over its pages (mlq_paged_attention_prefill)."""
+    every sequence over its pages (mlq_paged_attention_prefill). max_len and
+    workspace as in attention_decode, the workspace of
+    attention_workspace_bytes(..., rows=q.shape[0])."""
     index = cache.index
     if stream is not None or index != torch.cuda.current_device():
-        return _elsewhere(lambda: attention_prefill(cache, layer, batch, q, out, rule), index, stream)
+        return _elsewhere(lambda: attention_prefill(cache, layer, batch, q, out, rule, max_len,
+                                                    workspace), index, stream)
     heads, qp, qs, out, op, os, ref = _attention_args(cache, batch, q, out, rule)
     if batch.row_start is None:
         raise ValueError("attention_prefill needs a batch with row_start")
     n = q.shape[0]
     if n:
+        if max_len is None:
+            max_len = batch.max_pages * cache.page_size
+        rows = n if batch.max_rows is None else min(n, batch.max_rows)
+        workspace, wp, size = _workspace(cache, workspace, heads, batch.n_seqs, max_len, rows)
         _check(lib().mlq_paged_attention_prefill(cache.ref, layer, batch.bounded(n), ref, heads, qp, qs,
-                                                 op, os, _raw_stream(index)),
+                                                 op, os, max_len, wp, size, _raw_stream(index)),
                "mlq_paged_attention_prefill")
     return out

@@ -492,6 +492,47 @@ def test_prefill_long(paged, heads, kv, hd, lengths, new, kind):
     assert torch.equal(out, again)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,kv,hd,lengths,new", [
+    (28, 4, 128, [5000], [3]), (8, 8, 64, [3000, 10, 900, 0], [20, 10, 1, 0]), (16, 1, 256, [1300, 2000], [5, 4]), (33, 1, 128, [700], [9]),
+    (12, 4, 80, [4000, 130, 2000, 20], [1, 2, 40, 20]), (4, 4, 128, [600, 600], [300, 5])])
+def test_prefill_of_few_rows_behind_long_contexts(pkg, paged, heads, kv, hd, lengths, new, kind):
+    """Their keys are shared by several workgroups and joined: plain, with a rule, with a bad page, with a NaN that some rows see."""
+    import torch
+    p = Problem(paged, kind, lengths, heads, kv, hd, 16, seed=27, new=new)
+    need = paged.attention_workspace_bytes(p.cache, heads, len(lengths), p.table.shape[1] * 16, rows=p.rows)
+    assert need > 0
+    ws = torch.full((need,), 255, dtype=torch.uint8, device="cuda")  # (NaN wherever nothing is written)
+    rows = set(range(0, p.rows, max(1, p.rows // 40))) | {p.rows - 1}
+    for rule in (dict(), dict(softcap=20.0, slopes=True), dict(window=300), dict(scale=-0.1)):
+        own, plain = rule_of(paged, heads, **rule)
+        out = paged.attention_prefill(p.cache, 0, p.batch, p.qd, rule=own, workspace=ws)
+        again = paged.attention_prefill(p.cache, 0, p.batch, p.qd, rule=own)
+        torch.cuda.synchronize()
+        p.compare(out, p.want(rows=rows, **plain), rule)
+        assert torch.equal(out, again)
+    with pytest.raises(pkg.MLQError):
+        paged.attention_prefill(p.cache, 0, p.batch, p.qd, workspace=ws[:need - 256])
+    # the first sequence's key 100 holds an infinite value, key 300 lies on a page outside the cache
+    clean = out.clone()
+    page = int(p.table[0, 100 // 16])
+    p.cache.values[0, page, kv - 1, 100 % 16, 3] = math.inf
+    out = paged.attention_prefill(p.cache, 0, p.batch, p.qd, rule=own, workspace=ws)
+    torch.cuda.synchronize()
+    hit = heads - heads // kv
+    n0 = int(p.start[1])
+    assert torch.equal(out[n0:], clean[n0:]) and torch.equal(out[:n0, :hit], clean[:n0, :hit])
+    first = int(p.lengths[0]) - n0  # (rows before key 100 do not see it)
+    assert torch.all(~torch.isfinite(out[max(0, 100 - first):n0, hit:, 3]))
+    assert torch.all(torch.isfinite(out[:max(0, 100 - first)]))
+    p.batch.block_table[0, 300 // 16] = -7
+    out = paged.attention_prefill(p.cache, 0, p.batch, p.qd, rule=own, workspace=ws)
+    torch.cuda.synchronize()
+    assert torch.equal(out[n0:], clean[n0:])
+    assert torch.all(torch.isnan(out[max(0, 304 - first):n0]))
+    assert torch.all(torch.isfinite(out[:max(0, 100 - first)]))
+
+
 def test_decode_matches_the_single_sequence_attention(pkg, paged):
     """One sequence's attention through mlq_attention_decode over its own layout."""
     import ctypes

@@ -109,7 +109,7 @@ def test_attention_refusals(pkg, prefill):
         args = [ctypes.byref(c), layer, ctypes.byref(b), ctypes.byref(r) if r else None, heads, q, qs,
                 out, os]
         if prefill:
-            return pkg.lib().mlq_paged_attention_prefill(*args, None)
+            return pkg.lib().mlq_paged_attention_prefill(*args, max_len, ws, ws_bytes, None)
         return pkg.lib().mlq_paged_attention_decode(*args, max_len, ws, ws_bytes, None)
     for kw, want in [(dict(c=cache(pkg, keys=None)), ARG), (dict(c=cache(pkg, values=FAKE + 8)), ARG),
                      (dict(c=cache(pkg, head_dim=12)), UNSUPPORTED), (dict(layer=2), SHAPE),
@@ -125,33 +125,37 @@ def test_attention_refusals(pkg, prefill):
         assert call(**kw) == want, kw
     if prefill:
         assert call(b=batch(pkg, row_start=None)) == ARG
-    else:
-        assert call(max_len=0) == SHAPE and call(max_len=129) == SHAPE
-        assert call(ws=FAKE + 16) == ARG
-        # one sequence of 100000 keys is split over workgroups: it needs its partials
-        n = ctypes.c_size_t()
-        c = cache(pkg, n_pages=10000)
-        assert pkg.lib().mlq_paged_attention_workspace(ctypes.byref(c), 28, 1, 100000,
-                                                       ctypes.byref(n)) == OK
-        if n.value:
-            long = dict(c=c, b=batch(pkg, n_seqs=1, max_pages=6250), max_len=100000)
-            assert call(ws_bytes=n.value - 1, **long) == SMALL
-            assert call(ws=None, **long) == SMALL
+    assert call(max_len=0) == SHAPE and call(max_len=129) == SHAPE
+    assert call(ws=FAKE + 16) == ARG
+    # the keys of one sequence of 100000 are shared by workgroups: it needs their partials
+    n = ctypes.c_size_t()
+    c = cache(pkg, n_pages=10000)
+    assert pkg.lib().mlq_paged_attention_workspace(ctypes.byref(c), 28, 1, 5 if prefill else 0, 100000,
+                                                   ctypes.byref(n)) == OK
+    assert n.value > 0
+    long = dict(c=c, b=batch(pkg, n_seqs=1, max_pages=6250), max_len=100000)
+    assert call(ws_bytes=n.value - 1, **long) == SMALL
+    assert call(ws=None, **long) == SMALL
 
 
 def test_attention_workspace(pkg):
     lib, n = pkg.lib(), ctypes.c_size_t()
     c = cache(pkg, keys=None, values=None)
-    for heads, seqs, max_len, want in [(0, 1, 1, SHAPE), (30, 1, 1, SHAPE), (28, 0, 1, SHAPE),
-                                       (28, 1, 0, SHAPE), (28, 1, 1, OK)]:
-        assert lib.mlq_paged_attention_workspace(ctypes.byref(c), heads, seqs, max_len,
+    for heads, seqs, rows, max_len, want in [(0, 1, 0, 1, SHAPE), (30, 1, 0, 1, SHAPE), (28, 0, 0, 1, SHAPE),
+                                             (28, 1, 0, 0, SHAPE), (28, 1, -1, 1, SHAPE), (28, 1, 7, 1, OK),
+                                             (28, 1, 0, 1, OK)]:
+        n.value = 77
+        assert lib.mlq_paged_attention_workspace(ctypes.byref(c), heads, seqs, rows, max_len,
                                                  ctypes.byref(n)) == want
-    assert n.value == 0  # a single key is never split
+        assert n.value == (0 if want == OK else 77)  # a single key is never split
     sizes = []
     for max_len in (16, 100, 1000, 10000, 100000, 1000000):
-        assert lib.mlq_paged_attention_workspace(ctypes.byref(c), 28, 4, max_len, ctypes.byref(n)) == OK
+        assert lib.mlq_paged_attention_workspace(ctypes.byref(c), 28, 4, 0, max_len, ctypes.byref(n)) == OK
         sizes.append(n.value)
     assert sizes == sorted(sizes)  # one sized for the longest serves the shorter ones
+    # many rows fill the chip by themselves
+    assert lib.mlq_paged_attention_workspace(ctypes.byref(c), 28, 4, 20000, 100000, ctypes.byref(n)) == OK
+    assert n.value == 0
 
 
 @pytest.mark.parametrize("theta,rot,factor,original,fast,slow", [
