@@ -506,8 +506,8 @@ enum mlq_kv_type { MLQ_KV_F32 = 0, MLQ_KV_F16 = 1, MLQ_KV_BF16 = 2 };
 /* keys and values: [n_layers][n_pages][n_kv_heads][page_size][head_dim] each,
  * 16-byte aligned; token t of a sequence is token t % page_size of the page
  * that its block table names at t / page_size. page_size: a power of two,
- * 16 .. 4096; head_dim: a multiple of 8 up to 256 (MLQ_ERR_UNSUPPORTED
- * otherwise). */
+ * 16 .. 4096; head_dim: a multiple of 8 up to 256; a block table holds at most
+ * 2^30 tokens a sequence (MLQ_ERR_UNSUPPORTED otherwise). */
 typedef struct mlq_paged_cache {
   void* keys;
   void* values;
@@ -547,8 +547,9 @@ enum mlq_plan_status {
  * b->status. With another status than MLQ_PLAN_OK nothing is allocated,
  * released or counted and there are no rows. b->lengths may be `lengths`
  * and n_free_out may be n_free (a loop's state); no other arrays overlap.
- * Entries of block_table are not checked here. page_size as in
- * mlq_paged_cache. */
+ * Entries of block_table are not checked here, and a page that several
+ * sequences share is not counted: the first of them to end releases it.
+ * page_size as in mlq_paged_cache. */
 int mlq_paged_plan(const mlq_paged_batch* b, int page_size, int n_pages, const int32_t* lengths,
                    const int32_t* n_new, int32_t* free_pages, const int32_t* n_free,
                    int32_t* n_free_out, mlq_stream_t stream);
@@ -622,7 +623,7 @@ int mlq_paged_attention_workspace(const mlq_paged_cache* c, int n_heads, int n_s
  * the cache already. A length of 0 gives zeros; a length above max_len or
  * the block table, or a page outside the cache, NaN. q and out: rows of
  * n_heads * head_dim floats at strides in floats (multiples of 4, pointers
- * 16-byte aligned); b's block_table, lengths and row_start are read. max_len
+ * 16-byte aligned), out apart from everything else; b's block_table, lengths and row_start are read. max_len
  * bounds the lengths (grid and workspace; at most max_pages * page_size).
  * Keys behind a sequence's end are not read into results, whatever the pages
  * hold there. Sums and softmax in fp32; fp16 and bf16 caches multiply on

@@ -728,21 +728,31 @@ void decode_launch_hd(const PagedAttnArgs& a, int grid, hipStream_t stream) {
 }
 
 // ---- prefill -----------------------------------------------------------------------
-// Causal attention of every new row of every sequence. Bound by the matrix
-// instructions. A workgroup owns 128 consecutive (row, query head) pairs of one
-// sequence and kv head (pairs r * group + h: no padding whatever the group), a
-// wave 32 of them as the columns of both products, S^T = K Q^T and
-// O^T = V^T P^T on 32 x 32 x 16 instructions. A lane then holds 16 keys of one
-// column: the softmax is in registers but for one lane swap, and P^T is the
-// second product's B operand as it stands, V^T lying in LDS in the order in
-// which the first product leaves the keys. q and the weights are split into
-// parts as in the decode kernel; fp32 caches into three bf16 parts too, of whose
-// nine part products the six largest are taken (the others are below 2^-25 of
-// the product). Tiles of 32 keys pass through LDS: K's next tile is in flight
-// during the output's products, V's during the scores'.
-// A value that a masked weight of 0 does not silence (infinite or NaN), or that
-// the split does not carry, and a page outside the cache send the workgroup's
-// rows to slow_row.
+// Causal attention of every new row of every sequence. A workgroup owns 128
+// consecutive (row, query head) pairs of one sequence and kv head (pairs
+// r * group + h: no padding whatever the group), a wave 32 of them as the
+// columns of both products, S^T = K Q^T and O^T = V^T P^T on 32 x 32 x 16
+// instructions. A lane then holds 16 keys of one column: the softmax is in
+// registers but for one lane swap, and P^T is the second product's B operand as
+// it stands, V^T lying in LDS in the order in which the first product leaves
+// the keys. q and the weights are split into parts as in the decode kernel;
+// fp32 caches into three bf16 parts too, of whose nine part products the six
+// largest are taken (the others are below 2^-25 of the product).
+//  - Tiles of 32 keys pass through LDS; the next tile is on its way to registers
+//    during the products, and the page that the one after it lies in is asked
+//    for before that (a load that waits for its page waits twice).
+//  - Infinities and NaN, also those that a weight of 0 was to silence, end up in
+//    the output: such columns, and those of a workgroup that met a page outside
+//    the cache, go to slow_row.
+//  - Tiles with the most keys start first (6 sequences, 8000 rows behind up to
+//    2000 tokens, 32 heads on 8 of 128, bf16: 565 -> 552 us); where the tiles
+//    leave CUs idle, several workgroups share a tile's keys (64 rows of 16
+//    sequences behind up to 8000 tokens, 28 heads on 4, bf16: 342 -> 83 us).
+// That case's 620 GFLOP of part products (three for each of the two) take 550
+// us, 1.13 PFLOP/s where a library product of 8192^3 reaches 1.2: the chip's
+// power bounds both, its clock falls to 1.9 GHz. One barrier a tile instead of
+// two, fewer vector instructions and no spills brought 691 to 543; raising the
+// waves' priority around the products cost 5 %.
 constexpr int kPreCols = 128, kPreKeys = 32, kPreThreads = 256;
 typedef float f16v __attribute__((ext_vector_type(16)));
 

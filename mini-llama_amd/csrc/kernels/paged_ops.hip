@@ -21,12 +21,12 @@ namespace {
 // the prefix sums run in registers with one barrier a tile, a thread writes a
 // few pages and rows of its sequence itself and the wave many of them, and a
 // row takes its page from the stack or the table as they were, not from what
-// was just written. 48 sequences, a
-// token each: 4.1 us, of them about 2 for the launch.
-// Row arrays up to this size are written by the scanning workgroup itself,
-// larger ones by a second launch over the whole chip (4096 rows: 5.5 us against
-// 4.4 + 2.9).
-constexpr int kPlanInlineRows = 4096;
+// was just written. 48 sequences, a token each: 3.4 us in a graph.
+// The scanning workgroup writes the rows itself where there are few of them or
+// about one a sequence, else a second launch over the whole chip does (us in a
+// graph, itself and second launch: a token each for 1000 sequences 5.1 and 8.7,
+// for 3000 15.4 and 19.4; 100 prompts of up to 60 tokens 17.3 and 7.6).
+constexpr int kPlanFewRows = 1024, kPlanMostRows = 16384;
 constexpr int kPlanOwn = 8;  // pages or rows of a sequence that its own thread writes
 
 // Last i with start[i] <= r; start[0] <= r. The one that r falls into: an
@@ -353,7 +353,8 @@ void rotary_launch(RotaryArgs a, hipStream_t stream) {
 }  // namespace
 
 hipError_t launch_paged_plan(const PlanArgs& a, hipStream_t stream) {
-  const bool rows = a.max_rows <= kPlanInlineRows;
+  const bool rows = a.max_rows <= kPlanFewRows ||
+                    (a.max_rows <= kPlanMostRows && a.max_rows <= 2 * (int64_t)a.n_seqs);
   // (a workgroup of the sequences' size: a barrier of four waves costs less
   // than one of sixteen)
   if (a.n_seqs <= 256 && a.max_rows <= 1024)

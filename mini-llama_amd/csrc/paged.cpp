@@ -16,6 +16,9 @@ namespace {
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
+// Of a sequence: the kernels count positions, padded to whole tiles, in 32 bits.
+constexpr int64_t kMaxTokens = (int64_t)1 << 30;
+
 size_t kv_bytes(int type) { return type == MLQ_KV_F32 ? 4 : 2; }
 
 int page_shift_of(int page_size) {
@@ -66,7 +69,7 @@ int check_attention(const mlq_paged_cache* c, int layer, const mlq_paged_batch* 
   if (b->n_seqs <= 0 || b->max_pages <= 0 || n_heads <= 0 || n_heads % c->n_kv_heads != 0)
     return MLQ_ERR_SHAPE;
   if (layer < 0 || layer >= c->n_layers) return MLQ_ERR_SHAPE;
-  if ((int64_t)b->max_pages * c->page_size > INT32_MAX) return MLQ_ERR_UNSUPPORTED;
+  if ((int64_t)b->max_pages * c->page_size > kMaxTokens) return MLQ_ERR_UNSUPPORTED;
   const int64_t floats = (int64_t)n_heads * c->head_dim;
   if ((rc = check_rows(q, q_stride, floats)) != MLQ_OK) return rc;
   if ((rc = check_rows(out, out_stride, floats)) != MLQ_OK) return rc;
@@ -123,7 +126,7 @@ int mlq_paged_plan(const mlq_paged_batch* b, int page_size, int n_pages, const i
   if (b->n_seqs <= 0 || b->max_pages <= 0 || b->max_rows <= 0 || n_pages <= 0 || page_size <= 0)
     return MLQ_ERR_SHAPE;
   const int shift = page_shift_of(page_size);
-  if (shift < 0 || (int64_t)b->max_pages * page_size > INT32_MAX) return MLQ_ERR_UNSUPPORTED;
+  if (shift < 0 || (int64_t)b->max_pages * page_size > kMaxTokens) return MLQ_ERR_UNSUPPORTED;
   PlanArgs a = {};
   a.n_seqs = b->n_seqs;
   a.max_pages = b->max_pages;
@@ -258,6 +261,7 @@ int mlq_paged_attention_workspace(const mlq_paged_cache* c, int n_heads, int n_s
   if (bytes == nullptr) return MLQ_ERR_INVALID_ARG;
   if (n_heads <= 0 || n_heads % c->n_kv_heads != 0 || n_seqs <= 0 || max_rows < 0 || max_len <= 0)
     return MLQ_ERR_SHAPE;
+  if (max_len > kMaxTokens) return MLQ_ERR_UNSUPPORTED;
   PagedAttnArgs a = {};
   a.type = c->type;
   a.n_kv = c->n_kv_heads;
