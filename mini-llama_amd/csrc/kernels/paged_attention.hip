@@ -303,7 +303,8 @@ __global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_k
     __syncthreads();
   }
   const int64_t all = (int64_t)total * n_tiles;
-  const int64_t range = max((all + (int64_t)a.ranges * kDecWaves - 1) / ((int64_t)a.ranges * kDecWaves), (int64_t)1) * kDecWaves;
+  const int64_t share = (int64_t)a.ranges * kDecWaves;
+  const int64_t range = max(quotient(all + share - 1, share), (int64_t)1) * kDecWaves;
   if (blockIdx.x == 0 && a.part != nullptr) {
     if (tid == 0) *pp.range = range;
     for (int i = tid; i < a.n_seqs; i += kDecThreads) {
@@ -316,7 +317,7 @@ __global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_k
   if (u >= uend) return;
   int seq = 0, first, count;  // of the piece's sequence
   {
-    const int at = (int)(u / n_tiles);
+    const int at = (int)quotient(u, n_tiles);
     if (few) {
       seq = __builtin_ctzll(__ballot(my_first + my_count > at));
     } else {
@@ -334,7 +335,7 @@ __global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_k
     count = few ? __builtin_amdgcn_readlane(my_count, seq) : __builtin_amdgcn_readfirstlane(base[seq + 1]) - first;
   };
   take();
-  int tile = (int)((u - (int64_t)first * n_tiles) / count);
+  int tile = (int)quotient(u - (int64_t)first * n_tiles, count);
   int k_at = (int)(u - (int64_t)first * n_tiles - (int64_t)tile * count);
 
   // ---- the range's pieces
@@ -656,7 +657,7 @@ __global__ __launch_bounds__(kDecThreads) void paged_combine_kernel(PagedAttnArg
   const int kvh = head / a.group, g = head - kvh * a.group;
   const int tile = kvh * head_tiles + g / 16;
   const int64_t start = (int64_t)first_tile * n_tiles + (int64_t)tile * count;
-  const int w0 = (int)(start / range), parts = (int)((start + count - 1) / range) - w0 + 1;
+  const int w0 = (int)quotient(start, range), parts = (int)quotient(start + count - 1, range) - w0 + 1;
   if (parts <= 1) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   float m = -INFINITY, l = 0.0f, acc[KD] = {};
