@@ -64,8 +64,9 @@ struct PagedAttnArgs {
   int window;
   const float* slopes;
   // decode: launches of launch_seqs sequences, at most `ranges` workgroups;
-  // `part`: the workspace, null when every sequence is one piece
-  int launch_seqs, ranges;
+  // `part`: the workspace, null when every sequence is one piece, of `whole`
+  // key tiles
+  int launch_seqs, ranges, whole;
   // prefill: workgroups that share a tile's keys
   int splits;
   void* part;

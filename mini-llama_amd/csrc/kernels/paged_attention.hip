@@ -270,6 +270,7 @@ __global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_k
   // ---- the ranges
   auto tiles_of = [&](const DecodeRow& r) {
     if (r.row < 0) return 0;
+    if (a.part == nullptr) return a.whole;  // a range for each, as long as the longest
     const int tiles = (r.len - (first_key(a, r.len) & ~(KT - 1)) + KT - 1) / KT;
     return max((tiles + kDecWaves - 1) / kDecWaves, 1) * kDecWaves;
   };
@@ -304,7 +305,7 @@ __global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_k
   }
   const int64_t all = (int64_t)total * n_tiles;
   const int64_t share = (int64_t)a.ranges * kDecWaves;
-  const int64_t range = max(quotient(all + share - 1, share), (int64_t)1) * kDecWaves;
+  const int64_t range = a.part == nullptr ? a.whole : max(quotient(all + share - 1, share), (int64_t)1) * kDecWaves;
   if (blockIdx.x == 0 && a.part != nullptr) {
     if (tid == 0) *pp.range = range;
     for (int i = tid; i < a.n_seqs; i += kDecThreads) {
@@ -1473,8 +1474,16 @@ size_t plan_paged_decode(PagedAttnArgs& a) {
   const int cus = device_cus();
   // sequences of a launch: their prefix sums lie in LDS and fit 32 bits
   a.launch_seqs = (int)std::min((int64_t)std::min(a.n_seqs, kDecMaxSeqs), std::max(((int64_t)1 << 28) / units, (int64_t)1));
+  a.whole = (int)units * kDecWaves;
+  // Short ones are left whole, without a second launch (units of 128 keys, 64 of
+  // fp32; us of both and of a cut, in a graph, 28 heads on 4 of 128, bf16: one
+  // sequence of 250 9.4 and 10.2, of 500 12.9 and 10.4; 100 of up to 500 18.9 and
+  // 23.2; head dim 64, 16 heads, 16 of up to 500: 9.0 and 9.8).
+  if (units <= 2 || (units <= 4 && (a.hd <= 64 || a.launch_seqs * n_tiles >= cus))) {
+    a.ranges = (int)(a.launch_seqs * n_tiles);
+    return 0;
+  }
   a.ranges = (int)std::min(a.launch_seqs * n_tiles * units, (int64_t)dec_per_cu(a.hd, a.launch_seqs * n_tiles, cus) * cus);
-  if (units <= 1) return 0;  // every sequence is one piece
   const size_t tg = std::min(a.group, 16);
   return dec_header(std::min(a.n_seqs, kDecMaxSeqs)) + dec_align((size_t)2 * a.ranges * tg * 8) +
          (size_t)2 * a.ranges * tg * a.hd * sizeof(float);
