@@ -99,9 +99,17 @@ def gather(pool, table, length):
         np.zeros((pool.shape[1], 0, pool.shape[3]))
 
 
-def attention(q, k, v, pos, scale, softcap=0.0, window=0, slopes=None):
+# fp16 matrix products: a sum is aligned by the exponent fields of its factors
+# and keeps 24 bits from its largest term. A subnormal's field is that of 2^-14,
+# the smallest normal number, so a product with one is off by up to 2^-24 2^-14
+# of the other factor, whatever its own size; with two parts of that factor
+# twice that. (The stored value itself is off by up to 2^-25.)
+SUBNORMAL = 2.0 ** -37
+
+
+def attention(q, k, v, pos, scale, softcap=0.0, window=0, slopes=None, kind=None):
     """(out, bound) [heads, hd] of one row q [heads, hd] at pos over k and v
-    [kv, keys, hd] (keys 0 .. pos)."""
+    [kv, keys, hd] (keys 0 .. pos), for a cache of `kind`."""
     heads, hd = q.shape
     kv = k.shape[0]
     q = np.asarray(q, np.float64)
@@ -116,6 +124,8 @@ def attention(q, k, v, pos, scale, softcap=0.0, window=0, slopes=None):
         s = kk @ q[h] * scale
         # hd products summed in any order, q in parts of 22 bits and more (4 u), scale (2 u)
         err = (hd + 8) * U * (np.abs(kk) @ np.abs(q[h])) * abs(scale)
+        if kind == "f16":
+            err = err + SUBNORMAL * np.abs(q[h]).sum() * abs(scale)
         if softcap:
             s = softcap * np.tanh(s / softcap)
             err = err + 6 * U * np.abs(s)  # division, tanh (3 u), product (derivative at most 1)
@@ -135,6 +145,8 @@ def attention(q, k, v, pos, scale, softcap=0.0, window=0, slopes=None):
         bound[h] = (p * (err + mean + (2 * n + 24) * U)) @ np.abs(vv)
         # fp16 parts hold a weight down to 2^-39 of the largest
         bound[h] += n * 2.0 ** -39 * np.abs(vv).max() + 2.0 ** -140
+        if kind == "f16":  # (the weights add up to 1)
+            bound[h] += SUBNORMAL
     return out, bound
 
 

@@ -262,7 +262,7 @@ class Problem:
             for r in range(self.start[i], self.start[i + 1]):
                 if rows is None or r in rows:
                     pos = int(n) - (self.start[i + 1] - r)
-                    got[r] = ref.attention(self.q[r], k, v, pos, scale, **rule)
+                    got[r] = ref.attention(self.q[r], k, v, pos, scale, kind=self.kind, **rule)
         return got
 
     def compare(self, out, want, what=""):
@@ -445,6 +445,44 @@ def test_large_and_tiny_queries(paged, kind):
             out = call(p.cache, 0, p.batch, p.qd, rule=own)
             torch.cuda.synchronize()
             p.compare(out, p.want(**plain), scale)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("size", [1e-6, 1e-3, 1e3])
+def test_values_of_other_sizes(paged, size, kind):
+    """Cached keys and values far from 1, for fp16 subnormals among them: as they are stored."""
+    import torch
+    p = Problem(paged, kind, [1, 70, 300, 40], 8, 4, 64, 16, seed=15, new=[1, 70, 9, 0])
+    for pool in (p.cache.keys, p.cache.values):
+        pool.copy_((pool.float() * size).to(pool.dtype))
+    p.k, p.v = host(p.cache.keys), host(p.cache.values)
+    own, plain = rule_of(paged, 8, scale=0.2 / max(size, 1.0))
+    out = paged.attention_prefill(p.cache, 0, p.batch, p.qd, rule=own)
+    last = paged.attention_decode(p.cache, 0, p.batch, p.qd, rule=own)
+    torch.cuda.synchronize()
+    want = p.want(**plain)
+    p.compare(out, want, size)
+    p.compare(last, {int(s) - 1: want[int(s) - 1] for s in p.start[1:]}, size)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_query_that_is_not_finite_stays_alone(paged, kind):
+    import torch
+    p = Problem(paged, kind, [150, 200, 90], 8, 2, 64, 16, seed=17, new=[60, 1, 90])
+    clean = paged.attention_prefill(p.cache, 0, p.batch, p.qd)
+    last = paged.attention_decode(p.cache, 0, p.batch, p.qd)
+    q = p.qd.clone()
+    q[30, 2, 5], q[60, 4, 0], q[100, 7, 63] = math.nan, math.inf, -math.inf
+    out = paged.attention_prefill(p.cache, 0, p.batch, q)
+    one = paged.attention_decode(p.cache, 0, p.batch, q)
+    torch.cuda.synchronize()
+    hit = torch.zeros(p.rows, 8, dtype=torch.bool, device="cuda")
+    for r, h in ((30, 2), (60, 4), (100, 7)):
+        hit[r, h] = True
+    assert torch.all(torch.isnan(out[hit])) and torch.equal(out[~hit], clean[~hit])
+    assert torch.all(torch.isnan(one[60, 4]))
+    hit[30, 2] = hit[100, 7] = False  # (not the last rows of their sequences)
+    assert torch.equal(one[~hit], last[~hit])
 
 
 PREFILL = [  # lengths, new
@@ -696,6 +734,41 @@ def test_serving_step_in_a_graph(paged, kind):
             g.replay()
             loop.compare(want, (j, step))
             torch.zeros(1000, device="cuda").sum().item()
+
+
+def test_two_captured_calls_at_once(paged):
+    """Attention of two batches captured apart, replayed on two streams at once while lengths change between the replays."""
+    import torch
+    problems = [Problem(paged, "bf16", [4000, 2100, 900], 28, 4, 128, 16, seed=51, new=[1, 3, 2]),
+                Problem(paged, "f32", [3000, 5000], 8, 8, 64, 32, seed=53, new=[2, 1])]
+    calls = []
+    for p in problems:
+        outs = [torch.zeros_like(p.qd).contiguous() for _ in range(2)]
+        both = lambda p=p, outs=outs: (paged.attention_decode(p.cache, 0, p.batch, p.qd, out=outs[0]),  # noqa: E731
+                                       paged.attention_prefill(p.cache, 0, p.batch, p.qd, out=outs[1]))
+        both()
+        torch.cuda.synchronize()
+        g, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        with torch.cuda.graph(g):
+            both()
+        calls.append((both, outs, g, s))
+    for step in range(5):
+        want = []
+        for p, (both, outs, g, s) in zip(problems, calls):
+            p.batch.lengths.copy_(dev((p.lengths - 17 * step).astype(np.int32)))
+            both()
+            want.append([o.clone() for o in outs])
+            for o in outs:
+                o.zero_()
+        torch.cuda.synchronize()
+        for both, outs, g, s in calls:
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for w, (both, outs, g, s) in zip(want, calls):
+            n = [torch.equal(a, b) for a, b in zip(w, outs)]
+            assert n[1] and torch.equal(w[0][outs[0] != 0], outs[0][outs[0] != 0]), step
+            assert bool((outs[0] != 0).any())
 
 
 def _prompts(loop):
