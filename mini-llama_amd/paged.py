@@ -43,6 +43,7 @@ _F32, _I32, _I64 = torch.float32, torch.int32, torch.int64
 # object where torch gives it.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _elsewhere(call, index: int, stream):
@@ -60,28 +61,28 @@ def _elsewhere(call, index: int, stream):
 def _ints(name: str, t, dtype, index: int, n=None, least: int = 0):
     """Address of a contiguous 1-D device tensor of that type with n elements
     (or at least `least`)."""
-    if t.dtype is not dtype or t.dim() != 1 or t.get_device() != index or \
-       not t.is_contiguous() or (n is not None and t.shape[0] != n) or t.shape[0] < least:
-        size = n if n is not None else f"at least {least}" if least else "any number of"
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor of {size} elements on "
-                         f"cuda:{index}")
-    return t.data_ptr()
+    size = t.shape
+    if t.dtype is dtype and len(size) == 1 and t.get_device() == index and t.is_contiguous():
+        if size[0] == n or (n is None and size[0] >= least):
+            return t.data_ptr()
+    size = n if n is not None else f"at least {least}" if least else "any number of"
+    raise ValueError(f"{name} must be a contiguous {dtype} tensor of {size} elements on "
+                     f"cuda:{index}")
 
 
 def _rows(name: str, t, rows, heads, head_dim: int, index: int):
     """(address, row stride) of a [rows, heads, head_dim] float32 tensor whose
     heads lie side by side; rows, heads None: any."""
-    shape = t.shape
-    if t.dtype is not _F32 or t.get_device() != index or len(shape) != 3 or \
-       shape[2] != head_dim or (heads is not None and shape[1] != heads) or \
-       (rows is not None and shape[0] != rows):
-        raise ValueError(f"{name} must be float32 [{'rows' if rows is None else rows}, "
-                         f"{'heads' if heads is None else heads}, {head_dim}] on cuda:{index}")
-    s0, s1, s2 = t.stride()
-    if s2 != 1 or (s1 != head_dim and shape[1] > 1):
-        raise ValueError(f"the heads of {name} must lie side by side")
-    # (a single row's stride says nothing)
-    return t.data_ptr(), s0 if shape[0] > 1 else shape[1] * head_dim
+    if t.dtype is _F32 and t.dim() == 3 and t.get_device() == index:
+        n, h, d = t.shape
+        if d == head_dim and (h == heads or heads is None) and (n == rows or rows is None):
+            s0, s1, s2 = t.stride()
+            if s2 == 1 and (s1 == d or h <= 1):
+                # (a single row's stride says nothing)
+                return t.data_ptr(), s0 if n > 1 else h * d
+            raise ValueError(f"the heads of {name} must lie side by side")
+    raise ValueError(f"{name} must be float32 [{'rows' if rows is None else rows}, "
+                     f"{'heads' if heads is None else heads}, {head_dim}] on cuda:{index}")
 
 
 class PagedCache:
@@ -182,7 +183,7 @@ def plan(batch: PagedBatch, lengths, n_new, free_pages, n_free, page_size: int, 
     place unless n_free_out is given. batch.status says whether the step was
     planned (PLAN_STATUS)."""
     index, n = batch.index, batch.n_seqs
-    if stream is not None or index != torch.cuda.current_device():
+    if stream is not None or index != _current_device():
         return _elsewhere(lambda: plan(batch, lengths, n_new, free_pages, n_free, page_size,
                                        n_free_out), index, stream)
     if batch.row_start is None or batch.positions is None or batch.slots is None or \
@@ -250,14 +251,15 @@ def qk_norm_rope(rotary: Rotary, q, k, v, positions, q_out=None, k_out=None, cac
     index, hd = q.get_device(), rotary.head_dim
     if index < 0 or (rotary.index is not None and rotary.index != index):
         raise ValueError("q must be a device tensor, on the device of the rotary")
-    if stream is not None or index != torch.cuda.current_device():
+    if stream is not None or index != _current_device():
         return _elsewhere(lambda: qk_norm_rope(rotary, q, k, v, positions, q_out, k_out, cache, layer,
                                                slots), index, stream)
     qp, qs = _rows("q", q, None, None, hd, index)
-    n, heads = q.shape[:2]
+    q_shape = q.shape
+    n, heads = q_shape[0], q_shape[1]
     kp, ks = _rows("k", k, n, None, hd, index)
-    kv = k.shape[1]
-    pp = _ints("positions", positions, _I32, index, None, n)
+    k_shape = k.shape
+    kv = k_shape[1]
     vp = sp = cp = kop = None
     vs = kos = 0
     if cache is not None:
@@ -266,12 +268,13 @@ def qk_norm_rope(rotary: Rotary, q, k, v, positions, q_out=None, k_out=None, cac
         vp, vs = _rows("v", v, n, kv, hd, index)
         sp, cp = _ints("slots", slots, _I64, index, None, n), cache.ref
     elif k_out is None:
-        k_out = torch.empty((n, kv, hd), dtype=_F32, device=q.device)
+        k_out = torch.empty(k_shape, dtype=_F32, device=q.device)
     if q_out is None:
-        q_out = torch.empty((n, heads, hd), dtype=_F32, device=q.device)
+        q_out = torch.empty(q_shape, dtype=_F32, device=q.device)
     qop, qos = (qp, qs) if q_out is q else _rows("q_out", q_out, n, heads, hd, index)
     if k_out is not None:
         kop, kos = _rows("k_out", k_out, n, kv, hd, index)
+    pp = _ints("positions", positions, _I32, index, None, n)
     if n:
         _check(lib().mlq_qk_norm_rope(rotary.ref, n, pp, heads, kv, qp, qs, kp, ks, vp, vs, qop, qos,
                                       kop, kos, cp, layer, sp, _raw_stream(index)),
@@ -359,7 +362,7 @@ def attention_decode(cache: PagedCache, layer: int, batch: PagedBatch, q, out=No
     workspace: a uint8 device tensor of attention_workspace_bytes, or None for
     one of the call's own."""
     index = cache.index
-    if stream is not None or index != torch.cuda.current_device():
+    if stream is not None or index != _current_device():
         return _elsewhere(lambda: attention_decode(cache, layer, batch, q, out, rule, max_len,
                                                    workspace), index, stream)
     heads, qp, qs, out, op, os, ref = _attention_args(cache, batch, q, out, rule)
@@ -384,7 +387,7 @@ def attention_prefill(cache: PagedCache, layer: int, batch: PagedBatch, q, out=N
     workspace as in attention_decode, the workspace of
     attention_workspace_bytes(..., rows=q.shape[0])."""
     index = cache.index
-    if stream is not None or index != torch.cuda.current_device():
+    if stream is not None or index != _current_device():
         return _elsewhere(lambda: attention_prefill(cache, layer, batch, q, out, rule, max_len,
                                                     workspace), index, stream)
     heads, qp, qs, out, op, os, ref = _attention_args(cache, batch, q, out, rule)
