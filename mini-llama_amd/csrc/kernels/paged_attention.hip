@@ -787,10 +787,13 @@ struct PreTile {
 template <typename T, int HD>
 struct PreLds {
   // 16-bit caches: the next tile is written beside the one that is read, a
-  // barrier a tile; fp32's parts leave no room for it (two barriers)
-  static constexpr int kBuf = sizeof(T) == 4 ? 1 : 2;
-  // steps of q's last part per wave and lane (in registers they spill)
-  static constexpr int kQ = PreTraits<T>::kParts < 3 || HD < 128 ? 0 : sizeof(T) == 4 ? HD / 32 : HD / 16;
+  // barrier a tile; fp32's parts leave no room for it (two barriers), and at
+  // head dim 256 its registers spill (8000 rows, 16 heads on 2: bf16 988 -> 681
+  // us with one buffer, fp16 706 -> 620)
+  static constexpr int kBuf = sizeof(T) == 4 || HD > 128 ? 1 : 2;
+  // steps of q's last part per wave and lane (in registers they spill: fp16 at
+  // head dim 256 1058 -> 706 us)
+  static constexpr int kQ = HD < 128 || (PreTraits<T>::kParts < 3 && HD < 256) ? 0 : sizeof(T) == 4 ? (HD > 128 ? 12 : 5) : HD / 16;
   PreTile<T, HD> tile[kBuf];
   u32x4_t q[kQ > 0 ? kQ : 1][kPreThreads];
   int count[kPreThreads / 64];
@@ -1200,6 +1203,8 @@ __global__ __launch_bounds__(kPreThreads, HD <= 128 ? 2 : 1) void paged_prefill_
         for (int x = NK - 1; x >= 0; --x)
           if (sum - x >= 0 && sum - x < NP) c = Tr::mfma32(kk[x], q_part(sum - x, i), c);
     }
+    // (fp32's parts are read again: held across the loops they spill)
+    if constexpr (NK > 1 && HD <= 128) asm volatile("" ::: "memory");
 #pragma unroll
     for (int i = 0; i < KT; ++i) {
       f16v& c = i % 2 == 0 ? s : s1;
