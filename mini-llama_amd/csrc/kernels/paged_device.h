@@ -28,12 +28,12 @@ __device__ __forceinline__ int64_t wave_scan64(int64_t v) {
   const int64_t a = readlane64(v, 15), b = a + readlane64(v, 31), c = b + readlane64(v, 47);
   return v + (row == 0 ? 0 : row == 1 ? a : row == 2 ? b : c);
 }
+
 // a / b for a >= 0, b > 0, in 32 bits where they fit (a 64-bit division is a
 // hundred instructions).
 __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
   if (((a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
   return a / b;
 }
-__device__ __forceinline__ int64_t wave_last64(int64_t v) { return readlane64(v, 63); }
 
 }  // namespace mlq
