@@ -902,7 +902,7 @@ __device__ __forceinline__ PreWork by_row(const PagedAttnArgs& a, int x, int* ld
 struct PreSpan {
   int row0, pos0, len;  // of the sequence
   int64_t pairs, c0;    // its pairs, the tile's first
-  int kfirst, kmax;     // first key (a multiple of kPreKeys) and last; kmax < 0: none
+  int kfirst, kmax;     // first key (a multiple of kPreKeys) and last; kmax < 0 or len > max_len: none
   int tiles, each;      // key tiles, and of a workgroup when `splits` share them
   bool live;
 };
@@ -916,9 +916,10 @@ __device__ __forceinline__ PreSpan prefill_span(const PagedAttnArgs& a, const Pr
   s.c0 = (int64_t)w.tile * kPreCols;
   if (s.row0 < 0 || s.c0 < 0 || s.c0 >= s.pairs) return s;
   s.live = true;
-  s.len = a.lengths[w.seq];
+  s.len = max(a.lengths[w.seq], 0);  // (below: any number, but no overflow)
   s.pos0 = s.len - (end - s.row0);
   const int ja = (int)(s.c0 / a.group), jb = (int)((min(s.c0 + kPreCols, s.pairs) - 1) / a.group);
+  if (s.len > a.max_len) return s;
   s.kmax = s.pos0 + jb;
   s.kfirst = (a.window > 0 ? max(0, s.pos0 + ja + 1 - a.window) : 0) & ~(kPreKeys - 1);
   s.tiles = s.kmax < 0 ? 0 : (s.kmax - s.kfirst) / kPreKeys + 1;

@@ -391,10 +391,11 @@ def test_bad_device_numbers_give_nan_rows_alone(paged, prefill, kind):
         if r in bad:
             assert np.all(np.isnan(o[r])), r
     p.compare(out, {r: w for r, w in want.items() if r not in bad})
-    n.fill_(-5)  # negative lengths: nothing to see
-    out = call(p.cache, 0, p.batch, p.qd)
-    torch.cuda.synchronize()
-    assert np.all(host(out) == 0.0)
+    for length, value in ((-5, 0.0), (-2 ** 31, 0.0), (2 ** 31 - 1, math.nan)):  # negative: nothing to see
+        n.fill_(length)
+        out = call(p.cache, 0, p.batch, p.qd)
+        torch.cuda.synchronize()
+        assert np.array_equal(host(out), np.full(out.shape, value), equal_nan=True), length
 
 
 @pytest.mark.parametrize("kind", KINDS)
