@@ -532,6 +532,26 @@ def test_prefill_long(paged, heads, kv, hd, lengths, new, kind):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n", [255, 256, 257, 700])
+@pytest.mark.parametrize("heads,kv,hd", [(28, 4, 128), (4, 4, 64), (5, 1, 80)])
+def test_prefill_of_many_sequences(paged, heads, kv, hd, n, kind):
+    """Tiles are given out in another way from 257 sequences on; some have no rows, one has several tiles."""
+    import torch
+    r = np.random.default_rng(n)
+    lengths = r.integers(0, 50, n)
+    lengths[n // 2] = 300
+    new = np.minimum(r.choice([0, 1, 1, 2, 40], n), lengths)
+    new[n // 2], new[-1], new[0] = 290, 0, 0
+    p = Problem(paged, kind, lengths, heads, kv, hd, 16, seed=31, new=new)
+    out = torch.full((p.rows + 3, heads, hd), 9.0, device="cuda")
+    q = torch.cat([p.qd, p.qd[:1], p.qd[:1], p.qd[:1]])
+    paged.attention_prefill(p.cache, 0, p.batch, q, out=out)
+    torch.cuda.synchronize()
+    p.compare(out, p.want(rows=set(range(0, p.rows, 7)) | {p.rows - 1}))
+    assert torch.all(torch.isfinite(out)) and torch.all(out[p.rows:] == 9.0)
+
+
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("heads,kv,hd,lengths,new", [
     (28, 4, 128, [5000], [3]), (8, 8, 64, [3000, 10, 900, 0], [20, 10, 1, 0]), (16, 1, 256, [1300, 2000], [5, 4]), (33, 1, 128, [700], [9]),
     (12, 4, 80, [4000, 130, 2000, 20], [1, 2, 40, 20]), (4, 4, 128, [600, 600], [300, 5])])
