@@ -103,6 +103,13 @@ int check_attention(const mlq_paged_cache* c, int layer, const mlq_paged_batch* 
   return MLQ_OK;
 }
 
+// A window that every sequence fits in is none (and positions minus a window
+// stay within 32 bits).
+void bound_lengths(PagedAttnArgs* a, int max_len) {
+  a->max_len = max_len;
+  if (a->window >= max_len) a->window = 0;
+}
+
 }  // namespace
 
 extern "C" {
@@ -286,7 +293,7 @@ int mlq_paged_attention_decode(const mlq_paged_cache* c, int layer, const mlq_pa
     a.max_rows = b->n_seqs;
   else if (b->max_rows <= 0)
     return MLQ_ERR_SHAPE;
-  a.max_len = max_len;
+  bound_lengths(&a, max_len);
   const size_t need = plan_paged_decode(a);
   if (((uintptr_t)ws & 255u) != 0) return MLQ_ERR_INVALID_ARG;
   if (ws_bytes < need || (need > 0 && ws == nullptr)) return MLQ_ERR_BUFFER_TOO_SMALL;
@@ -304,7 +311,7 @@ int mlq_paged_attention_prefill(const mlq_paged_cache* c, int layer, const mlq_p
   if (b->row_start == nullptr) return MLQ_ERR_INVALID_ARG;
   if (b->max_rows <= 0 || max_len <= 0 || max_len > (int64_t)b->max_pages * c->page_size)
     return MLQ_ERR_SHAPE;
-  a.max_len = max_len;
+  bound_lengths(&a, max_len);
   const size_t need = plan_paged_prefill(a);
   if (((uintptr_t)ws & 255u) != 0) return MLQ_ERR_INVALID_ARG;
   if (ws_bytes < need || (need > 0 && ws == nullptr)) return MLQ_ERR_BUFFER_TOO_SMALL;

@@ -291,6 +291,8 @@ class AttentionRule:
                  slopes=None):
         if scale == 0.0:
             raise ValueError("a scale of 0 would weigh every key alike")
+        if not 0 <= window < 1 << 31:
+            raise ValueError("a window is a number of keys below 2^31 (0: none)")
         if slopes is not None and (slopes.dtype != torch.float32 or not slopes.is_cuda or
                                    slopes.dim() != 1 or not slopes.is_contiguous()):
             raise ValueError("slopes must be a contiguous float32 device vector")

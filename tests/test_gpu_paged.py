@@ -520,6 +520,21 @@ def test_prefill_rules(paged, heads, kv, hd, rule, kind):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("window", [64, 2 ** 31 - 1])
+def test_prefill_rows_before_the_first_key(paged, window, kind):
+    """More rows than tokens: the first ones see nothing and are zeros, the last ones what they would."""
+    import torch
+    p = Problem(paged, kind, [150, 40, 90], 8, 2, 64, 16, seed=33, new=[150, 40, 90])
+    kept = p.lengths = np.array([30, 0, 89])
+    p.batch.lengths.copy_(dev(kept.astype(np.int32)))
+    out = paged.attention_prefill(p.cache, 0, p.batch, p.qd, rule=paged.AttentionRule(window=window))
+    torch.cuda.synchronize()
+    lost = {int(p.start[i]) + j for i, n in enumerate(kept) for j in range(int(p.new[i] - n))}
+    assert torch.all(out[sorted(lost)] == 0.0)
+    p.compare(out, p.want(rows=set(range(p.rows)) - lost, window=window))
+
+
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("heads,kv,hd,lengths,new", [(28, 4, 128, [2100, 1500, 60], [1900, 800, 60]), (8, 8, 64, [3000], [1537]), (16, 1, 256, [1300], [700])])
 def test_prefill_long(paged, heads, kv, hd, lengths, new, kind):
     import torch

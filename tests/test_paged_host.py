@@ -207,6 +207,9 @@ def test_python_refusals(pkg):
         paged.Rotary(64, torch.zeros(32, dtype=torch.float64))
     with pytest.raises(ValueError):
         paged.AttentionRule(scale=0.0)
+    for window in (-1, 1 << 31, (1 << 32) + 5):  # (a C int would hold another number)
+        with pytest.raises(ValueError):
+            paged.AttentionRule(window=window)
     with pytest.raises(ValueError):
         paged.AttentionRule(slopes=torch.zeros(4))
     with pytest.raises(ValueError):
