@@ -297,6 +297,7 @@ int mlq_paged_attention_decode(const mlq_paged_cache* c, int layer, const mlq_pa
   const size_t need = plan_paged_decode(a);
   if (((uintptr_t)ws & 255u) != 0) return MLQ_ERR_INVALID_ARG;
   if (ws_bytes < need || (need > 0 && ws == nullptr)) return MLQ_ERR_BUFFER_TOO_SMALL;
+  if (out == q) return MLQ_ERR_INVALID_ARG;  // (q is read again after some of out is written)
   a.part = need > 0 ? ws : nullptr;
   return record_hip(launch_paged_decode(a, (hipStream_t)stream));
 }
@@ -315,6 +316,7 @@ int mlq_paged_attention_prefill(const mlq_paged_cache* c, int layer, const mlq_p
   const size_t need = plan_paged_prefill(a);
   if (((uintptr_t)ws & 255u) != 0) return MLQ_ERR_INVALID_ARG;
   if (ws_bytes < need || (need > 0 && ws == nullptr)) return MLQ_ERR_BUFFER_TOO_SMALL;
+  if (out == q) return MLQ_ERR_INVALID_ARG;  // (q is read again after some of out is written)
   a.part = need > 0 ? ws : nullptr;
   return record_hip(launch_paged_prefill(a, (hipStream_t)stream));
 }

@@ -136,6 +136,7 @@ def test_attention_refusals(pkg, prefill):
     long = dict(c=c, b=batch(pkg, n_seqs=1, max_pages=6250), max_len=100000)
     assert call(ws_bytes=n.value - 1, **long) == SMALL
     assert call(ws=None, **long) == SMALL
+    assert call(**long) == ARG  # out is q
 
 
 def test_attention_workspace(pkg):
