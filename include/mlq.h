@@ -591,7 +591,8 @@ typedef struct mlq_rotary {
  * side by side; 16-byte aligned float pointers. q_out may be q, k_out k (same
  * strides then; no other overlap). k_out may be NULL with a cache; without
  * one (c NULL) k_out is needed and v, slots and layer are not read.
- * Distinct rows need distinct slots. rows = 0 does nothing. */
+ * Distinct rows need distinct slots. rows = 0 does nothing. Up to 2048 heads and
+ * fewer than 2^24 rows (MLQ_ERR_UNSUPPORTED otherwise). */
 int mlq_qk_norm_rope(const mlq_rotary* r, int rows, const int32_t* positions, int n_heads,
                      int n_kv_heads, const float* q, int64_t q_stride, const float* k,
                      int64_t k_stride, const float* v, int64_t v_stride, float* q_out,
@@ -632,7 +633,8 @@ int mlq_paged_attention_workspace(const mlq_paged_cache* c, int n_heads, int n_s
  * error of up to 2^-37; storing them rounds by up to 2^-25).
  * NaN / inf among the seen keys and values give NaN / inf outputs. ws:
  * 256-byte aligned, scratch, may be NULL when its size is 0; calls that
- * share one (two captured graphs, too) must be ordered. */
+ * share one (two captured graphs, too) must be ordered. n_heads: up to 2048
+ * (MLQ_ERR_UNSUPPORTED otherwise). */
 int mlq_paged_attention_decode(const mlq_paged_cache* c, int layer, const mlq_paged_batch* b,
                                const mlq_attention_rule* rule, int n_heads, const float* q,
                                int64_t q_stride, float* out, int64_t out_stride, int max_len,
@@ -641,7 +643,8 @@ int mlq_paged_attention_decode(const mlq_paged_cache* c, int layer, const mlq_pa
  * cached): row j of n new ones of sequence i is at position lengths[i] - n + j
  * and sees the keys up to it. Same rule, layouts, checks and workspace
  * contract. b->max_rows bounds row_start[n_seqs] (rows past it are not
- * computed). */
+ * computed). (max_rows * n_heads / n_kv_heads / 128 + n_seqs) * n_kv_heads is
+ * less than 2^24 (MLQ_ERR_UNSUPPORTED otherwise). */
 int mlq_paged_attention_prefill(const mlq_paged_cache* c, int layer, const mlq_paged_batch* b,
                                 const mlq_attention_rule* rule, int n_heads, const float* q,
                                 int64_t q_stride, float* out, int64_t out_stride, int max_len,

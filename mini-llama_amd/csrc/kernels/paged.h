@@ -74,6 +74,8 @@ struct PagedAttnArgs {
 // Sets launch_seqs and ranges for lengths up to a.max_len; the workspace.
 size_t plan_paged_decode(PagedAttnArgs& a);
 hipError_t launch_paged_decode(const PagedAttnArgs& a, hipStream_t stream);
+// Workgroups of a launch, without the splits'.
+int64_t prefill_groups(const PagedAttnArgs& a);
 // Sets splits for a.max_rows rows and lengths up to a.max_len; the workspace.
 size_t plan_paged_prefill(PagedAttnArgs& a);
 hipError_t launch_paged_prefill(const PagedAttnArgs& a, hipStream_t stream);

@@ -852,7 +852,7 @@ __device__ __forceinline__ PreWork longest_first(const PagedAttnArgs& a, int x) 
   longest = wave_max_int(longest);
 #pragma unroll
   for (int n = 0; n < kPreSeqsPerLane; ++n) {
-    level[n] = (int)((int64_t)(longest - min(level[n], longest)) * a.group / kPreCols);
+    level[n] = (int)min((int64_t)(longest - min(level[n], longest)) * a.group / kPreCols, (int64_t)1 << 30);
     if (tiles[n] > 0) end = max(end, level[n] + tiles[n]);
   }
   if (x >= wave_sum_int(total)) return {-1, 0};
@@ -874,7 +874,7 @@ __device__ __forceinline__ PreWork longest_first(const PagedAttnArgs& a, int x) 
   for (int n = 0; n < kPreSeqsPerLane; ++n) {
     uint64_t has = __ballot(tiles[n] > 0 && lo >= level[n] && lo < level[n] + tiles[n]);
     const int count = __builtin_popcountll(has);
-    if (w.seq < 0 && rank < count) {
+    if (w.seq < 0 && rank >= 0 && rank < count) {
       for (int r = 0; r < rank; ++r) has &= has - 1;
       const int from = __builtin_ctzll(has);
       w.seq = from + 64 * n;
@@ -888,14 +888,14 @@ __device__ __forceinline__ PreWork longest_first(const PagedAttnArgs& a, int x) 
 // on, at least as many as it needs, found without a sum over the sequences
 // before it.
 __device__ __forceinline__ PreWork by_row(const PagedAttnArgs& a, int x, int* lds) {
-  auto first_tile = [&](int i) { return (int)((int64_t)a.row_start[i] * a.group / kPreCols) + i; };
+  auto first_tile = [&](int i) { return (int64_t)a.row_start[i] * a.group / kPreCols + i; };
   int before = 0;
   for (int i = threadIdx.x; i < a.n_seqs; i += kPreThreads) before += first_tile(i) <= x;
   before = wave_sum_int(before);
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = before;
   __syncthreads();
   const int seq = __builtin_amdgcn_readfirstlane(lds[0] + lds[1] + lds[2] + lds[3]) - 1;
-  return {seq, seq < 0 ? 0 : x - first_tile(seq)};
+  return {seq, seq < 0 ? 0 : (int)(x - first_tile(seq))};
 }
 
 // A workgroup's tile of rows: its pairs, positions and the keys that they see.
@@ -1435,12 +1435,6 @@ __global__ __launch_bounds__(kPreJoinThreads) void paged_prefill_join_kernel(Pag
     }
 }
 
-// Tiles of rows that the grid has to hold: one more for each sequence than its
-// rows fill.
-int64_t prefill_tiles(const PagedAttnArgs& a) {
-  return (int64_t)a.max_rows * a.group / kPreCols + a.n_seqs;
-}
-
 template <typename T, int HD, bool FULL, bool RULE>
 hipError_t prefill_launch(const PagedAttnArgs& a, hipStream_t stream) {
   constexpr size_t lds = sizeof(PreLds<T, HD>);
@@ -1448,8 +1442,7 @@ hipError_t prefill_launch(const PagedAttnArgs& a, hipStream_t stream) {
   const auto kernel = paged_prefill_kernel<T, HD, FULL, RULE>;
   hipError_t e = allow_dynamic_lds((const void*)kernel, lds);
   if (e != hipSuccess) return e;
-  const int64_t grid = prefill_tiles(a) * a.n_kv;
-  if (grid > INT32_MAX) return hipErrorInvalidValue;
+  const int64_t grid = prefill_groups(a);
   hipLaunchKernelGGL(kernel, dim3((unsigned)grid, a.splits), dim3(kPreThreads), lds, stream, a);
   e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
@@ -1525,10 +1518,16 @@ hipError_t launch_paged_decode(const PagedAttnArgs& all, hipStream_t stream) {
   return hipSuccess;
 }
 
+// Tiles of rows that the grid has to hold, one more for each sequence than its
+// rows fill, for every kv head.
+int64_t prefill_groups(const PagedAttnArgs& a) {
+  return ((int64_t)a.max_rows * a.group / kPreCols + a.n_seqs) * a.n_kv;
+}
+
 // Where the tiles of rows leave most of the chip idle, a tile's keys are shared
 // by several workgroups and joined.
 size_t plan_paged_prefill(PagedAttnArgs& a) {
-  const int64_t tiles = prefill_tiles(a) * a.n_kv, slots = (int64_t)(a.hd <= 128 ? 2 : 1) * device_cus();
+  const int64_t tiles = prefill_groups(a), slots = (int64_t)(a.hd <= 128 ? 2 : 1) * device_cus();
   const int64_t keys = ((int64_t)a.max_len + kPreKeys - 1) / kPreKeys;
   a.splits = (int)std::max(std::min(std::min(slots / tiles, keys / kPreLeast), (int64_t)kPreMaxSplits), (int64_t)1);
   if (a.n_seqs > kPreSorted) a.splits = 1;

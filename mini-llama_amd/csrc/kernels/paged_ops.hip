@@ -363,7 +363,7 @@ hipError_t launch_paged_plan(const PlanArgs& a, hipStream_t stream) {
     hipLaunchKernelGGL(plan_kernel<1024>, dim3(1), dim3(1024), 0, stream, a, rows ? 1 : 0);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || rows) return e;
-  hipLaunchKernelGGL(plan_rows_kernel, dim3((a.max_rows + 255) / 256), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL(plan_rows_kernel, dim3((unsigned)(((int64_t)a.max_rows + 255) / 256)), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 

@@ -18,6 +18,10 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
 // Of a sequence: the kernels count positions, padded to whole tiles, in 32 bits.
 constexpr int64_t kMaxTokens = (int64_t)1 << 30;
+// A launch holds fewer than 2^32 threads, 2^24 workgroups of 256; with so many
+// heads those of a decode launch's sequences stay below that.
+constexpr int kMaxHeads = 2048;
+constexpr int64_t kMaxGroups = ((int64_t)1 << 24) - 1;
 
 size_t kv_bytes(int type) { return type == MLQ_KV_F32 ? 4 : 2; }
 
@@ -69,7 +73,8 @@ int check_attention(const mlq_paged_cache* c, int layer, const mlq_paged_batch* 
   if (b->n_seqs <= 0 || b->max_pages <= 0 || n_heads <= 0 || n_heads % c->n_kv_heads != 0)
     return MLQ_ERR_SHAPE;
   if (layer < 0 || layer >= c->n_layers) return MLQ_ERR_SHAPE;
-  if ((int64_t)b->max_pages * c->page_size > kMaxTokens) return MLQ_ERR_UNSUPPORTED;
+  if ((int64_t)b->max_pages * c->page_size > kMaxTokens || n_heads > kMaxHeads)
+    return MLQ_ERR_UNSUPPORTED;
   const int64_t floats = (int64_t)n_heads * c->head_dim;
   if ((rc = check_rows(q, q_stride, floats)) != MLQ_OK) return rc;
   if ((rc = check_rows(out, out_stride, floats)) != MLQ_OK) return rc;
@@ -200,7 +205,9 @@ int mlq_qk_norm_rope(const mlq_rotary* r, int rows, const int32_t* positions, in
   if (rows < 0 || n_heads <= 0 || n_kv_heads <= 0 || r->head_dim <= 0 || r->rot_dim < 0 ||
       r->rot_dim % 2 != 0 || r->rot_dim > r->head_dim)
     return MLQ_ERR_SHAPE;
-  if (r->head_dim % 8 != 0 || r->head_dim > 256) return MLQ_ERR_UNSUPPORTED;
+  if (r->head_dim % 8 != 0 || r->head_dim > 256 || n_heads > kMaxHeads || n_kv_heads > kMaxHeads ||
+      rows > kMaxGroups)
+    return MLQ_ERR_UNSUPPORTED;
   if (r->rope_type != MLQ_ROPE_NORMAL && r->rope_type != MLQ_ROPE_NEOX)
     return MLQ_ERR_INVALID_ARG;
   if (r->rot_dim > 0 && (r->freqs == nullptr || !std::isfinite(r->magnitude)))
@@ -268,7 +275,7 @@ int mlq_paged_attention_workspace(const mlq_paged_cache* c, int n_heads, int n_s
   if (bytes == nullptr) return MLQ_ERR_INVALID_ARG;
   if (n_heads <= 0 || n_heads % c->n_kv_heads != 0 || n_seqs <= 0 || max_rows < 0 || max_len <= 0)
     return MLQ_ERR_SHAPE;
-  if (max_len > kMaxTokens) return MLQ_ERR_UNSUPPORTED;
+  if (max_len > kMaxTokens || n_heads > kMaxHeads) return MLQ_ERR_UNSUPPORTED;
   PagedAttnArgs a = {};
   a.type = c->type;
   a.n_kv = c->n_kv_heads;
@@ -277,6 +284,7 @@ int mlq_paged_attention_workspace(const mlq_paged_cache* c, int n_heads, int n_s
   a.n_seqs = n_seqs;
   a.max_len = max_len;
   a.max_rows = max_rows;
+  if (max_rows > 0 && prefill_groups(a) > kMaxGroups) return MLQ_ERR_UNSUPPORTED;
   *bytes = max_rows == 0 ? plan_paged_decode(a) : plan_paged_prefill(a);
   return MLQ_OK;
 }
@@ -313,6 +321,7 @@ int mlq_paged_attention_prefill(const mlq_paged_cache* c, int layer, const mlq_p
   if (b->max_rows <= 0 || max_len <= 0 || max_len > (int64_t)b->max_pages * c->page_size)
     return MLQ_ERR_SHAPE;
   bound_lengths(&a, max_len);
+  if (prefill_groups(a) > kMaxGroups) return MLQ_ERR_UNSUPPORTED;
   const size_t need = plan_paged_prefill(a);
   if (((uintptr_t)ws & 255u) != 0) return MLQ_ERR_INVALID_ARG;
   if (ws_bytes < need || (need > 0 && ws == nullptr)) return MLQ_ERR_BUFFER_TOO_SMALL;

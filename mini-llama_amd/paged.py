@@ -309,6 +309,8 @@ def attention_workspace_bytes(cache: PagedCache, n_heads: int, n_seqs: int, max_
     key = (n_heads, n_seqs, rows, max_len)
     need = cache._workspaces.get(key)
     if need is None:
+        if max(key) >= 1 << 31:  # (a C int would hold another number)
+            raise ValueError("more heads, sequences, rows or tokens than 2^31")
         nbytes = ctypes.c_size_t()
         _check(lib().mlq_paged_attention_workspace(cache.ref, n_heads, n_seqs, rows, max_len,
                                                    ctypes.byref(nbytes)),
@@ -329,6 +331,8 @@ def _workspace(cache, workspace, n_heads: int, n_seqs: int, max_len: int, rows: 
             return None, None, 0
         workspace = torch.empty(size, dtype=torch.uint8, device=cache.device)
         return workspace, workspace.data_ptr(), size
+    if max_len >= 1 << 31:
+        raise ValueError("max_len is below 2^31")
     if workspace.get_device() != cache.index or not workspace.is_contiguous():
         raise ValueError("the workspace must be a contiguous tensor on the cache's device")
     return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()

@@ -93,7 +93,9 @@ def test_rotary_refusals(pkg):
                      (dict(c=cache(pkg, n_kv_heads=2)), SHAPE),
                      (dict(c=cache(pkg, head_dim=64)), SHAPE),
                      (dict(c=cache(pkg, keys=None)), ARG), (dict(c=cache(pkg, keys=FAKE + 2)), ARG),
-                     (dict(c=None), ARG)]:
+                     (dict(c=None), ARG), (dict(rows=1 << 24), UNSUPPORTED),
+                     (dict(heads=2049, qs=2049 * 128, qos=2049 * 128), UNSUPPORTED),
+                     (dict(kv=2049, ks=2049 * 128, vs=2049 * 128), UNSUPPORTED)]:
         assert call(**kw) == want, kw
     assert call(rows=0, c=None, ko=FAKE + 4096, kos=512, v=None, slots=None) == OK
     assert call(rows=0, rot_dim=0, freqs=None) == OK
@@ -123,8 +125,11 @@ def test_attention_refusals(pkg, prefill):
                      (dict(rule=(0.0, -1.0, 0, None)), ARG), (dict(rule=(0.0, math.inf, 0, None)), ARG),
                      (dict(rule=(0.0, 0.0, -1, None)), ARG)]:
         assert call(**kw) == want, kw
+    assert call(heads=2052, qs=2052 * 128, os=2052 * 128) == UNSUPPORTED
     if prefill:
         assert call(b=batch(pkg, row_start=None)) == ARG
+        assert call(b=batch(pkg, n_seqs=1 << 22)) == UNSUPPORTED
+        assert call(b=batch(pkg, max_rows=2 ** 31 - 1)) == UNSUPPORTED
     assert call(max_len=0) == SHAPE and call(max_len=129) == SHAPE
     assert call(ws=FAKE + 16) == ARG
     # the keys of one sequence of 100000 are shared by workgroups: it needs their partials
@@ -144,6 +149,7 @@ def test_attention_workspace(pkg):
     c = cache(pkg, keys=None, values=None)
     for heads, seqs, rows, max_len, want in [(0, 1, 0, 1, SHAPE), (30, 1, 0, 1, SHAPE), (28, 0, 0, 1, SHAPE),
                                              (28, 1, 0, 0, SHAPE), (28, 1, -1, 1, SHAPE), (28, 1, 7, 1, OK),
+                                             (2052, 1, 0, 1, UNSUPPORTED), (28, 1 << 22, 1, 1, UNSUPPORTED),
                                              (28, 1, 0, 1, OK)]:
         n.value = 77
         assert lib.mlq_paged_attention_workspace(ctypes.byref(c), heads, seqs, rows, max_len,
