@@ -603,7 +603,9 @@ int mlq_qk_norm_rope(const mlq_rotary* r, int rows, const int32_t* positions, in
 /* How a score s = q . k becomes the softmax's input for a query at position p
  * and a key at position t <= p: s * scale, then softcap * tanh(that /
  * softcap) if softcap > 0, then + slopes[head] * (t - p) if slopes is given;
- * keys with t <= p - window are not seen if window > 0. */
+ * keys with t <= p - window are not seen if window > 0. Block table entries
+ * whose whole page is behind the windows of all of a sequence's rows of the
+ * call are not read: a caller may have given such pages to others. */
 typedef struct mlq_attention_rule {
   float scale;                       /* 0: 1 / sqrt(head_dim) */
   float softcap;                     /* 0: none */

@@ -406,9 +406,11 @@ __global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_k
   const int mask = (1 << a.page_shift) - 1;
   bool bad = dr.bad;
   const int32_t* table = a.block_table + (size_t)seq * a.max_pages;
-  // The rows of the run of 16 keys at k, or of the sequence's last run.
+  // The rows of the run of 16 keys at k, or of the nearest run that holds a key
+  // which is seen: a tile may begin before the window, on a page that nobody
+  // keeps any more.
   auto row_of = [&](int k) __attribute__((always_inline)) {
-    const int kk = min(k, pos);
+    const int kk = min(max(k, key_begin), pos);
     int page = __builtin_amdgcn_readfirstlane(table[kk >> a.page_shift]);
     const bool out = page < 0 || page >= a.n_pages;
     bad |= out;
@@ -902,7 +904,8 @@ __device__ __forceinline__ PreWork by_row(const PagedAttnArgs& a, int x, int* ld
 struct PreSpan {
   int row0, pos0, len;  // of the sequence
   int64_t pairs, c0;    // its pairs, the tile's first
-  int kfirst, kmax;     // first key (a multiple of kPreKeys) and last; kmax < 0 or len > max_len: none
+  int kseen, kmax;      // first key that a row sees and last; kmax < 0 or len > max_len: none
+  int kfirst;           // the tiles' first key: kseen down to a multiple of kPreKeys
   int tiles, each;      // key tiles, and of a workgroup when `splits` share them
   bool live;
 };
@@ -921,7 +924,8 @@ __device__ __forceinline__ PreSpan prefill_span(const PagedAttnArgs& a, const Pr
   const int ja = (int)(s.c0 / a.group), jb = (int)((min(s.c0 + kPreCols, s.pairs) - 1) / a.group);
   if (s.len > a.max_len) return s;
   s.kmax = s.pos0 + jb;
-  s.kfirst = (a.window > 0 ? max(0, s.pos0 + ja + 1 - a.window) : 0) & ~(kPreKeys - 1);
+  s.kseen = a.window > 0 ? max(0, s.pos0 + ja + 1 - a.window) : 0;
+  s.kfirst = s.kseen & ~(kPreKeys - 1);
   s.tiles = s.kmax < 0 ? 0 : (s.kmax - s.kfirst) / kPreKeys + 1;
   s.each = max((s.tiles + a.splits - 1) / a.splits, kPreLeast);
   return s;
@@ -1063,13 +1067,14 @@ __global__ __launch_bounds__(kPreThreads, HD <= 128 ? 2 : 1) void paged_prefill_
   // ---- staging: a wave's keys lie in one run of 16 (and so in one page)
   const int32_t* table = a.block_table + (size_t)seq * a.max_pages;
   const int mask = (1 << a.page_shift) - 1, row_bytes = a.hd * (int)sizeof(T);
+  // The wave's run, or the nearest that holds a key which a row sees (a tile may
+  // begin before the window, on a page that nobody keeps any more).
+  auto key_of = [&](int k0) __attribute__((always_inline)) { return min(max(k0 + 16 * (wave >> 1), sp.kseen), kmax); };
   // Asked for a tile ahead of the rows it names: a load that waits for it waits
   // twice.
-  auto page_of = [&](int k0) __attribute__((always_inline)) {
-    return table[min(k0 + 16 * (wave >> 1), kmax) >> a.page_shift];
-  };
+  auto page_of = [&](int k0) __attribute__((always_inline)) { return table[key_of(k0) >> a.page_shift]; };
   auto run_of = [&](int k0, int id) __attribute__((always_inline)) {
-    const int kk = min(k0 + 16 * (wave >> 1), kmax);
+    const int kk = key_of(k0);
     int page = __builtin_amdgcn_readfirstlane(id);
     const bool outside = page < 0 || page >= a.n_pages;
     odd |= outside;

@@ -848,3 +848,34 @@ def test_offsets_past_32_bits(paged):
         y, bound = ref.attention(host(q)[r_], kk, vv, r_, 1 / math.sqrt(hd))
         check(host(out[r_]), y, bound, r_)
     check(host(one[199]), y, bound, "decode")
+
+
+# ---- pages behind a window ---------------------------------------------------------------
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("page", [16, 32, 64])
+@pytest.mark.parametrize("heads,kv,hd", [(8, 2, 64), (28, 4, 128), (4, 1, 256)])
+def test_pages_behind_the_window_are_not_asked_for(paged, heads, kv, hd, page, kind):
+    """Wherever the window begins in a tile of keys or a page: a table entry of a page wholly behind the window of the
+    sequence's first new row may be anything, and the results are those of a whole table, bit for bit."""
+    import torch
+    window = 50
+    ends = [1, 50, 51, 65, 66, 67, 81, 82, 83, 97, 98, 99, 113, 114, 130, 200, 1003, 2000]
+    for new in (None, [min(n, 1 + 7 * i % 40) for i, n in enumerate(ends)]):
+        p = Problem(paged, kind, ends, heads, kv, hd, page, seed=61, new=new)
+        own, plain = rule_of(paged, heads, window=window)
+        call = paged.attention_decode if new is None else paged.attention_prefill
+        whole = call(p.cache, 0, p.batch, p.qd, rule=own)
+        torch.cuda.synchronize()
+        p.compare(whole, p.want(rows=set(range(0, p.rows, 3)) | {int(s) - 1 for s in p.start[1:]}, **plain))
+        first = p.lengths - p.new + 1 - window  # the first key that a row sees
+        for junk in (-1, p.cache.n_pages, 2 ** 31 - 1):
+            table = p.table.copy()
+            for i, f in enumerate(first):
+                table[i, :max(0, int(f)) // page] = junk
+            assert (table != p.table).any()
+            p.batch.block_table.copy_(dev(table))
+            out = call(p.cache, 0, p.batch, p.qd, rule=own)
+            torch.cuda.synchronize()
+            bad = [int(n) for i, n in enumerate(p.lengths)
+                   if not torch.equal(out[p.start[i]:p.start[i + 1]], whole[p.start[i]:p.start[i + 1]])]
+            assert not bad, (junk, bad)
