@@ -1487,7 +1487,10 @@ size_t plan_paged_decode(PagedAttnArgs& a) {
     a.ranges = (int)(a.launch_seqs * n_tiles);
     return 0;
   }
-  a.ranges = (int)std::min(a.launch_seqs * n_tiles * units, (int64_t)dec_per_cu(a.hd, a.launch_seqs * n_tiles, cus) * cus);
+  // (pieces of as many sequences as a launch takes under the smallest bounds: the
+  // ranges, and so the workspace, are then no fewer for a longer one)
+  const int64_t pieces = std::min(a.n_seqs, kDecMaxSeqs) * n_tiles;
+  a.ranges = (int)std::min(a.launch_seqs * n_tiles * units, (int64_t)dec_per_cu(a.hd, pieces, cus) * cus);
   const size_t tg = std::min(a.group, 16);
   return dec_header(std::min(a.n_seqs, kDecMaxSeqs)) + dec_align((size_t)2 * a.ranges * tg * 8) +
          (size_t)2 * a.ranges * tg * a.hd * sizeof(float);

@@ -879,3 +879,22 @@ def test_pages_behind_the_window_are_not_asked_for(paged, heads, kv, hd, page, k
             bad = [int(n) for i, n in enumerate(p.lengths)
                    if not torch.equal(out[p.start[i]:p.start[i + 1]], whole[p.start[i]:p.start[i + 1]])]
             assert not bad, (junk, bad)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_decode_of_many_short_pieces_in_a_workspace_of_the_longest_bound(paged, kind):
+    """Small heads, many of them: twice the ranges a CU, several pieces each; a workspace sized for the longest bound
+    that a table can have serves a call with a small one."""
+    import torch
+    r = np.random.default_rng(12)
+    lengths = np.concatenate([[0, 1, 899], r.integers(1, 900, 117)])
+    p = Problem(paged, kind, lengths, 16, 16, 64, 16, seed=63)
+    bound = p.batch.max_pages * 16
+    need = [paged.attention_workspace_bytes(p.cache, 16, len(lengths), n) for n in (bound, 2 ** 30)]
+    assert 0 < need[0] <= need[1]
+    ws = torch.full((need[1],), 255, dtype=torch.uint8, device="cuda")
+    out = paged.attention_decode(p.cache, 0, p.batch, p.qd, workspace=ws)
+    again = paged.attention_decode(p.cache, 0, p.batch, p.qd)
+    torch.cuda.synchronize()
+    p.compare(out, p.want(rows={0, 1, 2} | set(range(3, p.rows, 4))))
+    assert torch.equal(out, again)

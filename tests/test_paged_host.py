@@ -252,3 +252,16 @@ def test_reference_attention_matches_a_softmax():
         np.testing.assert_allclose(out[h], p @ v[h // 2, 5:9], rtol=1e-12)
     assert np.all(bound < 1e-4) and np.all(bound > 0)
     assert np.all(paged_ref.attention(q, k, v, -1, 0.3)[0] == 0)
+
+
+@pytest.mark.parametrize("kind", [0, 1, 2])
+@pytest.mark.parametrize("heads,kv,hd,seqs", [(16, 16, 64, 200), (40, 8, 64, 5000), (8, 8, 8, 190), (2, 1, 64, 4096), (28, 4, 128, 3000),
+                                              (16, 1, 256, 700), (16, 16, 64, 1)])
+def test_a_decode_workspace_serves_every_smaller_bound(pkg, heads, kv, hd, seqs, kind):
+    """Up to the longest bound, where a launch takes fewer sequences than the batch has."""
+    lib, n, sizes = pkg.lib(), ctypes.c_size_t(), []
+    c = cache(pkg, keys=None, values=None, type=kind, n_kv_heads=kv, head_dim=hd)
+    for max_len in sorted({max(1, (1 << s) + d) for s in range(3, 31) for d in (-1, 0)} | {300, 700, 10000, 5 * 10 ** 8}):
+        assert lib.mlq_paged_attention_workspace(ctypes.byref(c), heads, seqs, 0, max_len, ctypes.byref(n)) == OK
+        sizes.append(n.value)
+    assert sizes == sorted(sizes)
