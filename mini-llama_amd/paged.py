@@ -85,7 +85,22 @@ def _rows(name: str, t, rows, heads, head_dim: int, index: int):
                      f"{'heads' if heads is None else heads}, {head_dim}] on cuda:{index}")
 
 
-class PagedCache:
+class _Fixed:
+    """Attributes that are set once. The C structs hold the tensors' addresses:
+    another tensor in a tensor's place would not reach the device, and the old
+    one's memory could be given away under the kernels' writes."""
+
+    def __setattr__(self, name, value):
+        if name in self.__dict__:
+            raise AttributeError(f"{type(self).__name__}.{name} cannot be replaced: write into the "
+                                 "tensor, or make another object")
+        self.__dict__[name] = value
+
+    def __delattr__(self, name):
+        raise AttributeError(f"{type(self).__name__}.{name} cannot be deleted")
+
+
+class PagedCache(_Fixed):
     """keys and values [n_layers, n_pages, n_kv_heads, page_size, head_dim]."""
 
     def __init__(self, keys, values):
@@ -119,11 +134,12 @@ class PagedCache:
                    torch.empty(shape, dtype=dtype, device=device))
 
 
-class PagedBatch:
+class PagedBatch(_Fixed):
     """The device arrays of a batch (mlq_paged_batch): block_table int32
     [n_seqs, max_pages], lengths int32 [n_seqs], row_start int32 [n_seqs + 1]
     (None for a decode batch whose row i is sequence i), and for plan():
-    positions int32 and slots int64 [max_rows], status int32 [1]."""
+    positions int32 and slots int64 [max_rows], status int32 [1]. What they hold
+    may change, the tensors themselves are the batch's for good."""
 
     def __init__(self, block_table, lengths, row_start=None, positions=None, slots=None,
                  status=None):
@@ -213,7 +229,7 @@ def rope_frequencies(theta: float, rot_dim: int, scaling: str = "none", factor: 
     return freqs, magnitude.value
 
 
-class Rotary:
+class Rotary(_Fixed):
     """What a model does to each query and key head (mlq_rotary): freqs, a
     float64 device tensor [rot_dim / 2] of radians per position (None: no
     rotation), and the float32 norm weights [head_dim] of queries and keys."""
@@ -282,7 +298,7 @@ def qk_norm_rope(rotary: Rotary, q, k, v, positions, q_out=None, k_out=None, cac
     return q_out, k_out
 
 
-class AttentionRule:
+class AttentionRule(_Fixed):
     """How scores enter the softmax (mlq_attention_rule): scale (None:
     1 / sqrt(head_dim)), softcap, window and slopes, a float32 device tensor
     [n_heads] of biases per token of distance."""

@@ -898,3 +898,21 @@ def test_decode_of_many_short_pieces_in_a_workspace_of_the_longest_bound(paged, 
     torch.cuda.synchronize()
     p.compare(out, p.want(rows={0, 1, 2} | set(range(3, p.rows, 4))))
     assert torch.equal(out, again)
+
+
+def test_tensors_of_a_batch_and_a_cache_are_not_replaced(paged):
+    """Their contents change in place; another tensor in a tensor's place is refused."""
+    import torch
+    p = Problem(paged, "bf16", [40, 90], 8, 2, 64, 16, seed=65)
+    for obj, names in ((p.batch, ("block_table", "lengths", "row_start", "positions", "max_rows", "n_seqs")),
+                       (p.cache, ("keys", "values", "n_pages"))):
+        for name in names:
+            was = getattr(obj, name)
+            with pytest.raises(AttributeError):
+                setattr(obj, name, torch.zeros(2, dtype=torch.int32, device="cuda"))
+            assert getattr(obj, name) is was
+    p.lengths = np.array([33, 71])
+    p.batch.lengths.copy_(dev(p.lengths.astype(np.int32)))
+    out = paged.attention_decode(p.cache, 0, p.batch, p.qd)
+    torch.cuda.synchronize()
+    p.compare(out, p.want())

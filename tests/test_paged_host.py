@@ -265,3 +265,24 @@ def test_a_decode_workspace_serves_every_smaller_bound(pkg, heads, kv, hd, seqs,
         assert lib.mlq_paged_attention_workspace(ctypes.byref(c), heads, seqs, 0, max_len, ctypes.byref(n)) == OK
         sizes.append(n.value)
     assert sizes == sorted(sizes)
+
+
+def test_handles_keep_what_they_were_made_of(pkg):
+    """Their addresses are taken once: another tensor in a tensor's place is refused, not passed by."""
+    import torch
+    from mini_llama_amd import paged
+    rule, rotary = paged.AttentionRule(window=7), paged.Rotary(64)
+    for obj, names in ((rule, ("slopes", "struct", "ref")), (rotary, ("head_dim", "rot_dim", "struct"))):
+        for name in names:
+            was = getattr(obj, name)
+            with pytest.raises(AttributeError):
+                setattr(obj, name, torch.zeros(4))
+            with pytest.raises(AttributeError):
+                delattr(obj, name)
+            assert getattr(obj, name) is was
+    for cls in (paged.PagedCache, paged.PagedBatch):  # (made of device tensors only)
+        obj = object.__new__(cls)
+        obj.lengths = 1
+        with pytest.raises(AttributeError):
+            obj.lengths = 2
+        assert obj.lengths == 1
