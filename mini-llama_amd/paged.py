@@ -58,6 +58,13 @@ def _elsewhere(call, index: int, stream):
         return call()
 
 
+def _int32(name: str, value) -> int:
+    """value, if a C int holds it (ctypes keeps the low 32 bits of any other)."""
+    if not -(1 << 31) <= value < 1 << 31:
+        raise ValueError(f"{name} does not fit 32 bits")
+    return value
+
+
 def _ints(name: str, t, dtype, index: int, n=None, least: int = 0):
     """Address of a contiguous 1-D device tensor of that type with n elements
     (or at least `least`)."""
@@ -206,9 +213,10 @@ def plan(batch: PagedBatch, lengths, n_new, free_pages, n_free, page_size: int, 
        batch.status is None:
         raise ValueError("plan needs a batch with row_start, positions, slots and status")
     height = _ints("n_free", n_free, _I32, index, 1)
+    stack = _ints("free_pages", free_pages, _I32, index)
     _check(lib().mlq_paged_plan(
-        batch.ref, page_size, free_pages.shape[0], _ints("lengths", lengths, _I32, index, n),
-        _ints("n_new", n_new, _I32, index, n), _ints("free_pages", free_pages, _I32, index), height,
+        batch.ref, _int32("page_size", page_size), _int32("the size of free_pages", free_pages.shape[0]),
+        _ints("lengths", lengths, _I32, index, n), _ints("n_new", n_new, _I32, index, n), stack, height,
         height if n_free_out is None else _ints("n_free_out", n_free_out, _I32, index, 1),
         _raw_stream(index)), "mlq_paged_plan")
 
@@ -220,7 +228,8 @@ def rope_frequencies(theta: float, rot_dim: int, scaling: str = "none", factor: 
     (YaRN)."""
     if scaling not in SCALINGS:
         raise ValueError(f"scaling must be one of {sorted(SCALINGS)}")
-    freqs = np.zeros(max(rot_dim // 2, 1), np.float64)
+    _int32("original_len", original_len)
+    freqs = np.zeros(max(_int32("rot_dim", rot_dim) // 2, 1), np.float64)
     magnitude = ctypes.c_float()
     _check(lib().mlq_rope_frequencies(theta, rot_dim, SCALINGS[scaling], factor, original_len,
                                       beta_fast, beta_slow,
@@ -244,6 +253,7 @@ class Rotary(_Fixed):
                (name != "freqs" and t.shape[0] != head_dim):
                 raise ValueError(f"{name} must be a contiguous {dtype} device vector" +
                                  ("" if name == "freqs" else f" of {head_dim}"))
+        _int32("rope_type", rope_type)
         given = [t for t in (freqs, q_norm, k_norm) if t is not None]
         if len({t.device for t in given}) > 1:
             raise ValueError("freqs and norms must be on one device")
@@ -281,6 +291,7 @@ def qk_norm_rope(rotary: Rotary, q, k, v, positions, q_out=None, k_out=None, cac
     if cache is not None:
         if cache.index != index or v is None or slots is None:
             raise ValueError("v and slots, on the cache's device, are needed")
+        _int32("layer", layer)
         vp, vs = _rows("v", v, n, kv, hd, index)
         sp, cp = _ints("slots", slots, _I64, index, None, n), cache.ref
     elif k_out is None:
@@ -305,8 +316,10 @@ class AttentionRule(_Fixed):
 
     def __init__(self, scale: float | None = None, softcap: float = 0.0, window: int = 0,
                  slopes=None):
-        if scale == 0.0:
-            raise ValueError("a scale of 0 would weigh every key alike")
+        if scale is not None and ctypes.c_float(scale).value == 0.0:
+            raise ValueError("a scale of 0 (in float32) would weigh every key alike")
+        if softcap != 0.0 and ctypes.c_float(softcap).value == 0.0:
+            raise ValueError("a softcap that is 0 in float32 would be none")
         if not 0 <= window < 1 << 31:
             raise ValueError("a window is a number of keys below 2^31 (0: none)")
         if slopes is not None and (slopes.dtype != torch.float32 or not slopes.is_cuda or
@@ -325,8 +338,8 @@ def attention_workspace_bytes(cache: PagedCache, n_heads: int, n_seqs: int, max_
     key = (n_heads, n_seqs, rows, max_len)
     need = cache._workspaces.get(key)
     if need is None:
-        if max(key) >= 1 << 31:  # (a C int would hold another number)
-            raise ValueError("more heads, sequences, rows or tokens than 2^31")
+        for name, value in zip(("n_heads", "n_seqs", "rows", "max_len"), key):
+            _int32(name, value)
         nbytes = ctypes.c_size_t()
         _check(lib().mlq_paged_attention_workspace(cache.ref, n_heads, n_seqs, rows, max_len,
                                                    ctypes.byref(nbytes)),
@@ -347,19 +360,19 @@ def _workspace(cache, workspace, n_heads: int, n_seqs: int, max_len: int, rows: 
             return None, None, 0
         workspace = torch.empty(size, dtype=torch.uint8, device=cache.device)
         return workspace, workspace.data_ptr(), size
-    if max_len >= 1 << 31:
-        raise ValueError("max_len is below 2^31")
+    _int32("max_len", max_len)
     if workspace.get_device() != cache.index or not workspace.is_contiguous():
         raise ValueError("the workspace must be a contiguous tensor on the cache's device")
     return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
-def _attention_args(cache, batch, q, out, rule):
+def _attention_args(cache, layer, batch, q, out, rule):
     """(heads, q's address and stride, out, its address and stride, the rule's
     reference), checked."""
     index, hd = cache.index, cache.head_dim
     if batch.index != index:
         raise ValueError("the batch must be on the cache's device")
+    _int32("layer", layer)
     qp, qs = _rows("q", q, None, None, hd, index)
     n, heads = q.shape[:2]
     ref = None
@@ -387,7 +400,7 @@ def attention_decode(cache: PagedCache, layer: int, batch: PagedBatch, q, out=No
     if stream is not None or index != _current_device():
         return _elsewhere(lambda: attention_decode(cache, layer, batch, q, out, rule, max_len,
                                                    workspace), index, stream)
-    heads, qp, qs, out, op, os, ref = _attention_args(cache, batch, q, out, rule)
+    heads, qp, qs, out, op, os, ref = _attention_args(cache, layer, batch, q, out, rule)
     n = q.shape[0]
     if batch.row_start is None and n < batch.n_seqs:
         raise ValueError("a row for each sequence is needed")
@@ -412,7 +425,7 @@ def attention_prefill(cache: PagedCache, layer: int, batch: PagedBatch, q, out=N
     if stream is not None or index != _current_device():
         return _elsewhere(lambda: attention_prefill(cache, layer, batch, q, out, rule, max_len,
                                                     workspace), index, stream)
-    heads, qp, qs, out, op, os, ref = _attention_args(cache, batch, q, out, rule)
+    heads, qp, qs, out, op, os, ref = _attention_args(cache, layer, batch, q, out, rule)
     if batch.row_start is None:
         raise ValueError("attention_prefill needs a batch with row_start")
     n = q.shape[0]

@@ -916,3 +916,24 @@ def test_tensors_of_a_batch_and_a_cache_are_not_replaced(paged):
     out = paged.attention_decode(p.cache, 0, p.batch, p.qd)
     torch.cuda.synchronize()
     p.compare(out, p.want())
+
+
+def test_a_layer_or_page_size_past_32_bits_is_refused(pkg, paged):
+    """(ctypes would pass the low 32 bits: layer 0, pages of 16)"""
+    import torch
+    p = Problem(paged, "bf16", [40, 90], 8, 2, 64, 16, seed=67)
+    at = torch.zeros(2, dtype=torch.int32, device="cuda")
+    rotary, v = paged.Rotary(64), torch.zeros((2, 2, 64), device="cuda")
+    calls = [lambda n: paged.attention_decode(p.cache, n, p.batch, p.qd), lambda n: paged.attention_prefill(p.cache, n, p.batch, p.qd),
+             lambda n: paged.qk_norm_rope(rotary, p.qd, v, v, at, cache=p.cache, layer=n, slots=at.long())]
+    for call in calls:
+        for n in (1 << 32, -1 << 32):
+            with pytest.raises(ValueError):
+                call(n)
+        for n in (1, -1):
+            with pytest.raises(pkg.MLQError):
+                call(n)
+    batch = paged.PagedBatch.empty(2, 4, 8)
+    for n in (16 + (1 << 32), 16 - (1 << 32)):
+        with pytest.raises(ValueError):
+            paged.plan(batch, batch.lengths, at, at, at[:1], n)

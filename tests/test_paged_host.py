@@ -286,3 +286,28 @@ def test_handles_keep_what_they_were_made_of(pkg):
         with pytest.raises(AttributeError):
             obj.lengths = 2
         assert obj.lengths == 1
+
+
+def test_numbers_that_a_c_type_would_hold_as_others(pkg):
+    """A float that fp32 rounds to 0 is another rule, an int past 32 bits another number."""
+    from types import SimpleNamespace
+
+    from mini_llama_amd import paged
+    for kw in (dict(scale=1e-60), dict(scale=-1e-60), dict(softcap=1e-60), dict(softcap=-1e-60)):
+        with pytest.raises(ValueError):
+            paged.AttentionRule(**kw)
+    assert paged.AttentionRule(scale=1e-30, softcap=0.0).struct.scale == np.float32(1e-30)
+    wrap = 1 << 32
+    for kw in (dict(rot_dim=wrap + 8), dict(rot_dim=8 - wrap), dict(original_len=wrap + 4096), dict(original_len=4096 - wrap)):
+        with pytest.raises(ValueError):
+            paged.rope_frequencies(**{**dict(theta=1e4, rot_dim=8, scaling="parts", factor=2.0, original_len=4096), **kw})
+    for rope_type in (wrap, wrap + 1, -wrap):
+        with pytest.raises(ValueError):
+            paged.Rotary(64, rope_type=rope_type)
+    c = SimpleNamespace(ref=ctypes.byref(cache(pkg)), _workspaces={})
+    for n in (wrap + 100, 100 - wrap):
+        for args in ((28, 1, n, 0), (28, n, 100, 0), (28, 1, 100, n), (n, 1, 100, 0)):
+            with pytest.raises(ValueError):
+                paged.attention_workspace_bytes(c, *args)
+        with pytest.raises(ValueError):
+            paged._workspace(c, object(), 28, 1, n, 0)
