@@ -608,7 +608,7 @@ int mlq_qk_norm_rope(const mlq_rotary* r, int rows, const int32_t* positions, in
  * call are not read: a caller may have given such pages to others. */
 typedef struct mlq_attention_rule {
   float scale;                       /* 0: 1 / sqrt(head_dim) */
-  float softcap;                     /* 0: none */
+  float softcap;                     /* 0: none; scale / softcap is finite */
   int32_t window;                    /* 0: none */
   const float* slopes;               /* [n_heads] (device) or NULL */
 } mlq_attention_rule;

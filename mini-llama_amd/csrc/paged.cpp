@@ -82,6 +82,9 @@ int check_attention(const mlq_paged_cache* c, int layer, const mlq_paged_batch* 
   const mlq_attention_rule& r = rule != nullptr ? *rule : none;
   if (!std::isfinite(r.scale) || !std::isfinite(r.softcap) || r.softcap < 0.0f || r.window < 0)
     return MLQ_ERR_INVALID_ARG;
+  const float scale = r.scale != 0.0f ? r.scale : sqrtf(1.0f / (float)c->head_dim);
+  // (scores are multiplied by this, and 0 * inf is not 0)
+  if (r.softcap > 0.0f && !std::isfinite(scale / r.softcap)) return MLQ_ERR_INVALID_ARG;
   *a = {};
   a->keys = (const char*)c->keys + layer * layer_bytes(c);
   a->values = (const char*)c->values + layer * layer_bytes(c);
@@ -101,7 +104,7 @@ int check_attention(const mlq_paged_cache* c, int layer, const mlq_paged_batch* 
   a->out = out != nullptr ? const_cast<float*>(out) : nullptr;
   a->q_stride = q_stride;
   a->out_stride = out_stride;
-  a->scale = r.scale != 0.0f ? r.scale : sqrtf(1.0f / (float)c->head_dim);
+  a->scale = scale;
   a->softcap = r.softcap;
   a->window = r.window;
   a->slopes = r.slopes;

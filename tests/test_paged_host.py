@@ -311,3 +311,14 @@ def test_numbers_that_a_c_type_would_hold_as_others(pkg):
                 paged.attention_workspace_bytes(c, *args)
         with pytest.raises(ValueError):
             paged._workspace(c, object(), 28, 1, n, 0)
+
+
+def test_a_cap_that_no_score_can_be_divided_by(pkg):
+    """scale / softcap past fp32 would make a score of 0 NaN."""
+    n = ctypes.c_size_t()
+    c, b = cache(pkg), batch(pkg)
+    for call in (pkg.lib().mlq_paged_attention_decode, pkg.lib().mlq_paged_attention_prefill):
+        for scale, cap in ((0.0, 1e-42), (1e30, 1e-10), (-1e30, 1e-10)):
+            rule = pkg.MlqAttentionRule(scale, cap, 0, None)
+            assert call(ctypes.byref(c), 0, ctypes.byref(b), ctypes.byref(rule), 28, FAKE, 3584, FAKE + 4096, 3584, 0, FAKE, 1 << 40,
+                        None) == ARG, (scale, cap)  # (max_len 0: nothing is launched if the rule passes)
