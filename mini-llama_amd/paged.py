@@ -420,7 +420,8 @@ def attention_prefill(cache: PagedCache, layer: int, batch: PagedBatch, q, out=N
     """out [rows, n_heads, head_dim]: causal attention of every new row of
     every sequence over its pages (mlq_paged_attention_prefill). max_len and
     workspace as in attention_decode, the workspace of
-    attention_workspace_bytes(..., rows=q.shape[0])."""
+    attention_workspace_bytes(..., rows) for the rows that q has, or the batch
+    if it holds fewer (batch.max_rows)."""
     index = cache.index
     if stream is not None or index != _current_device():
         return _elsewhere(lambda: attention_prefill(cache, layer, batch, q, out, rule, max_len,

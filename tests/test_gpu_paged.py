@@ -937,3 +937,19 @@ def test_a_layer_or_page_size_past_32_bits_is_refused(pkg, paged):
     for n in (16 + (1 << 32), 16 - (1 << 32)):
         with pytest.raises(ValueError):
             paged.plan(batch, batch.lengths, at, at, at[:1], n)
+
+
+def test_prefill_workspace_of_a_batch_that_holds_fewer_rows_than_q(paged):
+    """The rows that count are the batch's: few of them share their keys, whatever q is padded to."""
+    import torch
+    p = Problem(paged, "bf16", [3000, 900], 8, 2, 64, 16, seed=69, new=[5, 3])
+    rows = torch.full((8,), -1, dtype=torch.int32, device="cuda")
+    p.batch = paged.PagedBatch(p.batch.block_table, p.batch.lengths, p.batch.row_start, rows, rows.long())
+    q = torch.cat([p.qd, torch.zeros((9000, 8, 64), device="cuda")])
+    bound = p.batch.max_pages * 16
+    need = [paged.attention_workspace_bytes(p.cache, 8, 2, bound, rows=n) for n in (p.batch.max_rows, q.shape[0])]
+    assert need[0] > need[1] == 0  # (so many rows would fill the chip)
+    out = paged.attention_prefill(p.cache, 0, p.batch, q, workspace=torch.empty(need[0], dtype=torch.uint8, device="cuda"))
+    torch.cuda.synchronize()
+    p.compare(out, p.want())
+    assert torch.all(out[p.rows:] == 0.0)
