@@ -646,7 +646,10 @@ int mlq_paged_attention_decode(const mlq_paged_cache* c, int layer, const mlq_pa
  * and sees the keys up to it. Same rule, layouts, checks and workspace
  * contract. b->max_rows bounds row_start[n_seqs] (rows past it are not
  * computed). (max_rows * n_heads / n_kv_heads / 128 + n_seqs) * n_kv_heads is
- * less than 2^24 (MLQ_ERR_UNSUPPORTED otherwise). */
+ * less than 2^24 (MLQ_ERR_UNSUPPORTED otherwise). Where a row sees values that
+ * are not finite, the 128 rows x heads around it take three times as long;
+ * where it sees a page outside the cache they are computed one by one (0.2 ms
+ * become 40 for 1000 rows behind 1000 tokens). */
 int mlq_paged_attention_prefill(const mlq_paged_cache* c, int layer, const mlq_paged_batch* b,
                                 const mlq_attention_rule* rule, int n_heads, const float* q,
                                 int64_t q_stride, float* out, int64_t out_stride, int max_len,

@@ -16,8 +16,8 @@ namespace {
 
 // One row of one query head by one wave, in plain fp32: a lane scores a key of
 // a tile of 64 against q in LDS, then takes head dims lane, lane + 64, .. of
-// the output. What the matrix kernels hand to it: rows that could see a value
-// or page that those do not carry. Writes dims d0 .. d1 - 1; `lds`: kSlowFloats
+// the output. What the prefill kernels hand to it: rows that could see a page
+// outside the cache, or that overflow the parts alone. Writes dims d0 .. d1 - 1; `lds`: kSlowFloats
 // of the wave's own.
 constexpr int kSlowFloats = 256 + 64 + 128;
 template <typename T>
@@ -746,8 +746,13 @@ void decode_launch_hd(const PagedAttnArgs& a, int grid, hipStream_t stream) {
 //    during the products, and the page that the one after it lies in is asked
 //    for before that (a load that waits for its page waits twice).
 //  - Infinities and NaN, also those that a weight of 0 was to silence, end up in
-//    the output: such columns, and those of a workgroup that met a page outside
-//    the cache, go to slow_row.
+//    the output: the workgroup computes such columns again with values that are
+//    not finite as 0, and once more with their places as 1 and every seen key's
+//    weight as 1: NaN where the sum is positive.
+//    (2000 rows of 6 sequences, 32 heads on 8 of 128, bf16, one infinite value
+//    in a kv head of one: 0.49 ms, 0.16 without that value, 37.8 with such
+//    columns in slow_row.) What met a page outside the cache goes to slow_row,
+//    a wave for a row and head.
 //  - Tiles with the most keys start first (6 sequences, 8000 rows behind up to
 //    2000 tokens, 32 heads on 8 of 128, bf16: 565 -> 552 us); where the tiles
 //    leave CUs idle, several workgroups share a tile's keys (64 rows of 16
@@ -951,10 +956,36 @@ __device__ __forceinline__ PrePartial prefill_partial(const PagedAttnArgs& a, in
   return {p, p + kPreCols, p + 2 * kPreCols};
 }
 
+// A word of values for the passes after the first: those that are not finite as
+// 0; or, to count them, as 1 and the others as 0.
+template <typename T>
+__device__ __forceinline__ uint32_t settled(uint32_t w, bool count) {
+  constexpr bool F32 = sizeof(T) == 4, F16 = std::is_same<T, _Float16>::value;
+  constexpr uint32_t kExp = F32 ? 0x7f800000u : F16 ? 0x7c00u : 0x7f80u, kOne = F32 ? 0x3f800000u : F16 ? 0x3c00u : 0x3f80u;
+  if constexpr (F32) {
+    const bool bad = (w & kExp) == kExp;
+    return count ? (bad ? kOne : 0u) : (bad ? 0u : w);
+  }
+  const bool lo = (w & kExp) == kExp, hi = (w >> 16 & kExp) == kExp;
+  if (count) return (lo ? kOne : 0u) | (hi ? kOne << 16 : 0u);
+  return w & ((lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u));
+}
+template <typename T>
+__device__ __forceinline__ bool not_finite(uint32_t w) {
+  return settled<T>(w, true) != 0;
+}
+
+// One pass of a workgroup over its keys. The first writes the columns (or their
+// partials) that are finite and returns the others; AGAIN, for those: `count` 0
+// with values that are not finite as 0, 1 to mark where they are seen.
 // RULE: scores are capped or biased (a variant of its own: its values spill
 // beside the others').
-template <typename T, int HD, bool FULL, bool RULE>
-__global__ __launch_bounds__(kPreThreads, HD <= 128 ? 2 : 1) void paged_prefill_kernel(PagedAttnArgs a) {
+struct PreDirty {
+  bool column, any;  // this lane's, any of the workgroup
+};
+template <typename T, int HD, bool FULL, bool RULE, bool AGAIN>
+__device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const PreSpan& sp, int seq, PreLds<T, HD>& lds,
+                                                 bool dirty, bool count) {
   using Tr = PreTraits<T>;
   using M = typename Tr::mat;
   using vec = typename Tr::vec;
@@ -966,28 +997,16 @@ __global__ __launch_bounds__(kPreThreads, HD <= 128 ? 2 : 1) void paged_prefill_
   constexpr int VDT = HD / 32;       // dims of V per thread, of 4 keys
   constexpr int VWT = VDT * (int)sizeof(T) / 4;     // their words a key (fp16 / bf16, HD 64: 1)
   constexpr float kSlack = Tr::kLift == 0.0f ? 8.0f : 0.0f;
-  extern __shared__ __align__(16) uint8_t pre_smem[];
-  PreLds<T, HD>& lds = *(PreLds<T, HD>*)pre_smem;
   constexpr int BUF = PreLds<T, HD>::kBuf, QL = PreLds<T, HD>::kQ;
   int* const count_lds = lds.count;
-  const int tid = threadIdx.x, lane = tid & 63;
+  int tid = threadIdx.x;
+  if constexpr (AGAIN) asm volatile("" : "+v"(tid));  // (no lane's numbers are kept for it from the first pass)
+  const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int G = a.group;
-  const int kvh = blockIdx.x % a.n_kv;
-  const PreWork work = a.n_seqs <= kPreSorted ? longest_first(a, (int)(blockIdx.x / a.n_kv))
-                                              : by_row(a, (int)(blockIdx.x / a.n_kv), count_lds);
-  const PreSpan sp = prefill_span(a, work);
-  const int seq = work.seq, split = blockIdx.y;
-  if (split == 0 && a.part != nullptr && tid == 0) {
-    const int j = (int)(sp.c0 / G);
-    const bool join = sp.live && sp.len <= a.max_len && sp.tiles > sp.each;
-    ((PreJoin*)a.part)[blockIdx.x] = {join ? (sp.tiles + sp.each - 1) / sp.each : 0,
-                                      (int)min((int64_t)kPreCols, sp.pairs - sp.c0), seq, sp.row0 + j, sp.pos0 + j,
-                                      (int)(sp.c0 - (int64_t)j * G)};
-  }
-  if (!sp.live) return;
-  const int row0 = sp.row0, pos0 = sp.pos0, len = sp.len;
+  const int kvh = blockIdx.x % a.n_kv, split = blockIdx.y;
+  const int row0 = sp.row0, pos0 = sp.pos0;
   const int64_t pairs = sp.pairs, c0 = sp.c0;
   // this lane's column
   const int64_t cc = c0 + wave * 32 + col;
@@ -1001,22 +1020,12 @@ __global__ __launch_bounds__(kPreThreads, HD <= 128 ? 2 : 1) void paged_prefill_
   const int kmax = min(sp.kmax, key0 + sp.each * kPreKeys - 1);
   const int wave_first = __builtin_amdgcn_readfirstlane(__shfl(qpos, 0));
   const int wave_last = __builtin_amdgcn_readfirstlane(__shfl(qpos, 63));
-  if (len > a.max_len || sp.kmax < 0) {  // (kmax < 0: nothing to see)
-    if (live && split == 0)
-      for (int d = 4 * half; d < a.hd; d += 8) {
-        const float x = len > a.max_len ? __builtin_nanf("") : 0.0f;
-        *(f4*)(out + d) = f4{x, x, x, x};
-      }
-    return;
-  }
-
-  if (key0 > kmax) return;
-
   // ---- q
   int q_exp = 0;
   vec q[NP][KT];
-  bool odd = false;  // a page outside the cache
-  bool cut = false;  // this column is written already
+  bool odd = false;    // a page outside the cache
+  bool k_bad = false;  // AGAIN: a key that is not finite
+  float q_zero = 0.0f;  // AGAIN: NaN where q is not finite
   {
     const float* qp = a.q + row * a.q_stride + (int64_t)head * a.hd + 8 * half;
     auto q_at = [&](int s, int u) __attribute__((always_inline)) {
@@ -1043,6 +1052,7 @@ __global__ __launch_bounds__(kPreThreads, HD <= 128 ? 2 : 1) void paged_prefill_
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         f4 x = q_at(s, u) * turned;
+        if constexpr (AGAIN) q_zero += (x.x * 0.0f + x.y * 0.0f) + (x.z * 0.0f + x.w * 0.0f);
         if constexpr (Tr::kLift != 0.0f)
           x = f4{ldexp_f(x.x, q_exp), ldexp_f(x.y, q_exp), ldexp_f(x.z, q_exp), ldexp_f(x.w, q_exp)};
 #pragma unroll
@@ -1118,7 +1128,12 @@ __global__ __launch_bounds__(kPreThreads, HD <= 128 ? 2 : 1) void paged_prefill_
       }
     }
   };
-  auto put_k = [&](PreTile<T, HD>& tl) __attribute__((always_inline)) {
+  auto put_k = [&](PreTile<T, HD>& tl, int k0) __attribute__((always_inline)) {
+    if constexpr (AGAIN)
+      if (k0 + kkey <= kmax) {
+#pragma unroll
+        for (int w = 0; w < KW; ++w) k_bad |= not_finite<T>(kw[w]);
+      }
     if constexpr (F32) {
 #pragma unroll
       for (int w = 0; w < KW; w += 4) {
@@ -1142,6 +1157,12 @@ __global__ __launch_bounds__(kPreThreads, HD <= 128 ? 2 : 1) void paged_prefill_
 #pragma unroll
           for (int w = 0; w < VWT; ++w) vw[e][w] = 0;
         }
+    }
+    if constexpr (AGAIN) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int w = 0; w < VWT; ++w) vw[e][w] = settled<T>(vw[e][w], count);
     }
     // the key group's slots in its run of 16: keys 0-3, 8-11 | 4-7, 12-15
     const int unit = 2 * (vkg >> 2) + (vkg & 1), sub = 4 * ((vkg >> 1) & 1);
@@ -1177,7 +1198,7 @@ __global__ __launch_bounds__(kPreThreads, HD <= 128 ? 2 : 1) void paged_prefill_
   };
   if constexpr (BUF == 2) {
     load_v(run);
-    put_k(lds.tile[0]);
+    put_k(lds.tile[0], k0);
     put_v(lds.tile[0], k0);
     __syncthreads();
   }
@@ -1191,7 +1212,7 @@ __global__ __launch_bounds__(kPreThreads, HD <= 128 ? 2 : 1) void paged_prefill_
         load_v(run);
       }
     } else {
-      put_k(tl);  // (the last tile's K is done with since its second barrier)
+      put_k(tl, k0);  // (the last tile's K is done with since its second barrier)
       load_v(run);
       __syncthreads();
     }
@@ -1238,6 +1259,15 @@ __global__ __launch_bounds__(kPreThreads, HD <= 128 ? 2 : 1) void paged_prefill_
         if (k > qpos || (a.window > 0 && k <= qpos - a.window)) s[i] = -INFINITY;
       }
     }
+    if constexpr (AGAIN)
+      if (count) {  // every key that is seen weighs the same
+        sl = 1.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int k = k0 + 8 * (i >> 2) + 4 * half + (i & 3);
+          s[i] = k > qpos || (a.window > 0 && k <= qpos - a.window) ? -INFINITY : 0.0f;
+        }
+      }
     float mx = s[0];
 #pragma unroll
     for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
@@ -1291,78 +1321,156 @@ __global__ __launch_bounds__(kPreThreads, HD <= 128 ? 2 : 1) void paged_prefill_
       }
     if constexpr (BUF == 2) {
       if (more) {
-        put_k(lds.tile[cur ^ 1]);
+        put_k(lds.tile[cur ^ 1], k0 + kPreKeys);
         put_v(lds.tile[cur ^ 1], k0 + kPreKeys);
         __syncthreads();
       }
     }
   }
+  // (without this the loop copies acc once a tile, for what follows)
+#pragma unroll
+  for (int b = 0; b < VB; ++b) asm volatile("" : "+v"(acc[b]));
   const float sum = xor32_sum(l);
+  const int at = wave * 32 + col;
+  PrePartial pp = {};
+  if (parts) pp = prefill_partial(a, split);
+  if (AGAIN && count) {  // NaN where a value that is not finite is seen
+#pragma unroll
+    for (int b = 0; b < VB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int d = 32 * b + 8 * (i >> 2) + 4 * half + (i & 3);
+        if (dirty && (FULL || d < a.hd) && acc[b][i] > 0.0f)
+          *(parts ? pp.acc + ((size_t)(d >> 2) * kPreCols + at) * 4 + (d & 3) : out + d) = __builtin_nanf("");
+      }
+    return {};
+  }
+  float zeros = sum * 0.0f;
+#pragma unroll
+  for (int b = 0; b < VB; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) zeros = __builtin_fmaf(acc[b][i], 0.0f, zeros);
+  const bool odd_column = live && !(xor32_sum(zeros) == 0.0f);
+  // (the waves tell each other: 1 a page outside the cache, 2 a key that is not
+  // finite, 4 a column that is not)
+  const int mine = (__any(odd) ? 1 : 0) | (__any(k_bad) ? 2 : 0) | (__any(odd_column) ? 4 : 0);
+  __syncthreads();  // every wave is done with the tile
+  if (lane == 0) count_lds[wave] = mine;
+  __syncthreads();
+  const int all = __builtin_amdgcn_readfirstlane(count_lds[0] | count_lds[1] | count_lds[2] | count_lds[3]);
+  bool write = live, slow = false;
+  if constexpr (AGAIN) {
+    // What no key or query explains is an overflow of the parts, which plain
+    // fp32 may not share.
+    slow = dirty && ((all & 1) != 0 || (odd_column && (all & 2) == 0 && xor32_sum(q_zero) == 0.0f));
+    write = dirty && !slow;
+  } else {
+    dirty = live && (odd_column || (all & 1) != 0);
+    write = live && !dirty;
+  }
   if (parts) {
-    // (a page outside the cache shows up as a NaN sum in the join)
-    if (lane == 0) count_lds[wave] = 0;
-    __syncthreads();
-    if (__any(odd) && lane == 0) count_lds[wave] = 1;
-    __syncthreads();
-    const bool outside = (count_lds[0] | count_lds[1] | count_lds[2] | count_lds[3]) != 0;
-    const PrePartial pp = prefill_partial(a, split);
-    const int at = wave * 32 + col;
-    if (half == 0) {
-      pp.m[at] = m;
-      pp.l[at] = outside ? __builtin_nanf("") : sum;
+    // (a maximum of NaN: the join computes the column in plain fp32)
+    if (half == 0 && (write || slow)) {
+      pp.m[at] = slow ? __builtin_nanf("") : m;
+      pp.l[at] = sum;
     }
+    if (write) {
+#pragma unroll
+      for (int b = 0; b < VB; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int d = 32 * b + 8 * i + 4 * half;
+          if (FULL || d < a.hd)
+            *(f4*)(pp.acc + ((size_t)(d >> 2) * kPreCols + at) * 4) =
+                f4{acc[b][4 * i], acc[b][4 * i + 1], acc[b][4 * i + 2], acc[b][4 * i + 3]};
+        }
+    }
+    return {dirty, all != 0};
+  }
+  if constexpr (AGAIN) {
+    uint64_t redo = __ballot(slow);
+    redo = (redo | redo >> 32) & 0xffffffffu;
+    while (redo != 0) {
+      const int c = __builtin_ctzll(redo);
+      redo &= redo - 1;
+      const int64_t p = c0 + wave * 32 + c;
+      const int j = (int)(p / G);
+      slow_row<T>(a, seq, row0 + j, pos0 + j, kvh * G + (int)(p - (int64_t)j * G), (float*)&lds + wave * kSlowFloats, 0, a.hd);
+    }
+  }
+  if (write) {
+    const float f = qpos < 0 ? 1.0f : sum;  // (a row before the first key: zeros)
 #pragma unroll
     for (int b = 0; b < VB; ++b)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int d = 32 * b + 8 * i + 4 * half;
         if (FULL || d < a.hd)
-          *(f4*)(pp.acc + ((size_t)(d >> 2) * kPreCols + at) * 4) =
-              f4{acc[b][4 * i], acc[b][4 * i + 1], acc[b][4 * i + 2], acc[b][4 * i + 3]};
+          *(f4*)(out + d) = f4{acc[b][4 * i] / f, acc[b][4 * i + 1] / f, acc[b][4 * i + 2] / f, acc[b][4 * i + 3] / f};
       }
+  }
+  return {dirty, all != 0};
+}
+
+// The tile of rows that a workgroup takes.
+struct PreTask {
+  int seq;
+  PreSpan span;
+};
+__device__ __forceinline__ PreTask prefill_task(const PagedAttnArgs& a, int x, int* lds) {
+  const PreWork work = a.n_seqs <= kPreSorted ? longest_first(a, x / a.n_kv) : by_row(a, x / a.n_kv, lds);
+  return {work.seq, prefill_span(a, work)};
+}
+
+template <typename T, int HD, bool FULL, bool RULE>
+__global__ __launch_bounds__(kPreThreads, HD <= 128 ? 2 : 1) void paged_prefill_kernel(PagedAttnArgs a) {
+  extern __shared__ __align__(16) uint8_t pre_smem[];
+  PreLds<T, HD>& lds = *(PreLds<T, HD>*)pre_smem;
+  const int tid = threadIdx.x, G = a.group, kvh = blockIdx.x % a.n_kv, split = blockIdx.y;
+  const PreTask task = prefill_task(a, (int)blockIdx.x, lds.count);
+  const PreSpan& sp = task.span;
+  if (split == 0 && a.part != nullptr && tid == 0) {
+    const int j = (int)(sp.c0 / G);
+    const bool join = sp.live && sp.len <= a.max_len && sp.tiles > sp.each;
+    ((PreJoin*)a.part)[blockIdx.x] = {join ? (sp.tiles + sp.each - 1) / sp.each : 0,
+                                      (int)min((int64_t)kPreCols, sp.pairs - sp.c0), task.seq, sp.row0 + j, sp.pos0 + j,
+                                      (int)(sp.c0 - (int64_t)j * G)};
+  }
+  if (!sp.live) return;
+  if (sp.len > a.max_len || sp.kmax < 0) {  // (kmax < 0: nothing to see)
+    const int64_t cc = sp.c0 + (tid >> 1);
+    const int j = (int)(cc / G);
+    if (cc < sp.pairs && split == 0) {
+      float* out = a.out + (sp.row0 + j) * a.out_stride + (int64_t)(kvh * G + (int)(cc - (int64_t)j * G)) * a.hd;
+      const float x = sp.len > a.max_len ? __builtin_nanf("") : 0.0f;
+      for (int d = 4 * (tid & 1); d < a.hd; d += 8) *(f4*)(out + d) = f4{x, x, x, x};
+    }
     return;
   }
-  // Infinities and NaN end up in the output, also those that a weight of 0 was
-  // to silence: columns that hold any, and all of a workgroup that met a page
-  // outside the cache, are computed again.
-  float zeros = sum * 0.0f;
-#pragma unroll
-  for (int b = 0; b < VB; ++b)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) zeros = __builtin_fmaf(acc[b][i], 0.0f, zeros);
-  __syncthreads();  // every wave is done with the tile
-  if (lane == 0) count_lds[wave] = 0;
-  __builtin_amdgcn_wave_barrier();
-  if (__any(odd) && lane == 0) count_lds[wave] = 1;
-  __syncthreads();
-  const bool again = (count_lds[0] | count_lds[1] | count_lds[2] | count_lds[3]) != 0;
-  uint64_t redo = __ballot(live && (again || !(zeros == 0.0f)));
-  redo = (redo | redo >> 32) & 0xffffffffu;
-  while (redo != 0) {
-    const int c = __builtin_ctzll(redo);
-    redo &= redo - 1;
-    const int64_t p = c0 + wave * 32 + c;
-    const int j = (int)(p / G);
-    slow_row<T>(a, seq, row0 + j, pos0 + j, kvh * G + (int)(p - (int64_t)j * G),
-                (float*)pre_smem + wave * kSlowFloats, 0, a.hd);
-    if (c == col) cut = true;
+  if (sp.kfirst + split * sp.each * kPreKeys > sp.kmax) return;
+
+  const PreDirty dirty = prefill_pass<T, HD, FULL, RULE, false>(a, sp, task.seq, lds, false, false);
+  if (__builtin_expect(!dirty.any, 1)) return;
+  // From here on everything but `dirty` is made anew, the arguments read again:
+  // what the compiler keeps for this through the first pass's loop spills there
+  // (8000 rows, 32 heads on 8, bf16: 557 -> 582 us).
+  auto args = (const __attribute__((address_space(4))) PagedAttnArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(args));
+  PagedAttnArgs b;
+  __builtin_memcpy(&b, (const void*)args, sizeof(b));
+  __syncthreads();  // (every wave has read what the waves told each other)
+  const PreTask same = prefill_task(b, (int)blockIdx.x, lds.count);
+#pragma nounroll
+  for (int count = 0; count < 2; ++count) {
+    __syncthreads();  // (every wave is done with the LDS)
+    prefill_pass<T, HD, FULL, RULE, true>(b, same.span, same.seq, lds, dirty.column, count != 0);
   }
-  if (!live || cut) return;
-  const float f = qpos < 0 ? 1.0f : sum;  // (a row before the first key: zeros)
-#pragma unroll
-  for (int b = 0; b < VB; ++b)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int d = 32 * b + 8 * i + 4 * half;
-      if (FULL || d < a.hd)
-        *(f4*)(out + d) = f4{acc[b][4 * i] / f, acc[b][4 * i + 1] / f, acc[b][4 * i + 2] / f, acc[b][4 * i + 3] / f};
-    }
 }
 
 // The splits of a tile of rows and kv head joined: a thread has one column and
 // two quads of dims, a workgroup 32 dims, four splits' loads are asked for at
-// once. Columns that are not finite go to slow_row, as in a workgroup that has
-// all keys.
+// once. Columns that a split marked, and those that overflow only here, go to
+// slow_row.
 constexpr int kPreJoinThreads = 512, kPreJoinDims = 32, kPreMaxSplits = 32, kPreJoinAhead = 4;
 template <typename T>
 __global__ __launch_bounds__(kPreJoinThreads) void paged_prefill_join_kernel(PagedAttnArgs a) {
@@ -1379,6 +1487,7 @@ __global__ __launch_bounds__(kPreJoinThreads) void paged_prefill_join_kernel(Pag
   const PrePartial first = prefill_partial(a, 0);
   const size_t stride = prefill_partial_floats(a.hd);
   float m = -INFINITY, l = 0.0f;
+  bool again = false;
   f4 o[N];
 #pragma unroll
   for (int n = 0; n < N; ++n) o[n] = f4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -1397,7 +1506,10 @@ __global__ __launch_bounds__(kPreJoinThreads) void paged_prefill_join_kernel(Pag
     float mx = m;
 #pragma unroll
     for (int i = 0; i < kPreJoinAhead; ++i)
-      if (i0 + i < info.parts) mx = fmaxf(mx, pm[i]);
+      if (i0 + i < info.parts) {
+        mx = fmaxf(mx, pm[i]);
+        again |= pm[i] != pm[i];
+      }
     const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mx);
     m = mx;
     l *= f;
@@ -1430,7 +1542,19 @@ __global__ __launch_bounds__(kPreJoinThreads) void paged_prefill_join_kernel(Pag
       zeros += (z.x + z.y) + (z.z + z.w);
       if (q0 + kStep * n <= last) *(f4*)(out + 4 * (q0 + kStep * n)) = f4{o[n].x / f, o[n].y / f, o[n].z / f, o[n].w / f};
     }
-    if (!(zeros == 0.0f)) redo[col] = 1;
+    if (!again && !(zeros == 0.0f)) {
+      again = true;
+      for (int i = 0; i < info.parts; ++i) {
+        float given = first.l[i * stride + col] * 0.0f;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          const f4 z = *(const f4*)(first.acc + i * stride + (size_t)min(q0 + kStep * n, last) * (4 * kPreCols) + 4 * col) * 0.0f;
+          given += (z.x + z.y) + (z.z + z.w);
+        }
+        if (!(given == 0.0f)) again = false;
+      }
+    }
+    if (again) redo[col] = 1;
   }
   __syncthreads();
   for (int c = tid >> 6; c < info.cols; c += kPreJoinThreads / 64)

@@ -953,3 +953,47 @@ def test_prefill_workspace_of_a_batch_that_holds_fewer_rows_than_q(paged):
     torch.cuda.synchronize()
     p.compare(out, p.want())
     assert torch.all(out[p.rows:] == 0.0)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,kv,hd,lengths,new", [(8, 2, 64, [400, 90], [400, 30]), (6, 2, 128, [700, 90], [650, 30]), (4, 1, 256, [300, 500], [300, 100]),
+                                                     (12, 4, 80, [3000, 40], [40, 3]), (4, 2, 128, [2500], [60]),
+                                                     (4, 2, 64, [200] + [9] * 300, [200] + [3] * 300)])
+def test_prefill_where_values_are_not_finite(paged, heads, kv, hd, lengths, new, kind):
+    """A value that overflowed early, a channel of infinite values, a last token of NaN, infinite keys: NaN or infinite where
+    they are seen, and the right numbers everywhere else, in one piece and where workgroups share the keys."""
+    import torch
+    n = lengths[0]
+    where = {"early": ("values", [5], 3, math.inf), "late": ("values", [n - 2], 1, -math.inf), "channel": ("values", range(n), 2, math.inf),
+             "middle": ("values", [n // 2, n // 2 + 1, n - 20], 7, math.nan), "token": ("values", [n - 1], slice(None), math.nan),
+             "key": ("keys", [n - 40], 4, math.nan), "far key": ("keys", [n // 3], slice(None), math.inf)}
+    for name, (pool, tokens, dim, value) in where.items():
+        p = Problem(paged, kind, lengths, heads, kv, hd, 16, seed=71, new=new)
+        t = getattr(p.cache, pool)
+        for k in tokens:
+            t[0, int(p.table[0, k // 16]), kv - 1, k % 16, dim] = value
+        clean_k, clean_v = (np.nan_to_num(x, nan=0, posinf=0, neginf=0) for x in (p.k, p.v))
+        p.k, p.v = clean_k, clean_v
+        hurt = np.zeros(hd, bool)
+        hurt[dim] = True
+        if pool == "values":  # (their dims, not the others)
+            for k in tokens:
+                p.v[0, int(p.table[0, k // 16]), kv - 1, k % 16, hurt] = 0
+        for rule in (dict(), dict(window=100, softcap=20.0), dict(window=33)):
+            own, plain = rule_of(paged, heads, **rule)
+            out = paged.attention_prefill(p.cache, 0, p.batch, p.qd, rule=own)
+            torch.cuda.synchronize()
+            out = host(out)
+            rows = set(range(0, p.rows, max(1, p.rows // 60))) | set(range(max(0, p.start[1] - 44), p.rows)) | set(range(12))
+            for r, (y, bound) in p.want(rows=rows, **plain).items():
+                pos = n - (p.start[1] - r) if r < p.start[1] else -1
+                first = max(0, pos + 1 - rule["window"]) if rule else 0
+                sees = any(first <= k <= pos for k in tokens)
+                for h in range(heads):
+                    whole = sees and h * kv // heads == kv - 1
+                    if whole and pool == "keys":
+                        assert np.all(np.isnan(out[r, h])) if value != value else True, (name, r, h)
+                        continue
+                    bad = hurt & whole
+                    assert not np.isfinite(out[r, h, bad]).any(), (name, rule, r, h)
+                    check(out[r, h, ~bad], y[h, ~bad], bound[h, ~bad], (name, rule, r, h))
