@@ -997,3 +997,28 @@ def test_prefill_where_values_are_not_finite(paged, heads, kv, hd, lengths, new,
                     bad = hurt & whole
                     assert not np.isfinite(out[r, h, bad]).any(), (name, rule, r, h)
                     check(out[r, h, ~bad], y[h, ~bad], bound[h, ~bad], (name, rule, r, h))
+
+
+@pytest.mark.parametrize("row_start", [False, True])
+@pytest.mark.parametrize("n", [4100, 4200])
+def test_decode_cut_into_ranges_over_several_launches(paged, n, row_start):
+    """A loose bound cuts the sequences, a tight one does not; the second launch has fewer sequences than a wave has lanes
+    (4100) or more (4200), in the first one's workspace."""
+    import torch
+    r = np.random.default_rng(n)
+    lengths = r.integers(0, 40, n)
+    lengths[[7, 2000, 4090, 4095, 4096, 4098, n - 1]] = [500, 333, 200, 480, 470, 350, 129]
+    p = Problem(paged, "bf16", lengths, 4, 2, 64, 16, seed=73, new=(r.random(n) < 0.9).astype(int) if row_start else None, extra_pages=100)
+    if not row_start:
+        p.batch = paged.PagedBatch(p.batch.block_table, p.batch.lengths)
+    loose = p.batch.max_pages * 16
+    assert paged.attention_workspace_bytes(p.cache, 4, n, loose) > 0
+    assert paged.attention_workspace_bytes(p.cache, 4, n, 500) == 0
+    want = p.want(rows=set(range(0, p.rows, 40)) | set(range(p.rows - (n - 4080), p.rows)) |
+                  {int(p.start[i]) for i in np.flatnonzero(lengths > 100) if p.new[i]})
+    for bound in (loose, 500):
+        out = torch.full((p.rows, 4, 64), 9.0, device="cuda")
+        paged.attention_decode(p.cache, 0, p.batch, p.qd, out=out, max_len=bound)
+        torch.cuda.synchronize()
+        p.compare(out, want, bound)
+        assert not torch.any(out == 9.0)
