@@ -1022,3 +1022,40 @@ def test_decode_cut_into_ranges_over_several_launches(paged, n, row_start):
         torch.cuda.synchronize()
         p.compare(out, want, bound)
         assert not torch.any(out == 9.0)
+
+
+@pytest.mark.parametrize("decode", [True, False])
+def test_replays_at_once_write_what_the_eager_calls_do(paged, decode):
+    """Two batches' calls captured apart and replayed on two streams at once: all of each output, rows that the call leaves
+    among it, bit for bit."""
+    import torch
+    problems = [Problem(paged, "bf16", [4000, 2100, 900, 30], 28, 4, 128, 16, seed=75, new=[1, 3, 2, 0]),
+                Problem(paged, "f16", [3000, 5000, 77], 8, 8, 64, 32, seed=77, new=[2, 1, 1])]
+    call = paged.attention_decode if decode else paged.attention_prefill
+    jobs = []
+    for p in problems:
+        out = torch.zeros_like(p.qd).contiguous()
+        run = lambda p=p, out=out: call(p.cache, 0, p.batch, p.qd, out=out)  # noqa: E731
+        run()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            run()
+        jobs.append((p, run, out, g, torch.cuda.Stream()))
+    for step in range(6):
+        want = []
+        for p, run, out, g, s in jobs:
+            p.batch.lengths.copy_(dev(np.maximum(p.lengths - 13 * step, 0).astype(np.int32)))
+            out.fill_(9.0)
+            run()
+            want.append(out.clone())
+            out.fill_(9.0)
+        torch.cuda.synchronize()
+        for p, run, out, g, s in jobs:
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for w, (p, run, out, g, s) in zip(want, jobs):
+            assert torch.equal(out, w), step
+            last = sorted({int(b) - 1 for a, b in zip(p.start, p.start[1:]) if b > a}) if decode else list(range(p.rows))
+            assert not torch.any(out[last] == 9.0)
