@@ -630,9 +630,13 @@ int mlq_paged_attention_workspace(const mlq_paged_cache* c, int n_heads, int n_s
  * bounds the lengths (grid and workspace; at most max_pages * page_size).
  * Keys behind a sequence's end are not read into results, whatever the pages
  * hold there. Sums and softmax in fp32; fp16 and bf16 caches multiply on
- * 16-bit matrix instructions with q and the weights split into exact parts
- * (fp16 values below its smallest normal number, 6.1e-5, enter with an absolute
- * error of up to 2^-37; storing them rounds by up to 2^-25).
+ * 16-bit matrix instructions with q and the weights split into parts. bf16:
+ * three, exact. fp16: two, 22 bits of each element, and an absolute error of
+ * up to 2^-39 of the head's largest |q| in each of its elements (far smaller
+ * ones are lost: a score is off by up to 2^-39 max|q| sum|k| scale) and of
+ * the largest weight in each weight; cached fp16 values below the smallest
+ * normal number, 6.1e-5, enter with an absolute error of up to 2^-37 (storing
+ * them rounds by up to 2^-25).
  * NaN / inf among the seen keys and values give NaN / inf outputs. ws:
  * 256-byte aligned, scratch, may be NULL when its size is 0; calls that
  * share one (two captured graphs, too) must be ordered. n_heads: up to 2048

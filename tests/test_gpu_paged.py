@@ -1059,3 +1059,24 @@ def test_replays_at_once_write_what_the_eager_calls_do(paged, decode):
             assert torch.equal(out, w), step
             last = sorted({int(b) - 1 for a, b in zip(p.start, p.start[1:]) if b > a}) if decode else list(range(p.rows))
             assert not torch.any(out[last] == 9.0)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("size", [1e3, 1e6, 1e10])
+def test_a_query_element_far_above_the_others(paged, size, kind):
+    """One element of q is huge where every key is 0. The others' scores are right to fp32's last bits, and for an fp16 cache
+    to the 2^-39 of the head's largest |q| that an element may be off by: e = 2^-39 max|q| sum|k| scale in a score, which
+    moves a weight p by at most 2 e p."""
+    import torch
+    p = Problem(paged, kind, [1, 70, 300], 8, 4, 64, 16, seed=79, new=[1, 50, 9])
+    p.cache.keys[..., 5] = 0
+    p.k = host(p.cache.keys)
+    p.q[..., 5] = size
+    p.qd = dev(p.q)
+    keys = np.abs(np.nan_to_num(p.k)).sum(-1).max()
+    more = 2 * 2.0 ** -39 * size * keys / 8 * np.abs(p.v[np.isfinite(p.v)]).max() if kind == "f16" else 0.0
+    want = {r: (y, bound + more) for r, (y, bound) in p.want().items()}
+    out, last = paged.attention_prefill(p.cache, 0, p.batch, p.qd), paged.attention_decode(p.cache, 0, p.batch, p.qd)
+    torch.cuda.synchronize()
+    p.compare(out, want, size)
+    p.compare(last, {int(s) - 1: want[int(s) - 1] for s in p.start[1:]}, size)
