@@ -499,8 +499,8 @@ int mlq_greedy_next(const float* logits, int vocab, int32_t* token_dev, int32_t*
  * is on the device unless noted; sizes come from the host, so a step can be
  * captured in a graph and replayed while lengths, pages and tokens change on
  * the device. What the device arrays hold is checked there: a length or page
- * that is out of range gives NaN outputs or writes nothing, never a wild
- * access. */
+ * that is out of range gives NaN outputs (a negative length zeros) or writes
+ * nothing, never a wild access. */
 enum mlq_kv_type { MLQ_KV_F32 = 0, MLQ_KV_F16 = 1, MLQ_KV_BF16 = 2 };
 
 /* keys and values: [n_layers][n_pages][n_kv_heads][page_size][head_dim] each,
@@ -623,7 +623,7 @@ int mlq_paged_attention_workspace(const mlq_paged_cache* c, int n_heads, int n_s
  * NULL: row i of sequence i), out of its last row = attention of q's last row
  * at position lengths[i] - 1 over the sequence's pages, query head h reading
  * kv head h / (n_heads / n_kv_heads). The new tokens' keys and values are in
- * the cache already. A length of 0 gives zeros; a length above max_len or
+ * the cache already. A length of 0 or less gives zeros; one above max_len or
  * the block table, or a page outside the cache, NaN. q and out: rows of
  * n_heads * head_dim floats at strides in floats (multiples of 4, pointers
  * 16-byte aligned), out apart from everything else; b's block_table, lengths and row_start are read. max_len

@@ -11,6 +11,13 @@ A step of a serving loop, all stream-ordered and with no host round trip:
         attention_decode(cache, i, batch, q, max_len=...)    # one new token each, or
         attention_prefill(cache, i, batch, q)                # any numbers of them
 
+Where some sequences bring one token and others a prompt, a batch whose
+sequences are in that order is two: PagedBatch of block_table[:n], lengths[:n]
+and row_start[:n + 1] for attention_decode, of [n:] of each for
+attention_prefill, both with the whole step's q and out. attention_prefill alone
+takes any mixture, but a workgroup walks all keys of a sequence if the batch has
+rows enough to fill the chip: long contexts belong to attention_decode.
+
 Activations are float32, the cache float32, float16 or bfloat16. Tensors are
 passed as they are: q, k, v and outputs are [rows, heads, head_dim] with any
 row stride (views of a fused projection), heads contiguous. There is no CPU
@@ -125,7 +132,7 @@ class PagedCache(_Fixed):
                                     self.head_dim)
         self.ref = ctypes.byref(self.struct)
         self.index = keys.get_device()
-        self._workspaces = {}  # bytes by (n_heads, n_seqs, max_len)
+        self._workspaces = {}  # bytes by (n_heads, n_seqs, rows, max_len)
         nbytes = ctypes.c_size_t()
         _check(lib().mlq_paged_cache_bytes(self.ref, ctypes.byref(nbytes)),
                "mlq_paged_cache_bytes")

@@ -1080,3 +1080,28 @@ def test_a_query_element_far_above_the_others(paged, size, kind):
     torch.cuda.synchronize()
     p.compare(out, want, size)
     p.compare(last, {int(s) - 1: want[int(s) - 1] for s in p.start[1:]}, size)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("seqs,prompts", [(5, 2), (400, 90), (300, 290)])
+def test_decode_for_some_sequences_and_prefill_for_the_others(paged, seqs, prompts, kind):
+    """A step of both: views of the batch's arrays are batches of their own, with the whole step's q and out."""
+    import torch
+    r = np.random.default_rng(seqs)
+    ones = seqs - prompts
+    lengths = np.concatenate([r.integers(1, 200, ones), r.integers(10, 150, prompts)])
+    lengths[0], lengths[ones] = 3000, 700
+    new = np.concatenate([np.ones(ones, int), r.integers(1, 10, prompts)])
+    new[ones], new[-1] = 650, lengths[-1]
+    p = Problem(paged, kind, lengths, 8, 2, 64, 16, seed=81, new=new)
+    b = p.batch
+    first = paged.PagedBatch(b.block_table[:ones], b.lengths[:ones], b.row_start[:ones + 1])
+    rest = paged.PagedBatch(b.block_table[ones:], b.lengths[ones:], b.row_start[ones:])
+    out = torch.full((p.rows, 8, 64), 9.0, device="cuda")
+    paged.attention_decode(p.cache, 0, first, p.qd, out=out)
+    torch.cuda.synchronize()
+    assert torch.all(out[ones:] == 9.0) and not torch.any(out[:ones] == 9.0)
+    paged.attention_prefill(p.cache, 0, rest, p.qd, out=out)
+    torch.cuda.synchronize()
+    p.compare(out, p.want(rows=set(range(0, p.rows, max(1, p.rows // 150))) | {ones - 1, ones, p.rows - 1}))
+    assert not torch.any(out == 9.0)
