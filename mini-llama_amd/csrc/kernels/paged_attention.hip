@@ -758,8 +758,8 @@ void decode_launch_hd(const PagedAttnArgs& a, int grid, hipStream_t stream) {
 //    leave CUs idle, several workgroups share a tile's keys (64 rows of 16
 //    sequences behind up to 8000 tokens, 28 heads on 4, bf16: 342 -> 83 us).
 // That case's 620 GFLOP of part products (three for each of the two) take 550
-// us, 1.13 PFLOP/s where a library product of 8192^3 reaches 1.2: the chip's
-// power bounds both, its clock falls to 1.9 GHz. One barrier a tile instead of
+// to 566 us, 1.1 PFLOP/s where a library product of 8192^3 reaches 1.2: the
+// chip's power bounds both, its clock falls to 1.9 GHz. One barrier a tile instead of
 // two, fewer vector instructions and no spills brought 691 to 543; raising the
 // waves' priority around the products cost 5 %.
 constexpr int kPreCols = 128, kPreKeys = 32, kPreThreads = 256;

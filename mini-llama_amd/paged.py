@@ -23,7 +23,7 @@ passed as they are: q, k, v and outputs are [rows, heads, head_dim] with any
 row stride (views of a fused projection), heads contiguous. There is no CPU
 fallback. Tensors of a call live on one device; it need not be the current
 one. Given a `stream`, the call's work is ordered on it and so must be the
-tensors.
+tensors. Forward only: outputs carry no gradients.
 """
 from __future__ import annotations
 
