@@ -302,6 +302,9 @@ __global__ __launch_bounds__(kRotaryThreads) void qk_norm_rope_kernel(RotaryArgs
             p[c] = 0.0f;
             if (d + c < a.rot) p[c] = w != nullptr ? src[e] * w[e] * inv : src[e];
           }
+          // (in place: no lane stores before its partners have read)
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          __builtin_amdgcn_wave_barrier();
         }
 #pragma unroll
         for (int c = 0; c < 4; ++c)
