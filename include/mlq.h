@@ -501,13 +501,27 @@ int mlq_greedy_next(const float* logits, int vocab, int32_t* token_dev, int32_t*
  * the device. What the device arrays hold is checked there: a length or page
  * that is out of range gives NaN outputs (a negative length zeros) or writes
  * nothing, never a wild access. */
-enum mlq_kv_type { MLQ_KV_F32 = 0, MLQ_KV_F16 = 1, MLQ_KV_BF16 = 2 };
+enum mlq_kv_type { MLQ_KV_F32 = 0, MLQ_KV_F16 = 1, MLQ_KV_BF16 = 2, MLQ_KV_Q4 = 4, MLQ_KV_Q8 = 8 };
 
-/* keys and values: [n_layers][n_pages][n_kv_heads][page_size][head_dim] each,
+/* keys and values: [n_layers][n_pages][n_kv_heads][page_size][head_dim] each
+ * (Q4 and Q8: [page_size][row bytes]),
  * 16-byte aligned; token t of a sequence is token t % page_size of the page
  * that its block table names at t / page_size. page_size: a power of two,
  * 16 .. 4096; head_dim: a multiple of 8 up to 256; a block table holds at most
- * 2^30 tokens a sequence (MLQ_ERR_UNSUPPORTED otherwise). */
+ * 2^30 tokens a sequence (MLQ_ERR_UNSUPPORTED otherwise).
+ *
+ * Q4 and Q8 hold a head's elements in blocks of 32 as codes c of 0 .. L for
+ * d (c - z) + m, d and m in fp16 (Q4: L = 15, z = 8; Q8: L = 255, z = 128). Of a
+ * block whose least and largest elements are lo and hi, d is (hi - lo) / L and
+ * m is lo + z d, in fp32 operations whose results are rounded to fp16 (nearest,
+ * ties to even), and c the nearest code, upwards from halfway, as exact
+ * arithmetic has it; d = 0 gives c = z. A block that holds an element that is
+ * not finite, or whose d or m passes fp16's range, reads as NaN: it is stored
+ * with d and m NaN. A row has 2, 4 or 8 blocks (head_dim up to 64, 128, 256):
+ * unit i * blocks + b (i < 16) holds elements 2i and 2i + 1 of block b (Q4: one
+ * byte, 2i in its low half; Q8: two bytes), then come d and m of every block.
+ * 40, 80 or 160 bytes (Q4), 72, 144 or 288 (Q8). Elements behind head_dim have
+ * code z, blocks that lie wholly behind it d = m = 0. */
 typedef struct mlq_paged_cache {
   void* keys;
   void* values;
@@ -592,13 +606,30 @@ typedef struct mlq_rotary {
  * strides then; no other overlap). k_out may be NULL with a cache; without
  * one (c NULL) k_out is needed and v, slots and layer are not read.
  * Distinct rows need distinct slots. rows = 0 does nothing. Up to 2048 heads and
- * fewer than 2^24 rows (MLQ_ERR_UNSUPPORTED otherwise). */
+ * fewer than 2^24 rows (MLQ_ERR_UNSUPPORTED otherwise). A Q4 or Q8 cache gets
+ * what mlq_paged_write stores of v and of the rotated keys as k_out has them. */
 int mlq_qk_norm_rope(const mlq_rotary* r, int rows, const int32_t* positions, int n_heads,
                      int n_kv_heads, const float* q, int64_t q_stride, const float* k,
                      int64_t k_stride, const float* v, int64_t v_stride, float* q_out,
                      int64_t q_out_stride, float* k_out, int64_t k_out_stride,
                      const mlq_paged_cache* c, int layer, const int64_t* slots,
                      mlq_stream_t stream);
+
+/* Rows of keys and values as they are (rotated already, where they are to be) to
+ * their slots of `layer`, rounded or quantised to the cache's type; a row whose
+ * slot is outside the cache is left out. k_out and v_out, NULL or not each by
+ * itself, receive the values that the cache now stands for (k_out may be k,
+ * v_out v, with the same strides; no other overlap). Strides, alignment, distinct
+ * slots and rows = 0 as in mlq_qk_norm_rope. Fewer than 2^28 / n_kv_heads rows
+ * (MLQ_ERR_UNSUPPORTED otherwise). */
+int mlq_paged_write(const mlq_paged_cache* c, int layer, int rows, const int64_t* slots,
+                    const float* k, int64_t k_stride, const float* v, int64_t v_stride,
+                    float* k_out, int64_t k_out_stride, float* v_out, int64_t v_out_stride,
+                    mlq_stream_t stream);
+/* The other way: rows of k and v = the values of their slots. A row whose slot is
+ * outside the cache is left as it was; several rows may name one slot. */
+int mlq_paged_read(const mlq_paged_cache* c, int layer, int rows, const int64_t* slots, float* k,
+                   int64_t k_stride, float* v, int64_t v_stride, mlq_stream_t stream);
 
 /* How a score s = q . k becomes the softmax's input for a query at position p
  * and a key at position t <= p: s * scale, then softcap * tanh(that /

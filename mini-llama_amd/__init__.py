@@ -204,6 +204,8 @@ SIGNATURES = {
     "mlq_paged_plan": ([_PBP, _I, _I, _P, _P, _P, _P, _P, _P], _I),
     "mlq_rope_frequencies": ([_D, _I, _I, _D, _I, _D, _D, ctypes.POINTER(_D),
                               ctypes.POINTER(_F)], _I),
+    "mlq_paged_write": ([_PCP, _I, _I, _P, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _P], _I),
+    "mlq_paged_read": ([_PCP, _I, _I, _P, _P, _I64, _P, _I64, _P], _I),
     "mlq_qk_norm_rope": ([_RTP, _I, _P, _I, _I, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I64,
                           _PCP, _I, _P, _P], _I),
     "mlq_paged_attention_workspace": ([_PCP, _I, _I, _I, _I, ctypes.POINTER(_Z)], _I),

@@ -48,6 +48,22 @@ struct RotaryArgs {
 };
 hipError_t launch_qk_norm_rope(const RotaryArgs& a, hipStream_t stream);
 
+struct RowsArgs {
+  int rows, n_kv, hd, type, page_shift;
+  const int64_t* slots;
+  int64_t n_slots;
+  void* keys;    // of the layer
+  void* values;
+  const float* k;  // written rows
+  const float* v;
+  float* k_out;    // what is read, or what was written now stands for (may be null then)
+  float* v_out;
+  int64_t k_stride, v_stride, k_out_stride, v_out_stride;
+};
+// Workgroups of a launch.
+int64_t rows_groups(int rows, int n_kv);
+hipError_t launch_paged_rows(const RowsArgs& a, bool write, hipStream_t stream);
+
 // paged_attention.hip
 struct PagedAttnArgs {
   const void* keys;    // of the layer

@@ -1,12 +1,14 @@
 // The paged cache's bookkeeping and what writes it: the plan of a step (block
-// tables, positions, slots) and the per-head norm + rotation of queries and
-// keys with the cache write.
+// tables, positions, slots), the per-head norm + rotation of queries and keys
+// with the cache write, and rows written to a cache or read back as they are.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "device_common.h"
+#include "kv_quant.h"
 #include "paged.h"
 #include "paged_device.h"
 
@@ -237,8 +239,38 @@ __device__ __forceinline__ void store_kv(void* base, int type, int64_t at, float
   else *(bv4*)((__bf16*)base + at) = __builtin_convertvector(f, bv4);
 }
 
-template <int LG>
+// A head's row of 4 or 8 bits from 4 elements a lane (lane l of the head's has
+// dims 4l ..): a block lies in 8 lanes, and a lane's two units in two places.
+template <typename Q>
+__device__ __forceinline__ void store_quantised(char* row, int l, int hd, float4 x) {
+  const int nb = kv_blocks(hd), b = l >> 3, d = 4 * l;
+  const float v[4] = {x.x, x.y, x.z, x.w};
+  float lo = INFINITY, hi = -INFINITY;
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    if (d + c < hd) kv_range(v[c], lo, hi);
+  lo = -row_max<8>(-lo);
+  hi = row_max<8>(hi);
+  if (lo > hi) lo = hi = 0.0f;  // (a block behind the head's end)
+  const KvScale s = kv_scale<Q>(lo, hi);
+  const float inv = 1.0f / (float)s.d;
+  int code[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) code[c] = d + c < hd ? kv_code<Q>(v[c], s, inv) : Q::kMiddle;
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const int unit = (2 * (l & 7) + c) * nb + b;
+    if constexpr (Q::kUnit == 1) ((uint8_t*)row)[unit] = (uint8_t)(code[2 * c] | code[2 * c + 1] << 4);
+    else ((uint16_t*)row)[unit] = (uint16_t)(code[2 * c] | code[2 * c + 1] << 8);
+  }
+  if ((l & 7) == 0) *(KvScale*)(row + 16 * nb * Q::kUnit + 4 * b) = s;
+}
+
+// Q: KvQ4 or KvQ8 for a cache of those bits, void for the others. The rotated
+// fp32 key is quantised, the one that k_out holds.
+template <int LG, typename Q>
 __global__ __launch_bounds__(kRotaryThreads) void qk_norm_rope_kernel(RotaryArgs a) {
+  constexpr bool QUANT = !std::is_void<Q>::value;
   __shared__ float2 turn[kRotaryMaxHalf];  // cos, sin, times the magnitude
   const int row = blockIdx.x;
   const int pos = a.positions[row];
@@ -276,8 +308,16 @@ __global__ __launch_bounds__(kRotaryThreads) void qk_norm_rope_kernel(RotaryArgs
                                   (int64_t)kh * a.hd;
     float4 x = in ? *(const float4*)(src + d) : float4{0.0f, 0.0f, 0.0f, 0.0f};
     const int64_t at = ((page * a.n_kv + kh) << a.page_shift) * a.hd + off * a.hd + d;
+    auto quantise = [&](void* base) {
+      if constexpr (QUANT)
+        store_quantised<Q>((char*)base + (((page * a.n_kv + kh) << a.page_shift) + off) * kv_row_bytes(Q::kType, a.hd), l, a.hd, x);
+    };
     if (is_v) {
-      if (in && slot >= 0) store_kv(a.values, a.type, at, x);
+      if constexpr (QUANT) {
+        if (slot >= 0) quantise(a.values);
+      } else {
+        if (in && slot >= 0) store_kv(a.values, a.type, at, x);
+      }
       continue;
     }
     const float* w = is_q ? a.q_norm : a.k_norm;
@@ -328,6 +368,8 @@ __global__ __launch_bounds__(kRotaryThreads) void qk_norm_rope_kernel(RotaryArgs
         }
       }
     }
+    if constexpr (QUANT)
+      if (!is_q && slot >= 0) quantise(a.keys);
     if (!in) continue;
     if (is_q) {
       float* to = a.q_out + row * a.q_out_stride + (int64_t)h * a.hd + d;
@@ -336,12 +378,172 @@ __global__ __launch_bounds__(kRotaryThreads) void qk_norm_rope_kernel(RotaryArgs
     } else {
       if (a.k_out != nullptr)
         *(float4*)(a.k_out + row * a.k_out_stride + (int64_t)kh * a.hd + d) = x;
-      if (slot >= 0) store_kv(a.keys, a.type, at, x);
+      if constexpr (!QUANT)
+        if (slot >= 0) store_kv(a.keys, a.type, at, x);
     }
   }
 }
 
-template <int LG>
+// ---- rows written and read back ----------------------------------------------------
+// Bytes bound both: for each element 4 in or out and the cache's share. 16
+// lanes have a head, lane i dims 2i and 2i + 1 of every block: loads and stores
+// of 128 bytes a block, and the lane's units lie side by side.
+constexpr int kRowsThreads = 256, kRowsGroup = 16;
+
+// Which (row, kv head, keys or values) the x-th is.
+struct RowItem {
+  int64_t row;
+  int head;
+  bool is_v;
+};
+__device__ __forceinline__ RowItem row_item(int64_t x, int n_kv) {
+  const int64_t row = quotient(x, 2 * n_kv);
+  const int of = (int)(x - row * 2 * n_kv);
+  return {row, of < n_kv ? of : of - n_kv, of >= n_kv};
+}
+// The place of a row's head in the cache, in rows; -1: outside.
+__device__ __forceinline__ int64_t row_place(const RowsArgs& a, const RowItem& it) {
+  const int64_t slot = a.slots[it.row];
+  if (slot < 0 || slot >= a.n_slots) return -1;
+  const int64_t page = slot >> a.page_shift;
+  return ((page * a.n_kv + it.head) << a.page_shift) + (slot & (((int64_t)1 << a.page_shift) - 1));
+}
+
+template <typename Q, int NB>
+__global__ __launch_bounds__(kRowsThreads) void write_rows_quantised_kernel(RowsArgs a) {
+  constexpr int kBytes = NB * (16 * Q::kUnit + 4);
+  const int i = threadIdx.x % kRowsGroup;
+  const int64_t x = (int64_t)blockIdx.x * (kRowsThreads / kRowsGroup) + threadIdx.x / kRowsGroup;
+  if (x >= (int64_t)a.rows * 2 * a.n_kv) return;
+  const RowItem it = row_item(x, a.n_kv);
+  const int64_t at = row_place(a, it);
+  if (at < 0) return;
+  const float* src = (it.is_v ? a.v + it.row * a.v_stride : a.k + it.row * a.k_stride) + (int64_t)it.head * a.hd;
+  float2 v[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) v[b] = 32 * b + 2 * i < a.hd ? *(const float2*)(src + 32 * b + 2 * i) : float2{0.0f, 0.0f};
+  KvScale s[NB];
+  uint32_t unit[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const bool in = 32 * b + 2 * i < a.hd;  // (both dims: head dims are even)
+    float lo = INFINITY, hi = -INFINITY;
+    if (in) {
+      kv_range(v[b].x, lo, hi);
+      kv_range(v[b].y, lo, hi);
+    }
+    lo = -row_max<16>(-lo);
+    hi = row_max<16>(hi);
+    if (lo > hi) lo = hi = 0.0f;  // (a block behind the head's end)
+    s[b] = kv_scale<Q>(lo, hi);
+    const float inv = 1.0f / (float)s[b].d;
+    const int c0 = in ? kv_code<Q>(v[b].x, s[b], inv) : Q::kMiddle, c1 = in ? kv_code<Q>(v[b].y, s[b], inv) : Q::kMiddle;
+    unit[b] = c0 | c1 << (4 * Q::kUnit);
+    v[b] = float2{kv_value<Q>(c0, s[b]), kv_value<Q>(c1, s[b])};
+  }
+  char* row = (char*)(it.is_v ? a.values : a.keys) + at * kBytes;
+  uint32_t w[(NB * Q::kUnit + 3) / 4] = {};
+#pragma unroll
+  for (int b = 0; b < NB; ++b) w[b * Q::kUnit / 4] |= unit[b] << (8 * (b * Q::kUnit % 4));
+  char* to = row + i * NB * Q::kUnit;
+  if constexpr (NB * Q::kUnit == 2) *(uint16_t*)to = (uint16_t)w[0];
+  else if constexpr (NB * Q::kUnit == 4) *(uint32_t*)to = w[0];
+  else if constexpr (NB * Q::kUnit == 8) *(u32x2_t*)to = u32x2_t{w[0], w[1]};
+  else *(u32x4_t*)to = u32x4_t{w[0], w[1], w[2], w[3]};
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+    if (i == b) *(KvScale*)(row + 16 * NB * Q::kUnit + 4 * b) = s[b];
+  float* out = it.is_v ? a.v_out : a.k_out;
+  if (out == nullptr) return;
+  out += it.row * (it.is_v ? a.v_out_stride : a.k_out_stride) + (int64_t)it.head * a.hd;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+    if (32 * b + 2 * i < a.hd) *(float2*)(out + 32 * b + 2 * i) = v[b];
+}
+
+template <typename Q, int NB>
+__global__ __launch_bounds__(kRowsThreads) void read_rows_quantised_kernel(RowsArgs a) {
+  constexpr int kBytes = NB * (16 * Q::kUnit + 4), W = NB * Q::kUnit;
+  const int i = threadIdx.x % kRowsGroup;
+  const int64_t x = (int64_t)blockIdx.x * (kRowsThreads / kRowsGroup) + threadIdx.x / kRowsGroup;
+  if (x >= (int64_t)a.rows * 2 * a.n_kv) return;
+  const RowItem it = row_item(x, a.n_kv);
+  const int64_t at = row_place(a, it);
+  if (at < 0) return;
+  const char* row = (const char*)(it.is_v ? a.values : a.keys) + at * kBytes;
+  uint32_t w[(W + 3) / 4];
+  const char* from = row + i * W;
+  if constexpr (W == 2) {
+    w[0] = *(const uint16_t*)from;
+  } else {
+#pragma unroll
+    for (int j = 0; j < W / 4; ++j) w[j] = ((const uint32_t*)from)[j];
+  }
+  float* out = (it.is_v ? a.v_out + it.row * a.v_out_stride : a.k_out + it.row * a.k_out_stride) + (int64_t)it.head * a.hd;
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    if (32 * b + 2 * i >= a.hd) break;
+    const KvScale s = *(const KvScale*)(row + 16 * W + 4 * b);
+    constexpr int kMask = Q::kLevels;
+    const uint32_t unit = w[b * Q::kUnit / 4] >> (8 * (b * Q::kUnit % 4));
+    *(float2*)(out + 32 * b + 2 * i) =
+        float2{kv_value<Q>(unit & kMask, s), kv_value<Q>(unit >> (4 * Q::kUnit) & kMask, s)};
+  }
+}
+
+// Caches of 16 and 32 bits: 4 elements a lane.
+__device__ __forceinline__ float4 load_kv(const void* base, int type, int64_t at) {
+  typedef float v4 __attribute__((ext_vector_type(4)));
+  typedef _Float16 hv4 __attribute__((ext_vector_type(4)));
+  typedef __bf16 bv4 __attribute__((ext_vector_type(4)));
+  v4 f;
+  if (type == MLQ_KV_F32) f = *(const v4*)((const float*)base + at);
+  else if (type == MLQ_KV_F16) f = __builtin_convertvector(*(const hv4*)((const _Float16*)base + at), v4);
+  else f = __builtin_convertvector(*(const bv4*)((const __bf16*)base + at), v4);
+  return float4{f.x, f.y, f.z, f.w};
+}
+template <bool WRITE>
+__global__ __launch_bounds__(kRowsThreads) void plain_rows_kernel(RowsArgs a) {
+  const int64_t x = (int64_t)blockIdx.x * (kRowsThreads / kRowsGroup) + threadIdx.x / kRowsGroup;
+  if (x >= (int64_t)a.rows * 2 * a.n_kv) return;
+  const RowItem it = row_item(x, a.n_kv);
+  const int64_t at = row_place(a, it);
+  if (at < 0) return;
+  void* base = it.is_v ? a.values : a.keys;
+  float* out = it.is_v ? a.v_out : a.k_out;
+  if (out != nullptr) out += it.row * (it.is_v ? a.v_out_stride : a.k_out_stride) + (int64_t)it.head * a.hd;
+  const float* src = nullptr;
+  if constexpr (WRITE)
+    src = (it.is_v ? a.v + it.row * a.v_stride : a.k + it.row * a.k_stride) + (int64_t)it.head * a.hd;
+  for (int d = 4 * (threadIdx.x % kRowsGroup); d < a.hd; d += 4 * kRowsGroup) {
+    float4 f;
+    if constexpr (WRITE) {
+      f = *(const float4*)(src + d);
+      if (a.type == MLQ_KV_F16) f = float4{(float)(_Float16)f.x, (float)(_Float16)f.y, (float)(_Float16)f.z, (float)(_Float16)f.w};
+      else if (a.type == MLQ_KV_BF16) f = float4{(float)(__bf16)f.x, (float)(__bf16)f.y, (float)(__bf16)f.z, (float)(__bf16)f.w};
+      store_kv(base, a.type, at * a.hd + d, f);
+    } else {
+      f = load_kv(base, a.type, at * a.hd + d);
+    }
+    if (out != nullptr) *(float4*)(out + d) = f;
+  }
+}
+
+template <typename Q, int NB>
+void rows_launch(const RowsArgs& a, bool write, dim3 grid, hipStream_t stream) {
+  if (write) hipLaunchKernelGGL((write_rows_quantised_kernel<Q, NB>), grid, dim3(kRowsThreads), 0, stream, a);
+  else hipLaunchKernelGGL((read_rows_quantised_kernel<Q, NB>), grid, dim3(kRowsThreads), 0, stream, a);
+}
+template <typename Q>
+void rows_launch_blocks(const RowsArgs& a, bool write, dim3 grid, hipStream_t stream) {
+  switch (kv_blocks(a.hd)) {
+    case 2: return rows_launch<Q, 2>(a, write, grid, stream);
+    case 4: return rows_launch<Q, 4>(a, write, grid, stream);
+    default: return rows_launch<Q, 8>(a, write, grid, stream);
+  }
+}
+
+template <int LG, typename Q>
 void rotary_launch(RotaryArgs a, hipStream_t stream) {
   const int heads = a.n_heads + (a.keys != nullptr ? 2 : 1) * a.n_kv;
   const int per = kRotaryThreads / LG;
@@ -349,8 +551,16 @@ void rotary_launch(RotaryArgs a, hipStream_t stream) {
   const int most = (heads + per - 1) / per;
   const int split = std::min(most, std::max(1, 2 * device_cus() / a.rows));
   a.stream = (int64_t)a.rows * a.n_heads * a.hd * 4 > kRotaryStreamBytes;
-  hipLaunchKernelGGL(qk_norm_rope_kernel<LG>, dim3(a.rows, split), dim3(kRotaryThreads), 0,
+  hipLaunchKernelGGL((qk_norm_rope_kernel<LG, Q>), dim3(a.rows, split), dim3(kRotaryThreads), 0,
                      stream, a);
+}
+// (a row of 4 or 8 bits has two blocks at least)
+template <typename Q>
+void rotary_launch_hd(const RotaryArgs& a, hipStream_t stream) {
+  if (a.hd <= 32 && std::is_void<Q>::value) rotary_launch<8, Q>(a, stream);
+  else if (a.hd <= 64) rotary_launch<16, Q>(a, stream);
+  else if (a.hd <= 128) rotary_launch<32, Q>(a, stream);
+  else rotary_launch<64, Q>(a, stream);
 }
 
 }  // namespace
@@ -371,10 +581,23 @@ hipError_t launch_paged_plan(const PlanArgs& a, hipStream_t stream) {
 }
 
 hipError_t launch_qk_norm_rope(const RotaryArgs& a, hipStream_t stream) {
-  if (a.hd <= 32) rotary_launch<8>(a, stream);
-  else if (a.hd <= 64) rotary_launch<16>(a, stream);
-  else if (a.hd <= 128) rotary_launch<32>(a, stream);
-  else rotary_launch<64>(a, stream);
+  if (a.keys != nullptr && a.type == MLQ_KV_Q4) rotary_launch_hd<KvQ4>(a, stream);
+  else if (a.keys != nullptr && a.type == MLQ_KV_Q8) rotary_launch_hd<KvQ8>(a, stream);
+  else rotary_launch_hd<void>(a, stream);
+  return hipGetLastError();
+}
+
+int64_t rows_groups(int rows, int n_kv) {
+  constexpr int per = kRowsThreads / kRowsGroup;
+  return ((int64_t)rows * 2 * n_kv + per - 1) / per;
+}
+
+hipError_t launch_paged_rows(const RowsArgs& a, bool write, hipStream_t stream) {
+  const dim3 grid((unsigned)rows_groups(a.rows, a.n_kv));
+  if (a.type == MLQ_KV_Q4) rows_launch_blocks<KvQ4>(a, write, grid, stream);
+  else if (a.type == MLQ_KV_Q8) rows_launch_blocks<KvQ8>(a, write, grid, stream);
+  else if (write) hipLaunchKernelGGL(plain_rows_kernel<true>, grid, dim3(kRowsThreads), 0, stream, a);
+  else hipLaunchKernelGGL(plain_rows_kernel<false>, grid, dim3(kRowsThreads), 0, stream, a);
   return hipGetLastError();
 }
 

@@ -6,6 +6,7 @@
 #include <cmath>
 #include <cstdint>
 
+#include "kernels/kv_quant.h"
 #include "kernels/launch.h"
 #include "kernels/paged.h"
 #include "mlq.h"
@@ -23,8 +24,6 @@ constexpr int64_t kMaxTokens = (int64_t)1 << 30;
 constexpr int kMaxHeads = 2048;
 constexpr int64_t kMaxGroups = ((int64_t)1 << 24) - 1;
 
-size_t kv_bytes(int type) { return type == MLQ_KV_F32 ? 4 : 2; }
-
 int page_shift_of(int page_size) {
   for (int s = 4; s <= 12; ++s)
     if (page_size == 1 << s) return s;
@@ -34,7 +33,8 @@ int page_shift_of(int page_size) {
 // Everything but the pointers.
 int check_geometry(const mlq_paged_cache* c) {
   if (c == nullptr) return MLQ_ERR_INVALID_ARG;
-  if (c->type != MLQ_KV_F32 && c->type != MLQ_KV_F16 && c->type != MLQ_KV_BF16)
+  if (c->type != MLQ_KV_F32 && c->type != MLQ_KV_F16 && c->type != MLQ_KV_BF16 &&
+      !kv_quantised(c->type))
     return MLQ_ERR_INVALID_ARG;
   if (c->n_layers <= 0 || c->n_pages <= 0 || c->page_size <= 0 || c->n_kv_heads <= 0 ||
       c->head_dim <= 0)
@@ -54,7 +54,7 @@ int check_paged_cache(const mlq_paged_cache* c) {
 
 // Bytes of one layer of one of the arrays.
 size_t layer_bytes(const mlq_paged_cache* c) {
-  return (size_t)c->n_pages * c->n_kv_heads * c->page_size * c->head_dim * kv_bytes(c->type);
+  return (size_t)c->n_pages * c->n_kv_heads * c->page_size * kv_row_bytes(c->type, c->head_dim);
 }
 
 // A row array of `heads` heads: 16-byte aligned rows that do not overlap.
@@ -68,6 +68,7 @@ int check_attention(const mlq_paged_cache* c, int layer, const mlq_paged_batch* 
                     int64_t q_stride, const float* out, int64_t out_stride, PagedAttnArgs* a) {
   int rc = check_paged_cache(c);
   if (rc != MLQ_OK) return rc;
+  if (kv_quantised(c->type)) return MLQ_ERR_UNSUPPORTED;
   if (b == nullptr || b->block_table == nullptr || b->lengths == nullptr)
     return MLQ_ERR_INVALID_ARG;
   if (b->n_seqs <= 0 || b->max_pages <= 0 || n_heads <= 0 || n_heads % c->n_kv_heads != 0)
@@ -271,10 +272,65 @@ int mlq_qk_norm_rope(const mlq_rotary* r, int rows, const int32_t* positions, in
   return record_hip(launch_qk_norm_rope(a, (hipStream_t)stream));
 }
 
+static int paged_rows(const mlq_paged_cache* c, int layer, int rows, const int64_t* slots,
+                      const float* k, int64_t k_stride, const float* v, int64_t v_stride,
+                      float* k_out, int64_t k_out_stride, float* v_out, int64_t v_out_stride,
+                      bool write, mlq_stream_t stream) {
+  int rc = check_paged_cache(c);
+  if (rc != MLQ_OK) return rc;
+  if (rows < 0 || layer < 0 || layer >= c->n_layers) return MLQ_ERR_SHAPE;
+  if (slots == nullptr) return MLQ_ERR_INVALID_ARG;
+  const int64_t floats = (int64_t)c->n_kv_heads * c->head_dim;
+  if (write) {
+    if ((rc = check_rows(k, k_stride, floats)) != MLQ_OK) return rc;
+    if ((rc = check_rows(v, v_stride, floats)) != MLQ_OK) return rc;
+    if (k_out == k && k_out_stride != k_stride) return MLQ_ERR_INVALID_ARG;
+    if (v_out == v && v_out_stride != v_stride) return MLQ_ERR_INVALID_ARG;
+  }
+  if ((!write || k_out != nullptr) && (rc = check_rows(k_out, k_out_stride, floats)) != MLQ_OK) return rc;
+  if ((!write || v_out != nullptr) && (rc = check_rows(v_out, v_out_stride, floats)) != MLQ_OK) return rc;
+  if (rows_groups(rows, c->n_kv_heads) > kMaxGroups) return MLQ_ERR_UNSUPPORTED;
+  if (rows == 0) return MLQ_OK;
+  RowsArgs a = {};
+  a.rows = rows;
+  a.n_kv = c->n_kv_heads;
+  a.hd = c->head_dim;
+  a.type = c->type;
+  a.page_shift = page_shift_of(c->page_size);
+  a.slots = slots;
+  a.n_slots = (int64_t)c->n_pages * c->page_size;
+  a.keys = (char*)c->keys + layer * layer_bytes(c);
+  a.values = (char*)c->values + layer * layer_bytes(c);
+  a.k = k;
+  a.v = v;
+  a.k_out = k_out;
+  a.v_out = v_out;
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.k_out_stride = k_out_stride;
+  a.v_out_stride = v_out_stride;
+  return record_hip(launch_paged_rows(a, write, (hipStream_t)stream));
+}
+
+int mlq_paged_write(const mlq_paged_cache* c, int layer, int rows, const int64_t* slots,
+                    const float* k, int64_t k_stride, const float* v, int64_t v_stride,
+                    float* k_out, int64_t k_out_stride, float* v_out, int64_t v_out_stride,
+                    mlq_stream_t stream) {
+  return paged_rows(c, layer, rows, slots, k, k_stride, v, v_stride, k_out, k_out_stride, v_out,
+                    v_out_stride, true, stream);
+}
+
+int mlq_paged_read(const mlq_paged_cache* c, int layer, int rows, const int64_t* slots, float* k,
+                   int64_t k_stride, float* v, int64_t v_stride, mlq_stream_t stream) {
+  return paged_rows(c, layer, rows, slots, nullptr, 0, nullptr, 0, k, k_stride, v, v_stride, false,
+                    stream);
+}
+
 int mlq_paged_attention_workspace(const mlq_paged_cache* c, int n_heads, int n_seqs, int max_rows,
                                   int max_len, size_t* bytes) {
   const int rc = check_geometry(c);
   if (rc != MLQ_OK) return rc;
+  if (kv_quantised(c->type)) return MLQ_ERR_UNSUPPORTED;
   if (bytes == nullptr) return MLQ_ERR_INVALID_ARG;
   if (n_heads <= 0 || n_heads % c->n_kv_heads != 0 || n_seqs <= 0 || max_rows < 0 || max_len <= 0)
     return MLQ_ERR_SHAPE;

@@ -11,6 +11,9 @@ A step of a serving loop, all stream-ordered and with no host round trip:
         attention_decode(cache, i, batch, q, max_len=...)    # one new token each, or
         attention_prefill(cache, i, batch, q)                # any numbers of them
 
+write() stores rows that need no rotation, read() gives tokens back, of any
+type of cache.
+
 Where some sequences bring one token and others a prompt, a batch whose
 sequences are in that order is two: PagedBatch of block_table[:n], lengths[:n]
 and row_start[:n + 1] for attention_decode, of [n:] of each for
@@ -18,7 +21,8 @@ attention_prefill, both with the whole step's q and out. attention_prefill alone
 takes any mixture, but a workgroup walks all keys of a sequence if the batch has
 rows enough to fill the chip: long contexts belong to attention_decode.
 
-Activations are float32, the cache float32, float16 or bfloat16. Tensors are
+Activations are float32, the cache float32, float16 or bfloat16, or of 4 or 8
+bits ("q4", "q8": 5 and 9 bits an element with their scales). Tensors are
 passed as they are: q, k, v and outputs are [rows, heads, head_dim] with any
 row stride (views of a fused projection), heads contiguous. There is no CPU
 fallback. Tensors of a call live on one device; it need not be the current
@@ -36,13 +40,15 @@ from . import (ROPE_NEOX, ROPE_NORMAL, MlqAttentionRule, MlqPagedBatch, MlqPaged
                _check, lib)
 
 __all__ = ["ROPE_NEOX", "ROPE_NORMAL", "PLAN_STATUS", "PagedCache", "PagedBatch", "Rotary",
-           "AttentionRule", "plan", "rope_frequencies", "qk_norm_rope", "attention_decode",
-           "attention_prefill", "attention_workspace_bytes"]
+           "AttentionRule", "plan", "rope_frequencies", "qk_norm_rope", "write", "read",
+           "attention_decode", "attention_prefill", "attention_workspace_bytes"]
 
 PLAN_STATUS = {0: "ok", 1: "count out of range", 2: "more rows than the batch holds",
                3: "not enough free pages"}
 SCALINGS = {"none": 0, "linear": 1, "parts": 2}
 _KV_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+# of 4 and 8 bits: enum mlq_kv_type, bytes of a block
+_KV_QUANT = {"q4": (4, 20), "q8": (8, 36)}
 _F32, _I32, _I64 = torch.float32, torch.int32, torch.int64
 
 # A step's calls are a few microseconds each: the checks below ask a tensor for
@@ -115,19 +121,36 @@ class _Fixed:
 
 
 class PagedCache(_Fixed):
-    """keys and values [n_layers, n_pages, n_kv_heads, page_size, head_dim]."""
+    """keys and values [n_layers, n_pages, n_kv_heads, page_size, head_dim]; with
+    quant "q4" or "q8" uint8 [n_layers, n_pages, n_kv_heads, page_size, bytes of a
+    row] (mlq_paged_cache says what they hold), for heads of head_dim elements
+    (None: as many as the row has)."""
 
-    def __init__(self, keys, values):
-        if keys.dtype not in _KV_TYPES:
-            raise ValueError("the cache must be float32, float16 or bfloat16")
+    def __init__(self, keys, values, quant: str | None = None, head_dim: int | None = None):
+        if quant is not None and quant not in _KV_QUANT:
+            raise ValueError(f"quant must be one of {sorted(_KV_QUANT)}")
+        if keys.dtype not in _KV_TYPES if quant is None else keys.dtype is not torch.uint8:
+            raise ValueError("the cache must be float32, float16 or bfloat16, or uint8 with quant")
         if keys.dim() != 5 or keys.shape != values.shape or keys.dtype != values.dtype or \
            keys.device != values.device or not keys.is_cuda or not keys.is_contiguous() or \
            not values.is_contiguous():
             raise ValueError("keys and values must be contiguous device tensors [n_layers, "
                              "n_pages, n_kv_heads, page_size, head_dim] of one type and device")
         self.keys, self.values, self.device = keys, values, keys.device
-        self.n_layers, self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = keys.shape
-        self.struct = MlqPagedCache(keys.data_ptr(), values.data_ptr(), _KV_TYPES[keys.dtype],
+        self.n_layers, self.n_pages, self.n_kv_heads, self.page_size, width = keys.shape
+        self.quant = quant
+        if quant is None:
+            if head_dim is not None and head_dim != width:
+                raise ValueError("head_dim is the last size of keys and values")
+            head_dim, kind = width, _KV_TYPES[keys.dtype]
+        else:
+            kind, block = _KV_QUANT[quant]
+            if head_dim is None:
+                head_dim = width // block * 32
+            if not 0 < head_dim <= 256 or quant_row_bytes(quant, head_dim) != width:
+                raise ValueError(f"a row of {head_dim} elements in {quant} does not have {width} bytes")
+        self.head_dim = head_dim
+        self.struct = MlqPagedCache(keys.data_ptr(), values.data_ptr(), kind,
                                     self.n_layers, self.n_pages, self.page_size, self.n_kv_heads,
                                     self.head_dim)
         self.ref = ctypes.byref(self.struct)
@@ -141,11 +164,23 @@ class PagedCache(_Fixed):
     @classmethod
     def empty(cls, n_layers: int, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int,
               dtype=None, device: str = "cuda") -> "PagedCache":
-        """Uninitialised pages: what lies behind a sequence's end is never used."""
-        shape = (n_layers, n_pages, n_kv_heads, page_size, head_dim)
+        """Uninitialised pages: what lies behind a sequence's end is never used.
+        dtype: a torch type, "q4" or "q8"."""
         dtype = torch.float32 if dtype is None else dtype
+        quant = dtype if isinstance(dtype, str) else None
+        if quant is not None and (quant not in _KV_QUANT or not 0 < head_dim <= 256):
+            raise ValueError(f"dtype must be a torch type or one of {sorted(_KV_QUANT)}, the "
+                             "latter with heads of up to 256")
+        width = head_dim if quant is None else quant_row_bytes(quant, head_dim)
+        shape = (n_layers, n_pages, n_kv_heads, page_size, width)
+        dtype = dtype if quant is None else torch.uint8
         return cls(torch.empty(shape, dtype=dtype, device=device),
-                   torch.empty(shape, dtype=dtype, device=device))
+                   torch.empty(shape, dtype=dtype, device=device), quant, head_dim)
+
+
+def quant_row_bytes(quant: str, head_dim: int) -> int:
+    """Bytes of a head's row in a cache of "q4" or "q8": 2, 4 or 8 blocks."""
+    return _KV_QUANT[quant][1] * (2 if head_dim <= 64 else 4 if head_dim <= 128 else 8)
 
 
 class PagedBatch(_Fixed):
@@ -314,6 +349,53 @@ def qk_norm_rope(rotary: Rotary, q, k, v, positions, q_out=None, k_out=None, cac
                                       kop, kos, cp, layer, sp, _raw_stream(index)),
                "mlq_qk_norm_rope")
     return q_out, k_out
+
+
+def write(cache: PagedCache, layer: int, k, v, slots, k_out=None, v_out=None, stream=None) -> None:
+    """Rows of keys and values [rows, n_kv_heads, head_dim], as they are, to
+    their slots of the layer (mlq_paged_write): rounded or quantised to the
+    cache's type; a slot outside the cache leaves its row out. k_out and v_out
+    (k and v themselves for in place) receive the values that the cache now
+    stands for."""
+    index, hd, kv = cache.index, cache.head_dim, cache.n_kv_heads
+    if stream is not None or index != _current_device():
+        return _elsewhere(lambda: write(cache, layer, k, v, slots, k_out, v_out), index, stream)
+    _int32("layer", layer)
+    kp, ks = _rows("k", k, None, kv, hd, index)
+    n = k.shape[0]
+    vp, vs = _rows("v", v, n, kv, hd, index)
+    kop = vop = None
+    kos = vos = 0
+    if k_out is not None:
+        kop, kos = (kp, ks) if k_out is k else _rows("k_out", k_out, n, kv, hd, index)
+    if v_out is not None:
+        vop, vos = (vp, vs) if v_out is v else _rows("v_out", v_out, n, kv, hd, index)
+    sp = _ints("slots", slots, _I64, index, None, n)
+    if n:
+        _check(lib().mlq_paged_write(cache.ref, layer, n, sp, kp, ks, vp, vs, kop, kos, vop, vos,
+                                     _raw_stream(index)), "mlq_paged_write")
+
+
+def read(cache: PagedCache, layer: int, slots, k_out=None, v_out=None, stream=None):
+    """(k_out, v_out) [rows, n_kv_heads, head_dim] float32: the values at each
+    slot of the layer (mlq_paged_read), in new tensors unless given. A row whose
+    slot is outside the cache is left as it was (new ones: zeros)."""
+    index, hd, kv = cache.index, cache.head_dim, cache.n_kv_heads
+    if stream is not None or index != _current_device():
+        return _elsewhere(lambda: read(cache, layer, slots, k_out, v_out), index, stream)
+    _int32("layer", layer)
+    sp = _ints("slots", slots, _I64, index)
+    n = _int32("the number of slots", slots.shape[0])
+    if k_out is None:
+        k_out = torch.zeros((n, kv, hd), dtype=_F32, device=cache.device)
+    if v_out is None:
+        v_out = torch.zeros((n, kv, hd), dtype=_F32, device=cache.device)
+    kp, ks = _rows("k_out", k_out, n, kv, hd, index)
+    vp, vs = _rows("v_out", v_out, n, kv, hd, index)
+    if n:
+        _check(lib().mlq_paged_read(cache.ref, layer, n, sp, kp, ks, vp, vs, _raw_stream(index)),
+               "mlq_paged_read")
+    return k_out, v_out
 
 
 class AttentionRule(_Fixed):

@@ -1,0 +1,105 @@
+"""CPU: argument checks of what a paged cache of 4 or 8 bits adds to the C ABI
+(every case returns before a launch), its sizes, and the definition's own
+properties that the GPU tests rely on."""
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import pytest
+
+import kv_quant_ref as kvq
+
+FAKE = 1 << 20  # a non-null, aligned pointer that no check dereferences
+OK, ARG, SHAPE, SMALL, UNSUPPORTED = 0, -1, -2, -4, -5
+TYPE = {"q4": 4, "q8": 8}
+
+
+def cache(pkg, **kw):
+    f = dict(keys=FAKE, values=FAKE, type=4, n_layers=2, n_pages=9, page_size=16, n_kv_heads=4, head_dim=128)
+    f.update(kw)
+    return pkg.MlqPagedCache(*(f[n] for n, _ in pkg.MlqPagedCache._fields_))
+
+
+@pytest.mark.parametrize("kind", ["q4", "q8"])
+@pytest.mark.parametrize("hd", [8, 64, 72, 128, 136, 256])
+def test_cache_bytes(pkg, kind, hd):
+    n = ctypes.c_size_t(7)
+    c = cache(pkg, keys=None, values=None, type=TYPE[kind], head_dim=hd)
+    assert pkg.lib().mlq_paged_cache_bytes(ctypes.byref(c), ctypes.byref(n)) == OK
+    assert n.value == 2 * 9 * 4 * 16 * kvq.row_bytes(hd, kind)
+
+
+@pytest.mark.parametrize("kw,want", [(dict(type=5), ARG), (dict(type=7), ARG), (dict(type=9), ARG), (dict(head_dim=100), UNSUPPORTED),
+                                     (dict(head_dim=264), UNSUPPORTED), (dict(page_size=8), UNSUPPORTED), (dict(n_pages=0), SHAPE)])
+def test_geometry(pkg, kw, want):
+    n = ctypes.c_size_t()
+    c = cache(pkg, **kw)
+    assert pkg.lib().mlq_paged_cache_bytes(ctypes.byref(c), ctypes.byref(n)) == want
+
+
+def test_write_and_read_refusals(pkg):
+    def write(c=None, layer=0, rows=3, slots=FAKE, k=FAKE, ks=512, v=FAKE, vs=512, ko=None, kos=0, vo=None, vos=0):
+        c = cache(pkg) if c is None else c
+        return pkg.lib().mlq_paged_write(ctypes.byref(c), layer, rows, slots, k, ks, v, vs, ko, kos, vo, vos, None)
+
+    def read(c=None, layer=0, rows=3, slots=FAKE, k=FAKE, ks=512, v=FAKE, vs=512):
+        c = cache(pkg) if c is None else c
+        return pkg.lib().mlq_paged_read(ctypes.byref(c), layer, rows, slots, k, ks, v, vs, None)
+
+    for call in (write, read):
+        for kw, want in [(dict(layer=2), SHAPE), (dict(layer=-1), SHAPE), (dict(rows=-1), SHAPE), (dict(slots=None), ARG), (dict(k=None), ARG),
+                         (dict(v=None), ARG), (dict(k=FAKE + 4), ARG), (dict(v=FAKE + 8), ARG), (dict(ks=510), ARG), (dict(ks=508), SHAPE),
+                         (dict(vs=508), SHAPE), (dict(vs=-512), SHAPE), (dict(rows=1 << 26), UNSUPPORTED), (dict(rows=2 ** 31 - 1), UNSUPPORTED),
+                         (dict(rows=0), OK)]:
+            assert call(**kw) == want, (call, kw)
+        for kw, want in [(dict(keys=None), ARG), (dict(values=FAKE + 8), ARG), (dict(type=3), ARG), (dict(head_dim=12), UNSUPPORTED)]:
+            assert call(c=cache(pkg, **kw)) == want, (call, kw)
+    assert pkg.lib().mlq_paged_write(None, 0, 3, FAKE, FAKE, 512, FAKE, 512, None, 0, None, 0, None) == ARG
+    assert pkg.lib().mlq_paged_read(None, 0, 3, FAKE, FAKE, 512, FAKE, 512, None) == ARG
+    other = 2 * FAKE
+    for kw, want in [(dict(ko=other, kos=508), SHAPE), (dict(vo=other, vos=508), SHAPE), (dict(ko=other + 4, kos=512), ARG),
+                     (dict(ko=FAKE, kos=516), ARG), (dict(vo=FAKE, vos=516), ARG), (dict(vo=other, vos=514), ARG),
+                     (dict(rows=0, ko=other, kos=512, vo=other, vos=512), OK)]:
+        assert write(**kw) == want, kw
+    # (the largest number of rows that a launch of this cache holds is checked, not launched)
+    assert write(rows=0) == OK and read(rows=0) == OK
+
+
+def test_front_end_refusals(pkg):
+    import torch
+    from mini_llama_amd import paged
+    rows = torch.zeros((1, 2, 4, 16, 80), dtype=torch.uint8)
+    for kw in (dict(), dict(quant="q5"), dict(quant="q4"), dict(quant="q8", head_dim=128)):  # (a CPU tensor is refused last)
+        with pytest.raises(ValueError):
+            paged.PagedCache(rows, rows, **kw)
+    with pytest.raises(ValueError):
+        paged.PagedCache(rows.float(), rows.float(), quant="q4")
+    with pytest.raises(ValueError):
+        paged.PagedCache.empty(1, 2, 16, 4, 128, "q6", device="cpu")
+    with pytest.raises(ValueError):
+        paged.PagedCache.empty(1, 2, 16, 4, 264, "q4", device="cpu")
+    assert [paged.quant_row_bytes(k, hd) for k in ("q4", "q8") for hd in (8, 64, 128, 256)] == [40, 40, 80, 160, 72, 72, 144, 288]
+
+
+@pytest.mark.parametrize("kind", ["q4", "q8"])
+@pytest.mark.parametrize("hd", [8, 40, 64, 80, 128, 200, 256])
+def test_definition(kind, hd):
+    """Values lie within half a step of what was quantised, and a little more
+    at the ends: m is off by half an fp16 step, d by half of its own a level."""
+    r = np.random.default_rng(hd)
+    x = (r.standard_normal((40, 3, hd)) * np.exp(r.uniform(-3, 3, (40, 3, 1)))).astype(np.float32)
+    levels, middle, _ = kvq.KINDS[kind]
+    rows = kvq.quantise(x, kind)
+    assert rows.shape == (40, 3, kvq.row_bytes(hd, kind))
+    y = kvq.values(rows, kind, hd)
+    for b in range(0, hd, 32):
+        e, f = x[..., b:b + 32].astype(np.float64), y[..., b:b + 32]
+        d = (e.max(-1) - e.min(-1)) / levels
+        big = np.abs(e).max(-1) + levels * d
+        bound = 0.5 * d * (1 + 2.0 ** -10) + big * 2.0 ** -11 + levels * (d * 2.0 ** -11 + 2.0 ** -25) + 1e-12
+        assert (np.abs(e - f).max(-1) <= bound).all()
+    # what was read is written back as it was, but for m and d: both ends have their codes, so lo, hi
+    # and d come back to half an fp16 step each, 2^-11 (|m| + levels d) in all, at most three times max |y|
+    again = kvq.values(kvq.quantise(y.astype(np.float32), kind), kind, hd)
+    assert np.abs(again - y).max() <= np.abs(y).max() * 2.0 ** -9
