@@ -8,11 +8,42 @@
 #include <type_traits>
 
 #include "device_common.h"
+#include "kv_quant.h"
 #include "paged.h"
 #include "paged_device.h"
 
 namespace mlq {
 namespace {
+
+// A cache's type: float, _Float16 and __bf16 are the elements as they lie, KvQ4
+// and KvQ8 rows of codes and scales.
+template <typename T>
+constexpr int kUnitBytes = 4;  // (of no meaning but for the last two)
+template <>
+constexpr int kUnitBytes<KvQ4> = KvQ4::kUnit;
+template <>
+constexpr int kUnitBytes<KvQ8> = KvQ8::kUnit;
+template <typename T>
+constexpr bool kQuantised = kUnitBytes<T> < 4;
+template <typename T>
+__device__ __forceinline__ int row_bytes_of(int hd) {
+  if constexpr (kQuantised<T>) return kv_row_bytes(T::kType, hd);
+  else return hd * (int)sizeof(T);
+}
+// Element d of a head's row.
+template <typename T>
+__device__ __forceinline__ float row_element(const char* row, int d, int hd) {
+  if constexpr (kQuantised<T>) {
+    const int nb = kv_blocks(hd), b = d >> 5, unit = ((d & 31) >> 1) * nb + b;
+    const KvScale s = *(const KvScale*)(row + 16 * nb * T::kUnit + 4 * b);
+    int code;
+    if constexpr (T::kUnit == 1) code = (uint8_t)row[unit] >> (4 * (d & 1)) & 15;
+    else code = (uint8_t)row[2 * unit + (d & 1)];
+    return kv_value<T>(code, s);
+  } else {
+    return (float)((const T*)row)[d];
+  }
+}
 
 // One row of one query head by one wave, in plain fp32: a lane scores a key of
 // a tile of 64 against q in LDS, then takes head dims lane, lane + 64, .. of
@@ -49,10 +80,10 @@ __device__ void slow_row(const PagedAttnArgs& a, int seq, int row, int pos, int 
       if (page < 0 || page >= a.n_pages) {
         bad = true;
       } else {
-        base = ((((int64_t)page * a.n_kv + kvh) << a.page_shift) + (t & ((1 << a.page_shift) - 1))) * a.hd;
-        const T* k = (const T*)a.keys + base;
+        base = ((((int64_t)page * a.n_kv + kvh) << a.page_shift) + (t & ((1 << a.page_shift) - 1))) * row_bytes_of<T>(a.hd);
+        const char* k = (const char*)a.keys + base;
         s = 0.0f;
-        for (int d = 0; d < a.hd; ++d) s += qs[d] * (float)k[d];
+        for (int d = 0; d < a.hd; ++d) s += qs[d] * row_element<T>(k, d, a.hd);
         s *= a.scale;
         if (a.softcap > 0.0f) s = a.softcap * tanhf(s / a.softcap);
         s += slope * (float)(t - pos);
@@ -73,10 +104,10 @@ __device__ void slow_row(const PagedAttnArgs& a, int seq, int row, int pos, int 
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[j] *= al;
     for (int i = 0; i < min(64, len - t0); ++i) {
-      const T* v = (const T*)a.values + at[i];
+      const char* v = (const char*)a.values + at[i];
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (lane + 64 * j < a.hd) acc[j] += ps[i] * (float)v[lane + 64 * j];
+        if (lane + 64 * j < a.hd) acc[j] += ps[i] * row_element<T>(v, lane + 64 * j, a.hd);
     }
   }
   float* out = a.out + row * a.out_stride + (int64_t)head * a.hd;
@@ -123,6 +154,10 @@ constexpr int kDecWaves = 4, kDecThreads = 64 * kDecWaves;
 constexpr int dec_per_cu(int hd, int64_t pieces, int cus) {
   return hd <= 64 ? (pieces >= 6 * (int64_t)cus ? 6 : 3) : hd <= 128 ? 2 : 1;
 }
+// Weights times d, for the products over codes, have a power of two of their own:
+// 2^15 less that of the largest d so far, which fp16's least normal numbers leave
+// at 2^29 and an infinite or NaN one at 2^-2.
+constexpr float kMostLift = 29.0f;
 constexpr int kDecMaxSeqs = 4096;  // sequences of a launch: their prefix sums lie in LDS
 
 typedef float f4 __attribute__((ext_vector_type(4)));
@@ -157,6 +192,56 @@ struct KvTraits<__bf16> {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
 };
+
+// Codes are whole numbers that fp16 holds: the parts are those of an fp16 cache.
+template <>
+struct KvTraits<KvQ4> : KvTraits<_Float16> {};
+template <>
+struct KvTraits<KvQ8> : KvTraits<_Float16> {};
+
+// Codes less their middle as fp16: those of unit p0 of word w0 and unit p1 of
+// w1, the lower dims in lo, the others in hi. A code in the mantissa of an fp16
+// is an exact sum (device_common.h).
+template <typename T>
+__device__ __forceinline__ void code_pairs(uint32_t w0, int p0, uint32_t w1, int p1, uint32_t& lo, uint32_t& hi) {
+  if constexpr (T::kUnit == 1) {
+    const uint32_t x = __builtin_amdgcn_perm(w1, w0, 0x0c000c00u | (uint32_t)p0 | (uint32_t)(4 + p1) << 16);
+    lo = as_u32(as_h2(and_or(x, 0x000F000Fu, 0x64006400u)) - h2_t{1032, 1032});
+    hi = as_u32(as_h2(and_or(x, 0x00F000F0u, 0x54005400u)) - h2_t{72, 72});
+  } else {
+    const uint32_t x = __builtin_amdgcn_perm(w1, w0, (uint32_t)(2 * p0) | (uint32_t)(2 * p0 + 1) << 8 |
+                                                         (uint32_t)(4 + 2 * p1) << 16 | (uint32_t)(5 + 2 * p1) << 24);
+    uint32_t a, b;
+    q8_pairs(x, a, b);
+    lo = as_u32(as_h2(a) - h2_t{1152, 1152});
+    hi = as_u32(as_h2(b) - h2_t{1152, 1152});
+  }
+}
+// d and m of a scale word.
+__device__ __forceinline__ float scale_d(uint32_t w) { return (float)as_h2(w).x; }
+__device__ __forceinline__ float scale_m(uint32_t w) { return (float)as_h2(w).y; }
+// N words (a half for 0) from an address that is a multiple of 4 (2).
+template <int N>
+__device__ __forceinline__ void load_words(const char* p, uint32_t* w) {
+  typedef uint32_t w4 __attribute__((ext_vector_type(4), aligned(4)));
+  typedef uint32_t w2 __attribute__((ext_vector_type(2), aligned(4)));
+  if constexpr (N == 0) {
+    w[0] = *(const uint16_t*)p;
+  } else if constexpr (N == 1) {
+    w[0] = *(const uint32_t*)p;
+  } else if constexpr (N == 2) {
+    const w2 x = *(const w2*)p;
+    w[0] = x.x;
+    w[1] = x.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const w4 x = *(const w4*)(p + 4 * i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[i + j] = x[j];
+    }
+  }
+}
 
 // a, b = the sum of p's parts, each rounded to nearest: two values of a vec.
 template <typename T>
@@ -246,12 +331,14 @@ __host__ __device__ inline DecodePartials decode_partials(void* ws, int n_seqs, 
 template <typename T, int HD, bool FULL>
 __global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_kernel(PagedAttnArgs a) {
   using Tr = KvTraits<T>;
-  constexpr bool F32 = sizeof(T) == 4;
+  constexpr bool F32 = sizeof(T) == 4, QUANT = kQuantised<T>;
   constexpr int KT = Tr::kKeys, NS = KT / 16;  // keys, runs of 16 keys
   constexpr int NP = Tr::kParts;
   constexpr int KS = F32 ? HD / 16 : HD / 32;  // 16-byte pieces of a K row per lane
   constexpr int VD = HD / 16;                  // dims of V (and of the output) per lane
   constexpr int VW = VD * (int)sizeof(T) / 4;  // their words
+  constexpr int NB = QUANT ? HD / 32 : 1;      // blocks of a quantised row
+  constexpr int UB = NB * kUnitBytes<T>;       // bytes of a unit of all of them
   constexpr int RD = VD < 8 ? VD : 8;          // output dims per lane merged at a time
   constexpr int OS = 16 * RD + 4;
   constexpr int kUnit = kDecWaves * KT;
@@ -364,6 +451,7 @@ __global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_k
   typedef typename std::conditional<F32, f4, bf8>::type raw8;  // (16 bytes of either)
   raw8 qv[F32 ? 1 : NP][F32 ? 1 : KS];
   int q_exp = 0;
+  float q_sum[NB];  // quantised: of each block, with q's power of two
   if constexpr (F32) {
 #pragma unroll
     for (int s = 0; s < KS; ++s) qf[s] = q_at(16 * s + 4 * ak);
@@ -379,12 +467,21 @@ __global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_k
                     fmaxf(fabsf(x[s][j].z), fabsf(x[s][j].w)));
       }
     if constexpr (Tr::kLift != 0.0f) q_exp = pow2_scale_exp(xor32_max(xor16_max(big)));
+    if constexpr (QUANT) {
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const f4 y = x[s][0] + x[s][1];
+        q_sum[s] = ldexp_f(xor32_sum(xor16_sum((y.x + y.y) + (y.z + y.w))), q_exp);
+      }
+    }
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       uint32_t w[NP][4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        float u = x[s][j >> 1][2 * (j & 1)], v = x[s][j >> 1][2 * (j & 1) + 1];
+        // (a quantised key's come as the lower dims of two units, then the others)
+        const int i0 = QUANT ? 4 * (j >> 1) + (j & 1) : 2 * j, i1 = QUANT ? i0 + 2 : i0 + 1;
+        float u = x[s][i0 >> 2][i0 & 3], v = x[s][i1 >> 2][i1 & 3];
         if constexpr (Tr::kLift != 0.0f) {
           u = ldexp_f(u, q_exp);
           v = ldexp_f(v, q_exp);
@@ -417,12 +514,25 @@ __global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_k
     page = out ? 0 : page;
     return (((int64_t)page * a.n_kv + kvh) << a.page_shift) + (kk & mask & ~15);
   };
-  u32x4_t kr[NS][KS];
-  uint32_t vr[F32 ? 4 : 8][VW];
+  u32x4_t kr[QUANT ? 1 : NS][QUANT ? 1 : KS];
+  uint32_t vr[F32 ? 4 : 8][QUANT ? (UB + 3) / 4 : VW];
+  // quantised: the key's units of quarter ak; scales of the quarter's keys
+  uint32_t kq[QUANT ? NS : 1][QUANT ? UB : 1], ks[QUANT ? 4 * NS : 1][NB], vs[QUANT ? 4 * NS : 1][NB];
   int64_t rows[NS];
   auto load_k = [&]() __attribute__((always_inline)) {
+    if constexpr (QUANT) {
+      constexpr int RB = 16 * UB + 4 * NB;
 #pragma unroll
-    for (int u = 0; u < NS; ++u) {
+      for (int u = 0; u < NS; ++u) {
+        const char* p = (const char*)a.keys + rows[u] * RB;
+        load_words<UB>(p + ai * RB + 4 * UB * ak, kq[u]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) load_words<NB>(p + (4 * ak + r) * RB + 16 * UB, ks[4 * u + r]);
+      }
+      return;
+    }
+#pragma unroll
+    for (int u = 0; u < (QUANT ? 0 : NS); ++u) {
       const char* p = (const char*)a.keys + rows[u] * a.hd * sizeof(T) + (size_t)ai * a.hd * sizeof(T);
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
@@ -434,8 +544,18 @@ __global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_k
   };
   // this lane's keys of quarter ak: 4 ak + r of each run
   auto load_v = [&]() __attribute__((always_inline)) {
+    if constexpr (QUANT) {
+      constexpr int RB = 16 * UB + 4 * NB;
 #pragma unroll
-    for (int e = 0; e < 4 * NS; ++e) {
+      for (int e = 0; e < 4 * NS; ++e) {
+        const char* p = (const char*)a.values + (rows[e >> 2] + 4 * ak + (e & 3)) * RB;
+        load_words<UB / 4>(p + UB * ai, vr[e]);
+        load_words<NB>(p + 16 * UB, vs[e]);
+      }
+      return;
+    }
+#pragma unroll
+    for (int e = 0; e < (QUANT ? 0 : 4 * NS); ++e) {
       const char* p = (const char*)a.values +
                       (rows[e >> 2] + 4 * ak + (e & 3)) * a.hd * (int64_t)sizeof(T);
 #pragma unroll
@@ -457,7 +577,13 @@ __global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_k
   };
 
   float m = -INFINITY, l = 0.0f;  // of head ai; l of this quarter's keys
-  f4 acc[VD];                     // dims VD (4 ak + r) + c of head ai in acc[c][r]
+  // dims VD (4 ak + r) + c of head ai in acc[c][r]; quantised: dims 2 (4 ak + r) + c % 2 of block c / 2
+  f4 acc[VD];
+  // quantised: the power of two that weights times d have, and the weights'
+  // sum times m, of this quarter's keys
+  float lift = QUANT ? kMostLift : Tr::kLift, acc_m[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) acc_m[b] = 0.0f;
 #pragma unroll
   for (int c = 0; c < VD; ++c) acc[c] = f4{0.0f, 0.0f, 0.0f, 0.0f};
   int k0 = lo + wave * KT;
@@ -482,6 +608,31 @@ __global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_k
           c = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f4, kr[0][st])[i], qf[st][i], c, 0, 0, 0);
         }
       s[0] = ((c8[0] + c8[1]) + (c8[2] + c8[3])) + ((c8[4] + c8[5]) + (c8[6] + c8[7]));
+    } else if constexpr (QUANT) {
+      // each block's sum over codes, then d times it and m times the sum of q
+#pragma unroll
+      for (int u = 0; u < NS; ++u) {
+        s[u] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          if (!FULL && 32 * b >= a.hd) break;
+          uint32_t w[4];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int x0 = 2 * j * UB + b * T::kUnit, x1 = x0 + UB;  // bytes of the two units
+            code_pairs<T>(kq[u][x0 / 4], x0 % 4 / T::kUnit, kq[u][x1 / 4], x1 % 4 / T::kUnit, w[2 * j], w[2 * j + 1]);
+          }
+          f4 c = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int i = NP - 1; i >= 0; --i)
+            c = Tr::mfma(__builtin_bit_cast(h8_t, u32x4_t{w[0], w[1], w[2], w[3]}), __builtin_bit_cast(h8_t, qv[i][b]), c);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const uint32_t sw = ks[4 * u + r][b];
+            s[u][r] = __builtin_fmaf(scale_m(sw), q_sum[b], __builtin_fmaf(scale_d(sw), c[r], s[u][r]));
+          }
+        }
+      }
     } else {
 #pragma unroll
       for (int u = 0; u < NS; ++u) s[u] = f4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -516,21 +667,46 @@ __global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_k
         if (k < key_begin || k >= hi) {
           p[e] = -INFINITY;
           // (what lies there may be anything, and 0 * inf is not 0)
+          if constexpr (QUANT) {
 #pragma unroll
-          for (int w = 0; w < VW; ++w) vr[e][w] = 0;
+            for (int b = 0; b < NB; ++b) vs[e][b] = 0;
+          } else {
+#pragma unroll
+            for (int w = 0; w < VW; ++w) vr[e][w] = 0;
+          }
         }
       }
     }
 #pragma unroll
     for (int e = 0; e < 4 * NS; ++e) mx = fmaxf(mx, p[e]);
     mx = fmaxf(m, xor32_max(xor16_max(mx)));
-    const float ref = (mx == -INFINITY ? 0.0f : mx) - Tr::kLift;
-    const float al = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mx);
+    float new_lift = Tr::kLift;
+    if constexpr (QUANT) {
+      // The largest d of the tile, by its exponent: a weight times it is to end
+      // below 2^15.
+      typedef uint16_t us2 __attribute__((ext_vector_type(2)));
+      us2 big = {0, 0};
+#pragma unroll
+      for (int e = 0; e < 4 * NS; ++e)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) big = __builtin_elementwise_max(big, __builtin_bit_cast(us2, vs[e][b]));
+      new_lift = fminf(lift, kMostLift - xor32_max(xor16_max((float)(big.x >> 10))));
+    }
+    const float ref = (mx == -INFINITY ? 0.0f : mx) - new_lift;
+    float al = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mx);
     m = mx;
+    if constexpr (QUANT) {
+      al *= __builtin_amdgcn_exp2f(new_lift - lift);
+      lift = new_lift;
+    }
     if (__any(al != 1.0f)) {
       l *= al;
 #pragma unroll
       for (int c = 0; c < VD; ++c) acc[c] *= al;
+      if constexpr (QUANT) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) acc_m[b] *= al;
+      }
     }
     if (plain && !edge) {
       // (scaled and shifted with one rounding)
@@ -555,6 +731,29 @@ __global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_k
 #pragma unroll
         for (int c = 0; c < VD; ++c)
           acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, vr[e][c]), p[e], acc[c], 0, 0, 0);
+    } else if constexpr (QUANT) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        if (!FULL && 32 * b >= a.hd) break;
+        uint32_t w[NP][4], v[2][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t q[NP];
+          split_pair<T>(p[2 * j] * scale_d(vs[2 * j][b]), p[2 * j + 1] * scale_d(vs[2 * j + 1][b]), q);
+#pragma unroll
+          for (int i = 0; i < NP; ++i) w[i][j] = q[i];
+          const int x = b * T::kUnit;
+          code_pairs<T>(vr[2 * j][x / 4], x % 4 / T::kUnit, vr[2 * j + 1][x / 4], x % 4 / T::kUnit, v[0][j], v[1][j]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4 * NS; ++e) acc_m[b] = __builtin_fmaf(scale_m(vs[e][b]), p[e], acc_m[b]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = NP - 1; i >= 0; --i)
+            acc[2 * b + h] = Tr::mfma(__builtin_bit_cast(h8_t, u32x4_t{v[h][0], v[h][1], v[h][2], v[h][3]}),
+                                      __builtin_bit_cast(h8_t, u32x4_t{w[i][0], w[i][1], w[i][2], w[i][3]}), acc[2 * b + h]);
+      }
     } else {
       uint32_t w[NP][4];
 #pragma unroll
@@ -581,6 +780,19 @@ __global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_k
     }
   }
   l = xor32_sum(xor16_sum(l));
+  if constexpr (QUANT) {
+    // (the waves, and the ranges, need not have met the same d)
+    const float down = __builtin_amdgcn_exp2f(-lift);
+    l *= down;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const float sum = xor32_sum(xor16_sum(acc_m[b])) * down;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[2 * b + h][r] = __builtin_fmaf(acc[2 * b + h][r], down, sum);
+    }
+  }
 
   // ---- the waves joined in their order
   __syncthreads();  // (the last piece's readers are done with the LDS)
@@ -593,6 +805,14 @@ __global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_k
 #pragma unroll
   for (int c0 = 0; c0 < VD; c0 += RD) {
     __syncthreads();
+    if constexpr (QUANT) {
+#pragma unroll
+      for (int c = 0; c < RD; c += 2)
+#pragma unroll
+        for (int r = 0; r < 4; r += 2)
+          *(f4*)&merge[wave][ai][16 * c + 8 * ak + 2 * r] =
+              f4{acc[c0 + c][r], acc[c0 + c + 1][r], acc[c0 + c][r + 1], acc[c0 + c + 1][r + 1]};
+    } else
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -602,7 +822,7 @@ __global__ __launch_bounds__(kDecThreads, HD <= 128 ? 2 : 1) void paged_decode_k
     __syncthreads();
     for (int e = tid; e < G * 16 * RD; e += kDecThreads) {
       const int g = e / (16 * RD), x = e % (16 * RD);
-      const int d = VD * (x / RD) + c0 + x % RD;
+      const int d = QUANT ? 16 * c0 + x : VD * (x / RD) + c0 + x % RD;
       if (!FULL && d >= a.hd) continue;
       float mx = -INFINITY;
 #pragma unroll
@@ -1634,6 +1854,8 @@ hipError_t launch_paged_decode(const PagedAttnArgs& all, hipStream_t stream) {
     }
     if (a.type == MLQ_KV_F32) decode_launch_hd<float>(a, a.ranges, stream);
     else if (a.type == MLQ_KV_F16) decode_launch_hd<_Float16>(a, a.ranges, stream);
+    else if (a.type == MLQ_KV_Q4) decode_launch_hd<KvQ4>(a, a.ranges, stream);
+    else if (a.type == MLQ_KV_Q8) decode_launch_hd<KvQ8>(a, a.ranges, stream);
     else decode_launch_hd<__bf16>(a, a.ranges, stream);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;

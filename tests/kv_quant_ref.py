@@ -82,3 +82,72 @@ def heads(r, rows, kv, hd):
             with np.errstate(all="ignore"):
                 flat[i, b:b + 32] = f(flat[i, b:b + 32].copy())
     return x
+
+
+# ---- attention over such rows ------------------------------------------------------
+U = 2.0 ** -24  # half a step of fp32
+
+
+def sizes(rows, kind, hd):
+    """d |c - middle| + |m|: what an element's terms add up to without their signs."""
+    levels, middle, unit = KINDS[kind]
+    nb = blocks(hd)
+    at = 16 * nb * unit
+    s = np.abs(np.ascontiguousarray(rows[..., at:]).view(np.float16).astype(np.float64)).reshape(rows.shape[:-1] + (nb, 2))
+    flat = rows.copy()
+    flat[..., at:] = np.stack([s[..., 0], np.zeros_like(s[..., 1])], -1).astype(np.float16).reshape(rows.shape[:-1] + (-1,)).view(np.uint8)
+    return np.abs(values(flat, kind, hd)) + np.repeat(s[..., 1], 32, -1)[..., :hd]
+
+
+def steps(rows, kind, hd):
+    """The largest d of each row."""
+    nb = blocks(hd)
+    at = 16 * nb * KINDS[kind][2]
+    return np.ascontiguousarray(rows[..., at:]).view(np.float16).astype(np.float64).reshape(rows.shape[:-1] + (nb, 2))[..., 0].max(-1)
+
+
+def attention(q, k, v, pos, scale, softcap=0.0, window=0, slopes=None, kind="q4"):
+    """(out, bound) [heads, hd] of one row q [heads, hd] at pos over the row
+    bytes k and v [kv, keys, bytes] (keys 0 .. pos)."""
+    heads, hd = q.shape
+    kv = k.shape[0]
+    q = np.asarray(q, np.float64)
+    out, bound = np.zeros((heads, hd)), np.zeros((heads, hd))
+    first = max(0, pos + 1 - window) if window else 0
+    n = pos + 1 - first
+    if n <= 0:
+        return out, bound
+    parts = {}
+    for h in range(heads):
+        g = h * kv // heads
+        if g not in parts:
+            kr, vr = k[g, first:pos + 1], v[g, first:pos + 1]
+            parts[g] = values(kr, kind, hd), sizes(kr, kind, hd), values(vr, kind, hd), sizes(vr, kind, hd), steps(vr, kind, hd).max()
+        kk, ks, vv, vs, step = parts[g]
+        s = kk @ q[h] * scale
+        # a block's 32 products and 32 elements of q summed in any order, or the head's products at once;
+        # two roundings a block for d and m; q, and elements, in parts of 22 bits, the parts of a product
+        # below 2^-24 left out, the value's own rounding, scale
+        err = (max(hd, 64) + 2 * blocks(hd) + 20) * U * (ks @ np.abs(q[h])) * abs(scale)
+        # (parts hold 2^-39 of the head's largest |q| and of the row's largest element)
+        err = err + 2.0 ** -38 * (np.abs(q[h]).max() * ks.sum(-1) + np.abs(q[h]).sum() * ks.max(-1)) * abs(scale)
+        if softcap:
+            s = softcap * np.tanh(s / softcap)
+            err = err + 6 * U * np.abs(s)  # division, tanh (3 u), product (derivative at most 1)
+        if slopes is not None:
+            bias = float(slopes[h]) * (np.arange(first, pos + 1) - pos)
+            s = s + bias
+            err = err + 2 * U * (np.abs(bias) + np.abs(s))
+        top = s.max()
+        p = np.exp(s - top)
+        p /= p.sum()
+        # (the exponent's own roundings, as for the other types)
+        err = err + 4 * U * np.abs(s - top) + 8 * U
+        mean = p @ err
+        out[h] = p @ vv
+        # the weights' sum and the output's: at most n roundings each; d, m, and parts of 22 bits
+        bound[h] = (p * (err + mean + (2 * n + 40) * U)) @ vs
+        # parts hold a weight times d down to 2^-39 of the largest weight times the largest d (2^-14 at
+        # least), each with a code of up to `middle`; an element down to 2^-39 of its row's largest
+        bound[h] += n * 2.0 ** -38 * (KINDS[kind][1] * max(step, 2.0 ** -14) + vs.max()) + 2.0 ** -140
+    return out, bound
