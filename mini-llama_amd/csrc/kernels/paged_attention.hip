@@ -1005,6 +1005,15 @@ struct PreTraits<float> : KvTraits<__bf16> {
   }
 };
 
+// Codes and scales are made fp32 values on their way to LDS and go on as those.
+template <>
+struct PreTraits<KvQ4> : PreTraits<float> {};
+template <>
+struct PreTraits<KvQ8> : PreTraits<float> {};
+// Bytes of an element in a thread's registers.
+template <typename T>
+constexpr int kPreBytes = kQuantised<T> ? 4 : (int)sizeof(T);
+
 template <typename T, int HD>
 struct PreTile {
   static constexpr int NK = PreTraits<T>::kCacheParts;
@@ -1017,10 +1026,10 @@ struct PreLds {
   // barrier a tile; fp32's parts leave no room for it (two barriers), and at
   // head dim 256 its registers spill (8000 rows, 16 heads on 2: bf16 988 -> 681
   // us with one buffer, fp16 706 -> 620)
-  static constexpr int kBuf = sizeof(T) == 4 || HD > 128 ? 1 : 2;
+  static constexpr int kBuf = kPreBytes<T> == 4 || HD > 128 ? 1 : 2;
   // steps of q's last part per wave and lane (in registers they spill: fp16 at
   // head dim 256 1058 -> 706 us)
-  static constexpr int kQ = HD < 128 || (PreTraits<T>::kParts < 3 && HD < 256) ? 0 : sizeof(T) == 4 ? (HD > 128 ? 12 : 5) : HD / 16;
+  static constexpr int kQ = HD < 128 || (PreTraits<T>::kParts < 3 && HD < 256) ? 0 : kPreBytes<T> == 4 ? (HD > 128 ? 12 : 5) : HD / 16;
   PreTile<T, HD> tile[kBuf];
   u32x4_t q[kQ > 0 ? kQ : 1][kPreThreads];
   int count[kPreThreads / 64];
@@ -1180,7 +1189,7 @@ __device__ __forceinline__ PrePartial prefill_partial(const PagedAttnArgs& a, in
 // 0; or, to count them, as 1 and the others as 0.
 template <typename T>
 __device__ __forceinline__ uint32_t settled(uint32_t w, bool count) {
-  constexpr bool F32 = sizeof(T) == 4, F16 = std::is_same<T, _Float16>::value;
+  constexpr bool F32 = kPreBytes<T> == 4, F16 = std::is_same<T, _Float16>::value;
   constexpr uint32_t kExp = F32 ? 0x7f800000u : F16 ? 0x7c00u : 0x7f80u, kOne = F32 ? 0x3f800000u : F16 ? 0x3c00u : 0x3f80u;
   if constexpr (F32) {
     const bool bad = (w & kExp) == kExp;
@@ -1209,13 +1218,16 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
   using Tr = PreTraits<T>;
   using M = typename Tr::mat;
   using vec = typename Tr::vec;
-  constexpr bool F32 = sizeof(T) == 4;
+  constexpr bool QUANT = kQuantised<T>;
+  constexpr int ES = kPreBytes<T>;
+  constexpr bool F32 = ES == 4;
   constexpr int NP = Tr::kParts, NK = Tr::kCacheParts;
   constexpr int KT = HD / 16;        // 16-dim steps of the scores
   constexpr int VB = HD / 32;        // 32-dim blocks of the output
-  constexpr int KW = HD / 8 * (int)sizeof(T) / 4;   // words of K per thread: HD / 8 dims of a key
+  constexpr int KW = HD / 8 * ES / 4;   // words of K per thread: HD / 8 dims of a key
   constexpr int VDT = HD / 32;       // dims of V per thread, of 4 keys
-  constexpr int VWT = VDT * (int)sizeof(T) / 4;     // their words a key (fp16 / bf16, HD 64: 1)
+  constexpr int VWT = VDT * ES / 4;     // their words a key (fp16 / bf16, HD 64: 1)
+  constexpr int NB = HD / 32, UB = NB * kUnitBytes<T>;  // quantised: blocks, bytes of a unit of all of them
   constexpr float kSlack = Tr::kLift == 0.0f ? 8.0f : 0.0f;
   constexpr int BUF = PreLds<T, HD>::kBuf, QL = PreLds<T, HD>::kQ;
   int* const count_lds = lds.count;
@@ -1296,7 +1308,7 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
 
   // ---- staging: a wave's keys lie in one run of 16 (and so in one page)
   const int32_t* table = a.block_table + (size_t)seq * a.max_pages;
-  const int mask = (1 << a.page_shift) - 1, row_bytes = a.hd * (int)sizeof(T);
+  const int mask = (1 << a.page_shift) - 1, row_bytes = QUANT ? 16 * UB + 4 * NB : a.hd * ES;
   // The wave's run, or the nearest that holds a key which a row sees (a tile may
   // begin before the window, on a page that nobody keeps any more).
   auto key_of = [&](int k0) __attribute__((always_inline)) { return min(max(k0 + 16 * (wave >> 1), sp.kseen), kmax); };
@@ -1311,17 +1323,36 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
     page = outside ? 0 : page;
     return ((((int64_t)page * a.n_kv + kvh) << a.page_shift) + (kk & mask & ~15)) * row_bytes;
   };
-  const int kkey = tid >> 3, kd = (tid & 7) * (16 / (int)sizeof(T));  // K: dims kd + 8 threads' pieces
-  const int vkg = tid >> 5, vd = (tid & 31) * VDT;                    // V: keys 4 vkg .. + 3
+  const int kkey = tid >> 3, kd = (tid & 7) * (16 / ES);  // K: dims kd + 8 threads' pieces
+  // V: keys 4 vkg .. + 3, VDT dims; quantised, two of each of VDT / 2 blocks
+  const int vkg = tid >> 5, vd = QUANT ? 32 * (VDT / 2) * ((tid & 31) >> 4) + 2 * (tid & 15) : (tid & 31) * VDT;
+  auto v_dim = [&](int j) __attribute__((always_inline)) { return QUANT ? vd + 32 * (j >> 1) + (j & 1) : vd + j; };
   uint32_t kw[KW], vw[4][VWT];
+  // quantised, as they lie: two units of every block and all scales of the key;
+  // a unit of VDT / 2 blocks and their scales of each of four
+  constexpr int VB2 = VDT / 2, VU = VB2 * kUnitBytes<T>;
+  uint32_t kc[QUANT ? (2 * UB + 3) / 4 : 1], kscale[QUANT ? NB : 1], vc[4][QUANT ? (VU + 3) / 4 : 1], vscale[4][QUANT ? VB2 : 1];
+  auto two_values = [&](uint32_t unit, uint32_t scale, uint32_t* w) __attribute__((always_inline)) {
+    if constexpr (QUANT) {
+      const KvScale sc = __builtin_bit_cast(KvScale, scale);
+      constexpr int kBits = 4 * T::kUnit;
+      w[0] = __builtin_bit_cast(uint32_t, kv_value<T>(unit & T::kLevels, sc));
+      w[1] = __builtin_bit_cast(uint32_t, kv_value<T>(unit >> kBits & T::kLevels, sc));
+    }
+  };
   // (a run's start is uniform, a lane's place in it never changes)
-  const uint32_t k_at = (kkey & 15) * row_bytes + kd * (int)sizeof(T);
-  const uint32_t v_at = 4 * (vkg & 3) * row_bytes + vd * (int)sizeof(T);
+  const uint32_t k_at = (kkey & 15) * row_bytes + (QUANT ? 2 * UB * (tid & 7) : kd * ES);
+  const uint32_t v_at = 4 * (vkg & 3) * row_bytes + (QUANT ? UB * (tid & 15) + VU * ((tid & 31) >> 4) : vd * ES);
   auto load_k = [&](int64_t run) __attribute__((always_inline)) {
     const char* p = (const char*)a.keys + run;
+    if constexpr (QUANT) {
+      load_words<2 * UB / 4>(p + k_at, kc);
+      load_words<NB>(p + (kkey & 15) * row_bytes + 16 * UB, kscale);
+      return;
+    }
 #pragma unroll
-    for (int w = 0; w < KW; w += 4) {
-      const bool in = FULL || kd + w * 32 / (int)sizeof(T) < a.hd;
+    for (int w = 0; w < (QUANT ? 0 : KW); w += 4) {
+      const bool in = FULL || kd + w * 32 / ES < a.hd;
       const u32x4_t x = in ? *(const u32x4_t*)(p + k_at + w * 32) : u32x4_t{0, 0, 0, 0};
 #pragma unroll
       for (int i = 0; i < 4; ++i) kw[w + i] = x[i];
@@ -1331,10 +1362,14 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const char* p = (const char*)a.values + run + e * row_bytes;
-      if constexpr (VWT >= 4) {
+      if constexpr (QUANT) {
+        if constexpr (VU == 1) vc[e][0] = *(const uint8_t*)(p + v_at);
+        else load_words<VU / 4>(p + v_at, vc[e]);
+        load_words<VB2>(p + 4 * (vkg & 3) * row_bytes + 16 * UB + 4 * VB2 * ((tid & 31) >> 4), vscale[e]);
+      } else if constexpr (VWT >= 4) {
 #pragma unroll
         for (int w = 0; w < VWT; w += 4) {
-          const bool in = FULL || vd + w * 4 / (int)sizeof(T) < a.hd;
+          const bool in = FULL || vd + w * 4 / ES < a.hd;
           const u32x4_t x = in ? *(const u32x4_t*)(p + v_at + 4 * w) : u32x4_t{0, 0, 0, 0};
 #pragma unroll
           for (int i = 0; i < 4; ++i) vw[e][w + i] = x[i];
@@ -1349,6 +1384,15 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
     }
   };
   auto put_k = [&](PreTile<T, HD>& tl, int k0) __attribute__((always_inline)) {
+    if constexpr (QUANT) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const int at = u * UB + b * kUnitBytes<T>;
+          two_values(kc[at / 4] >> (8 * (at % 4)), kscale[b], kw + 4 * b + 2 * u);
+        }
+    }
     if constexpr (AGAIN)
       if (k0 + kkey <= kmax) {
 #pragma unroll
@@ -1370,6 +1414,15 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
     }
   };
   auto put_v = [&](PreTile<T, HD>& tl, int k0) __attribute__((always_inline)) {
+    if constexpr (QUANT) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int b = 0; b < VB2; ++b) {
+          const int at = b * kUnitBytes<T>;
+          two_values(vc[e][at / 4] >> (8 * (at % 4)), vscale[e][b], vw[e] + 2 * b);
+        }
+    }
     if (k0 + kPreKeys - 1 > kmax) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -1388,13 +1441,13 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
     const int unit = 2 * (vkg >> 2) + (vkg & 1), sub = 4 * ((vkg >> 1) & 1);
 #pragma unroll
     for (int j = 0; j < VDT; ++j) {
-      const int at = v_slot(unit, vd + j) + sub;
+      const int at = v_slot(unit, v_dim(j)) + sub;
       if constexpr (F32) {
         uint32_t x[3], y[3];
         split_pair<__bf16>(__builtin_bit_cast(float, vw[0][j]), __builtin_bit_cast(float, vw[1][j]), x);
         split_pair<__bf16>(__builtin_bit_cast(float, vw[2][j]), __builtin_bit_cast(float, vw[3][j]), y);
 #pragma unroll
-        for (int i = 0; i < 3; ++i) *(u32x2_t*)&tl.v[i][vd + j][at] = u32x2_t{x[i], y[i]};
+        for (int i = 0; i < 3; ++i) *(u32x2_t*)&tl.v[i][v_dim(j)][at] = u32x2_t{x[i], y[i]};
       } else {
         const uint32_t sel = j & 1 ? 0x07060302u : 0x05040100u;
         *(u32x2_t*)&tl.v[0][vd + j][at] =
@@ -1892,6 +1945,8 @@ size_t plan_paged_prefill(PagedAttnArgs& a) {
 hipError_t launch_paged_prefill(const PagedAttnArgs& a, hipStream_t stream) {
   if (a.type == MLQ_KV_F32) return prefill_launch_type<float>(a, stream);
   if (a.type == MLQ_KV_F16) return prefill_launch_type<_Float16>(a, stream);
+  if (a.type == MLQ_KV_Q4) return prefill_launch_type<KvQ4>(a, stream);
+  if (a.type == MLQ_KV_Q8) return prefill_launch_type<KvQ8>(a, stream);
   return prefill_launch_type<__bf16>(a, stream);
 }
 

@@ -329,7 +329,6 @@ int mlq_paged_attention_workspace(const mlq_paged_cache* c, int n_heads, int n_s
                                   int max_len, size_t* bytes) {
   const int rc = check_geometry(c);
   if (rc != MLQ_OK) return rc;
-  if (kv_quantised(c->type) && max_rows > 0) return MLQ_ERR_UNSUPPORTED;
   if (bytes == nullptr) return MLQ_ERR_INVALID_ARG;
   if (n_heads <= 0 || n_heads % c->n_kv_heads != 0 || n_seqs <= 0 || max_rows < 0 || max_len <= 0)
     return MLQ_ERR_SHAPE;
@@ -375,7 +374,6 @@ int mlq_paged_attention_prefill(const mlq_paged_cache* c, int layer, const mlq_p
   PagedAttnArgs a;
   const int rc = check_attention(c, layer, b, rule, n_heads, q, q_stride, out, out_stride, &a);
   if (rc != MLQ_OK) return rc;
-  if (kv_quantised(c->type)) return MLQ_ERR_UNSUPPORTED;
   if (b->row_start == nullptr) return MLQ_ERR_INVALID_ARG;
   if (b->max_rows <= 0 || max_len <= 0 || max_len > (int64_t)b->max_pages * c->page_size)
     return MLQ_ERR_SHAPE;

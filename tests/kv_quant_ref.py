@@ -100,10 +100,12 @@ def sizes(rows, kind, hd):
 
 
 def steps(rows, kind, hd):
-    """The largest d of each row."""
+    """The largest d of each row; one that is not finite counts as 2^17, past the
+    largest that is."""
     nb = blocks(hd)
     at = 16 * nb * KINDS[kind][2]
-    return np.ascontiguousarray(rows[..., at:]).view(np.float16).astype(np.float64).reshape(rows.shape[:-1] + (nb, 2))[..., 0].max(-1)
+    d = np.ascontiguousarray(rows[..., at:]).view(np.float16).astype(np.float64).reshape(rows.shape[:-1] + (nb, 2))[..., 0]
+    return np.where(np.isfinite(d), d, 2.0 ** 17).max(-1)
 
 
 def attention(q, k, v, pos, scale, softcap=0.0, window=0, slopes=None, kind="q4"):
@@ -149,5 +151,5 @@ def attention(q, k, v, pos, scale, softcap=0.0, window=0, slopes=None, kind="q4"
         bound[h] = (p * (err + mean + (2 * n + 40) * U)) @ vs
         # parts hold a weight times d down to 2^-39 of the largest weight times the largest d (2^-14 at
         # least), each with a code of up to `middle`; an element down to 2^-39 of its row's largest
-        bound[h] += n * 2.0 ** -38 * (KINDS[kind][1] * max(step, 2.0 ** -14) + vs.max()) + 2.0 ** -140
+        bound[h] += n * 2.0 ** -38 * (KINDS[kind][1] * max(step, 2.0 ** -14) + np.nanmax(vs, initial=0.0)) + 2.0 ** -140
     return out, bound

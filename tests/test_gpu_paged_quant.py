@@ -239,7 +239,8 @@ class Problem:
     def compare(self, out, want, what=""):
         out = out.double().cpu().numpy()
         for r, (y, bound) in want.items():
-            bad = ~(np.abs(out[r] - y) <= bound)
+            # (a block past fp16's range reads as NaN, and so do the rows that see it)
+            bad = ~((np.abs(out[r] - y) <= bound) | (np.isnan(out[r]) & np.isnan(y)))
             assert not bad.any(), (what, r, int(bad.sum()), float(np.nanmax(np.abs(out[r] - y) / bound)), out[r][bad][:3], y[bad][:3])
 
     def some(self, n):
@@ -666,6 +667,8 @@ def test_serving_loop(paged, kind, graph):
         slots, start, lengths = (t.cpu().numpy() for t in (batch.slots, batch.row_start, batch.lengths))
         table, keys, vals = (t.cpu().numpy() for t in (batch.block_table, cache.keys[0], cache.values[0]))
         n = int(start[-1])
+        if n == 0:
+            continue
         at = (slots[:n] // page, slice(None), slots[:n] % page)
         assert kvq.same_rows(keys[at], kvq.quantise(k_out[:n].cpu().numpy(), kind), hd, kind)
         v = qkv[:n, (heads + kv) * hd:].view(n, kv, hd).cpu().numpy()
