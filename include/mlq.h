@@ -690,6 +690,41 @@ int mlq_paged_attention_prefill(const mlq_paged_cache* c, int layer, const mlq_p
                                 int64_t q_stride, float* out, int64_t out_stride, int max_len,
                                 void* ws, size_t ws_bytes, mlq_stream_t stream);
 
+/* ---------------------------------------------------------------------- */
+/* The tokens of a batched step                                             */
+/* ---------------------------------------------------------------------- */
+/* Settings of each row (device arrays [rows], each may be NULL: temperature 1, no
+ * filter). temperature: 0, negative or NaN takes the largest logit. top_k: 0 or
+ * less for none. top_p: 1, more or NaN for none. min_p: 0, less or NaN for none. */
+typedef struct mlq_sampling {
+  const float* temperature;
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+} mlq_sampling;
+
+/* tokens[r] from row r of logits (stride in floats, not negative; 0 draws from
+ * one row several times): weights
+ * w = exp((l - max) / temperature); tokens in the order of falling logits, equal
+ * ones by index; the first top_k of them; of those the fewest first ones whose
+ * weights add up to top_p of theirs; of those the ones with w >= min_p; the
+ * first of all always stays; of what stays the first token whose weights, added
+ * up to it, pass uniform[r] times their sum. uniform: in [0, 1) (below 0 and NaN count
+ * as 0, 1 and above as the last). Logits that are -inf or NaN are no tokens,
+ * inf counts as the largest finite number; a row without tokens gives -1. Sums are
+ * exact ones of weights in units of 2^-44, which a double exponential gives: the
+ * token is that of real arithmetic unless uniform or top_p times a sum is within
+ * about 2^-40 of a border, and the same in every call. Random
+ * numbers are the caller's: the reference's sampler draws them on the host
+ * (src/sampler.cc). vocab up to 2^19, rows up to 2^20 (MLQ_ERR_UNSUPPORTED
+ * otherwise); rows = 0 does nothing. s may be NULL. ws: mlq_sample_workspace bytes,
+ * 256-byte aligned, scratch, may be NULL when that is 0; calls that share one
+ * (two captured graphs, too) must be ordered. */
+int mlq_sample_workspace(int rows, int vocab, size_t* bytes);
+int mlq_sample(const mlq_sampling* s, int rows, int vocab, const float* logits, int64_t stride,
+               const float* uniform, int32_t* tokens, void* ws, size_t ws_bytes,
+               mlq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

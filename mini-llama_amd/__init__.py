@@ -137,6 +137,12 @@ class MlqAttentionRule(ctypes.Structure):
                 ("window", ctypes.c_int32), ("slopes", ctypes.c_void_p)]
 
 
+class MlqSampling(ctypes.Structure):
+    """struct mlq_sampling (include/mlq.h)."""
+    _fields_ = [("temperature", ctypes.c_void_p), ("top_k", ctypes.c_void_p),
+                ("top_p", ctypes.c_void_p), ("min_p", ctypes.c_void_p)]
+
+
 # Every symbol declared in include/mlq.h, with its ctypes signature.
 _P, _I, _Z = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t
 _WP = ctypes.POINTER(MlqWeight)
@@ -204,6 +210,8 @@ SIGNATURES = {
     "mlq_paged_plan": ([_PBP, _I, _I, _P, _P, _P, _P, _P, _P], _I),
     "mlq_rope_frequencies": ([_D, _I, _I, _D, _I, _D, _D, ctypes.POINTER(_D),
                               ctypes.POINTER(_F)], _I),
+    "mlq_sample_workspace": ([_I, _I, ctypes.POINTER(_Z)], _I),
+    "mlq_sample": ([ctypes.POINTER(MlqSampling), _I, _I, _P, _I64, _P, _P, _P, _Z, _P], _I),
     "mlq_paged_write": ([_PCP, _I, _I, _P, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _P], _I),
     "mlq_paged_read": ([_PCP, _I, _I, _P, _P, _I64, _P, _I64, _P], _I),
     "mlq_qk_norm_rope": ([_RTP, _I, _P, _I, _I, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I64,
