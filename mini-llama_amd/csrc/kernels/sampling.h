@@ -18,6 +18,7 @@ struct SampleArgs {
   const float* min_p;
   int32_t* tokens;
 };
-hipError_t launch_sample(const SampleArgs& a, hipStream_t stream);
+size_t sample_workspace(int rows, int vocab);
+hipError_t launch_sample(const SampleArgs& a, void* ws, hipStream_t stream);
 
 }  // namespace mlq

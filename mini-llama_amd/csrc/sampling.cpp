@@ -29,7 +29,7 @@ int mlq_sample_workspace(int rows, int vocab, size_t* bytes) {
   if (bytes == nullptr) return MLQ_ERR_INVALID_ARG;
   const int rc = check_sizes(rows, vocab);
   if (rc != MLQ_OK) return rc;
-  *bytes = 0;
+  *bytes = sample_workspace(rows, vocab);
   return MLQ_OK;
 }
 
@@ -41,8 +41,7 @@ int mlq_sample(const mlq_sampling* s, int rows, int vocab, const float* logits, 
   if (logits == nullptr || uniform == nullptr || tokens == nullptr || ((uintptr_t)ws & 255u) != 0)
     return MLQ_ERR_INVALID_ARG;
   if (stride < 0) return MLQ_ERR_SHAPE;
-  size_t need = 0;
-  if (mlq_sample_workspace(rows, vocab, &need) != MLQ_OK) return MLQ_ERR_SHAPE;
+  const size_t need = sample_workspace(rows, vocab);
   if (ws_bytes < need || (need > 0 && ws == nullptr)) return MLQ_ERR_BUFFER_TOO_SMALL;
   if (rows == 0) return MLQ_OK;
   const mlq_sampling none = {};
@@ -58,7 +57,7 @@ int mlq_sample(const mlq_sampling* s, int rows, int vocab, const float* logits, 
   a.top_p = r.top_p;
   a.min_p = r.min_p;
   a.tokens = tokens;
-  return record_hip(launch_sample(a, (hipStream_t)stream));
+  return record_hip(launch_sample(a, ws, (hipStream_t)stream));
 }
 
 }  // extern "C"
