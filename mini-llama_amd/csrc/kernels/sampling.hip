@@ -166,10 +166,14 @@ __device__ int index_of(const Row& r, SampleLds& lds, uint32_t key, uint64_t n) 
 }
 
 // What of a row is asked for.
+constexpr int kLightK = 1024;
 struct Ask {
   float t, p, least, u;
   int k;
   bool greedy;
+  // few enough are kept that no weight of others is asked for; tokens are counted
+  __device__ __forceinline__ bool light() const { return k > 0 && k <= kLightK; }
+  __device__ __forceinline__ bool counts() const { return k > 0; }
 };
 __device__ __forceinline__ Ask ask_of(const SampleArgs& a, int row) {
   Ask s;
@@ -218,17 +222,9 @@ __device__ __forceinline__ void for_each(const float* logits, int lo, int hi, F 
   }
 }
 
-// The largest of a range and the first index with it, as the key and the index
-// in one number, in every thread; a range without candidates: all ones.
-__device__ uint64_t first_top(const float* logits, int lo, int hi, uint64_t* lds) {
-  float top = -INFINITY;
-  int at = 0x7fffffff;
-  for_each(logits, lo, hi, [&](float l, int i) __attribute__((always_inline)) {
-    if (l > top) {
-      top = l;
-      at = i;
-    }
-  });
+// The largest of what the threads have and the first index with it, as the key
+// and the index in one number, in every thread; no candidates: all ones.
+__device__ __forceinline__ uint64_t first_of(float top, int at, uint64_t* lds) {
   const float best = wave_max(top);
   uint32_t first = top == best ? (uint32_t)at : 0x7fffffffu;
 #pragma unroll
@@ -240,6 +236,40 @@ __device__ uint64_t first_top(const float* logits, int lo, int hi, uint64_t* lds
 #pragma unroll
   for (int w = 0; w < kSampleWaves; ++w) least = min(least, lds[w]);
   return least;
+}
+// Calls `all` with the f that goes over the candidates of a range: up to kHeld of
+// them are asked for at once and stay in registers however often it is called.
+constexpr int kHeldQuads = 8, kHeld = 4 * kHeldQuads * kSampleThreads;
+template <typename A>
+__device__ __forceinline__ void over(const float* logits, int lo, int hi, A all) {
+  typedef float v4 __attribute__((ext_vector_type(4), aligned(4)));
+  constexpr int kStep = 4 * kSampleThreads;
+  if (hi - lo > kHeld) {
+    all([&](auto f) __attribute__((always_inline)) { for_each(logits, lo, hi, f); });
+    return;
+  }
+  v4 x[kHeldQuads];
+  const int i0 = lo + 4 * (int)threadIdx.x;
+#pragma unroll
+  for (int j = 0; j < kHeldQuads; ++j) {
+    const int i = i0 + j * kStep;
+    x[j] = v4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    if (i + 3 < hi) {
+      x[j] = *(const v4*)(logits + i);
+    } else if (i < hi) {
+      x[j].x = logits[i];
+      if (i + 1 < hi) x[j].y = logits[i + 1];
+      if (i + 2 < hi) x[j].z = logits[i + 2];
+    }
+  }
+  all([&](auto f) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < kHeldQuads; ++j)
+      if (i0 + j * kStep < hi) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) f(candidate(x[j][c]), i0 + j * kStep + c);
+      }
+  });
 }
 
 // A row by itself, whatever its logits: everything by histograms of the whole
@@ -295,7 +325,7 @@ __device__ int sample_row(const SampleArgs& a, int row, const Ask& s, float top,
 // longer than kListed, or a place lies behind the last bin, the row is done by
 // sample_row.
 constexpr int kGrid = 1024;     // bins, the last of them everything behind the others
-constexpr int kListed = 4096, kLightK = 1024;
+constexpr int kListed = 4096;
 constexpr int kPartLeast = 4096;
 constexpr int kRowsAtOnce = 1024;
 static_assert(kGrid == kSampleThreads, "a bin a thread");
@@ -322,7 +352,6 @@ struct PartsView {
   RowState* state;     // [rows]
   uint64_t* before_w;  // [rows][kGrid + 1] units before each bin
   uint32_t* before_c;  // [rows][kGrid + 1] tokens
-  uint32_t* listed;    // [rows][kGrid + 1] listed ones
   uint64_t* list;      // [rows][kListed] key and index
 };
 __host__ __device__ inline size_t parts_align(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -339,7 +368,6 @@ __host__ __device__ inline size_t parts_view(void* ws, int rows, int parts, Part
   take(&v->state, (size_t)rows);
   take(&v->before_w, (size_t)rows * (kGrid + 1));
   take(&v->before_c, (size_t)rows * (kGrid + 1));
-  take(&v->listed, (size_t)rows * (kGrid + 1));
   take(&v->list, (size_t)rows * kListed);
   return at;
 }
@@ -412,41 +440,49 @@ __global__ __launch_bounds__(kSampleThreads) void sample_parts_kernel(SampleArgs
   __shared__ float stats[3 * kSampleWaves];
   const int part = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
   const float* logits = a.logits + row * a.stride;
-  const int lo = part * part_len, hi = min(lo + part_len, a.vocab);
   const Ask s = ask_of(a, row);
   const size_t at = (size_t)row * parts + part;
   count[tid] = 0;
   units[tid] = 0;
-  const uint64_t first = first_top(logits, lo, hi, scan);
-  const float top = top_of(first);
   if (part == 0 && tid == 0) v.state[row].listed = 0;
-  if (s.greedy || top == -INFINITY) {
-    if (tid == 0) v.head[at] = {first, 0, 0.0, 0, 0};
-    if (s.greedy) return;
-  } else {
-    const double grid = grid_of(logits, a.vocab, s.t, stats), top_bin = floor((double)top * grid);
-    const double scale = kLog2e / (double)s.t;
-    const bool light = s.k > 0 && s.k <= kLightK;
+  const double grid = s.greedy ? 0.0 : grid_of(logits, a.vocab, s.t, stats);
+  over(logits, part * part_len, min((part + 1) * part_len, a.vocab), [&](auto each) __attribute__((always_inline)) {
+    float top = -INFINITY;
+    int index = 0x7fffffff;
+    each([&](float l, int i) __attribute__((always_inline)) {
+      if (l > top) {
+        top = l;
+        index = i;
+      }
+    });
+    const uint64_t first = first_of(top, index, scan);
+    top = top_of(first);
     uint64_t all = 0;
     uint32_t n = 0;
-    for_each(logits, lo, hi, [&](float l, int) __attribute__((always_inline)) {
-      if (l == -INFINITY) return;
-      const int b = bin_of(l, top_bin, grid);
-      atomicAdd(&count[b], 1u);
-      ++n;
-      if (light) return;
-      const uint64_t x = quick_units(((double)l - (double)top) * scale);
-      if (x == 0) return;
-      atomicAdd((unsigned long long*)&units[b], (unsigned long long)x);
-      all += x;
-    });
-    all = block_sum(all, scan);  // (its barriers are the histogram's, too)
-    n = (uint32_t)block_sum(n, scan);
+    if (!s.greedy && top != -INFINITY) {
+      const double top_bin = floor((double)top * grid), scale = kLog2e / (double)s.t;
+      if (s.counts())
+        each([&](float l, int) __attribute__((always_inline)) {
+          if (l == -INFINITY) return;
+          atomicAdd(&count[bin_of(l, top_bin, grid)], 1u);
+          ++n;
+        });
+      if (!s.light())
+        each([&](float l, int) __attribute__((always_inline)) {
+          const uint64_t x = quick_units(((double)l - (double)top) * scale);
+          if (x == 0) return;
+          atomicAdd((unsigned long long*)&units[bin_of(l, top_bin, grid)], (unsigned long long)x);
+          all += x;
+        });
+      all = block_sum(all, scan);  // (its barriers are the histogram's, too)
+      n = (uint32_t)block_sum(n, scan);
+    }
     if (tid == 0) v.head[at] = {first, all, grid, n, 0};
-  }
+  });
+  if (s.greedy) return;
   __syncthreads();
-  v.count[at * kGrid + tid] = count[tid];
-  v.units[at * kGrid + tid] = units[tid];
+  if (s.counts()) v.count[at * kGrid + tid] = count[tid];
+  if (!s.light()) v.units[at * kGrid + tid] = units[tid];
 }
 
 // Exclusive prefix sums over the workgroup.
@@ -466,11 +502,17 @@ __device__ __forceinline__ uint64_t block_before(uint64_t x, uint64_t* lds, uint
   return before + end - x;
 }
 
+constexpr int kMaxParts = 16;
 struct ListLds {
   uint64_t w[kGrid + 1];
   uint32_t c[kGrid + 1];
   uint64_t scan[kSampleWaves];
   int bins[8];
+  PartHead head[kMaxParts];
+  uint32_t found, place;
+  uint64_t list[kListed];
+  int off[kMaxParts];    // bins from the row's largest logit to the part's
+  double f[kMaxParts];   // what a unit of the part is in the row's
 };
 
 __global__ __launch_bounds__(kSampleThreads) void sample_list_kernel(SampleArgs a, PartsView v, int parts, int part_len) {
@@ -478,38 +520,48 @@ __global__ __launch_bounds__(kSampleThreads) void sample_list_kernel(SampleArgs 
   const int part = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
   const float* logits = a.logits + row * a.stride;
   const Ask s = ask_of(a, row);
+  if (tid < parts) lds.head[tid] = v.head[(size_t)row * parts + tid];
+  __syncthreads();
   uint64_t first = ~0ull;
   double grid = 0.0;
   for (int i = 0; i < parts; ++i) {
-    const PartHead h = v.head[(size_t)row * parts + i];
-    if (h.top < first) {
-      first = h.top;
-      grid = h.grid;
+    if (lds.head[i].top < first) {
+      first = lds.head[i].top;
+      grid = lds.head[i].grid;
     }
   }
   const float top = top_of(first);
   if (part == 0 && tid == 0) v.state[row].top = first;
   if (s.greedy || top == -INFINITY) return;
   const double top_bin = floor((double)top * grid);
-  const bool light = s.k > 0 && s.k <= kLightK;
+  const bool light = s.light();
 
   // ---- the parts' histograms added up, each moved to the row's largest logit
+  if (tid < parts) {
+    const float t = top_of(lds.head[tid].top);
+    lds.off[tid] = t == -INFINITY ? kGrid : (int)fmin(top_bin - floor((double)t * grid), (double)kGrid);
+    lds.f[tid] = t == -INFINITY ? 0.0 : exp2((((double)t - (double)top) * kLog2e) / (double)s.t);
+  }
+  __syncthreads();
   uint64_t w = 0, all_w = 0;
   uint32_t c = 0, all_c = 0;
+  const size_t at0 = (size_t)row * parts * kGrid;
+#pragma unroll 8
   for (int i = 0; i < parts; ++i) {
-    const size_t at = (size_t)row * parts + i;
-    const PartHead h = v.head[at];
-    const float t = top_of(h.top);
-    if (t == -INFINITY) continue;
-    const double down = top_bin - floor((double)t * grid);
-    const int off = (int)fmin(down, (double)kGrid);
-    const double f = exp2((((double)t - (double)top) * kLog2e) / (double)s.t);
-    if (tid >= off && tid < kGrid - 1) {
-      c += v.count[at * kGrid + tid - off];
-      if (!light) w += (uint64_t)((double)v.units[at * kGrid + tid - off] * f + 0.5);
+    // (loads without a condition are asked for together)
+    const int b = tid - lds.off[i];
+    const bool in = b >= 0 && tid < kGrid - 1;
+    const size_t at = at0 + i * kGrid + (in ? b : 0);
+    if (s.counts()) {
+      const uint32_t x = v.count[at];
+      c += in ? x : 0;
     }
-    all_c += h.count;
-    all_w += (uint64_t)((double)h.units * f + 0.5);
+    if (!light) {
+      const uint64_t x = v.units[at];
+      w += in ? (uint64_t)((double)x * lds.f[i] + 0.5) : 0;
+    }
+    all_c += lds.head[i].count;
+    all_w += (uint64_t)((double)lds.head[i].units * lds.f[i] + 0.5);
   }
   uint64_t sum_w, sum_c;
   const uint64_t before_w = block_before(w, lds.scan, &sum_w), before_c = block_before(c, lds.scan, &sum_c);
@@ -536,11 +588,12 @@ __global__ __launch_bounds__(kSampleThreads) void sample_list_kernel(SampleArgs 
   };
   // ---- the bins in question, from what the units kept are at least and at most
   bool mine = false;
-  int m_bin = 0;
+  int m_bin = 0, far = kGrid - 1;  // the last bin in question
   const bool cut = s.k > 0 && (uint32_t)s.k < all_c;
   if (light) {
     const int b = cut ? bin_by(true, s.k, 0) : kGrid - 1;
     mine = tid <= b;
+    far = b;
   } else {
     uint64_t lo = total, hi = total;
     if (cut) {
@@ -564,242 +617,303 @@ __global__ __launch_bounds__(kSampleThreads) void sample_list_kernel(SampleArgs 
       m_bin = bin(l + off);
       const int b1 = bin(l - off);
       mine |= tid >= m_bin && tid <= b1;
+      if (tid == 0) lds.bins[5] = b1;  // (read behind the next barrier)
       lo = min(lo, max(lds.w[m_bin], (uint64_t)1));
       hi = min(hi, lds.w[b1 + 1]);
     }
     const int b0 = bin_by(false, token_target(s.u, lo), 3), b1 = bin_by(false, token_target(s.u, hi), 4);
     mine |= tid >= b0 && tid <= b1;
+    far = max(max(cut ? lds.bins[0] : 0, s.p < 1.0f ? lds.bins[2] : 0), max(s.least > 0.0f ? lds.bins[5] : 0, b1));
+    if (w == 0 && !(cut && tid == lds.bins[0])) mine = false;
   }
-  if (c == 0) mine = false;
-  uint64_t n_listed;
-  const uint64_t listed = block_before(mine ? c : 0, lds.scan, &n_listed);
-  // a bin that is behind the grid's end has more in it than its place says
-  const bool slow = __syncthreads_or((mine && !light && tid == kGrid - 1) || n_listed > kListed);
+  // A place behind the grid's end, and more tokens than the list takes (where
+  // they are not counted, the list says so itself).
+  const bool slow = __syncthreads_or((mine && !light && tid == kGrid - 1) || (light && mine && end_c > kListed));
   if (part == 0) {
     if (tid == 0) {
       v.state[row].slow = slow;
       v.state[row].grid = grid;
       v.state[row].m_bin = m_bin;
     }
-    const size_t at = (size_t)row * (kGrid + 1) + tid;
-    v.before_w[at] = before_w;
-    v.before_c[at] = (uint32_t)before_c;
-    v.listed[at] = (uint32_t)listed;
-    if (tid == kGrid - 1) {
-      v.before_w[at + 1] = end_w;
-      v.before_c[at + 1] = (uint32_t)end_c;
-      v.listed[at + 1] = (uint32_t)n_listed;
+    if (!light) {
+      const size_t at = (size_t)row * (kGrid + 1) + tid;
+      v.before_w[at] = before_w;
+      v.before_c[at] = (uint32_t)before_c;
+      if (tid == kGrid - 1) {
+        v.before_w[at + 1] = end_w;
+        v.before_c[at + 1] = (uint32_t)end_c;
+      }
     }
   }
   if (slow) return;
   // ---- their tokens
-  __syncthreads();
   uint32_t* flags = lds.c;
+  __syncthreads();
   flags[tid] = mine;
+  if (tid == 0) lds.found = 0;
+  __syncthreads();
+  // (most tokens lie behind the last bin in question: told from its end, and a
+  // little before it, in 32 bits)
+  const double end = (top_bin - far) / grid;
+  const float below = far == kGrid - 1 || grid == 0.0 ? -INFINITY : (float)fmax(end - 1e-6 * fabs(end), -3e38);
+  over(logits, part * part_len, min((part + 1) * part_len, a.vocab), [&](auto each) __attribute__((always_inline)) {
+    each([&](float l, int i) __attribute__((always_inline)) {
+      if (l < below || l == -INFINITY || flags[bin_of(l, top_bin, grid)] == 0) return;
+      const uint32_t at = atomicAdd(&lds.found, 1u);
+      if (at < kListed) lds.list[at] = (uint64_t)key_of(l) << 32 | (uint32_t)i;
+    });
+  });
+  __syncthreads();
+  // (one atomic a part: a round trip of a microsecond)
+  if (tid == 0) lds.place = atomicAdd(&v.state[row].listed, lds.found);
   __syncthreads();
   uint64_t* list = v.list + (size_t)row * kListed;
-  for_each(logits, part * part_len, min((part + 1) * part_len, a.vocab), [&](float l, int i) __attribute__((always_inline)) {
-    if (l == -INFINITY || flags[bin_of(l, top_bin, grid)] == 0) return;
-    const uint32_t at = atomicAdd(&v.state[row].listed, 1u);
-    if (at < kListed) list[at] = (uint64_t)key_of(l) << 32 | (uint32_t)i;
-  });
+  for (uint32_t i = tid; i < min(lds.found, (uint32_t)kListed); i += kSampleThreads)
+    if (lds.place + i < kListed) list[lds.place + i] = lds.list[i];
 }
 
-// 64-bit numbers in ascending order: elements tid + kSampleThreads * q of n (a
-// power of two, n / kSampleThreads or 1 a thread; threads past n idle), by a
-// bitonic network: within the wave by lane swaps, across waves through LDS.
+// The value of the lane J away (a power of two).
+template <int J>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t x) {
+  if constexpr (J == 1) return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, kDppXor1, 0xF, 0xF, false);
+  if constexpr (J == 2) return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, kDppXor2, 0xF, 0xF, false);
+  if constexpr (J == 4)  // (7 away, then 3)
+    return (uint32_t)__builtin_amdgcn_mov_dpp(__builtin_amdgcn_mov_dpp((int)x, kDppHalfMirror, 0xF, 0xF, false), 0x1B, 0xF, 0xF, false);
+  if constexpr (J == 8) return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, kDppRor8, 0xF, 0xF, false);
+  if constexpr (J == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return threadIdx.x & 16 ? (uint32_t)r[0] : (uint32_t)r[1];
+  }
+  if constexpr (J == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return threadIdx.x & 32 ? (uint32_t)r[0] : (uint32_t)r[1];
+  }
+}
+// A bitonic network's steps J, J / 2 .. 1 within the wave; `up`: ascending.
+template <int J>
+__device__ __forceinline__ void sort_lanes(uint64_t& x, bool up) {
+  const uint64_t y = (uint64_t)lane_xor<J>((uint32_t)(x >> 32)) << 32 | lane_xor<J>((uint32_t)x);
+  const bool low = (threadIdx.x & J) == 0;
+  if ((y < x) == (up == low)) x = y;
+  if constexpr (J > 1) sort_lanes<J / 2>(x, up);
+}
+// Ascending: elements tid + kSampleThreads * q of n, a power of two of 64 and
+// more, by a bitonic network: lane swaps in a wave, LDS across waves. Elements
+// past n are left.
 template <int Q>
 __device__ __forceinline__ void sort_list(uint64_t (&x)[Q], uint64_t* lds, int n) {
   const int tid = threadIdx.x;
-  for (int k = 2; k <= n; k <<= 1)
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      if (j >= 64) {
-        __syncthreads();
 #pragma unroll
-        for (int q = 0; q < Q; ++q)
-          if (tid + kSampleThreads * q < n) lds[tid + kSampleThreads * q] = x[q];
-        __syncthreads();
-      }
+  for (int q = 0; q < Q; ++q) {
+    sort_lanes<1>(x[q], (tid & 2) == 0);
+    sort_lanes<2>(x[q], (tid & 4) == 0);
+    sort_lanes<4>(x[q], (tid & 8) == 0);
+    sort_lanes<8>(x[q], (tid & 16) == 0);
+    sort_lanes<16>(x[q], (tid & 32) == 0);
+    sort_lanes<32>(x[q], ((tid + kSampleThreads * q) & 64) == 0 || n == 64);
+  }
+#pragma nounroll
+  for (int k = 128; k <= n; k <<= 1) {
+#pragma nounroll
+    for (int j = k >> 1; j >= 64; j >>= 1) {
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < Q; ++q) lds[tid + kSampleThreads * q] = x[q];
+      __syncthreads();
 #pragma unroll
       for (int q = 0; q < Q; ++q) {
         const int i = tid + kSampleThreads * q;
-        if (i >= n) continue;  // (n is a multiple of 64: whole waves)
-        uint64_t y;
-        if (j >= 64) y = lds[i ^ j];
-        else y = (uint64_t)__shfl_xor((unsigned long long)x[q], j);
-        const bool up = (i & k) == 0, low = (i & j) == 0;
-        x[q] = up == low ? min(x[q], y) : max(x[q], y);
+        const uint64_t y = lds[i ^ j];
+        if ((y < x[q]) == (((i & k) == 0) == ((i & j) == 0)) && i < n) x[q] = y;
       }
     }
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const int i = tid + kSampleThreads * q;
+      if (i < n) sort_lanes<32>(x[q], (i & k) == 0);  // (whole waves)
+    }
+  }
 }
 
 struct TokenLds {
   union {
     SampleLds row;
-    uint64_t list[kListed];
+    struct {
+      uint64_t list[kListed];
+      uint16_t from[kGrid], to[kGrid];  // of each bin in the list
+    };
   };
   uint64_t scan[kSampleWaves];
-  uint64_t kept[3];
-  unsigned long long count[3];
-  int token;
+  uint64_t kept[2];
+  unsigned long long m_kept;
 };
+
+// The token from the list's tokens x (key and index; all ones: none), elements
+// tid + kSampleThreads * q.
+template <int Q, bool DIRECT>
+__device__ __forceinline__ void token_of_list(const SampleArgs& a, const PartsView& v, const RowState& state, int row, const Ask& s,
+                                              uint64_t (&x)[Q], TokenLds& lds) {
+  const int tid = threadIdx.x;
+  const float top = top_of(state.top);
+  const bool light = DIRECT || s.light();
+  int size = 64;
+  while (size < (int)state.listed) size <<= 1;
+  sort_list<Q>(x, lds.list, size);
+  if (tid == 0) {
+    lds.kept[0] = lds.kept[1] = 0;
+    lds.m_kept = 0;
+  }
+  // ---- in order, Q neighbours a thread; weights and running sums
+  if (Q > 1 || !light) {
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < Q; ++q) lds.list[tid + kSampleThreads * q] = x[q];
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < Q; ++q) x[q] = lds.list[Q * tid + q];
+  }
+  const Row r = {a.logits, a.vocab, top, 1.0 / (double)s.t};
+  double weight[Q];
+  uint64_t sum[Q], less[Q], mine = 0;  // up to and with each, and before it
+#pragma unroll
+  for (int q = 0; q < Q; ++q) {
+    weight[q] = x[q] == ~0ull ? 0.0 : r.weight(of_key((uint32_t)(x[q] >> 32)));
+    less[q] = mine;
+    mine += (uint64_t)(weight[q] * kUnits + 0.5);
+    sum[q] = mine;
+  }
+  uint64_t kept;
+  const uint64_t before = block_before(mine, lds.scan, &kept);
+  uint32_t rank[Q];
+#pragma unroll
+  for (int q = 0; q < Q; ++q) {
+    sum[q] += before;
+    less[q] += before;
+    rank[q] = Q * tid + q;
+  }
+  const size_t at = (size_t)row * (kGrid + 1);
+  if constexpr (!DIRECT)
+    if (!light) {
+      // (before each bin what the histogram says; a bin's last token brings it to
+      // the next one's)
+      const double grid = state.grid, top_bin = floor((double)top * grid);
+      int bin[Q];
+      uint64_t w0[Q], w1[Q];
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        const int i = Q * tid + q;
+        bin[q] = x[q] == ~0ull ? -1 : bin_of(of_key((uint32_t)(x[q] >> 32)), top_bin, grid);
+        if (bin[q] < 0) continue;
+        w0[q] = v.before_w[at + bin[q]];
+        w1[q] = v.before_w[at + bin[q] + 1];
+        // its bin begins or ends here, if its neighbours are of others
+        const uint64_t prev = i > 0 ? lds.list[i - 1] : ~0ull, next = i + 1 < Q * kSampleThreads ? lds.list[i + 1] : ~0ull;
+        if (prev == ~0ull || bin_of(of_key((uint32_t)(prev >> 32)), top_bin, grid) != bin[q]) lds.from[bin[q]] = (uint16_t)i;
+        if (next == ~0ull || bin_of(of_key((uint32_t)(next >> 32)), top_bin, grid) != bin[q]) lds.to[bin[q]] = (uint16_t)(i + 1);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < Q; ++q) lds.list[Q * tid + q] = less[q];
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        if (bin[q] < 0) continue;
+        const int from = lds.from[bin[q]], i = Q * tid + q;
+        const uint64_t p = lds.list[from];
+        less[q] = min(w0[q] + less[q] - p, w1[q]);
+        sum[q] = i + 1 == lds.to[bin[q]] ? w1[q] : min(w0[q] + sum[q] - p, w1[q]);
+        if (s.counts()) rank[q] = v.before_c[at + bin[q]] + i - from;
+      }
+      kept = v.before_w[at + kGrid];
+    }
+  // ---- the filters, each by the units that stay: the one token at which a
+  // number of them is reached says how many
+  if (s.k > 0) {
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+      if (x[q] != ~0ull && rank[q] == (uint32_t)s.k - 1) lds.kept[0] = sum[q];
+    __syncthreads();
+    if (lds.kept[0] != 0) kept = lds.kept[0];  // (0: there are not so many)
+  }
+  if (s.p < 1.0f) {
+    const uint64_t target = top_p_target(s.p, kept);
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+      if (x[q] != ~0ull && less[q] < target && target <= sum[q]) lds.kept[1] = sum[q];
+    __syncthreads();
+    kept = lds.kept[1];
+  }
+  if (s.least > 0.0f) {
+    uint64_t stay = light ? 0 : v.before_w[at + state.m_bin];
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+      if (x[q] != ~0ull && weight[q] >= (double)s.least) stay = max(stay, sum[q]);
+    __syncthreads();
+    atomicMax(&lds.m_kept, (unsigned long long)stay);
+    __syncthreads();
+    kept = min(kept, (uint64_t)lds.m_kept);
+  }
+  const uint64_t target = token_target(s.u, kept);
+#pragma unroll
+  for (int q = 0; q < Q; ++q)
+    if (x[q] != ~0ull && less[q] < target && target <= sum[q]) a.tokens[row] = (int32_t)(uint32_t)x[q];
+}
 
 // DIRECT: the list is the whole row (vocabularies of up to kListed), read here.
 template <bool DIRECT>
-__global__ __launch_bounds__(kSampleThreads) void sample_token_kernel(SampleArgs a, PartsView v, int parts) {
+__global__ __launch_bounds__(kSampleThreads) void sample_token_kernel(SampleArgs a, PartsView v) {
   constexpr int Q = kListed / kSampleThreads;
   __shared__ TokenLds lds;
   const int row = blockIdx.x, tid = threadIdx.x;
   const Ask s = ask_of(a, row);
   const float* logits = a.logits + row * a.stride;
-  const uint64_t first = DIRECT ? first_top(logits, 0, a.vocab, lds.scan) : v.state[row].top;
-  if (s.greedy || first == ~0ull) {
-    if (tid == 0) a.tokens[row] = first == ~0ull ? -1 : (int32_t)(uint32_t)first;
+  RowState state = {};
+  uint64_t x[Q];
+  if constexpr (DIRECT) {
+    float top = -INFINITY;
+    int index = 0x7fffffff;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const int i = tid + kSampleThreads * q;
+      const float l = i < a.vocab ? candidate(logits[i]) : -INFINITY;
+      x[q] = l == -INFINITY ? ~0ull : (uint64_t)key_of(l) << 32 | (uint32_t)i;
+      if (l > top) {
+        top = l;
+        index = i;
+      }
+    }
+    state.top = first_of(top, index, lds.scan);
+    state.listed = a.vocab;
+  } else {
+    state = v.state[row];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      x[q] = v.list[(size_t)row * kListed + tid + kSampleThreads * q];
+      if (tid + kSampleThreads * q >= state.listed) x[q] = ~0ull;
+    }
+  }
+  if (s.greedy || state.top == ~0ull) {
+    if (tid == 0) a.tokens[row] = state.top == ~0ull ? -1 : (int32_t)(uint32_t)state.top;
     return;
   }
-  const float top = top_of(first);
-  if (!DIRECT && v.state[row].slow) {
-    const int token = sample_row(a, row, s, top, lds.row);
+  if (!DIRECT && (state.slow || state.listed > kListed)) {
+    const int token = sample_row(a, row, s, top_of(state.top), lds.row);
     if (tid == 0) a.tokens[row] = token;
     return;
   }
-  // ---- the list, in order
-  const bool light = DIRECT || (s.k > 0 && s.k <= kLightK);
-  int n = DIRECT ? a.vocab : (int)min(v.state[row].listed, (uint32_t)kListed);
-  int size = 64;
-  while (size < n) size <<= 1;
-  uint64_t x[Q];
-#pragma unroll
-  for (int q = 0; q < Q; ++q) {
-    const int i = tid + kSampleThreads * q;
-    x[q] = ~0ull;  // (no token: behind all others)
-    if (i >= n) continue;
-    if constexpr (DIRECT) {
-      const float l = candidate(logits[i]);
-      if (l != -INFINITY) x[q] = (uint64_t)key_of(l) << 32 | (uint32_t)i;
-    } else {
-      x[q] = v.list[(size_t)row * kListed + i];
-    }
+  if (state.listed <= kSampleThreads) {
+    uint64_t y[1] = {x[0]};
+    token_of_list<1, DIRECT>(a, v, state, row, s, y, lds);
+  } else {
+    token_of_list<Q, DIRECT>(a, v, state, row, s, x, lds);
   }
-  sort_list<Q>(x, lds.list, size);
-  if (tid < 3) {
-    lds.count[tid] = 0;
-    lds.kept[tid] = 0;
-  }
-  __syncthreads();
-  // element order from here on: Q neighbours a thread
-#pragma unroll
-  for (int q = 0; q < Q; ++q) lds.list[tid + kSampleThreads * q] = x[q];
-  __syncthreads();
-#pragma unroll
-  for (int q = 0; q < Q; ++q) x[q] = lds.list[Q * tid + q];
-  // ---- weights, ranks and running sums
-  const Row r = {logits, a.vocab, top, 1.0 / (double)s.t};
-  double weight[Q];
-  uint64_t sum[Q], mine = 0;
-#pragma unroll
-  for (int q = 0; q < Q; ++q) {
-    weight[q] = x[q] == ~0ull ? 0.0 : r.weight(of_key((uint32_t)(x[q] >> 32)));
-    mine += (uint64_t)(weight[q] * kUnits + 0.5);
-    sum[q] = mine;
-  }
-  uint64_t all;
-  const uint64_t before = block_before(mine, lds.scan, &all);
-  uint32_t rank[Q];
-#pragma unroll
-  for (int q = 0; q < Q; ++q) {
-    rank[q] = Q * tid + q;
-    sum[q] += before;
-  }
-  if constexpr (!DIRECT)
-    if (!light) {
-      // (before each bin what the histogram says; a bin's last token brings it to
-      // the next one's)
-      __syncthreads();
-      uint64_t* sums = lds.list;
-#pragma unroll
-      for (int q = 0; q < Q; ++q) sums[Q * tid + q] = sum[q];
-      __syncthreads();
-      const double grid = v.state[row].grid, top_bin = floor((double)top * grid);
-      const size_t at = (size_t)row * (kGrid + 1);
-#pragma unroll
-      for (int q = 0; q < Q; ++q) {
-        if (x[q] == ~0ull) continue;
-        const int b = bin_of(of_key((uint32_t)(x[q] >> 32)), top_bin, grid);
-        const uint32_t from = v.listed[at + b], to = v.listed[at + b + 1], i = rank[q];
-        const uint64_t w0 = v.before_w[at + b], w1 = v.before_w[at + b + 1];
-        sum[q] = i + 1 == to ? w1 : min(w0 + sum[q] - (from > 0 ? sums[from - 1] : 0), w1);
-        rank[q] = v.before_c[at + b] + i - from;
-      }
-    }
-  // ---- the filters, each by the token with which it ends
-  __syncthreads();
-  uint64_t count = DIRECT || light ? (uint64_t)n : v.before_c[(size_t)row * (kGrid + 1) + kGrid];
-  uint64_t kept = DIRECT || light ? all : v.before_w[(size_t)row * (kGrid + 1) + kGrid];
-  if (s.k > 0 && (uint64_t)s.k < count) {
-#pragma unroll
-    for (int q = 0; q < Q; ++q)
-      if (x[q] != ~0ull && rank[q] == (uint32_t)s.k - 1) lds.kept[0] = sum[q];
-    __syncthreads();
-    if (lds.kept[0] != 0) {
-      count = s.k;
-      kept = lds.kept[0];
-    }
-  }
-  // the first token that reaches a number of units: one whose sum does and whose
-  // predecessor's does not, the lowest rank if there are several
-  auto reached = [&](uint64_t target, int slot) __attribute__((always_inline)) {
-    uint32_t least = 0xffffffffu;
-#pragma unroll
-    for (int q = Q - 1; q >= 0; --q)
-      if (x[q] != ~0ull && sum[q] >= target) least = rank[q];
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) least = min(least, (uint32_t)__shfl_xor((int)least, d));
-    __syncthreads();
-    if ((tid & 63) == 0) lds.scan[tid >> 6] = least;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kSampleWaves; ++w) least = min(least, (uint32_t)lds.scan[w]);
-    return least;
-  };
-  if (s.p < 1.0f) {
-    const uint32_t last = reached(top_p_target(s.p, kept), 1);
-#pragma unroll
-    for (int q = 0; q < Q; ++q)
-      if (x[q] != ~0ull && rank[q] == last) lds.kept[1] = sum[q];
-    __syncthreads();
-    count = (uint64_t)last + 1;
-    kept = lds.kept[1];
-  }
-  if (s.least > 0.0f) {
-    uint64_t stay = 0, units = 0;
-    if (!light) {
-      const size_t at = (size_t)row * (kGrid + 1) + v.state[row].m_bin;
-      stay = v.before_c[at];
-      units = v.before_w[at];
-    }
-#pragma unroll
-    for (int q = 0; q < Q; ++q)
-      if (x[q] != ~0ull && weight[q] >= (double)s.least && rank[q] + 1 > stay) {
-        stay = rank[q] + 1;
-        units = sum[q];
-      }
-    atomicMax(&lds.count[2], (unsigned long long)stay);
-    __syncthreads();
-    if (stay == lds.count[2]) lds.kept[2] = units;
-    __syncthreads();
-    if (lds.count[2] < count) kept = lds.kept[2];
-  }
-  // ---- the token
-  const uint32_t last = reached(token_target(s.u, kept), 2);
-#pragma unroll
-  for (int q = 0; q < Q; ++q)
-    if (x[q] != ~0ull && rank[q] == last) a.tokens[row] = (int32_t)(uint32_t)x[q];
 }
 
 int parts_of(int rows, int vocab) {
   const int most = std::max(2 * device_cus() / std::min(rows, kRowsAtOnce), 1);
-  return std::min(std::min(most, 16), (vocab + kPartLeast - 1) / kPartLeast);
+  return std::min(std::min(most, kMaxParts), (vocab + kPartLeast - 1) / kPartLeast);
 }
 
 }  // namespace
@@ -813,7 +927,7 @@ size_t sample_workspace(int rows, int vocab) {
 hipError_t launch_sample(const SampleArgs& all, void* ws, hipStream_t stream) {
   PartsView v = {};
   if (all.vocab <= kListed) {
-    hipLaunchKernelGGL(sample_token_kernel<true>, dim3(all.rows), dim3(kSampleThreads), 0, stream, all, v, 1);
+    hipLaunchKernelGGL(sample_token_kernel<true>, dim3(all.rows), dim3(kSampleThreads), 0, stream, all, v);
     return hipGetLastError();
   }
   const int parts = parts_of(all.rows, all.vocab);
@@ -835,7 +949,7 @@ hipError_t launch_sample(const SampleArgs& all, void* ws, hipStream_t stream) {
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(sample_list_kernel, grid, dim3(kSampleThreads), 0, stream, a, v, parts, part_len);
     if ((e = hipGetLastError()) != hipSuccess) return e;
-    hipLaunchKernelGGL(sample_token_kernel<false>, dim3(a.rows), dim3(kSampleThreads), 0, stream, a, v, parts);
+    hipLaunchKernelGGL(sample_token_kernel<false>, dim3(a.rows), dim3(kSampleThreads), 0, stream, a, v);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   return hipSuccess;
