@@ -96,4 +96,12 @@ int64_t prefill_groups(const PagedAttnArgs& a);
 size_t plan_paged_prefill(PagedAttnArgs& a);
 hipError_t launch_paged_prefill(const PagedAttnArgs& a, hipStream_t stream);
 
+// paged_quant.hip, of caches of 4 and 8 bits: what launch_paged_decode and
+// launch_paged_prefill have planned and split up
+void launch_paged_decode_quantised(const PagedAttnArgs& a, hipStream_t stream);
+hipError_t launch_paged_prefill_quantised(const PagedAttnArgs& a, hipStream_t stream);
+// Workgroups of the decode kernel that a CU holds, sequences of a launch.
+int paged_decode_quantised_per_cu(const PagedAttnArgs& a);
+int paged_decode_quantised_seqs();
+
 }  // namespace mlq
