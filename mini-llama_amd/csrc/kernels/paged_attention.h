@@ -193,6 +193,28 @@ struct KvTraits<__bf16> {
   }
 };
 
+// Codes less their middle as fp16: those of unit p0 of word w0 and unit p1 of
+// w1, the lower dims in lo, the others in hi. A code in the mantissa of an fp16
+// is an exact sum (device_common.h).
+template <typename T>
+__device__ __forceinline__ void code_pairs(uint32_t w0, int p0, uint32_t w1, int p1, uint32_t& lo, uint32_t& hi) {
+  if constexpr (T::kUnit == 1) {
+    const uint32_t x = __builtin_amdgcn_perm(w1, w0, 0x0c000c00u | (uint32_t)p0 | (uint32_t)(4 + p1) << 16);
+    lo = as_u32(as_h2(and_or(x, 0x000F000Fu, 0x64006400u)) - h2_t{1032, 1032});
+    hi = as_u32(as_h2(and_or(x, 0x00F000F0u, 0x54005400u)) - h2_t{72, 72});
+  } else {
+    const uint32_t x = __builtin_amdgcn_perm(w1, w0, (uint32_t)(2 * p0) | (uint32_t)(2 * p0 + 1) << 8 |
+                                                         (uint32_t)(4 + 2 * p1) << 16 | (uint32_t)(5 + 2 * p1) << 24);
+    uint32_t a, b;
+    q8_pairs(x, a, b);
+    lo = as_u32(as_h2(a) - h2_t{1152, 1152});
+    hi = as_u32(as_h2(b) - h2_t{1152, 1152});
+  }
+}
+// d and m of a scale word.
+__device__ __forceinline__ float scale_d(uint32_t w) { return (float)as_h2(w).x; }
+__device__ __forceinline__ float scale_m(uint32_t w) { return (float)as_h2(w).y; }
+
 // N words (a half for 0) from an address that is a multiple of 4 (2).
 template <int N>
 __device__ __forceinline__ void load_words(const char* p, uint32_t* w) {
@@ -303,7 +325,10 @@ __host__ __device__ inline DecodePartials decode_partials(void* ws, int n_seqs, 
 
 // The cut of a launch and a workgroup's way through its range: `first` and
 // `count` are those of the piece's sequence, base and scan_lds the caller's LDS.
-template <int KT, int MAXS>
+// PAD: what a piece costs besides its tiles, in tiles: where ranges hold several
+// pieces, so many empty tiles follow each sequence's, and ranges of many short
+// sequences hold fewer real ones.
+template <int KT, int MAXS, int PAD = 0>
 struct DecodeWork {
   const PagedAttnArgs& a;
   int* base;      // [MAXS + 1]
@@ -321,7 +346,8 @@ struct DecodeWork {
     if (r.row < 0) return 0;
     if (a.part == nullptr) return a.whole;  // a range for each, as long as the longest
     const int tiles = (r.len - (first_key(a, r.len) & ~(KT - 1)) + KT - 1) / KT;
-    return max((tiles + kDecWaves - 1) / kDecWaves, 1) * kDecWaves;
+    if (tiles == 0) return kDecWaves;  // (one piece, which says that there is nothing)
+    return (tiles + kDecWaves - 1) / kDecWaves * kDecWaves + (PAD > 0 && 4 * (int64_t)a.n_seqs * n_tiles >= a.ranges ? PAD : 0);
   }
   __device__ __forceinline__ void take() {
     first = few ? __builtin_amdgcn_readlane(my_first, seq) : __builtin_amdgcn_readfirstlane(base[seq]);
@@ -789,11 +815,24 @@ struct PreTraits<float> : KvTraits<__bf16> {
   }
 };
 
-// Codes and scales are made fp32 values on their way to LDS and go on as those.
+// Codes and scales become values on their way to LDS, in two fp16 parts: 22
+// bits, under a power of two for each key's row, whose largest element could
+// otherwise overflow or all of them lose bits to fp16's subnormals. A score is
+// multiplied by its key's power, a weight by its value row's; the weights of a
+// column have another one, which follows the largest value row so far. Three
+// part products then make a product, as of a bf16 cache.
+template <typename Q>
+struct PreTraitsQuantised : KvTraits<_Float16> {
+  typedef _Float16 mat;
+  static constexpr int kCacheParts = 2;
+  static __device__ __forceinline__ f16v mfma32(h8_t a, h8_t b, f16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
 template <>
-struct PreTraits<KvQ4> : PreTraits<float> {};
+struct PreTraits<KvQ4> : PreTraitsQuantised<KvQ4> {};
 template <>
-struct PreTraits<KvQ8> : PreTraits<float> {};
+struct PreTraits<KvQ8> : PreTraitsQuantised<KvQ8> {};
 // Bytes of an element in a thread's registers.
 template <typename T>
 constexpr int kPreBytes = kQuantised<T> ? 4 : (int)sizeof(T);
@@ -810,13 +849,17 @@ struct PreLds {
   // barrier a tile; fp32's parts leave no room for it (two barriers), and at
   // head dim 256 its registers spill (8000 rows, 16 heads on 2: bf16 988 -> 681
   // us with one buffer, fp16 706 -> 620)
-  static constexpr int kBuf = kPreBytes<T> == 4 || HD > 128 ? 1 : 2;
+  static constexpr int kBuf = sizeof(T) == 4 || HD > 128 ? 1 : 2;
   // steps of q's last part per wave and lane (in registers they spill: fp16 at
   // head dim 256 1058 -> 706 us)
-  static constexpr int kQ = HD < 128 || (PreTraits<T>::kParts < 3 && HD < 256) ? 0 : kPreBytes<T> == 4 ? (HD > 128 ? 12 : 5) : HD / 16;
+  static constexpr int kQ = HD < 128 || (PreTraits<T>::kParts < 3 && HD < 256) ? 0 : sizeof(T) == 4 ? (HD > 128 ? 12 : 5) : HD / 16;
   PreTile<T, HD> tile[kBuf];
   u32x4_t q[kQ > 0 ? kQ : 1][kPreThreads];
   int count[kPreThreads / 64];
+  // quantised: the powers of two to take keys and values back by, of the tile
+  // that is read and the next one
+  static constexpr int kF = kQuantised<T> ? kPreKeys : 1;
+  alignas(16) float kf[2][kF], vf[2][kF];
 };
 
 // Where the 8-slot unit of a dim's row lies: a wave writes a few dims of four
@@ -1116,13 +1159,12 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
   // a unit of VDT / 2 blocks and their scales of each of four
   constexpr int VB2 = VDT / 2, VU = VB2 * kUnitBytes<T>;
   uint32_t kc[QUANT ? (2 * UB + 3) / 4 : 1], kscale[QUANT ? NB : 1], vc[4][QUANT ? (VU + 3) / 4 : 1], vscale[4][QUANT ? VB2 : 1];
-  auto two_values = [&](uint32_t unit, uint32_t scale, uint32_t* w) __attribute__((always_inline)) {
-    if constexpr (QUANT) {
-      const KvScale sc = __builtin_bit_cast(KvScale, scale);
-      constexpr int kBits = 4 * T::kUnit;
-      w[0] = __builtin_bit_cast(uint32_t, kv_value<T>(unit & T::kLevels, sc));
-      w[1] = __builtin_bit_cast(uint32_t, kv_value<T>(unit >> kBits & T::kLevels, sc));
-    }
+  // what a block's elements cannot exceed (0 for one that is not finite; what
+  // lies behind a sequence's end may hold a negative d)
+  auto bound_of = [&](uint32_t scale) __attribute__((always_inline)) {
+    float x = 0.0f;
+    if constexpr (QUANT) x = __builtin_fmaf(fabsf(scale_d(scale)), (float)T::kMiddle, fabsf(scale_m(scale)));
+    return x <= 3.402823466e38f ? x : 0.0f;
   };
   // (a run's start is uniform, a lane's place in it never changes)
   const uint32_t k_at = (kkey & 15) * row_bytes + (QUANT ? 2 * UB * (tid & 7) : kd * ES);
@@ -1167,22 +1209,38 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
       }
     }
   };
-  auto put_k = [&](PreTile<T, HD>& tl, int k0) __attribute__((always_inline)) {
+  int par = 0;  // of the tile that is read: which kf
+  auto put_k = [&](PreTile<T, HD>& tl, int k0, int par) __attribute__((always_inline)) {
     if constexpr (QUANT) {
+      float big = 0.0f;
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int b = 0; b < NB; ++b) big = fmaxf(big, bound_of(kscale[b]));
+      const int e = pow2_scale_exp(big);
+      if ((tid & 7) == 0) lds.kf[par][kkey] = ldexp_f(1.0f, -e);
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          const int at = u * UB + b * kUnitBytes<T>;
-          two_values(kc[at / 4] >> (8 * (at % 4)), kscale[b], kw + 4 * b + 2 * u);
-        }
+      for (int b = 0; b < NB; ++b) {
+        const int a0 = b * kUnitBytes<T>, a1 = UB + a0;
+        const float d = ldexp_f(scale_d(kscale[b]), e), mid = ldexp_f(scale_m(kscale[b]), e);
+        uint32_t lo, hi, x[NK], y[NK];
+        code_pairs<T>(kc[a0 / 4], a0 % 4 / kUnitBytes<T>, kc[a1 / 4], a1 % 4 / kUnitBytes<T>, lo, hi);
+        const float v0 = __builtin_fmaf((float)as_h2(lo).x, d, mid), v1 = __builtin_fmaf((float)as_h2(hi).x, d, mid);
+        const float v2 = __builtin_fmaf((float)as_h2(lo).y, d, mid), v3 = __builtin_fmaf((float)as_h2(hi).y, d, mid);
+        if constexpr (AGAIN)
+          if (k0 + kkey <= kmax) k_bad |= !((v0 * 0.0f + v1 * 0.0f) + (v2 * 0.0f + v3 * 0.0f) == 0.0f);
+        split_pair<_Float16>(v0, v1, x);
+        split_pair<_Float16>(v2, v3, y);
+#pragma unroll
+        for (int i = 0; i < NK; ++i) *(u32x2_t*)&tl.k[i][kkey][32 * b + 4 * (tid & 7)] = u32x2_t{x[i], y[i]};
+      }
+      return;
     }
-    if constexpr (AGAIN)
+    if constexpr (AGAIN && !QUANT)
       if (k0 + kkey <= kmax) {
 #pragma unroll
         for (int w = 0; w < KW; ++w) k_bad |= not_finite<T>(kw[w]);
       }
-    if constexpr (F32) {
+    if constexpr (QUANT) {
+    } else if constexpr (F32) {
 #pragma unroll
       for (int w = 0; w < KW; w += 4) {
         uint32_t x[3], y[3];
@@ -1197,15 +1255,56 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
         *(u32x4_t*)&tl.k[0][kkey][kd + w * 16] = u32x4_t{kw[w], kw[w + 1], kw[w + 2], kw[w + 3]};
     }
   };
-  auto put_v = [&](PreTile<T, HD>& tl, int k0) __attribute__((always_inline)) {
+  auto put_v = [&](PreTile<T, HD>& tl, int k0, int par) __attribute__((always_inline)) {
+    // the key group's slots in its run of 16: keys 0-3, 8-11 | 4-7, 12-15
+    const int unit = 2 * (vkg >> 2) + (vkg & 1), sub = 4 * ((vkg >> 1) & 1);
     if constexpr (QUANT) {
+      int e[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int i = 0; i < 4; ++i) {
+        float big = 0.0f;
 #pragma unroll
-        for (int b = 0; b < VB2; ++b) {
-          const int at = b * kUnitBytes<T>;
-          two_values(vc[e][at / 4] >> (8 * (at % 4)), vscale[e][b], vw[e] + 2 * b);
+        for (int b = 0; b < VB2; ++b) big = fmaxf(big, bound_of(vscale[i][b]));
+        e[i] = pow2_scale_exp(xor16_max(big));  // (the row's other blocks are 16 lanes away)
+        const bool out = k0 + 4 * vkg + i > kmax;
+        if (out) {
+#pragma unroll
+          for (int b = 0; b < VB2; ++b) vscale[i][b] = 0;
         }
+        if ((tid & 31) == 0) lds.vf[par][4 * vkg + i] = out ? 0.0f : ldexp_f(1.0f, -e[i]);
+      }
+#pragma unroll
+      for (int b = 0; b < VB2; ++b) {
+        const int a0 = b * kUnitBytes<T>;
+        uint32_t c[2][2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          code_pairs<T>(vc[2 * i][a0 / 4], a0 % 4 / kUnitBytes<T>, vc[2 * i + 1][a0 / 4], a0 % 4 / kUnitBytes<T>, c[0][i], c[1][i]);
+        float d[4], mid[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          d[i] = ldexp_f(scale_d(vscale[i][b]), e[i]);
+          mid[i] = ldexp_f(scale_m(vscale[i][b]), e[i]);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t x[2][NK];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float v0 = __builtin_fmaf((float)as_h2(c[h][i]).x, d[2 * i], mid[2 * i]);
+            float v1 = __builtin_fmaf((float)as_h2(c[h][i]).y, d[2 * i + 1], mid[2 * i + 1]);
+            if constexpr (AGAIN) {
+              v0 = __builtin_bit_cast(float, settled<T>(__builtin_bit_cast(uint32_t, v0), count));
+              v1 = __builtin_bit_cast(float, settled<T>(__builtin_bit_cast(uint32_t, v1), count));
+            }
+            split_pair<_Float16>(v0, v1, x[i]);
+          }
+          const int dim = v_dim(2 * b + h);
+#pragma unroll
+          for (int i = 0; i < NK; ++i) *(u32x2_t*)&tl.v[i][dim][v_slot(unit, dim) + sub] = u32x2_t{x[0][i], x[1][i]};
+        }
+      }
+      return;
     }
     if (k0 + kPreKeys - 1 > kmax) {
 #pragma unroll
@@ -1215,16 +1314,14 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
           for (int w = 0; w < VWT; ++w) vw[e][w] = 0;
         }
     }
-    if constexpr (AGAIN) {
+    if constexpr (AGAIN && !QUANT) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
 #pragma unroll
         for (int w = 0; w < VWT; ++w) vw[e][w] = settled<T>(vw[e][w], count);
     }
-    // the key group's slots in its run of 16: keys 0-3, 8-11 | 4-7, 12-15
-    const int unit = 2 * (vkg >> 2) + (vkg & 1), sub = 4 * ((vkg >> 1) & 1);
 #pragma unroll
-    for (int j = 0; j < VDT; ++j) {
+    for (int j = 0; j < (QUANT ? 0 : VDT); ++j) {
       const int at = v_slot(unit, v_dim(j)) + sub;
       if constexpr (F32) {
         uint32_t x[3], y[3];
@@ -1245,6 +1342,8 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
 #pragma unroll
   for (int b = 0; b < VB; ++b) acc[b] = (f16v){};
   float m = -INFINITY, l = 0.0f;  // of the column; l of this half's keys
+  // quantised: the largest value row's power of two so far, and the weights'
+  float vtop = 0.0f, lift = Tr::kLift;
   int k0 = key0;
   int64_t run = run_of(k0, page_of(k0));
   load_k(run);
@@ -1255,11 +1354,11 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
   };
   if constexpr (BUF == 2) {
     load_v(run);
-    put_k(lds.tile[0], k0);
-    put_v(lds.tile[0], k0);
+    put_k(lds.tile[0], k0, 0);
+    put_v(lds.tile[0], k0, 0);
     __syncthreads();
   }
-  for (int cur = 0; k0 <= kmax; k0 += kPreKeys, cur ^= BUF - 1) {
+  for (int cur = 0; k0 <= kmax; k0 += kPreKeys, cur ^= BUF - 1, par ^= 1) {
     PreTile<T, HD>& tl = lds.tile[cur];
     const bool more = k0 + kPreKeys <= kmax;
     if constexpr (BUF == 2) {
@@ -1269,7 +1368,7 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
         load_v(run);
       }
     } else {
-      put_k(tl, k0);  // (the last tile's K is done with since its second barrier)
+      put_k(tl, k0, par);  // (the last tile's K is done with since its second barrier)
       load_v(run);
       __syncthreads();
     }
@@ -1288,7 +1387,7 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
           if (sum - x >= 0 && sum - x < NP) c = Tr::mfma32(kk[x], q_part(sum - x, i), c);
     }
     // (fp32's parts are read again: held across the loops they spill)
-    if constexpr (NK > 1 && HD <= 128) asm volatile("" ::: "memory");
+    if constexpr (NK > 2 && HD <= 128) asm volatile("" ::: "memory");
 #pragma unroll
     for (int i = 0; i < KT; ++i) {
       f16v& c = i % 2 == 0 ? s : s1;
@@ -1296,7 +1395,7 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
     }
     s += s1;
     if constexpr (BUF == 1) {
-      put_v(tl, k0);
+      put_v(tl, k0, par);
       if (more) {
         next(k0 + kPreKeys);
         load_k(run);
@@ -1304,6 +1403,26 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
       __syncthreads();
     }
     // lane: keys 8 (i / 4) + 4 half + i % 4 of its column
+    float vf[QUANT ? 16 : 1];
+    if constexpr (QUANT) {
+      float big = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f4 x = *(const f4*)&lds.kf[par][8 * j + 4 * half], y = *(const f4*)&lds.vf[par][8 * j + 4 * half];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[4 * j + i] *= x[i];
+          vf[4 * j + i] = y[i];
+          big = fmaxf(big, y[i]);
+        }
+      }
+      vtop = fmaxf(vtop, xor32_max(big));
+      if constexpr (AGAIN)
+        if (count) {  // (no row's mark is to fall below fp16)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) vf[i] = vtop;
+        }
+    }
     const bool edge = k0 + kPreKeys - 1 > wave_first || (a.window > 0 && k0 <= wave_last - a.window);
     float sl = rule.sl2;  // what is left to multiply
     if (RULE || edge) {
@@ -1333,9 +1452,15 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
     // behind (bf16 parts hold any size): less to rescale.
     if constexpr (kSlack > 0.0f) mx = mx > m + kSlack ? mx : m;
     // rows with nothing visible yet keep m = -inf and weight 0
-    const float ref = (mx == -INFINITY ? 0.0f : mx) - Tr::kLift;
-    if (__any(mx != m)) {
-      const float alpha = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mx);
+    // (a weight times its value row's power ends below 2^15)
+    const float new_lift = QUANT ? Tr::kLift - (float)((int)(__builtin_bit_cast(uint32_t, vtop) >> 23) - 127) : Tr::kLift;
+    const float ref = (mx == -INFINITY ? 0.0f : mx) - new_lift;
+    if (__any(mx != m || (QUANT && new_lift != lift))) {
+      float alpha = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mx);
+      if constexpr (QUANT) {
+        alpha *= __builtin_amdgcn_exp2f(new_lift - lift);
+        lift = new_lift;
+      }
 #pragma unroll
       for (int b = 0; b < VB; ++b) acc[b] *= alpha;
       l *= alpha;
@@ -1352,7 +1477,8 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         uint32_t x[NP];
-        split_pair<M>(s[2 * j], s[2 * j + 1], x);
+        if constexpr (QUANT) split_pair<M>(s[2 * j] * vf[2 * j], s[2 * j + 1] * vf[2 * j + 1], x);
+        else split_pair<M>(s[2 * j], s[2 * j + 1], x);
 #pragma unroll
         for (int i = 0; i < NP; ++i) w[i][j] = x[i];
       }
@@ -1378,8 +1504,8 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
       }
     if constexpr (BUF == 2) {
       if (more) {
-        put_k(lds.tile[cur ^ 1], k0 + kPreKeys);
-        put_v(lds.tile[cur ^ 1], k0 + kPreKeys);
+        put_k(lds.tile[cur ^ 1], k0 + kPreKeys, par ^ 1);
+        put_v(lds.tile[cur ^ 1], k0 + kPreKeys, par ^ 1);
         __syncthreads();
       }
     }
@@ -1387,10 +1513,17 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
   // (without this the loop copies acc once a tile, for what follows)
 #pragma unroll
   for (int b = 0; b < VB; ++b) asm volatile("" : "+v"(acc[b]));
-  const float sum = xor32_sum(l);
+  float sum = xor32_sum(l);
   const int at = wave * 32 + col;
   PrePartial pp = {};
   if (parts) pp = prefill_partial(a, split);
+  if constexpr (QUANT)
+    if (parts) {  // (the splits need not have met the same values)
+      const float down = __builtin_amdgcn_exp2f(-lift);
+      sum *= down;
+#pragma unroll
+      for (int b = 0; b < VB; ++b) acc[b] *= down;
+    }
   if (AGAIN && count) {  // NaN where a value that is not finite is seen
 #pragma unroll
     for (int b = 0; b < VB; ++b)

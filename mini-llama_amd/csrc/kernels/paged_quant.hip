@@ -39,32 +39,14 @@ struct DecQuant {
   static constexpr int kPerCu = HD == 64 ? (T::kUnit == 1 ? 4 : 3) : HD == 128 ? (T::kUnit == 1 ? 3 : 2) : 1;
 };
 constexpr int kDecQuantSeqs = 1024;  // sequences of a launch
+// What a piece costs besides its tiles, in tiles (us with 0 / 4 / 8 / 16: 64
+// sequences of up to 8000, 28 heads on 4 of 128, q4, 56.0 / 50.7 / 46.9 / 46.6; 180
+// of up to 2500 with a window of 1000, 16 of 64, q8, 96.8 / 71.1 / 64.7 / 70.0).
+constexpr int kDecPad = 8;
 
 // Weights times d are lifted to 2^15 less the exponent of the largest d; fp16's
 // least normal numbers leave that at 2^29, an infinite or NaN one at 2^-2.
 constexpr float kMostLift = 29.0f;
-
-// Codes less their middle as fp16: those of unit p0 of word w0 and unit p1 of
-// w1, the lower dims in lo, the others in hi. A code in the mantissa of an fp16
-// is an exact sum (device_common.h).
-template <typename T>
-__device__ __forceinline__ void code_pairs(uint32_t w0, int p0, uint32_t w1, int p1, uint32_t& lo, uint32_t& hi) {
-  if constexpr (T::kUnit == 1) {
-    const uint32_t x = __builtin_amdgcn_perm(w1, w0, 0x0c000c00u | (uint32_t)p0 | (uint32_t)(4 + p1) << 16);
-    lo = as_u32(as_h2(and_or(x, 0x000F000Fu, 0x64006400u)) - h2_t{1032, 1032});
-    hi = as_u32(as_h2(and_or(x, 0x00F000F0u, 0x54005400u)) - h2_t{72, 72});
-  } else {
-    const uint32_t x = __builtin_amdgcn_perm(w1, w0, (uint32_t)(2 * p0) | (uint32_t)(2 * p0 + 1) << 8 |
-                                                         (uint32_t)(4 + 2 * p1) << 16 | (uint32_t)(5 + 2 * p1) << 24);
-    uint32_t a, b;
-    q8_pairs(x, a, b);
-    lo = as_u32(as_h2(a) - h2_t{1152, 1152});
-    hi = as_u32(as_h2(b) - h2_t{1152, 1152});
-  }
-}
-// d and m of a scale word.
-__device__ __forceinline__ float scale_d(uint32_t w) { return (float)as_h2(w).x; }
-__device__ __forceinline__ float scale_m(uint32_t w) { return (float)as_h2(w).y; }
 
 template <int N>
 __device__ __forceinline__ float row_ror(float v) { return dpp<0x120 + N>(v); }
@@ -102,7 +84,7 @@ __global__ __launch_bounds__(kDecThreads, (DecQuant<T, HD>::kPerCu)) void paged_
   const int ai = lane & 15, ak = lane >> 4, rep = ai / HPR;
   const int head_tiles = (a.group + 15) / 16, n_tiles = a.n_kv * head_tiles, TG = min(a.group, 16);
   const DecodePartials pp = decode_partials(a.part, a.n_seqs, a.ranges, TG);
-  DecodeWork<KT, kDecQuantSeqs> work(a, base, scan_lds, n_tiles);
+  DecodeWork<KT, kDecQuantSeqs, kDecPad> work(a, base, scan_lds, n_tiles);
   if (!work.start(pp)) return;
 
   while (true) {
@@ -152,6 +134,17 @@ __global__ __launch_bounds__(kDecThreads, (DecQuant<T, HD>::kPerCu)) void paged_
                                            (__attribute__((address_space(3))) void*)(to + 1024 * j), 16, 0, 0);
       }
     };
+    // ---- q, asked for before the tiles
+    const bool has_head = ai % HPR < G;
+    const float* qp = a.q + dr.row * a.q_stride + (int64_t)(head0 + (has_head ? ai % HPR : 0)) * a.hd;
+    f4 x[BR][2];
+#pragma unroll
+    for (int c = 0; c < BR; ++c)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int d = 32 * (rep * BR + c) + 8 * ak + 4 * j;
+        x[c][j] = has_head && d < a.hd ? *(const f4*)(qp + d) : f4{0.0f, 0.0f, 0.0f, 0.0f};
+      }
     __syncthreads();  // (the last piece's readers are done with the LDS)
     if (tiles > 0) {
       places(0);
@@ -159,21 +152,15 @@ __global__ __launch_bounds__(kDecThreads, (DecQuant<T, HD>::kPerCu)) void paged_
       if (tiles > 1) fetch(1);
     }
 
-    // ---- q
-    const bool has_head = ai % HPR < G;
-    const float* qp = a.q + dr.row * a.q_stride + (int64_t)(head0 + (has_head ? ai % HPR : 0)) * a.hd;
     h8_t qv[NP][NB];
     int q_exp = 0;
     float q_sum[BR];  // of the replica's blocks, with q's power of two
     {
-      f4 x[BR][2];
       float big = 0.0f;
 #pragma unroll
       for (int c = 0; c < BR; ++c)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const int d = 32 * (rep * BR + c) + 8 * ak + 4 * j;
-          x[c][j] = has_head && d < a.hd ? *(const f4*)(qp + d) : f4{0.0f, 0.0f, 0.0f, 0.0f};
           big = fmaxf(fmaxf(big, fmaxf(fabsf(x[c][j].x), fabsf(x[c][j].y))), fmaxf(fabsf(x[c][j].z), fabsf(x[c][j].w)));
         }
       q_exp = pow2_scale_exp(replica_max<R>(xor32_max(xor16_max(big))));
