@@ -215,6 +215,26 @@ __device__ __forceinline__ void code_pairs(uint32_t w0, int p0, uint32_t w1, int
 __device__ __forceinline__ float scale_d(uint32_t w) { return (float)as_h2(w).x; }
 __device__ __forceinline__ float scale_m(uint32_t w) { return (float)as_h2(w).y; }
 
+// d times x in one instruction that takes the half as it lies (a product is a
+// conversion and a multiplication).
+__device__ __forceinline__ float times_d(uint32_t w, float x) { return __builtin_fmaf((float)as_h2(w).x, x, 0.0f); }
+__device__ __forceinline__ float times_m(uint32_t w, float x) { return __builtin_fmaf((float)as_h2(w).y, x, 0.0f); }
+// -1 that the compiler does not know: the remainder of a split is then one
+// instruction that takes the half as it lies, not a conversion and a difference.
+__device__ __forceinline__ float hidden_minus_one() {
+  float x;
+  asm("v_mov_b32 %0, -1.0" : "=v"(x));
+  return x;
+}
+// a, b = the sum of two fp16 parts each, rounded to nearest.
+__device__ __forceinline__ void split_halves(float a, float b, float minus_one, uint32_t (&p)[2]) {
+  f2_t x = {a, b};
+  const h2_t h = __builtin_convertvector(x, h2_t);
+  p[0] = as_u32(h);
+  x.x = __builtin_fmaf((float)h.x, minus_one, a);
+  x.y = __builtin_fmaf((float)h.y, minus_one, b);
+  p[1] = as_u32(__builtin_convertvector(x, h2_t));
+}
 // N words (a half for 0) from an address that is a multiple of 4 (2).
 template <int N>
 __device__ __forceinline__ void load_words(const char* p, uint32_t* w) {
@@ -1055,7 +1075,8 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
   constexpr int VDT = HD / 32;       // dims of V per thread, of 4 keys
   constexpr int VWT = VDT * ES / 4;     // their words a key (fp16 / bf16, HD 64: 1)
   constexpr int NB = HD / 32, UB = NB * kUnitBytes<T>;  // quantised: blocks, bytes of a unit of all of them
-  constexpr float kSlack = Tr::kLift == 0.0f ? 8.0f : 0.0f;
+  constexpr float kSlack = QUANT ? 4.0f : Tr::kLift == 0.0f ? 8.0f : 0.0f;
+  constexpr float kLift = Tr::kLift == 0.0f ? 0.0f : Tr::kLift - kSlack;  // (weights of up to 2^kSlack stay below fp16's range)
   constexpr int BUF = PreLds<T, HD>::kBuf, QL = PreLds<T, HD>::kQ;
   int* const count_lds = lds.count;
   int tid = threadIdx.x;
@@ -1159,6 +1180,13 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
   // a unit of VDT / 2 blocks and their scales of each of four
   constexpr int VB2 = VDT / 2, VU = VB2 * kUnitBytes<T>;
   uint32_t kc[QUANT ? (2 * UB + 3) / 4 : 1], kscale[QUANT ? NB : 1], vc[4][QUANT ? (VU + 3) / 4 : 1], vscale[4][QUANT ? VB2 : 1];
+  // the one of four with the lane's last two bits (by masks: selects of array
+  // elements become an array in memory)
+  const uint32_t mask1 = 0u - (uint32_t)(tid & 1), mask2 = 0u - (uint32_t)(tid >> 1 & 1);
+  auto by_lane = [&](uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) __attribute__((always_inline)) {
+    const uint32_t x = (a0 & ~mask1) | (a1 & mask1), y = (a2 & ~mask1) | (a3 & mask1);
+    return (x & ~mask2) | (y & mask2);
+  };
   // what a block's elements cannot exceed (0 for one that is not finite; what
   // lies behind a sequence's end may hold a negative d)
   auto bound_of = [&](uint32_t scale) __attribute__((always_inline)) {
@@ -1210,25 +1238,34 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
     }
   };
   int par = 0;  // of the tile that is read: which kf
+  const float minus_one = QUANT ? hidden_minus_one() : 0.0f;
   auto put_k = [&](PreTile<T, HD>& tl, int k0, int par) __attribute__((always_inline)) {
     if constexpr (QUANT) {
+      // (each of the key's 8 threads has a block of it, or two of 8)
       float big = 0.0f;
-#pragma unroll
-      for (int b = 0; b < NB; ++b) big = fmaxf(big, bound_of(kscale[b]));
+      if constexpr (NB == 2) {
+        big = fmaxf(bound_of(kscale[0]), bound_of(kscale[1]));
+      } else {
+        big = bound_of(by_lane(kscale[0], kscale[1], kscale[2], kscale[3]));
+        if constexpr (NB == 8) big = fmaxf(big, bound_of(by_lane(kscale[4], kscale[5], kscale[6], kscale[7])));
+        big = fmaxf(big, dpp<kDppXor1>(big));
+        big = fmaxf(big, dpp<kDppXor2>(big));
+      }
       const int e = pow2_scale_exp(big);
+      const float up = ldexp_f(1.0f, e);
       if ((tid & 7) == 0) lds.kf[par][kkey] = ldexp_f(1.0f, -e);
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         const int a0 = b * kUnitBytes<T>, a1 = UB + a0;
-        const float d = ldexp_f(scale_d(kscale[b]), e), mid = ldexp_f(scale_m(kscale[b]), e);
+        const float d = times_d(kscale[b], up), mid = times_m(kscale[b], up);
         uint32_t lo, hi, x[NK], y[NK];
         code_pairs<T>(kc[a0 / 4], a0 % 4 / kUnitBytes<T>, kc[a1 / 4], a1 % 4 / kUnitBytes<T>, lo, hi);
         const float v0 = __builtin_fmaf((float)as_h2(lo).x, d, mid), v1 = __builtin_fmaf((float)as_h2(hi).x, d, mid);
         const float v2 = __builtin_fmaf((float)as_h2(lo).y, d, mid), v3 = __builtin_fmaf((float)as_h2(hi).y, d, mid);
         if constexpr (AGAIN)
           if (k0 + kkey <= kmax) k_bad |= !((v0 * 0.0f + v1 * 0.0f) + (v2 * 0.0f + v3 * 0.0f) == 0.0f);
-        split_pair<_Float16>(v0, v1, x);
-        split_pair<_Float16>(v2, v3, y);
+        split_halves(v0, v1, minus_one, x);
+        split_halves(v2, v3, minus_one, y);
 #pragma unroll
         for (int i = 0; i < NK; ++i) *(u32x2_t*)&tl.k[i][kkey][32 * b + 4 * (tid & 7)] = u32x2_t{x[i], y[i]};
       }
@@ -1259,19 +1296,26 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
     // the key group's slots in its run of 16: keys 0-3, 8-11 | 4-7, 12-15
     const int unit = 2 * (vkg >> 2) + (vkg & 1), sub = 4 * ((vkg >> 1) & 1);
     if constexpr (QUANT) {
-      int e[4];
+      // (lane 4n + i of the row's threads has key i of the four, the row's other
+      // blocks are 16 lanes away)
+      float big = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float big = 0.0f;
+      for (int b = 0; b < VB2; ++b) {
+        big = fmaxf(big, bound_of(by_lane(vscale[0][b], vscale[1][b], vscale[2][b], vscale[3][b])));
+      }
+      const int e = pow2_scale_exp(xor16_max(big));
+      const bool out = k0 + 4 * vkg + (tid & 3) > kmax;
+      if ((tid & 31) < 4) lds.vf[par][4 * vkg + (tid & 3)] = out ? 0.0f : ldexp_f(1.0f, -e);
+      const float mine = out ? 0.0f : ldexp_f(1.0f, e);
+      // (zeros take a key behind the end out: its scales may be anything, and 0
+      // times them is not 0)
+      const float up[4] = {dpp<0x00>(mine), dpp<0x55>(mine), dpp<0xAA>(mine), dpp<0xFF>(mine)};
+      if (k0 + kPreKeys - 1 > kmax) {
 #pragma unroll
-        for (int b = 0; b < VB2; ++b) big = fmaxf(big, bound_of(vscale[i][b]));
-        e[i] = pow2_scale_exp(xor16_max(big));  // (the row's other blocks are 16 lanes away)
-        const bool out = k0 + 4 * vkg + i > kmax;
-        if (out) {
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int b = 0; b < VB2; ++b) vscale[i][b] = 0;
-        }
-        if ((tid & 31) == 0) lds.vf[par][4 * vkg + i] = out ? 0.0f : ldexp_f(1.0f, -e[i]);
+          for (int b = 0; b < VB2; ++b)
+            if (up[i] == 0.0f) vscale[i][b] = 0;
       }
 #pragma unroll
       for (int b = 0; b < VB2; ++b) {
@@ -1283,8 +1327,8 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
         float d[4], mid[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          d[i] = ldexp_f(scale_d(vscale[i][b]), e[i]);
-          mid[i] = ldexp_f(scale_m(vscale[i][b]), e[i]);
+          d[i] = times_d(vscale[i][b], up[i]);
+          mid[i] = times_m(vscale[i][b], up[i]);
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -1297,7 +1341,7 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
               v0 = __builtin_bit_cast(float, settled<T>(__builtin_bit_cast(uint32_t, v0), count));
               v1 = __builtin_bit_cast(float, settled<T>(__builtin_bit_cast(uint32_t, v1), count));
             }
-            split_pair<_Float16>(v0, v1, x[i]);
+            split_halves(v0, v1, minus_one, x[i]);
           }
           const int dim = v_dim(2 * b + h);
 #pragma unroll
@@ -1343,7 +1387,7 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
   for (int b = 0; b < VB; ++b) acc[b] = (f16v){};
   float m = -INFINITY, l = 0.0f;  // of the column; l of this half's keys
   // quantised: the largest value row's power of two so far, and the weights'
-  float vtop = 0.0f, lift = Tr::kLift;
+  float vtop = 0.0f, lift = kLift;
   int k0 = key0;
   int64_t run = run_of(k0, page_of(k0));
   load_k(run);
@@ -1362,7 +1406,7 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
     PreTile<T, HD>& tl = lds.tile[cur];
     const bool more = k0 + kPreKeys <= kmax;
     if constexpr (BUF == 2) {
-      if (more) {
+      if (more && !QUANT) {
         next(k0 + kPreKeys);
         load_k(run);
         load_v(run);
@@ -1373,25 +1417,44 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
       __syncthreads();
     }
     f16v s = {}, s1 = {};
-    // the small part products of all dims first: few roundings at a score's own size
+    if constexpr (QUANT) {
+      // the small part products apart: few roundings at a score's own size. A
+      // step's parts are asked for before the last one's products (left to
+      // itself the compiler waits for each: 745 -> 7xx us).
+      auto part = [&](int x, int i) __attribute__((always_inline)) { return *(const vec*)&tl.k[x][col][16 * i + 8 * half]; };
+      vec k0 = part(0, 0), k1 = part(1, 0);
 #pragma unroll
-    for (int i = 0; i < KT; ++i) {
-      f16v& c = i % 2 == 0 ? s : s1;
-      vec kk[NK];
+      for (int i = 0; i < KT; ++i) {
+        const vec n0 = part(0, i + 1 < KT ? i + 1 : i), n1 = part(1, i + 1 < KT ? i + 1 : i);
+        __builtin_amdgcn_sched_barrier(0);
+        s1 = Tr::mfma32(k1, q[0][i], s1);
+        s = Tr::mfma32(k0, q[0][i], s);
+        s1 = Tr::mfma32(k0, q_part(1, i), s1);
+        __builtin_amdgcn_sched_barrier(0);
+        k0 = n0;
+        k1 = n1;
+      }
+    } else {
+      // the small part products of all dims first: few roundings at a score's own size
 #pragma unroll
-      for (int x = 0; x < NK; ++x) kk[x] = *(const vec*)&tl.k[x][col][16 * i + 8 * half];
+      for (int i = 0; i < KT; ++i) {
+        f16v& c = i % 2 == 0 ? s : s1;
+        vec kk[NK];
 #pragma unroll
-      for (int sum = NP - 1; sum > 0; --sum)
+        for (int x = 0; x < NK; ++x) kk[x] = *(const vec*)&tl.k[x][col][16 * i + 8 * half];
 #pragma unroll
-        for (int x = NK - 1; x >= 0; --x)
-          if (sum - x >= 0 && sum - x < NP) c = Tr::mfma32(kk[x], q_part(sum - x, i), c);
-    }
-    // (fp32's parts are read again: held across the loops they spill)
-    if constexpr (NK > 2 && HD <= 128) asm volatile("" ::: "memory");
+        for (int sum = NP - 1; sum > 0; --sum)
 #pragma unroll
-    for (int i = 0; i < KT; ++i) {
-      f16v& c = i % 2 == 0 ? s : s1;
-      c = Tr::mfma32(*(const vec*)&tl.k[0][col][16 * i + 8 * half], q[0][i], c);
+          for (int x = NK - 1; x >= 0; --x)
+            if (sum - x >= 0 && sum - x < NP) c = Tr::mfma32(kk[x], q_part(sum - x, i), c);
+      }
+      // (fp32's parts are read again: held across the loops they spill)
+      if constexpr (NK > 2 && HD <= 128) asm volatile("" ::: "memory");
+#pragma unroll
+      for (int i = 0; i < KT; ++i) {
+        f16v& c = i % 2 == 0 ? s : s1;
+        c = Tr::mfma32(*(const vec*)&tl.k[0][col][16 * i + 8 * half], q[0][i], c);
+      }
     }
     s += s1;
     if constexpr (BUF == 1) {
@@ -1453,7 +1516,7 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
     if constexpr (kSlack > 0.0f) mx = mx > m + kSlack ? mx : m;
     // rows with nothing visible yet keep m = -inf and weight 0
     // (a weight times its value row's power ends below 2^15)
-    const float new_lift = QUANT ? Tr::kLift - (float)((int)(__builtin_bit_cast(uint32_t, vtop) >> 23) - 127) : Tr::kLift;
+    const float new_lift = QUANT ? kLift - (float)((int)(__builtin_bit_cast(uint32_t, vtop) >> 23) - 127) : kLift;
     const float ref = (mx == -INFINITY ? 0.0f : mx) - new_lift;
     if (__any(mx != m || (QUANT && new_lift != lift))) {
       float alpha = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mx);
@@ -1477,7 +1540,7 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         uint32_t x[NP];
-        if constexpr (QUANT) split_pair<M>(s[2 * j] * vf[2 * j], s[2 * j + 1] * vf[2 * j + 1], x);
+        if constexpr (QUANT) split_halves(s[2 * j] * vf[2 * j], s[2 * j + 1] * vf[2 * j + 1], minus_one, x);
         else split_pair<M>(s[2 * j], s[2 * j + 1], x);
 #pragma unroll
         for (int i = 0; i < NP; ++i) w[i][j] = x[i];
@@ -1488,20 +1551,46 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
         for (int u = 0; u < 2; ++u)
           p[i][u] = __builtin_bit_cast(vec, u32x4_t{w[i][4 * u], w[i][4 * u + 1], w[i][4 * u + 2], w[i][4 * u + 3]});
     }
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int b = 0; b < VB; ++b) {
-        const int at = v_slot(2 * u + half, 32 * b + col);
-        vec vv[NK];
-#pragma unroll
-        for (int x = 0; x < NK; ++x) vv[x] = *(const vec*)&tl.v[x][32 * b + col][at];
-#pragma unroll
-        for (int sum = NP - 1; sum >= 0; --sum)
-#pragma unroll
-          for (int x = NK - 1; x >= 0; --x)
-            if (sum - x >= 0 && sum - x < NP) acc[b] = Tr::mfma32(vv[x], p[sum - x][u], acc[b]);
+    if constexpr (BUF == 2 && QUANT)
+      if (more) {
+        next(k0 + kPreKeys);
+        load_k(run);
+        load_v(run);
       }
+    if constexpr (QUANT) {
+      auto part = [&](int x, int n) __attribute__((always_inline)) {
+        const int u = n / VB, dim = 32 * (n % VB) + col;
+        return *(const vec*)&tl.v[x][dim][v_slot(2 * u + half, dim)];
+      };
+      vec v0 = part(0, 0), v1 = part(1, 0);
+#pragma unroll
+      for (int n = 0; n < 2 * VB; ++n) {
+        const vec n0 = part(0, n + 1 < 2 * VB ? n + 1 : n), n1 = part(1, n + 1 < 2 * VB ? n + 1 : n);
+        __builtin_amdgcn_sched_barrier(0);
+        f16v& c = acc[n % VB];
+        c = Tr::mfma32(v1, p[0][n / VB], c);
+        c = Tr::mfma32(v0, p[1][n / VB], c);
+        c = Tr::mfma32(v0, p[0][n / VB], c);
+        __builtin_amdgcn_sched_barrier(0);
+        v0 = n0;
+        v1 = n1;
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int b = 0; b < VB; ++b) {
+          const int at = v_slot(2 * u + half, 32 * b + col);
+          vec vv[NK];
+#pragma unroll
+          for (int x = 0; x < NK; ++x) vv[x] = *(const vec*)&tl.v[x][32 * b + col][at];
+#pragma unroll
+          for (int sum = NP - 1; sum >= 0; --sum)
+#pragma unroll
+            for (int x = NK - 1; x >= 0; --x)
+              if (sum - x >= 0 && sum - x < NP) acc[b] = Tr::mfma32(vv[x], p[sum - x][u], acc[b]);
+        }
+    }
     if constexpr (BUF == 2) {
       if (more) {
         put_k(lds.tile[cur ^ 1], k0 + kPreKeys, par ^ 1);

@@ -192,6 +192,7 @@ __global__ __launch_bounds__(kDecThreads, (DecQuant<T, HD>::kPerCu)) void paged_
     float m = -INFINITY, l = 0.0f;  // of the column's head; l of this quarter's keys
     f4 acc[VD];                     // dims 2 (4 ak + r) + c % 2 of block c / 2 of the column
     float lift = kMostLift, acc_m[BR];
+    const float minus_one = hidden_minus_one();
 #pragma unroll
     for (int c = 0; c < VD; ++c) acc[c] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -304,7 +305,7 @@ __global__ __launch_bounds__(kDecThreads, (DecQuant<T, HD>::kPerCu)) void paged_
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           uint32_t q[NP];
-          split_pair<_Float16>(p[2 * j] * scale_d(vs[2 * j][c]), p[2 * j + 1] * scale_d(vs[2 * j + 1][c]), q);
+          split_halves(times_d(vs[2 * j][c], p[2 * j]), times_d(vs[2 * j + 1][c], p[2 * j + 1]), minus_one, q);
 #pragma unroll
           for (int n = 0; n < NP; ++n) w[n][j] = q[n];
         }
