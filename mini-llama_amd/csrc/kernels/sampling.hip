@@ -40,6 +40,23 @@ __device__ __forceinline__ float of_key(uint32_t k) {
   return __builtin_bit_cast(float, k & 0x80000000u ? k : ~k & 0x7fffffffu);
 }
 
+// The value of the lane J away (a power of two).
+template <int J>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t x) {
+  if constexpr (J == 1) return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, kDppXor1, 0xF, 0xF, false);
+  if constexpr (J == 2) return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, kDppXor2, 0xF, 0xF, false);
+  if constexpr (J == 4)  // (7 away, then 3)
+    return (uint32_t)__builtin_amdgcn_mov_dpp(__builtin_amdgcn_mov_dpp((int)x, kDppHalfMirror, 0xF, 0xF, false), 0x1B, 0xF, 0xF, false);
+  if constexpr (J == 8) return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, kDppRor8, 0xF, 0xF, false);
+  if constexpr (J == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return threadIdx.x & 16 ? (uint32_t)r[0] : (uint32_t)r[1];
+  }
+  if constexpr (J == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return threadIdx.x & 32 ? (uint32_t)r[0] : (uint32_t)r[1];
+  }
+}
 struct SampleLds {
   uint32_t count[kBins];
   uint64_t weight[kBins];
@@ -223,14 +240,21 @@ __device__ __forceinline__ void for_each(const float* logits, int lo, int hi, F 
 }
 
 // The largest of what the threads have and the first index with it, as the key
-// and the index in one number, in every thread; no candidates: all ones.
+// and the index in one number; no candidates: all ones.
+template <int J>
+__device__ __forceinline__ uint64_t wave_least(uint64_t x) {
+  x = min(x, (uint64_t)lane_xor<J>((uint32_t)(x >> 32)) << 32 | lane_xor<J>((uint32_t)x));
+  if constexpr (J > 1) return wave_least<J / 2>(x);
+  return x;
+}
+__device__ __forceinline__ uint64_t first_of_wave(float top, int at) {
+  return wave_least<32>(top == -INFINITY ? ~0ull : (uint64_t)key_of(top) << 32 | (uint32_t)at);
+}
+// (in every thread of the workgroup)
 __device__ __forceinline__ uint64_t first_of(float top, int at, uint64_t* lds) {
-  const float best = wave_max(top);
-  uint32_t first = top == best ? (uint32_t)at : 0x7fffffffu;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) first = min(first, (uint32_t)__shfl_xor((int)first, d));
+  const uint64_t mine = first_of_wave(top, at);
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = best == -INFINITY ? ~0ull : (uint64_t)key_of(best) << 32 | first;
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = mine;
   __syncthreads();
   uint64_t least = ~0ull;
 #pragma unroll
@@ -400,30 +424,22 @@ __device__ __forceinline__ uint64_t quick_units(double y) {  // y = (l - top) lo
   return __builtin_bit_cast(uint64_t, w) & ((1ull << 52) - 1);
 }
 
-// Bins a unit of logit, for a whole row the same in all its parts: from the
-// spread of a thousand of its logits. 32 T are e^-32, less than half a unit.
-__device__ double grid_of(const float* logits, int vocab, float t, float* lds) {
-  const int tid = threadIdx.x;
-  const float l = candidate(logits[(int)((int64_t)tid * vocab / kSampleThreads)]), ref = candidate(logits[0]);
-  const float x = l == -INFINITY ? 0.0f : l - (ref == -INFINITY ? 0.0f : ref);
-  const float n = wave_sum(l == -INFINITY ? 0.0f : 1.0f), s = wave_sum(x), q = wave_sum(x * x);
-  __syncthreads();
-  if ((tid & 63) == 0) {
-    lds[3 * (tid >> 6)] = n;
-    lds[3 * (tid >> 6) + 1] = s;
-    lds[3 * (tid >> 6) + 2] = q;
+// A thousand logits' number, sum and sum of squares about the row's first one,
+// one logit a thread.
+struct Spread {
+  float n, s, q;
+  __device__ __forceinline__ Spread(float l, float ref) {
+    const float x = l == -INFINITY ? 0.0f : l - (ref == -INFINITY ? 0.0f : ref);
+    n = wave_sum(l == -INFINITY ? 0.0f : 1.0f);
+    s = wave_sum(x);
+    q = wave_sum(x * x);
   }
-  __syncthreads();
-  float an = 0.0f, as = 0.0f, aq = 0.0f;
-#pragma unroll
-  for (int w = 0; w < kSampleWaves; ++w) {
-    an += lds[3 * w];
-    as += lds[3 * w + 1];
-    aq += lds[3 * w + 2];
-  }
-  const float var = aq / an - (as / an) * (as / an);
+};
+// Bins a unit of logit from that. 32 T are e^-32, less than half a unit, and 14
+// of the spread reach from the largest, 5 to 8 above the middle, far enough down.
+__device__ __forceinline__ double grid_of(float n, float s, float q, float t) {
+  const float var = q / n - (s / n) * (s / n);
   double span = 32.0 * (double)t;
-  // (14 of the spread: the largest lies 5 to 8 above the middle)
   if (var > 0.0f && var < 1e30f) span = fmin(span, 14.0 * (double)sqrtf(var));
   return (double)(kGrid - 1) / span;
 }
@@ -436,16 +452,20 @@ constexpr double kLog2e = 1.44269504088896340736;
 __global__ __launch_bounds__(kSampleThreads) void sample_parts_kernel(SampleArgs a, PartsView v, int parts, int part_len) {
   __shared__ uint64_t units[kGrid];
   __shared__ uint32_t count[kGrid];
-  __shared__ uint64_t scan[kSampleWaves];
-  __shared__ float stats[3 * kSampleWaves];
-  const int part = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
+  __shared__ uint64_t first_lds[kSampleWaves];
+  __shared__ float spread[kSampleWaves][3];
+  __shared__ uint64_t units_lds[kSampleWaves];
+  __shared__ uint32_t count_lds[kSampleWaves];
+  const int part = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, wave = tid >> 6;
+  const bool leads = (tid & 63) == 0;
   const float* logits = a.logits + row * a.stride;
   const Ask s = ask_of(a, row);
   const size_t at = (size_t)row * parts + part;
+  // (the same logits in every part of a row; asked for with the part's own)
+  const float sampled = logits[(int)((int64_t)tid * a.vocab / kSampleThreads)], zeroth = logits[0];
   count[tid] = 0;
   units[tid] = 0;
   if (part == 0 && tid == 0) v.state[row].listed = 0;
-  const double grid = s.greedy ? 0.0 : grid_of(logits, a.vocab, s.t, stats);
   over(logits, part * part_len, min((part + 1) * part_len, a.vocab), [&](auto each) __attribute__((always_inline)) {
     float top = -INFINITY;
     int index = 0x7fffffff;
@@ -455,8 +475,24 @@ __global__ __launch_bounds__(kSampleThreads) void sample_parts_kernel(SampleArgs
         index = i;
       }
     });
-    const uint64_t first = first_of(top, index, scan);
+    uint64_t first = first_of_wave(top, index);
+    const Spread sp(candidate(sampled), candidate(zeroth));
+    if (leads) {
+      first_lds[wave] = first;
+      spread[wave][0] = sp.n;
+      spread[wave][1] = sp.s;
+      spread[wave][2] = sp.q;
+    }
+    __syncthreads();
+    float n3[3] = {};
+#pragma unroll
+    for (int w = 0; w < kSampleWaves; ++w) {
+      first = min(first, first_lds[w]);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) n3[i] += spread[w][i];
+    }
     top = top_of(first);
+    const double grid = s.greedy ? 0.0 : grid_of(n3[0], n3[1], n3[2], s.t);
     uint64_t all = 0;
     uint32_t n = 0;
     if (!s.greedy && top != -INFINITY) {
@@ -474,13 +510,24 @@ __global__ __launch_bounds__(kSampleThreads) void sample_parts_kernel(SampleArgs
           atomicAdd((unsigned long long*)&units[bin_of(l, top_bin, grid)], (unsigned long long)x);
           all += x;
         });
-      all = block_sum(all, scan);  // (its barriers are the histogram's, too)
-      n = (uint32_t)block_sum(n, scan);
     }
-    if (tid == 0) v.head[at] = {first, all, grid, n, 0};
+    all = (uint64_t)readlane64(wave_scan64((int64_t)all), 63);
+    n = (uint32_t)readlane64(wave_scan64((int64_t)n), 63);
+    if (leads) {
+      units_lds[wave] = all;
+      count_lds[wave] = n;
+    }
+    __syncthreads();  // (and the histogram is whole)
+    if (tid == 0) {
+      all = n = 0;
+      for (int w = 0; w < kSampleWaves; ++w) {
+        all += units_lds[w];
+        n += count_lds[w];
+      }
+      v.head[at] = {first, all, grid, n, 0};
+    }
   });
   if (s.greedy) return;
-  __syncthreads();
   if (s.counts()) v.count[at * kGrid + tid] = count[tid];
   if (!s.light()) v.units[at * kGrid + tid] = units[tid];
 }
@@ -508,11 +555,8 @@ struct ListLds {
   uint32_t c[kGrid + 1];
   uint64_t scan[kSampleWaves];
   int bins[8];
-  PartHead head[kMaxParts];
   uint32_t found, place;
   uint64_t list[kListed];
-  int off[kMaxParts];    // bins from the row's largest logit to the part's
-  double f[kMaxParts];   // what a unit of the part is in the row's
 };
 
 __global__ __launch_bounds__(kSampleThreads) void sample_list_kernel(SampleArgs a, PartsView v, int parts, int part_len) {
@@ -520,49 +564,58 @@ __global__ __launch_bounds__(kSampleThreads) void sample_list_kernel(SampleArgs 
   const int part = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
   const float* logits = a.logits + row * a.stride;
   const Ask s = ask_of(a, row);
-  if (tid < parts) lds.head[tid] = v.head[(size_t)row * parts + tid];
-  __syncthreads();
-  uint64_t first = ~0ull;
-  double grid = 0.0;
-  for (int i = 0; i < parts; ++i) {
-    if (lds.head[i].top < first) {
-      first = lds.head[i].top;
-      grid = lds.head[i].grid;
-    }
-  }
+  // (lane i of every wave has part i's)
+  PartHead h = {~0ull, 0, 0.0, 0, 0};
+  if ((tid & 63) < parts) h = v.head[(size_t)row * parts + (tid & 63)];
+  const uint64_t first = wave_least<32>(h.top);
   const float top = top_of(first);
   if (part == 0 && tid == 0) v.state[row].top = first;
   if (s.greedy || top == -INFINITY) return;
+  const uint64_t grid_bits = __builtin_bit_cast(uint64_t, h.grid);
+  const double grid = __builtin_bit_cast(double, (uint64_t)readlane64((int64_t)grid_bits, __builtin_ctzll(__ballot(h.top == first))));
   const double top_bin = floor((double)top * grid);
   const bool light = s.light();
 
   // ---- the parts' histograms added up, each moved to the row's largest logit
-  if (tid < parts) {
-    const float t = top_of(lds.head[tid].top);
-    lds.off[tid] = t == -INFINITY ? kGrid : (int)fmin(top_bin - floor((double)t * grid), (double)kGrid);
-    lds.f[tid] = t == -INFINITY ? 0.0 : exp2((((double)t - (double)top) * kLog2e) / (double)s.t);
-  }
-  __syncthreads();
-  uint64_t w = 0, all_w = 0;
-  uint32_t c = 0, all_c = 0;
+  const bool any = h.top != ~0ull;
+  const float t = any ? top_of(h.top) : top;
+  // bins from the row's largest logit to the part's, what a unit of the part is in the row's
+  const int off_lane = any ? (int)fmin(top_bin - floor((double)t * grid), (double)kGrid) : kGrid;
+  const double f_lane = light || !any ? 0.0 : exp2((((double)t - (double)top) * kLog2e) / (double)s.t);
+  const uint32_t all_c = (uint32_t)readlane64(wave_scan64(any ? (int64_t)h.count : 0), 63);
+  const uint64_t all_w = (uint64_t)readlane64(wave_scan64((int64_t)((double)h.units * f_lane + 0.5)), 63);
+  uint64_t w = 0;
+  uint32_t c = 0;
   const size_t at0 = (size_t)row * parts * kGrid;
-#pragma unroll 8
-  for (int i = 0; i < parts; ++i) {
-    // (loads without a condition are asked for together)
-    const int b = tid - lds.off[i];
-    const bool in = b >= 0 && tid < kGrid - 1;
-    const size_t at = at0 + i * kGrid + (in ? b : 0);
-    if (s.counts()) {
-      const uint32_t x = v.count[at];
-      c += in ? x : 0;
+  // (loads without a condition between them are asked for together: a part that
+  // is not there has the last one's, and bins that are none the first one's)
+  constexpr int kAhead = 8;
+  auto place = [&](int i, bool* in) __attribute__((always_inline)) {
+    const int n = min(i, parts - 1), b = tid - __builtin_amdgcn_readlane(off_lane, n);
+    *in = i < parts && b >= 0 && tid < kGrid - 1;
+    return at0 + (size_t)n * kGrid + (b >= 0 ? b : 0);
+  };
+  if (s.counts())
+    for (int i0 = 0; i0 < parts; i0 += kAhead) {
+      uint32_t x[kAhead];
+      bool in[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) x[i] = v.count[place(i0 + i, &in[i])];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) c += in[i] ? x[i] : 0;
     }
-    if (!light) {
-      const uint64_t x = v.units[at];
-      w += in ? (uint64_t)((double)x * lds.f[i] + 0.5) : 0;
+  if (!light)
+    for (int i0 = 0; i0 < parts; i0 += kAhead) {
+      uint64_t x[kAhead];
+      bool in[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) x[i] = v.units[place(i0 + i, &in[i])];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const double f = __builtin_bit_cast(double, (uint64_t)readlane64((int64_t)__builtin_bit_cast(uint64_t, f_lane), min(i0 + i, parts - 1)));
+        w += in[i] ? (uint64_t)((double)x[i] * f + 0.5) : 0;
+      }
     }
-    all_c += lds.head[i].count;
-    all_w += (uint64_t)((double)lds.head[i].units * lds.f[i] + 0.5);
-  }
   uint64_t sum_w, sum_c;
   const uint64_t before_w = block_before(w, lds.scan, &sum_w), before_c = block_before(c, lds.scan, &sum_c);
   // (what is not in a bin of its own is in the last one)
@@ -672,23 +725,6 @@ __global__ __launch_bounds__(kSampleThreads) void sample_list_kernel(SampleArgs 
     if (lds.place + i < kListed) list[lds.place + i] = lds.list[i];
 }
 
-// The value of the lane J away (a power of two).
-template <int J>
-__device__ __forceinline__ uint32_t lane_xor(uint32_t x) {
-  if constexpr (J == 1) return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, kDppXor1, 0xF, 0xF, false);
-  if constexpr (J == 2) return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, kDppXor2, 0xF, 0xF, false);
-  if constexpr (J == 4)  // (7 away, then 3)
-    return (uint32_t)__builtin_amdgcn_mov_dpp(__builtin_amdgcn_mov_dpp((int)x, kDppHalfMirror, 0xF, 0xF, false), 0x1B, 0xF, 0xF, false);
-  if constexpr (J == 8) return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, kDppRor8, 0xF, 0xF, false);
-  if constexpr (J == 16) {
-    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-    return threadIdx.x & 16 ? (uint32_t)r[0] : (uint32_t)r[1];
-  }
-  if constexpr (J == 32) {
-    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-    return threadIdx.x & 32 ? (uint32_t)r[0] : (uint32_t)r[1];
-  }
-}
 // A bitonic network's steps J, J / 2 .. 1 within the wave; `up`: ascending.
 template <int J>
 __device__ __forceinline__ void sort_lanes(uint64_t& x, bool up) {
