@@ -1420,7 +1420,7 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
     if constexpr (QUANT) {
       // the small part products apart: few roundings at a score's own size. A
       // step's parts are asked for before the last one's products (left to
-      // itself the compiler waits for each: 745 -> 7xx us).
+      // itself the compiler waits for each: 745 -> 708 us).
       auto part = [&](int x, int i) __attribute__((always_inline)) { return *(const vec*)&tl.k[x][col][16 * i + 8 * half]; };
       vec k0 = part(0, 0), k1 = part(1, 0);
 #pragma unroll
