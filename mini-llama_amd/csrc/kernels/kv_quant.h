@@ -55,7 +55,8 @@ __device__ __forceinline__ KvScale kv_scale(float lo, float hi) {
 
 // The code of x: the nearest of d (c - z) + m, upwards from halfway. Decided
 // exactly: fp32 gives it but for a neighbour, and whether x is past that one's
-// border is asked in 64 bits, which hold the border and x - m.
+// border is asked in 64 bits, which hold the border (multiples of 2^-25 below
+// 2^25) where they do not hold x - m of a tiny x.
 template <typename Q>
 __device__ __forceinline__ int kv_code(float x, KvScale s, float inv) {
   constexpr float kLo = -(float)Q::kMiddle, kHi = (float)(Q::kLevels - Q::kMiddle);
@@ -63,9 +64,8 @@ __device__ __forceinline__ int kv_code(float x, KvScale s, float inv) {
   if (!(d > 0.0f)) return Q::kMiddle;
   float c = floorf(__builtin_fmaf(x - m, inv, 0.5f));
   c = fminf(fmaxf(c, kLo), kHi);
-  const double u = (double)x - (double)m;
-  if (u >= ((double)c + 0.5) * (double)d) c += 1.0f;
-  else if (u < ((double)c - 0.5) * (double)d) c -= 1.0f;
+  if ((double)x >= __builtin_fma((double)c + 0.5, (double)d, (double)m)) c += 1.0f;
+  else if ((double)x < __builtin_fma((double)c - 0.5, (double)d, (double)m)) c -= 1.0f;
   return (int)fminf(fmaxf(c, kLo), kHi) + Q::kMiddle;
 }
 

@@ -35,7 +35,10 @@ def quantise(x, kind):
             fine &= np.isfinite(d) & np.isfinite(m)
             d, m = np.where(fine, d, np.float16(np.nan)), np.where(fine, m, np.float16(np.nan))
             d64, m64 = d.astype(np.float64)[..., None], m.astype(np.float64)[..., None]
-            c = np.floor((e.astype(np.float64) - m64) / d64 + 0.5) + middle
+            # (64 bits hold the borders, not the quotient of an element that is tiny next to m)
+            e64 = e.astype(np.float64)
+            c = np.floor((e64 - m64) / d64 + 0.5)
+            c = c + (e64 >= (c + 0.5) * d64 + m64) - (e64 < (c - 0.5) * d64 + m64) + middle
             codes[..., b, :e.shape[-1]] = np.where(d64 > 0, np.clip(c, 0, levels), middle)
             scales[..., b, 0], scales[..., b, 1] = d, m
     pairs = np.moveaxis(codes.reshape(lead + (nb, 16, 2)), -3, -2)

@@ -72,6 +72,32 @@ def test_write_and_read(paged, kind, rows, kv, hd, page):
         assert np.array_equal(got.cpu().numpy(), y, equal_nan=True)
 
 
+@pytest.mark.parametrize("kind", ["q4", "q8"])
+def test_elements_next_to_a_border(paged, kind):
+    """x = m + (c + 1/2) d is rounded up, the float below it down, also where the border is 0 and x - m rounds to it."""
+    levels, middle, _ = kvq.KINDS[kind]
+    x = np.zeros((40, 1, 64), np.float32)
+    r = np.random.default_rng(2)
+    for i in range(40):
+        d = np.float32(2.0 ** r.integers(-12, 6))
+        m = np.float32(-(r.integers(-6, 6) + 0.5)) * d if i % 2 else np.float32(r.integers(-40, 40)) * d
+        for b in range(2):
+            border = m + (r.integers(0, levels, 32).astype(np.float32) - middle + np.float32(0.5)) * d
+            near = np.where(r.random(32) < 0.5, border, np.nextafter(border, np.float32(-np.inf), dtype=np.float32))
+            near = np.where((r.random(32) < 0.3) & (border == 0), np.float32(-1e-30), near)
+            if i % 2:
+                near[5:8] = -1e-30, -2.0 ** -149, 0.0
+            near[:2] = m - middle * d, m + (levels - middle) * d  # (the block's ends: they give d and m back)
+            x[i, 0, 32 * b:32 * b + 32] = near
+    rows = kvq.quantise(x, kind)
+    assert len(np.unique(rows[..., :16 * 2 * kvq.KINDS[kind][2]])) > 10
+    slots = np.arange(40, dtype=np.int64)
+    cache = paged.PagedCache.empty(1, 3, 16, 1, 64, kind)
+    paged.write(cache, 0, dev(x), dev(x), dev(slots))
+    for pool in (cache.keys, cache.values):
+        assert np.array_equal(pool[0].cpu().numpy()[slots // 16, :, slots % 16], rows)
+
+
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
 @pytest.mark.parametrize("rows,kv,hd,page", ROWS[:9])
 def test_write_and_read_of_other_types(paged, dtype, rows, kv, hd, page):

@@ -21,6 +21,16 @@ def cache(pkg, **kw):
     return pkg.MlqPagedCache(*(f[n] for n, _ in pkg.MlqPagedCache._fields_))
 
 
+def test_the_definition_at_a_border():
+    """A block of -8.5 .. 6.5 has d = 1 and m = -0.5: 0 is halfway from code 8 to 9, what is below it has code 8."""
+    x = np.full((1, 32), 1.0, np.float32)
+    x[0, :6] = -8.5, 6.5, 0.0, -1e-30, -2.0 ** -149, -1e-3
+    row = kvq.quantise(x, "q4")[0]
+    codes = np.stack([row[:32:2] & 15, row[:32:2] >> 4], -1).reshape(-1)
+    assert list(codes[:7]) == [0, 15, 9, 8, 8, 8, 10]
+    assert list(row[32:36].view(np.float16)) == [1.0, -0.5]
+
+
 @pytest.mark.parametrize("kind", ["q4", "q8"])
 @pytest.mark.parametrize("hd", [8, 64, 72, 128, 136, 256])
 def test_cache_bytes(pkg, kind, hd):
