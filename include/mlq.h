@@ -620,7 +620,7 @@ int mlq_qk_norm_rope(const mlq_rotary* r, int rows, const int32_t* positions, in
  * slot is outside the cache is left out. k_out and v_out, NULL or not each by
  * itself, receive the values that the cache now stands for (k_out may be k,
  * v_out v, with the same strides; no other overlap). Strides, alignment, distinct
- * slots and rows = 0 as in mlq_qk_norm_rope. Fewer than 2^28 / n_kv_heads rows
+ * slots and rows = 0 as in mlq_qk_norm_rope. Fewer than 2^27 / n_kv_heads rows
  * (MLQ_ERR_UNSUPPORTED otherwise). */
 int mlq_paged_write(const mlq_paged_cache* c, int layer, int rows, const int64_t* slots,
                     const float* k, int64_t k_stride, const float* v, int64_t v_stride,
@@ -667,7 +667,10 @@ int mlq_paged_attention_workspace(const mlq_paged_cache* c, int n_heads, int n_s
  * ones are lost: a score is off by up to 2^-39 max|q| sum|k| scale) and of
  * the largest weight in each weight; cached fp16 values below the smallest
  * normal number, 6.1e-5, enter with an absolute error of up to 2^-37 (storing
- * them rounds by up to 2^-25).
+ * them rounds by up to 2^-25). Q4 and Q8: what the codes stand for, not rounded
+ * again; q and the weights in two parts of fp16 with the same absolute errors, a
+ * weight's times the largest d among the keys; prefill has elements in two parts
+ * too, with one of up to 2^-39 of the largest in the key's or value's row.
  * NaN / inf among the seen keys and values give NaN / inf outputs. ws:
  * 256-byte aligned, scratch, may be NULL when its size is 0; calls that
  * share one (two captured graphs, too) must be ordered. n_heads: up to 2048

@@ -62,7 +62,7 @@ def test_rows_of_their_own_settings(sampling, vocab, sharp):
     check(sampling, x, r.random(rows), stride=vocab + 3, **settings(r, rows))
 
 
-@pytest.mark.parametrize("rows,vocab", [(1, 152064), (3, 40000), (130, 20000), (700, 5000), (3000, 700)])
+@pytest.mark.parametrize("rows,vocab", [(1, 152064), (3, 40000), (130, 20000), (700, 5000), (1500, 4500), (3000, 700)])
 def test_numbers_of_rows(sampling, rows, vocab):
     r = np.random.default_rng(rows)
     x = (r.standard_normal((rows, vocab)) * 3).astype(np.float32)
