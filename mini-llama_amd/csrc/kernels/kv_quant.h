@@ -40,14 +40,25 @@ struct KvScale {
   _Float16 d, m;
 };
 
+// A rounding of its own: the compiler makes one of a sum's to fp32 and its result's
+// to fp16 (an instruction that gives fp16 right away), which is off at fp16's ties.
+__device__ __forceinline__ _Float16 half_of_float(float x) {
+  asm("" : "+v"(x));
+  return (_Float16)x;
+}
+
 // From the block's least and largest element (-inf and inf where one is not
 // finite). A range or middle that fp16 does not hold gives NaN: the whole block
 // then reads as NaN.
 template <typename Q>
 __device__ __forceinline__ KvScale kv_scale(float lo, float hi) {
   KvScale s;
-  s.d = (_Float16)((hi - lo) / (float)Q::kLevels);
-  s.m = (_Float16)(lo + (float)Q::kMiddle * (float)s.d);
+  // (the quotient as a division rounds it: true of 15 and 255 for every fp32
+  // mantissa; where exponents end, fp16 has d 0 or NaN either way)
+  constexpr float kInv = 1.0f / (float)Q::kLevels;
+  const float q = (hi - lo) * kInv;
+  s.d = half_of_float(__builtin_fmaf(__builtin_fmaf(-q, (float)Q::kLevels, hi - lo), kInv, q));
+  s.m = half_of_float(lo + (float)Q::kMiddle * (float)s.d);
   const float all = (float)s.d * 0.0f + (float)s.m * 0.0f;
   if (!(all == 0.0f)) s.d = s.m = __builtin_bit_cast(_Float16, (uint16_t)0x7e00);
   return s;
@@ -57,6 +68,7 @@ __device__ __forceinline__ KvScale kv_scale(float lo, float hi) {
 // exactly: fp32 gives it but for a neighbour, and whether x is past that one's
 // border is asked in 64 bits, which hold the border (multiples of 2^-25 below
 // 2^25) where they do not hold x - m of a tiny x.
+// inv: 1 / d to a few units in its last place.
 template <typename Q>
 __device__ __forceinline__ int kv_code(float x, KvScale s, float inv) {
   constexpr float kLo = -(float)Q::kMiddle, kHi = (float)(Q::kLevels - Q::kMiddle);

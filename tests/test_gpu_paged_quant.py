@@ -98,6 +98,28 @@ def test_elements_next_to_a_border(paged, kind):
         assert np.array_equal(pool[0].cpu().numpy()[slots // 16, :, slots % 16], rows)
 
 
+@pytest.mark.parametrize("kind", ["q4", "q8"])
+def test_scales_are_rounded_twice(paged, kind):
+    """m = lo + z d is rounded to fp32 and then to fp16: 1 + 2^-11 + 2^-30 becomes 1 + 2^-11, a tie, and that 1."""
+    levels, middle, _ = kvq.KINDS[kind]
+    lo = np.float32(2.0 ** -11 + 2.0 ** -30)
+    x = np.full((16, 1, 64), lo, np.float32)
+    x[:, 0, 1::2] = lo + np.float32(levels / middle)
+    rows = kvq.quantise(x, kind)
+    scales = rows[0, 0, 16 * 2 * kvq.KINDS[kind][2]:].view(np.float16)
+    assert list(scales[:2]) == [1.0 / middle, 1.0]
+    slots = np.arange(16, dtype=np.int64)
+    cache = paged.PagedCache.empty(1, 1, 16, 1, 64, kind)
+    paged.write(cache, 0, dev(x), dev(x), dev(slots))
+    assert np.array_equal(cache.keys[0, 0, 0].cpu().numpy(), rows[:, 0])
+    # (and rotated by nothing, a position of 0)
+    cache.keys.zero_()
+    rotary = paged.Rotary(64, dev(paged.rope_frequencies(1e4, 64)[0]))
+    paged.qk_norm_rope(rotary, dev(x), dev(x), dev(x), dev(np.zeros(16, np.int32)), cache=cache, slots=dev(slots))
+    assert np.array_equal(cache.keys[0, 0, 0].cpu().numpy(), rows[:, 0])
+    assert np.array_equal(cache.values[0, 0, 0].cpu().numpy(), rows[:, 0])
+
+
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
 @pytest.mark.parametrize("rows,kv,hd,page", ROWS[:9])
 def test_write_and_read_of_other_types(paged, dtype, rows, kv, hd, page):
