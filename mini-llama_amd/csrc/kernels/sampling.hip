@@ -214,10 +214,10 @@ __device__ __forceinline__ uint64_t token_target(float u, uint64_t all) {
 
 // f(l, i) for the candidates l at lo <= i < hi, by the whole workgroup, several
 // loads at a time.
-template <typename F>
+template <int THREADS, typename F>
 __device__ __forceinline__ void for_each(const float* logits, int lo, int hi, F f) {
   typedef float v4 __attribute__((ext_vector_type(4), aligned(4)));
-  constexpr int kStep = 4 * kSampleThreads, kAhead = 4;
+  constexpr int kStep = 4 * THREADS, kAhead = 4;
   int i = lo + 4 * (int)threadIdx.x;
   for (; i + (kAhead - 1) * kStep + 3 < hi; i += kAhead * kStep) {
     v4 x[kAhead];
@@ -261,15 +261,15 @@ __device__ __forceinline__ uint64_t first_of(float top, int at, uint64_t* lds) {
   for (int w = 0; w < kSampleWaves; ++w) least = min(least, lds[w]);
   return least;
 }
-// Calls `all` with the f that goes over the candidates of a range: up to kHeld of
-// them are asked for at once and stay in registers however often it is called.
-constexpr int kHeldQuads = 8, kHeld = 4 * kHeldQuads * kSampleThreads;
-template <typename A>
+// Calls `all` with the f that goes over the candidates of a range: up to QUADS of
+// four a thread are asked for at once and stay in registers however often it is
+// called.
+template <int THREADS, int QUADS, typename A>
 __device__ __forceinline__ void over(const float* logits, int lo, int hi, A all) {
   typedef float v4 __attribute__((ext_vector_type(4), aligned(4)));
-  constexpr int kStep = 4 * kSampleThreads;
-  if (hi - lo > kHeld) {
-    all([&](auto f) __attribute__((always_inline)) { for_each(logits, lo, hi, f); });
+  constexpr int kStep = 4 * THREADS, kHeldQuads = QUADS;
+  if (hi - lo > kHeldQuads * kStep) {
+    all([&](auto f) __attribute__((always_inline)) { for_each<THREADS>(logits, lo, hi, f); });
     return;
   }
   v4 x[kHeldQuads];
@@ -302,7 +302,7 @@ __device__ int sample_row(const SampleArgs& a, int row, const Ask& s, float top,
   const Row r = {a.logits + row * a.stride, a.vocab, top, 1.0 / (double)s.t};
   // ---- all candidates, and those that min_p leaves
   uint64_t count = 0, units = 0, n_m = 0, w_m = 0;
-  for_each(r.logits, 0, a.vocab, [&](float l, int) __attribute__((always_inline)) {
+  for_each<kSampleThreads>(r.logits, 0, a.vocab, [&](float l, int) __attribute__((always_inline)) {
     if (l == -INFINITY) return;
     const double w = r.weight(l);
     const uint64_t x = (uint64_t)(w * kUnits + 0.5);
@@ -348,6 +348,10 @@ __device__ int sample_row(const SampleArgs& a, int row, const Ask& s, float top,
 // everything down to the bin that holds the k-th. Where the list would be
 // longer than kListed, or a place lies behind the last bin, the row is done by
 // sample_row.
+// Of the histograms' kernel: two workgroups a CU, one's loads beside the other's
+// exponentials (64 rows of 152064 logits: 80.0 us, 83.3 with 1024 threads, 85.7 with 256).
+constexpr int kPartThreads = 512, kPartWaves = kPartThreads / 64;
+constexpr int kPartQuads = 10;  // of four logits that a thread of it holds
 constexpr int kGrid = 1024;     // bins, the last of them everything behind the others
 constexpr int kListed = 4096;
 constexpr int kPartLeast = 4096;
@@ -424,15 +428,23 @@ __device__ __forceinline__ uint64_t quick_units(double y) {  // y = (l - top) lo
   return __builtin_bit_cast(uint64_t, w) & ((1ull << 52) - 1);
 }
 
-// A thousand logits' number, sum and sum of squares about the row's first one,
-// one logit a thread.
+// Logits' number, sum and sum of squares about the row's first one, kSpread of
+// them a thread.
+constexpr int kSpread = 1024 / kPartThreads;
 struct Spread {
   float n, s, q;
-  __device__ __forceinline__ Spread(float l, float ref) {
-    const float x = l == -INFINITY ? 0.0f : l - (ref == -INFINITY ? 0.0f : ref);
-    n = wave_sum(l == -INFINITY ? 0.0f : 1.0f);
-    s = wave_sum(x);
-    q = wave_sum(x * x);
+  __device__ __forceinline__ Spread(const float (&l)[kSpread], float ref) {
+    n = s = q = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kSpread; ++i) {
+      const float c = candidate(l[i]), x = c == -INFINITY ? 0.0f : c - (ref == -INFINITY ? 0.0f : ref);
+      n += c == -INFINITY ? 0.0f : 1.0f;
+      s += x;
+      q += x * x;
+    }
+    n = wave_sum(n);
+    s = wave_sum(s);
+    q = wave_sum(q);
   }
 };
 // Bins a unit of logit from that. 32 T are e^-32, less than half a unit, and 14
@@ -449,24 +461,30 @@ __device__ __forceinline__ int bin_of(float l, double top_bin, double grid) {
 
 constexpr double kLog2e = 1.44269504088896340736;
 
-__global__ __launch_bounds__(kSampleThreads) void sample_parts_kernel(SampleArgs a, PartsView v, int parts, int part_len) {
+__global__ __launch_bounds__(kPartThreads, 4) void sample_parts_kernel(SampleArgs a, PartsView v, int parts, int part_len) {
   __shared__ uint64_t units[kGrid];
   __shared__ uint32_t count[kGrid];
-  __shared__ uint64_t first_lds[kSampleWaves];
-  __shared__ float spread[kSampleWaves][3];
-  __shared__ uint64_t units_lds[kSampleWaves];
-  __shared__ uint32_t count_lds[kSampleWaves];
+  __shared__ uint64_t first_lds[kPartWaves];
+  __shared__ float spread[kPartWaves][3];
+  __shared__ uint64_t units_lds[kPartWaves];
+  __shared__ uint32_t count_lds[kPartWaves];
   const int part = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, wave = tid >> 6;
   const bool leads = (tid & 63) == 0;
   const float* logits = a.logits + row * a.stride;
   const Ask s = ask_of(a, row);
   const size_t at = (size_t)row * parts + part;
   // (the same logits in every part of a row; asked for with the part's own)
-  const float sampled = logits[(int)((int64_t)tid * a.vocab / kSampleThreads)], zeroth = logits[0];
-  count[tid] = 0;
-  units[tid] = 0;
+  float sampled[kSpread];
+#pragma unroll
+  for (int i = 0; i < kSpread; ++i) sampled[i] = logits[(int)((int64_t)(kSpread * tid + i) * a.vocab / 1024)];
+  const float zeroth = logits[0];
+#pragma unroll
+  for (int b = tid; b < kGrid; b += kPartThreads) {
+    count[b] = 0;
+    units[b] = 0;
+  }
   if (part == 0 && tid == 0) v.state[row].listed = 0;
-  over(logits, part * part_len, min((part + 1) * part_len, a.vocab), [&](auto each) __attribute__((always_inline)) {
+  over<kPartThreads, kPartQuads>(logits, part * part_len, min((part + 1) * part_len, a.vocab), [&](auto each) __attribute__((always_inline)) {
     float top = -INFINITY;
     int index = 0x7fffffff;
     each([&](float l, int i) __attribute__((always_inline)) {
@@ -476,7 +494,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_parts_kernel(SampleArgs
       }
     });
     uint64_t first = first_of_wave(top, index);
-    const Spread sp(candidate(sampled), candidate(zeroth));
+    const Spread sp(sampled, candidate(zeroth));
     if (leads) {
       first_lds[wave] = first;
       spread[wave][0] = sp.n;
@@ -486,7 +504,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_parts_kernel(SampleArgs
     __syncthreads();
     float n3[3] = {};
 #pragma unroll
-    for (int w = 0; w < kSampleWaves; ++w) {
+    for (int w = 0; w < kPartWaves; ++w) {
       first = min(first, first_lds[w]);
 #pragma unroll
       for (int i = 0; i < 3; ++i) n3[i] += spread[w][i];
@@ -520,7 +538,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_parts_kernel(SampleArgs
     __syncthreads();  // (and the histogram is whole)
     if (tid == 0) {
       all = n = 0;
-      for (int w = 0; w < kSampleWaves; ++w) {
+      for (int w = 0; w < kPartWaves; ++w) {
         all += units_lds[w];
         n += count_lds[w];
       }
@@ -528,8 +546,11 @@ __global__ __launch_bounds__(kSampleThreads) void sample_parts_kernel(SampleArgs
     }
   });
   if (s.greedy) return;
-  if (s.counts()) v.count[at * kGrid + tid] = count[tid];
-  if (!s.light()) v.units[at * kGrid + tid] = units[tid];
+#pragma unroll
+  for (int b = tid; b < kGrid; b += kPartThreads) {
+    if (s.counts()) v.count[at * kGrid + b] = count[b];
+    if (!s.light()) v.units[at * kGrid + b] = units[b];
+  }
 }
 
 // Exclusive prefix sums over the workgroup.
@@ -559,7 +580,7 @@ struct ListLds {
   uint64_t list[kListed];
 };
 
-__global__ __launch_bounds__(kSampleThreads) void sample_list_kernel(SampleArgs a, PartsView v, int parts, int part_len) {
+__global__ __launch_bounds__(kSampleThreads, 8) void sample_list_kernel(SampleArgs a, PartsView v, int parts, int part_len) {
   __shared__ ListLds lds;
   const int part = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
   const float* logits = a.logits + row * a.stride;
@@ -567,14 +588,21 @@ __global__ __launch_bounds__(kSampleThreads) void sample_list_kernel(SampleArgs 
   // (lane i of every wave has part i's)
   PartHead h = {~0ull, 0, 0.0, 0, 0};
   if ((tid & 63) < parts) h = v.head[(size_t)row * parts + (tid & 63)];
-  const uint64_t first = wave_least<32>(h.top);
+  // (what is the same in every lane lies in scalar registers: two workgroups a CU
+  // have 64 others a lane; 64 rows of 152064 logits 74.9 us, with one a CU 79.8)
+  auto uniform = [](double x) __attribute__((always_inline)) {
+    return __builtin_bit_cast(double, (uint64_t)readlane64((int64_t)__builtin_bit_cast(uint64_t, x), 0));
+  };
+  const uint64_t first = (uint64_t)readlane64((int64_t)wave_least<32>(h.top), 0);
   const float top = top_of(first);
   if (part == 0 && tid == 0) v.state[row].top = first;
   if (s.greedy || top == -INFINITY) return;
   const uint64_t grid_bits = __builtin_bit_cast(uint64_t, h.grid);
   const double grid = __builtin_bit_cast(double, (uint64_t)readlane64((int64_t)grid_bits, __builtin_ctzll(__ballot(h.top == first))));
-  const double top_bin = floor((double)top * grid);
+  const double top_bin = uniform(floor((double)top * grid));
   const bool light = s.light();
+  // the logit of a weight of min_p
+  const double least = s.least > 0.0f ? uniform((double)top + log((double)s.least) * (double)s.t) : 0.0;
 
   // ---- the parts' histograms added up, each moved to the row's largest logit
   const bool any = h.top != ~0ull;
@@ -586,21 +614,22 @@ __global__ __launch_bounds__(kSampleThreads) void sample_list_kernel(SampleArgs 
   const uint64_t all_w = (uint64_t)readlane64(wave_scan64((int64_t)((double)h.units * f_lane + 0.5)), 63);
   uint64_t w = 0;
   uint32_t c = 0;
-  const size_t at0 = (size_t)row * parts * kGrid;
+  const uint64_t* row_units = v.units + (size_t)row * parts * kGrid;
+  const uint32_t* row_count = v.count + (size_t)row * parts * kGrid;
   // (loads without a condition between them are asked for together: a part that
   // is not there has the last one's, and bins that are none the first one's)
   constexpr int kAhead = 8;
   auto place = [&](int i, bool* in) __attribute__((always_inline)) {
     const int n = min(i, parts - 1), b = tid - __builtin_amdgcn_readlane(off_lane, n);
     *in = i < parts && b >= 0 && tid < kGrid - 1;
-    return at0 + (size_t)n * kGrid + (b >= 0 ? b : 0);
+    return (uint32_t)(n * kGrid + (b >= 0 ? b : 0));
   };
   if (s.counts())
     for (int i0 = 0; i0 < parts; i0 += kAhead) {
       uint32_t x[kAhead];
       bool in[kAhead];
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) x[i] = v.count[place(i0 + i, &in[i])];
+      for (int i = 0; i < kAhead; ++i) x[i] = *(const uint32_t*)((const char*)row_count + 4 * place(i0 + i, &in[i]));
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) c += in[i] ? x[i] : 0;
     }
@@ -609,7 +638,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_list_kernel(SampleArgs 
       uint64_t x[kAhead];
       bool in[kAhead];
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) x[i] = v.units[place(i0 + i, &in[i])];
+      for (int i = 0; i < kAhead; ++i) x[i] = *(const uint64_t*)((const char*)row_units + 8 * place(i0 + i, &in[i]));
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         const double f = __builtin_bit_cast(double, (uint64_t)readlane64((int64_t)__builtin_bit_cast(uint64_t, f_lane), min(i0 + i, parts - 1)));
@@ -662,13 +691,13 @@ __global__ __launch_bounds__(kSampleThreads) void sample_list_kernel(SampleArgs 
       hi = lds.w[b1 + 1];
     }
     if (s.least > 0.0f) {
-      // (the logit of a weight of min_p, and what its logarithm may be off by)
-      const double l = (double)top + log((double)s.least) * (double)s.t, off = 1e-12 * (fabs((double)top) + fabs(l));
+      // (and what its logarithm may be off by)
+      const double off = 1e-12 * (fabs((double)top) + fabs(least));
       auto bin = [&](double x) __attribute__((always_inline)) {
         return (int)fmin(fmax(top_bin - floor(x * grid), 0.0), (double)(kGrid - 1));
       };
-      m_bin = bin(l + off);
-      const int b1 = bin(l - off);
+      m_bin = bin(least + off);
+      const int b1 = bin(least - off);
       mine |= tid >= m_bin && tid <= b1;
       if (tid == 0) lds.bins[5] = b1;  // (read behind the next barrier)
       lo = min(lo, max(lds.w[m_bin], (uint64_t)1));
@@ -709,12 +738,10 @@ __global__ __launch_bounds__(kSampleThreads) void sample_list_kernel(SampleArgs 
   // little before it, in 32 bits)
   const double end = (top_bin - far) / grid;
   const float below = far == kGrid - 1 || grid == 0.0 ? -INFINITY : (float)fmax(end - 1e-6 * fabs(end), -3e38);
-  over(logits, part * part_len, min((part + 1) * part_len, a.vocab), [&](auto each) __attribute__((always_inline)) {
-    each([&](float l, int i) __attribute__((always_inline)) {
-      if (l < below || l == -INFINITY || flags[bin_of(l, top_bin, grid)] == 0) return;
-      const uint32_t at = atomicAdd(&lds.found, 1u);
-      if (at < kListed) lds.list[at] = (uint64_t)key_of(l) << 32 | (uint32_t)i;
-    });
+  for_each<kSampleThreads>(logits, part * part_len, min((part + 1) * part_len, a.vocab), [&](float l, int i) __attribute__((always_inline)) {
+    if (l < below || l == -INFINITY || flags[bin_of(l, top_bin, grid)] == 0) return;
+    const uint32_t at = atomicAdd(&lds.found, 1u);
+    if (at < kListed) lds.list[at] = (uint64_t)key_of(l) << 32 | (uint32_t)i;
   });
   __syncthreads();
   // (one atomic a part: a round trip of a microsecond)
@@ -980,7 +1007,7 @@ hipError_t launch_sample(const SampleArgs& all, void* ws, hipStream_t stream) {
     if (a.top_p != nullptr) a.top_p += r0;
     if (a.min_p != nullptr) a.min_p += r0;
     const dim3 grid(parts, a.rows);
-    hipLaunchKernelGGL(sample_parts_kernel, grid, dim3(kSampleThreads), 0, stream, a, v, parts, part_len);
+    hipLaunchKernelGGL(sample_parts_kernel, grid, dim3(kPartThreads), 0, stream, a, v, parts, part_len);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(sample_list_kernel, grid, dim3(kSampleThreads), 0, stream, a, v, parts, part_len);
