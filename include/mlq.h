@@ -517,9 +517,11 @@ enum mlq_kv_type { MLQ_KV_F32 = 0, MLQ_KV_F16 = 1, MLQ_KV_BF16 = 2, MLQ_KV_Q4 = 
  * ties to even), and c the nearest code, upwards from halfway, as exact
  * arithmetic has it; d = 0 gives c = z. A block that holds an element that is
  * not finite, or whose d or m passes fp16's range, reads as NaN: it is stored
- * with d and m NaN. A row has 2, 4 or 8 blocks (head_dim up to 64, 128, 256):
- * unit i * blocks + b (i < 16) holds elements 2i and 2i + 1 of block b (Q4: one
- * byte, 2i in its low half; Q8: two bytes), then come d and m of every block.
+ * with d and m NaN. d is never negative (attention over rows from elsewhere that
+ * have such d keeps 21 bits of a weight). A row has 2, 4 or 8 blocks (head_dim up
+ * to 64, 128, 256): unit i * blocks + b (i < 16) holds elements 2i and 2i + 1 of
+ * block b (Q4: one byte, 2i in its low half; Q8: two bytes), then come d and m of
+ * every block:
  * 40, 80 or 160 bytes (Q4), 72, 144 or 288 (Q8). Elements behind head_dim have
  * code z, blocks that lie wholly behind it d = m = 0. */
 typedef struct mlq_paged_cache {
@@ -717,8 +719,9 @@ typedef struct mlq_sampling {
  * inf counts as the largest finite number; a row without tokens gives -1. Sums are
  * exact ones of weights in units of 2^-44, which a double exponential gives: the
  * token is that of real arithmetic unless uniform or top_p times a sum is within
- * about 2^-40 of a border, and the same in every call. Random
- * numbers are the caller's: the reference's sampler draws them on the host
+ * about 2^-40 of a border, and the same whenever the call is repeated (there, a
+ * batch of other size may give the neighbour). Random numbers are the caller's:
+ * the reference's sampler draws them on the host
  * (src/sampler.cc). vocab up to 2^19, rows up to 2^20 (MLQ_ERR_UNSUPPORTED
  * otherwise); rows = 0 does nothing. s may be NULL. ws: mlq_sample_workspace bytes,
  * 256-byte aligned, scratch, may be NULL when that is 0; calls that share one
