@@ -737,7 +737,7 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_list_kernel(SampleAr
   // (most tokens lie behind the last bin in question: told from its end, and a
   // little before it, in 32 bits)
   const double end = (top_bin - far) / grid;
-  const float below = far == kGrid - 1 || grid == 0.0 ? -INFINITY : (float)fmax(end - 1e-6 * fabs(end), -3e38);
+  const float below = far == kGrid - 1 || grid == 0.0 ? -INFINITY : (float)fmax(end - 1e-6 * fabs(end), -(double)3.402823466e38f);
   for_each<kSampleThreads>(logits, part * part_len, min((part + 1) * part_len, a.vocab), [&](float l, int i) __attribute__((always_inline)) {
     if (l < below || l == -INFINITY || flags[bin_of(l, top_bin, grid)] == 0) return;
     const uint32_t at = atomicAdd(&lds.found, 1u);

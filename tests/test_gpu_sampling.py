@@ -107,6 +107,21 @@ def test_masked_rows(sampling):
         assert got[14] == -1 and got[16] == 0 and got[19] == 0
 
 
+@pytest.mark.parametrize("vocab", [900, 2000, 6000, 40000])
+@pytest.mark.parametrize("low", [np.finfo(np.float32).min, -3.1e38, 3.3e38, np.finfo(np.float32).max, 0.0, -1e-45])
+def test_equal_logits_at_the_type_s_ends(sampling, vocab, low):
+    """A few thousand equal candidates among masked ones, and some neighbours of theirs."""
+    r = np.random.default_rng(6)
+    x = np.full((12, vocab), -np.inf, np.float32)
+    for row in range(12):
+        at = r.permutation(vocab)[:r.integers(1, min(vocab, 3500))]
+        x[row, at] = low
+        if row % 3 == 2:
+            x[row, at[:len(at) // 2]] = np.nextafter(np.float32(low), np.float32(0.0 if low else 1.0))
+    check(sampling, x, r.random(12), temperature=r.uniform(0.3, 2.0, 12), top_k=r.choice([0, 5, 900, 3000], 12), top_p=r.choice([1.0, 0.9], 12),
+          min_p=r.choice([0.0, 0.2], 12))
+
+
 @pytest.mark.parametrize("vocab", [300, 9000])
 def test_settings_at_their_ends(sampling, vocab):
     r = np.random.default_rng(5)
