@@ -354,6 +354,7 @@ constexpr int kPartThreads = 512, kPartWaves = kPartThreads / 64;
 constexpr int kPartQuads = 10;  // of four logits that a thread of it holds
 constexpr int kGrid = 1024;     // bins, the last of them everything behind the others
 constexpr int kListed = 4096;
+constexpr int kDirect = kSampleThreads;  // a row is its own list
 constexpr int kPartLeast = 4096;
 constexpr int kRowsAtOnce = 1024;
 static_assert(kGrid == kSampleThreads, "a bin a thread");
@@ -924,10 +925,12 @@ __device__ __forceinline__ void token_of_list(const SampleArgs& a, const PartsVi
     if (x[q] != ~0ull && less[q] < target && target <= sum[q]) a.tokens[row] = (int32_t)(uint32_t)x[q];
 }
 
-// DIRECT: the list is the whole row (vocabularies of up to kListed), read here.
+// DIRECT: the list is the whole row, read here (vocabularies of up to kDirect. Of
+// more tokens a sort of all costs more than the other two launches: 1 / 16 / 300 rows
+// of 2000 take 20 / 30 / 55 us so, 17 / 29 / 47 in parts; of 1000 9 / 16 / 26).
 template <bool DIRECT>
 __global__ __launch_bounds__(kSampleThreads) void sample_token_kernel(SampleArgs a, PartsView v) {
-  constexpr int Q = kListed / kSampleThreads;
+  constexpr int Q = DIRECT ? 1 : kListed / kSampleThreads;
   __shared__ TokenLds lds;
   const int row = blockIdx.x, tid = threadIdx.x;
   const Ask s = ask_of(a, row);
@@ -966,7 +969,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_token_kernel(SampleArgs
     if (tid == 0) a.tokens[row] = token;
     return;
   }
-  if (state.listed <= kSampleThreads) {
+  if (Q > 1 && state.listed <= kSampleThreads) {
     uint64_t y[1] = {x[0]};
     token_of_list<1, DIRECT>(a, v, state, row, s, y, lds);
   } else {
@@ -982,14 +985,14 @@ int parts_of(int rows, int vocab) {
 }  // namespace
 
 size_t sample_workspace(int rows, int vocab) {
-  if (rows == 0 || vocab <= kListed) return 0;
+  if (rows == 0 || vocab <= kDirect) return 0;
   PartsView v;
   return parts_view(nullptr, std::min(rows, kRowsAtOnce), parts_of(rows, vocab), &v);
 }
 
 hipError_t launch_sample(const SampleArgs& all, void* ws, hipStream_t stream) {
   PartsView v = {};
-  if (all.vocab <= kListed) {
+  if (all.vocab <= kDirect) {
     hipLaunchKernelGGL(sample_token_kernel<true>, dim3(all.rows), dim3(kSampleThreads), 0, stream, all, v);
     return hipGetLastError();
   }
