@@ -720,7 +720,9 @@ typedef struct mlq_sampling {
  * exact ones of weights in units of 2^-44, which a double exponential gives: the
  * token is that of real arithmetic unless uniform or top_p times a sum is within
  * about 2^-40 of a border, and the same whenever the call is repeated (there, a
- * batch of other size may give the neighbour). Random numbers are the caller's:
+ * batch of other size may give the neighbour). A row in whose order thousands of
+ * equal or nearly equal logits lie where a filter or the token falls is found by
+ * one workgroup (0.4 to 0.9 ms of 152064 logits). Random numbers are the caller's:
  * the reference's sampler draws them on the host
  * (src/sampler.cc). vocab up to 2^19, rows up to 2^20 (MLQ_ERR_UNSUPPORTED
  * otherwise); rows = 0 does nothing. s may be NULL. ws: mlq_sample_workspace bytes,

@@ -57,6 +57,33 @@ __device__ __forceinline__ uint32_t lane_xor(uint32_t x) {
     return threadIdx.x & 32 ? (uint32_t)r[0] : (uint32_t)r[1];
   }
 }
+// f(l, i) for the candidates l at lo <= i < hi, by the whole workgroup, several
+// loads at a time.
+template <int THREADS, typename F>
+__device__ __forceinline__ void for_each(const float* logits, int lo, int hi, F f) {
+  typedef float v4 __attribute__((ext_vector_type(4), aligned(4)));
+  constexpr int kStep = 4 * THREADS, kAhead = 4;
+  int i = lo + 4 * (int)threadIdx.x;
+  for (; i + (kAhead - 1) * kStep + 3 < hi; i += kAhead * kStep) {
+    v4 x[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) x[j] = *(const v4*)(logits + i + j * kStep);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) f(candidate(x[j][c]), i + j * kStep + c);
+  }
+  for (; i < hi; i += kStep) {
+    if (i + 3 < hi) {
+      const v4 x = *(const v4*)(logits + i);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) f(candidate(x[c]), i + c);
+    } else {
+      for (int c = 0; i + c < hi; ++c) f(candidate(logits[i + c]), i + c);
+    }
+  }
+}
+
 struct SampleLds {
   uint32_t count[kBins];
   uint64_t weight[kBins];
@@ -107,14 +134,25 @@ __device__ Place find(const Row& r, SampleLds& lds, uint64_t target) {
       lds.weight[i] = 0;
     }
     __syncthreads();
-    for (int i = tid; i < r.vocab; i += kSampleThreads) {
-      const float l = r.at(i);
+    for_each<kSampleThreads>(r.logits, 0, r.vocab, [&](float l, int) __attribute__((always_inline)) {
       const uint32_t k = key_of(l);
-      if (l == -INFINITY || (shift < 32 && k >> shift != p.key)) continue;
+      if (l == -INFINITY || (shift < 32 && k >> shift != p.key)) return;
       const uint32_t bin = k >> low & ((1u << bits) - 1);
-      atomicAdd(&lds.count[bin], 1u);
-      atomicAdd((unsigned long long*)&lds.weight[bin], (unsigned long long)r.units(l));
-    }
+      const uint64_t x = r.units(l), who = __ballot(true);
+      // (a row is here for its equal logits: a wave's go with one atomic, not 64 in
+      // turn; 152064 equal ones with top-k and top-p 2.4 -> 0.8 ms, loads ahead among it)
+      const int lead = __builtin_ctzll(who);
+      if (__ballot(k != (uint32_t)__builtin_amdgcn_readlane((int)k, lead)) == 0) {
+        if ((tid & 63) == lead) {
+          const int n = __builtin_popcountll(who);
+          atomicAdd(&lds.count[bin], (uint32_t)n);
+          atomicAdd((unsigned long long*)&lds.weight[bin], (unsigned long long)(n * x));
+        }
+      } else {
+        atomicAdd(&lds.count[bin], 1u);
+        atomicAdd((unsigned long long*)&lds.weight[bin], (unsigned long long)x);
+      }
+    });
     __syncthreads();
     // two bins a thread
     uint64_t c[2], w[2];
@@ -158,26 +196,32 @@ __device__ Place find(const Row& r, SampleLds& lds, uint64_t target) {
 __device__ int index_of(const Row& r, SampleLds& lds, uint32_t key, uint64_t n) {
   const int tid = threadIdx.x, wave = tid >> 6;
   uint64_t before = 0;
-  for (int i0 = 0; i0 < r.vocab; i0 += kSampleThreads) {
-    const int i = i0 + tid;
-    const float l = i < r.vocab ? r.at(i) : -INFINITY;
-    const uint64_t has = __ballot(l != -INFINITY && key_of(l) == key);
-    __syncthreads();
-    if ((tid & 63) == 0) lds.scan[0][wave] = __builtin_popcountll(has);
-    __syncthreads();
-    uint64_t mine = before, all = 0;
+  constexpr int kAhead = 8;
+  for (int i0 = 0; i0 < r.vocab; i0 += kAhead * kSampleThreads) {
+    float l[kAhead];
 #pragma unroll
-    for (int w = 0; w < kSampleWaves; ++w) {
-      if (w < wave) mine += lds.scan[0][w];
-      all += lds.scan[0][w];
-    }
-    if (before + all > n) {
-      const uint64_t lower = has & ((1ull << (tid & 63)) - 1);
-      if ((has >> (tid & 63) & 1) != 0 && mine + __builtin_popcountll(lower) == n) lds.found[0] = i;
+    for (int j = 0; j < kAhead; ++j) l[j] = r.at(min(i0 + j * kSampleThreads + tid, r.vocab - 1));
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int i = i0 + j * kSampleThreads + tid;
+      const uint64_t has = __ballot(i < r.vocab && l[j] != -INFINITY && key_of(l[j]) == key);
       __syncthreads();
-      return (int)lds.found[0];
+      if ((tid & 63) == 0) lds.scan[0][wave] = __builtin_popcountll(has);
+      __syncthreads();
+      uint64_t mine = before, all = 0;
+#pragma unroll
+      for (int w = 0; w < kSampleWaves; ++w) {
+        if (w < wave) mine += lds.scan[0][w];
+        all += lds.scan[0][w];
+      }
+      if (before + all > n) {
+        const uint64_t lower = has & ((1ull << (tid & 63)) - 1);
+        if ((has >> (tid & 63) & 1) != 0 && mine + __builtin_popcountll(lower) == n) lds.found[0] = i;
+        __syncthreads();
+        return (int)lds.found[0];
+      }
+      before += all;
     }
-    before += all;
   }
   return -1;
 }
@@ -210,33 +254,6 @@ __device__ __forceinline__ uint64_t top_p_target(float p, uint64_t all) {
 __device__ __forceinline__ uint64_t token_target(float u, uint64_t all) {
   const double past = u > 0.0f ? (double)u * (double)all : 0.0;
   return past < (double)all ? min((uint64_t)past + 1, all) : all;
-}
-
-// f(l, i) for the candidates l at lo <= i < hi, by the whole workgroup, several
-// loads at a time.
-template <int THREADS, typename F>
-__device__ __forceinline__ void for_each(const float* logits, int lo, int hi, F f) {
-  typedef float v4 __attribute__((ext_vector_type(4), aligned(4)));
-  constexpr int kStep = 4 * THREADS, kAhead = 4;
-  int i = lo + 4 * (int)threadIdx.x;
-  for (; i + (kAhead - 1) * kStep + 3 < hi; i += kAhead * kStep) {
-    v4 x[kAhead];
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) x[j] = *(const v4*)(logits + i + j * kStep);
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) f(candidate(x[j][c]), i + j * kStep + c);
-  }
-  for (; i < hi; i += kStep) {
-    if (i + 3 < hi) {
-      const v4 x = *(const v4*)(logits + i);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) f(candidate(x[c]), i + c);
-    } else {
-      for (int c = 0; i + c < hi; ++c) f(candidate(logits[i + c]), i + c);
-    }
-  }
 }
 
 // The largest of what the threads have and the first index with it, as the key
