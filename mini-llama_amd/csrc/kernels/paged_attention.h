@@ -1303,9 +1303,12 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
       for (int b = 0; b < VB2; ++b) {
         big = fmaxf(big, bound_of(by_lane(vscale[0][b], vscale[1][b], vscale[2][b], vscale[3][b])));
       }
-      const int e = pow2_scale_exp(xor16_max(big));
+      big = xor16_max(big);
+      const int e = pow2_scale_exp(big);
       const bool out = k0 + 4 * vkg + (tid & 3) > kmax;
-      if ((tid & 31) < 4) lds.vf[par][4 * vkg + (tid & 3)] = out ? 0.0f : ldexp_f(1.0f, -e);
+      // (a row of zeros has no power: 1 would be a large row's, and take the weights
+      // of small ones their bits. One that has no number makes NaN of 0 too)
+      if ((tid & 31) < 4) lds.vf[par][4 * vkg + (tid & 3)] = out || big == 0.0f ? 0.0f : ldexp_f(1.0f, -e);
       const float mine = out ? 0.0f : ldexp_f(1.0f, e);
       // (zeros take a key behind the end out: its scales may be anything, and 0
       // times them is not 0)
@@ -1386,8 +1389,9 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
 #pragma unroll
   for (int b = 0; b < VB; ++b) acc[b] = (f16v){};
   float m = -INFINITY, l = 0.0f;  // of the column; l of this half's keys
-  // quantised: the largest value row's power of two so far, and the weights'
-  float vtop = 0.0f, lift = kLift;
+  // quantised: the largest value row's power of two so far (at first that of fp16's
+  // least number, 2^-24), and the weights'
+  float vtop = 0x1p-38f, lift = kLift;
   int k0 = key0;
   int64_t run = run_of(k0, page_of(k0));
   load_k(run);

@@ -728,3 +728,83 @@ def test_serving_loop(paged, kind, graph):
             for r in range(start[s], start[s + 1]):
                 y, bound = kvq.attention(q_out[r].cpu().numpy(), kk, vv, int(lengths[s]) - (start[s + 1] - r), hd ** -0.5, kind=kind)
                 assert np.all(np.abs(out[r].double().cpu().numpy() - y) <= bound), (i, r)
+
+
+# ---- what values a row's weights are held beside ------------------------------------------
+def small_weights(paged, kind, heads, kv, hd, lengths, new, size, sink, seed):
+    """Values of `size`, and in each sequence a token `sink` (from its end) that weighs e^12 times what others do: what the
+    others add has to come out of weights far below the largest, which is the sink's, of a value a million times smaller."""
+    p = Problem(paged, kind, lengths, heads, kv, hd, 16, seed=seed, new=new, size=size)
+    r = np.random.default_rng(seed)
+    p.q = (0.3 * r.standard_normal(p.q.shape) + 4 * hd ** -0.5).astype(np.float32)
+    p.qd.copy_(dev(p.q))
+    for i, n in enumerate(lengths):
+        put(p.k, p, i, np.arange(n), (1.5 * r.standard_normal((n, kv, hd))).astype(np.float32))
+        put(p.k, p, i, n - sink, np.full((kv, hd), 3.0, np.float32))
+        put(p.v, p, i, n - sink, (1e-6 * size * r.standard_normal((kv, hd))).astype(np.float32))
+    return p
+
+
+def put(pool, p, i, t, x):
+    """Heads x in the place of token t, or of several, of sequence i."""
+    pool[0, p.table[i, t // p.page], :, t % p.page] = kvq.quantise(x, p.kind)
+
+
+def compare_prefill(paged, p, what, **rule):
+    """Both attentions against the definition. Prefill holds a weight beside its value row's bound |m| + middle d: a part's
+    last bit, 2^-24, is off by half of it, of weights lifted to 2^11 at least for the largest bound among the seen rows,
+    2^14 to 2^15 in the parts' own units: 2^-25 2^15 / 2^11 / 2^14 = 2^-35 of that bound a key."""
+    own, plain = rule_of(paged, p.heads, **rule)
+    p.cache.keys.copy_(dev(p.k))
+    p.cache.values.copy_(dev(p.v))
+    want = p.want(**plain)
+    p.compare(paged.attention_decode(p.cache, 0, p.batch, p.qd, rule=own), {int(s) - 1: want[int(s) - 1] for s in p.start[1:]}, what)
+    levels, middle, unit = kvq.KINDS[p.kind]
+    nb, window = kvq.blocks(p.hd), plain["window"]
+    for row, (y, bound) in want.items():
+        i = int(np.searchsorted(p.start, row, side="right")) - 1
+        pos = int(p.lengths[i]) - (p.start[i + 1] - row)
+        t = np.arange(max(0, pos + 1 - window) if window else 0, pos + 1)
+        s = np.ascontiguousarray(p.v[0, p.table[i, t // p.page], :, t % p.page][..., 16 * nb * unit:]).view(np.float16).astype(np.float64)
+        most = (np.abs(s[..., 1::2]) + middle * s[..., ::2]).max((0, 2))
+        bound += len(t) * 2.0 ** -35 * np.repeat(most, p.heads // p.kv)[:, None]
+    p.compare(paged.attention_prefill(p.cache, 0, p.batch, p.qd, rule=own), want, what)
+
+
+FEW_AND_SPLIT = [([170, 90], [150, 90]), ([1500], [3])]  # (the second one's keys are shared by workgroups)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("size", [1e-2, 1e-3])
+@pytest.mark.parametrize("lengths,new", FEW_AND_SPLIT)
+@pytest.mark.parametrize("heads,kv,hd", [(8, 2, 128), (4, 4, 64), (4, 1, 256), (6, 2, 80)])
+def test_value_rows_of_zeros_take_nothing_from_others(paged, heads, kv, hd, lengths, new, size, kind):
+    """A value row of zeros, first, in the middle, last or everywhere but in a few places: the weights of the others keep their
+    bits."""
+    for at in ([0], [lengths[0] // 2], [-1], "most", "all"):
+        p = small_weights(paged, kind, heads, kv, hd, lengths, new, size, sink=70, seed=71)
+        r = np.random.default_rng(5)
+        for i, n in enumerate(lengths):
+            t = np.flatnonzero(r.random(n) < (0.9 if at == "most" else 2.0)) if isinstance(at, str) else np.array(at) % n
+            put(p.v, p, i, t, np.zeros((len(t), kv, hd), np.float32))
+        compare_prefill(paged, p, at)
+        if at == "all":
+            assert not paged.attention_prefill(p.cache, 0, p.batch, p.qd).any()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,kv,hd", [(8, 2, 128), (4, 4, 64), (4, 1, 256)])
+def test_a_value_row_that_is_nan_among_zeros(paged, heads, kv, hd, kind):
+    """All values zero but for one row without a number: who sees it gets NaN, others zeros."""
+    p = Problem(paged, kind, [150, 700], heads, kv, hd, 16, seed=73, new=[150, 5])
+    for i, n in enumerate(p.lengths):
+        put(p.v, p, i, np.arange(n), np.zeros((n, kv, hd), np.float32))
+        put(p.v, p, i, 77, np.full((kv, hd), np.nan, np.float32))
+    p.cache.values.copy_(dev(p.v))
+    own, _ = rule_of(paged, heads, window=60)
+    for rule, last in ((None, 10 ** 9), (own, 60)):
+        out = paged.attention_prefill(p.cache, 0, p.batch, p.qd, rule=rule).cpu().numpy()
+        for row in range(p.rows):
+            i = int(np.searchsorted(p.start, row, side="right")) - 1
+            pos = int(p.lengths[i]) - (p.start[i + 1] - row)
+            assert np.isnan(out[row]).all() if 77 <= pos < 77 + last else (out[row] == 0.0).all(), (row, pos)
