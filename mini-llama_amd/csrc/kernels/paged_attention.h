@@ -1472,7 +1472,6 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
     // lane: keys 8 (i / 4) + 4 half + i % 4 of its column
     float vf[QUANT ? 16 : 1];
     if constexpr (QUANT) {
-      float big = 0.0f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const f4 x = *(const f4*)&lds.kf[par][8 * j + 4 * half], y = *(const f4*)&lds.vf[par][8 * j + 4 * half];
@@ -1480,15 +1479,8 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
         for (int i = 0; i < 4; ++i) {
           s[4 * j + i] *= x[i];
           vf[4 * j + i] = y[i];
-          big = fmaxf(big, y[i]);
         }
       }
-      vtop = fmaxf(vtop, xor32_max(big));
-      if constexpr (AGAIN)
-        if (count) {  // (no row's mark is to fall below fp16)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) vf[i] = vtop;
-        }
     }
     const bool edge = k0 + kPreKeys - 1 > wave_first || (a.window > 0 && k0 <= wave_last - a.window);
     float sl = rule.sl2;  // what is left to multiply
@@ -1499,8 +1491,23 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
         const int k = k0 + 8 * (i >> 2) + 4 * half + (i & 3);
         s[i] = RULE && a.softcap > 0.0f ? rule.cap_out * tanhf(s[i] * rule.cap_in) : s[i] * rule.sl2;
         if constexpr (RULE) s[i] += rule.slope2 * (float)(k - qpos);
-        if (k > qpos || (a.window > 0 && k <= qpos - a.window)) s[i] = -INFINITY;
+        if (k > qpos || (a.window > 0 && k <= qpos - a.window)) {
+          s[i] = -INFINITY;
+          // (what the column does not see has no say in its weights' power)
+          if constexpr (QUANT) vf[i] = 0.0f;
+        }
       }
+    }
+    if constexpr (QUANT) {
+      float big = vf[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) big = fmaxf(big, vf[i]);
+      vtop = fmaxf(vtop, xor32_max(big));
+      if constexpr (AGAIN)
+        if (count) {  // (no row's mark is to fall below fp16)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) vf[i] = vtop;
+        }
     }
     if constexpr (AGAIN)
       if (count) {  // every key that is seen weighs the same

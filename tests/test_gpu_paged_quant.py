@@ -808,3 +808,22 @@ def test_a_value_row_that_is_nan_among_zeros(paged, heads, kv, hd, kind):
             i = int(np.searchsorted(p.start, row, side="right")) - 1
             pos = int(p.lengths[i]) - (p.start[i + 1] - row)
             assert np.isnan(out[row]).all() if 77 <= pos < 77 + last else (out[row] == 0.0).all(), (row, pos)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("big", [1e2, 1e4])
+@pytest.mark.parametrize("heads,kv,hd,softcap", [(8, 2, 128, 0.0), (4, 4, 64, 0.0), (4, 1, 256, 0.0), (6, 2, 80, 0.0), (8, 2, 128, 50.0)])
+def test_large_value_rows_that_are_not_seen(paged, heads, kv, hd, softcap, big, kind):
+    """A later token's values in the same tile, and a token's just before the window: a row's bits do not hang on them."""
+    p = small_weights(paged, kind, heads, kv, hd, [170, 90], [150, 90], 1e-2, sink=70, seed=75)
+    r = np.random.default_rng(9)
+    for i, n in enumerate(p.lengths):
+        for t in [n - 1, n - 2] + ([95] if n > 95 else []):  # (95 is the last of its tile: 64 .. 94 do not see it)
+            put(p.v, p, i, t, (big * r.standard_normal((kv, hd))).astype(np.float32))
+    compare_prefill(paged, p, "later", softcap=softcap)
+    # the windows of the last rows begin in the tile of a large row, behind it
+    for n, window in ((170, 76), (1511, 100), (1511, 90)):
+        p = small_weights(paged, kind, heads, kv, hd, [n, n - 1], [4, 1], 1e-2, sink=40, seed=77)
+        for i, m in enumerate(p.lengths):
+            put(p.v, p, i, np.arange(m - 3 - window, m - window), (big * r.standard_normal((3, kv, hd))).astype(np.float32))
+        compare_prefill(paged, p, (n, window), window=window, softcap=softcap)
