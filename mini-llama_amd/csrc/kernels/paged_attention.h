@@ -1174,7 +1174,9 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
   const int kkey = tid >> 3, kd = (tid & 7) * (16 / ES);  // K: dims kd + 8 threads' pieces
   // V: keys 4 vkg .. + 3, VDT dims; quantised, two of each of VDT / 2 blocks
   const int vkg = tid >> 5, vd = QUANT ? 32 * (VDT / 2) * ((tid & 31) >> 4) + 2 * (tid & 15) : (tid & 31) * VDT;
-  auto v_dim = [&](int j) __attribute__((always_inline)) { return QUANT ? vd + 32 * (j >> 1) + (j & 1) : vd + j; };
+  // (of the other types vd + j, written out: fp32 of head dims 129 to 256 spills more
+  // if it comes from here, 2 x 1000 rows of 16 heads on 4 of 200 590 us, not 462)
+  auto v_dim = [&](int j) __attribute__((always_inline)) { return vd + 32 * (j >> 1) + (j & 1); };
   uint32_t kw[KW], vw[4][VWT];
   // quantised, as they lie: two units of every block and all scales of the key;
   // a unit of VDT / 2 blocks and their scales of each of four
@@ -1369,13 +1371,13 @@ __device__ __forceinline__ PreDirty prefill_pass(const PagedAttnArgs& a, const P
     }
 #pragma unroll
     for (int j = 0; j < (QUANT ? 0 : VDT); ++j) {
-      const int at = v_slot(unit, v_dim(j)) + sub;
+      const int at = v_slot(unit, vd + j) + sub;
       if constexpr (F32) {
         uint32_t x[3], y[3];
         split_pair<__bf16>(__builtin_bit_cast(float, vw[0][j]), __builtin_bit_cast(float, vw[1][j]), x);
         split_pair<__bf16>(__builtin_bit_cast(float, vw[2][j]), __builtin_bit_cast(float, vw[3][j]), y);
 #pragma unroll
-        for (int i = 0; i < 3; ++i) *(u32x2_t*)&tl.v[i][v_dim(j)][at] = u32x2_t{x[i], y[i]};
+        for (int i = 0; i < 3; ++i) *(u32x2_t*)&tl.v[i][vd + j][at] = u32x2_t{x[i], y[i]};
       } else {
         const uint32_t sel = j & 1 ? 0x07060302u : 0x05040100u;
         *(u32x2_t*)&tl.v[0][vd + j][at] =
