@@ -388,7 +388,7 @@ struct RowState {
   uint32_t slow;    // sample_row's
   uint64_t top;
   double grid;
-  int32_t m_bin;    // the first bin that min_p may cut
+  int32_t m_bin;    // the first bin that min_p may cut; kGrid: none
   uint32_t pad;
 };
 struct PartsView {
@@ -619,8 +619,10 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_list_kernel(SampleAr
   const double grid = __builtin_bit_cast(double, (uint64_t)readlane64((int64_t)grid_bits, __builtin_ctzll(__ballot(h.top == first))));
   const double top_bin = uniform(floor((double)top * grid));
   const bool light = s.light();
-  // the logit of a weight of min_p
-  const double least = s.least > 0.0f ? uniform((double)top + log((double)s.least) * (double)s.t) : 0.0;
+  // the logit of a weight of min_p (up to 1 here, and an infinite temperature makes
+  // every weight 1: nothing falls below it)
+  const bool m_cuts = s.least > 0.0f && s.t < INFINITY;
+  const double least = m_cuts ? uniform((double)top + log((double)s.least) * (double)s.t) : 0.0;
 
   // ---- the parts' histograms added up, each moved to the row's largest logit
   const bool any = h.top != ~0ull;
@@ -688,7 +690,7 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_list_kernel(SampleAr
   };
   // ---- the bins in question, from what the units kept are at least and at most
   bool mine = false;
-  int m_bin = 0, far = kGrid - 1;  // the last bin in question
+  int m_bin = kGrid, far = kGrid - 1;  // the last bin in question
   const bool cut = s.k > 0 && (uint32_t)s.k < all_c;
   if (light) {
     const int b = cut ? bin_by(true, s.k, 0) : kGrid - 1;
@@ -708,9 +710,10 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_list_kernel(SampleAr
       lo = max(lds.w[b0], (uint64_t)1);
       hi = lds.w[b1 + 1];
     }
-    if (s.least > 0.0f) {
-      // (and what its logarithm may be off by)
-      const double off = 1e-12 * (fabs((double)top) + fabs(least));
+    if (m_cuts) {
+      // (and what its logarithm may be off by, and a logit whose weight is rounded
+      // to min_p's: half a step of 64 bits is 1.1e-16 T)
+      const double off = 1e-12 * (fabs((double)top) + fabs(least)) + 1e-15 * (double)s.t;
       auto bin = [&](double x) __attribute__((always_inline)) {
         return (int)fmin(fmax(top_bin - floor(x * grid), 0.0), (double)(kGrid - 1));
       };
@@ -723,7 +726,7 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_list_kernel(SampleAr
     }
     const int b0 = bin_by(false, token_target(s.u, lo), 3), b1 = bin_by(false, token_target(s.u, hi), 4);
     mine |= tid >= b0 && tid <= b1;
-    far = max(max(cut ? lds.bins[0] : 0, s.p < 1.0f ? lds.bins[2] : 0), max(s.least > 0.0f ? lds.bins[5] : 0, b1));
+    far = max(max(cut ? lds.bins[0] : 0, s.p < 1.0f ? lds.bins[2] : 0), max(m_cuts ? lds.bins[5] : 0, b1));
     if (w == 0 && !(cut && tid == lds.bins[0])) mine = false;
   }
   // A place behind the grid's end, and more tokens than the list takes (where

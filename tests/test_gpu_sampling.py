@@ -230,3 +230,15 @@ def test_refusals_on_the_device(pkg, sampling):
         rule.temperature = u
     assert sampling.sample(None, x[:0], u[:0]).shape == (0,)
     assert sampling.sample(None, x, u).tolist() == [0] * 4
+
+
+@pytest.mark.parametrize("vocab", [900, 9000, 152064])
+@pytest.mark.parametrize("temperature", [np.inf, 1e30, 1e20])
+def test_min_p_at_temperatures_that_weigh_all_alike(sampling, vocab, temperature):
+    """Every weight is 1 in 64 bits: min_p leaves all tokens up to 1, and the first for more."""
+    r = np.random.default_rng(vocab)
+    rows = 6
+    x = (r.standard_normal((rows, vocab)) * 3).astype(np.float32)
+    for least in (1.0, 0.5, 1e-30):
+        for kw in (dict(), dict(top_k=[0, 5, 1500, 1024, 1025, 0], top_p=[0.9, 0.9, 1.0, 1.0, 0.5, 1.0])):
+            check(sampling, x, r.random(rows), temperature=temperature, min_p=least, **kw)
