@@ -715,12 +715,15 @@ typedef struct mlq_sampling {
  * weights add up to top_p of theirs; of those the ones with w >= min_p; the
  * first of all always stays; of what stays the first token whose weights, added
  * up to it, pass uniform[r] times their sum. uniform: in [0, 1) (below 0 and NaN count
- * as 0, 1 and above as the last). Logits that are -inf or NaN are no tokens,
- * inf counts as the largest finite number; a row without tokens gives -1. Sums are
- * exact ones of weights in units of 2^-44, which a double exponential gives: the
- * token is that of real arithmetic unless uniform or top_p times a sum is within
- * about 2^-40 of a border, and the same whenever the call is repeated (there, a
- * batch of other size may give the neighbour). A row in whose order thousands of
+ * as 0, 1 and above as the last whose weight is 2^-45 or more). Logits that are -inf
+ * or NaN are no tokens, inf counts as the largest finite number; a row without
+ * tokens gives -1. w is a double exponential, as such compared with min_p, and
+ * in sums rounded to units of 2^-44, so that their order does not matter: the token
+ * is that of real arithmetic unless uniform or top_p times a sum is within
+ * (vocab + 2^14) 2^-44, and 2^-40 of the sum, of a border (of 2^19 tokens half of
+ * uniform's last step before 1; the largest weight is 1). It is the same whenever the
+ * call is repeated (so near a border a batch of other size may give another, whose
+ * weights lie within that distance). A row in whose order thousands of
  * equal or nearly equal logits lie where a filter or the token falls is found by
  * one workgroup (0.4 to 0.9 ms of 152064 logits). Random numbers are the caller's:
  * the reference's sampler draws them on the host

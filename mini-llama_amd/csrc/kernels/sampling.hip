@@ -19,8 +19,10 @@ namespace {
 // where the sum of weights reaches top_p of those, and where it passes u times
 // what is kept. Sums are whole numbers, weights w = exp((l - max) / T) in units of
 // 2^-44: they do not depend on the order in which they are added, so neither does
-// the token, and 2^19 of them fit 64 bits. What a unit cannot hold could be asked
-// for by no u, whose last step is 2^-24 of the sum.
+// the token, and 2^19 of them fit 64 bits. Half a unit is rounded off each weight, and
+// where the parts' sums are brought together off each bin of each part: sums are off
+// by up to (vocab + 2^14) 2^-45 where the largest weight is 1, of 2^19 tokens by 2^-26
+// (a quarter of the last step of u before 1), and by 64 bits' roundings.
 constexpr int kSampleThreads = 1024, kSampleWaves = kSampleThreads / 64;
 constexpr double kUnits = 17592186044416.0;  // 2^44
 constexpr int kDigit = 11, kBins = 1 << kDigit;

@@ -242,3 +242,25 @@ def test_min_p_at_temperatures_that_weigh_all_alike(sampling, vocab, temperature
     for least in (1.0, 0.5, 1e-30):
         for kw in (dict(), dict(top_k=[0, 5, 1500, 1024, 1025, 0], top_p=[0.9, 0.9, 1.0, 1.0, 0.5, 1.0])):
             check(sampling, x, r.random(rows), temperature=temperature, min_p=least, **kw)
+
+
+@pytest.mark.parametrize("rows,vocab", [(177, 900), (3, 9000), (177, 152064), (8, 152064), (600, 152064), (5, 1 << 19)])
+@pytest.mark.parametrize("units", [0.4, 0.6, 300.5, 1000.5, 2000.4])
+def test_long_tails_of_equal_weights(sampling, rows, vocab, units):
+    """One token of weight 1 and all others of a few units of 2^-44, half of one rounded each: sums are off by up to
+    vocab 2^-45, and 2^-45 for each of 16 parts' 1024 bins, at the token and in the whole sum, and by 64 bits' roundings.
+    What uniform points at lies within that of the token."""
+    x = np.full(vocab, np.log(units * 2.0 ** -44), np.float32)
+    x[vocab // 3] = 0.0
+    w = np.exp(x.astype(np.float64)[0])
+    whole = 1.0 + (vocab - 1) * w
+    # from the peak's end to the last step of fp32 before 1
+    u = np.float32(1.0) - np.float32(2.0 ** -24) * np.arange(1, rows + 1, dtype=np.float32)
+    u[::2] = 1.0 - (np.linspace(0.01, 0.99, rows)[::2] * (vocab - 1) * w / whole)
+    u = np.minimum(u, np.float32(1 - 2.0 ** -24))
+    out = sampling.sample(None, dev(x)[None].expand(rows, vocab), dev(u)).cpu().numpy()
+    assert ((out >= 0) & (out < vocab)).all()
+    rank = np.where(out == vocab // 3, 0, out + (out < vocab // 3))
+    lo, hi = np.where(rank == 0, 0.0, 1.0 + (rank - 1) * w), 1.0 + rank * w
+    target = u.astype(np.float64) * whole
+    assert (np.maximum(lo - target, target - hi) <= (vocab + 2 ** 14) * 2.0 ** -44 + 2.0 ** -40 * whole).all()
