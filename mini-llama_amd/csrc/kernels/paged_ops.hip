@@ -579,8 +579,9 @@ void rotary_launch(RotaryArgs a, hipStream_t stream) {
 // (a row of 4 or 8 bits has two blocks at least)
 template <typename Q>
 void rotary_launch_hd(const RotaryArgs& a, hipStream_t stream) {
-  if (a.hd <= 32 && std::is_void<Q>::value) rotary_launch<8, Q>(a, stream);
-  else if (a.hd <= 64) rotary_launch<16, Q>(a, stream);
+  if constexpr (std::is_void<Q>::value)
+    if (a.hd <= 32) return rotary_launch<8, Q>(a, stream);
+  if (a.hd <= 64) rotary_launch<16, Q>(a, stream);
   else if (a.hd <= 128) rotary_launch<32, Q>(a, stream);
   else rotary_launch<64, Q>(a, stream);
 }
