@@ -729,8 +729,9 @@ typedef struct mlq_sampling {
  * the reference's sampler draws them on the host
  * (src/sampler.cc). vocab up to 2^19, rows up to 2^20 (MLQ_ERR_UNSUPPORTED
  * otherwise); rows = 0 does nothing. s may be NULL. ws: mlq_sample_workspace bytes,
- * 256-byte aligned, scratch, may be NULL when that is 0; calls that share one
- * (two captured graphs, too) must be ordered. */
+ * those of more rows or a larger vocab serve too, 256-byte aligned, scratch, may be
+ * NULL when that is 0; calls that share one (two captured graphs, too) must be
+ * ordered. */
 int mlq_sample_workspace(int rows, int vocab, size_t* bytes);
 int mlq_sample(const mlq_sampling* s, int rows, int vocab, const float* logits, int64_t stride,
                const float* uniform, int32_t* tokens, void* ws, size_t ws_bytes,

@@ -403,16 +403,17 @@ struct PartsView {
   uint64_t* list;      // [rows][kListed] key and index
 };
 __host__ __device__ inline size_t parts_align(size_t n) { return (n + 255) & ~(size_t)255; }
-__host__ __device__ inline size_t parts_view(void* ws, int rows, int parts, PartsView* v) {
+// (slots: parts of all rows)
+__host__ __device__ inline size_t parts_view(void* ws, int rows, int slots, PartsView* v) {
   size_t at = 0;
   auto take = [&](auto** p, size_t n) {
     typedef typename std::remove_reference<decltype(**p)>::type X;
     *p = (X*)((char*)ws + at);
     at += parts_align(n * sizeof(X));
   };
-  take(&v->head, (size_t)rows * parts);
-  take(&v->count, (size_t)rows * parts * kGrid);
-  take(&v->units, (size_t)rows * parts * kGrid);
+  take(&v->head, (size_t)slots);
+  take(&v->count, (size_t)slots * kGrid);
+  take(&v->units, (size_t)slots * kGrid);
   take(&v->state, (size_t)rows);
   take(&v->before_w, (size_t)rows * (kGrid + 1));
   take(&v->before_c, (size_t)rows * (kGrid + 1));
@@ -1003,13 +1004,19 @@ int parts_of(int rows, int vocab) {
   const int most = std::max(2 * device_cus() / std::min(rows, kRowsAtOnce), 1);
   return std::min(std::min(most, kMaxParts), (vocab + kPartLeast - 1) / kPartLeast);
 }
+// Parts of a launch's rows, or of any smaller one's: a workspace then serves every
+// smaller batch (256 rows have two parts each, 257 one).
+int part_slots(int rows, int vocab) {
+  const int r = std::min(rows, kRowsAtOnce);
+  return std::max(std::min(r * std::min(kMaxParts, (vocab + kPartLeast - 1) / kPartLeast), 2 * device_cus()), r);
+}
 
 }  // namespace
 
 size_t sample_workspace(int rows, int vocab) {
   if (rows == 0 || vocab <= kDirect) return 0;
   PartsView v;
-  return parts_view(nullptr, std::min(rows, kRowsAtOnce), parts_of(rows, vocab), &v);
+  return parts_view(nullptr, std::min(rows, kRowsAtOnce), part_slots(rows, vocab), &v);
 }
 
 hipError_t launch_sample(const SampleArgs& all, void* ws, hipStream_t stream) {
@@ -1020,7 +1027,7 @@ hipError_t launch_sample(const SampleArgs& all, void* ws, hipStream_t stream) {
   }
   const int parts = parts_of(all.rows, all.vocab);
   const int part_len = ((all.vocab + parts - 1) / parts + 3) & ~3;
-  parts_view(ws, std::min(all.rows, kRowsAtOnce), parts, &v);
+  parts_view(ws, std::min(all.rows, kRowsAtOnce), part_slots(all.rows, all.vocab), &v);
   for (int r0 = 0; r0 < all.rows; r0 += kRowsAtOnce) {
     SampleArgs a = all;
     a.rows = std::min(kRowsAtOnce, all.rows - r0);

@@ -64,8 +64,8 @@ def sample(rule, logits, uniform, out=None, workspace=None, stream=None):
     """Tokens int32 [rows] (out, a new tensor unless given) of logits float32
     [rows, vocab], whose rows may have any stride, by rule (a Sampling, or None:
     temperature 1 without filters) and uniform, float32 [rows] in [0, 1).
-    workspace: a uint8 device tensor of sample_workspace_bytes, or None for one
-    of the call's own."""
+    workspace: a uint8 device tensor of sample_workspace_bytes (of these rows and
+    vocab, or larger ones), or None for one of the call's own."""
     index = logits.get_device()
     if index < 0 or (rule is not None and rule.index is not None and rule.index != index):
         raise ValueError("logits must be a device tensor, on the device of the settings")

@@ -264,3 +264,19 @@ def test_long_tails_of_equal_weights(sampling, rows, vocab, units):
     lo, hi = np.where(rank == 0, 0.0, 1.0 + (rank - 1) * w), 1.0 + rank * w
     target = u.astype(np.float64) * whole
     assert (np.maximum(lo - target, target - hi) <= (vocab + 2 ** 14) * 2.0 ** -44 + 2.0 ** -40 * whole).all()
+
+
+def test_a_workspace_of_the_largest_batch(sampling):
+    """One workspace for every batch size of a server, other rows' numbers in it."""
+    import torch
+    vocab, most = 20000, 257
+    ws = torch.full((sampling.sample_workspace_bytes(most, vocab),), 255, dtype=torch.uint8, device="cuda")
+    g = torch.Generator(device="cuda")
+    g.manual_seed(3)
+    x, u = torch.randn(most, vocab, device="cuda", generator=g) * 3, torch.rand(most, device="cuda", generator=g)
+    k, p = torch.randint(0, 2000, (most,), device="cuda", generator=g).int(), torch.rand(most, device="cuda", generator=g) + 0.3
+    for rows in (257, 256, 255, 171, 128, 86, 33, 16, 1, 257):
+        rule = sampling.Sampling(top_k=k[:rows].contiguous(), top_p=p[:rows].contiguous())
+        for n in (vocab, 17000, 1025, 900):
+            got = sampling.sample(rule, x[:rows, :n], u[:rows].contiguous(), workspace=ws)
+            assert torch.equal(got, sampling.sample(rule, x[:rows, :n], u[:rows].contiguous())), (rows, n)

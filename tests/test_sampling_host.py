@@ -59,3 +59,17 @@ def test_definition():
     assert [got(u, min_p=0.4) for u in (0.66, 0.99)] == [1, 3] and got(0.99, min_p=2.0) == 1
     assert got(0.99, temperature=0.0) == 1 and got(0.9, temperature=1e-3) == 1 and got(0.76, temperature=1e6) == 2
     assert ref.token([np.nan, -np.inf], 0.3)[0] == -1 and ref.token([np.nan, 3, np.inf, np.inf], 0.6)[0] == 3
+
+
+@pytest.mark.parametrize("vocab", [1025, 5000, 32000, 152064, 1 << 19])
+def test_a_workspace_serves_smaller_calls(pkg, vocab):
+    """Bytes do not fall as rows or the vocabulary grow."""
+    n = ctypes.c_size_t()
+
+    def need(rows, vocab):
+        assert pkg.lib().mlq_sample_workspace(rows, vocab, ctypes.byref(n)) == OK
+        return n.value
+    sizes = [need(rows, vocab) for rows in range(1, 1100)]
+    assert sizes == sorted(sizes) and sizes[-1] == need(1 << 20, vocab)
+    for rows in (1, 3, 100, 257, 2000):
+        assert need(rows, 1024) == 0 < need(rows, vocab - 1 if vocab > 1025 else vocab) <= need(rows, vocab)
