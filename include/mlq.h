@@ -715,9 +715,9 @@ typedef struct mlq_sampling {
  * weights add up to top_p of theirs; of those the ones with w >= min_p; the
  * first of all always stays; of what stays the first token whose weights, added
  * up to it, pass uniform[r] times their sum. uniform: in [0, 1) (below 0 and NaN count
- * as 0, 1 and above as the last whose weight is 2^-45 or more). Logits that are -inf
- * or NaN are no tokens, inf counts as the largest finite number; a row without
- * tokens gives -1. w is a double exponential, as such compared with min_p, and
+ * as 0, 1 and above as the whole sum: the last token that adds to it, as it is held).
+ * Logits that are -inf or NaN are no tokens, inf counts as the largest finite
+ * number; a row without tokens gives -1. w is a double exponential, as such compared with min_p, and
  * in sums rounded to units of 2^-44, so that their order does not matter: the token
  * is that of real arithmetic unless uniform or top_p times a sum is within
  * (vocab + 2^14) 2^-44, and 2^-40 of the sum, of a border (of 2^19 tokens half of
