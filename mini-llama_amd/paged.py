@@ -221,6 +221,7 @@ class PagedBatch(_Fixed):
         ref = self._bounded.get(most)
         if ref is None:
             s = self.struct
+            _int32("the number of rows", most)
             ref = ctypes.byref(MlqPagedBatch(s.n_seqs, s.max_pages, most, s.block_table, s.lengths,
                                              s.row_start, s.positions, s.slots, s.status))
             if len(self._bounded) >= 64:
@@ -324,7 +325,7 @@ def qk_norm_rope(rotary: Rotary, q, k, v, positions, q_out=None, k_out=None, cac
                                                slots), index, stream)
     qp, qs = _rows("q", q, None, None, hd, index)
     q_shape = q.shape
-    n, heads = q_shape[0], q_shape[1]
+    n, heads = _int32("the number of rows", q_shape[0]), q_shape[1]
     kp, ks = _rows("k", k, n, None, hd, index)
     k_shape = k.shape
     kv = k_shape[1]
@@ -362,7 +363,7 @@ def write(cache: PagedCache, layer: int, k, v, slots, k_out=None, v_out=None, st
         return _elsewhere(lambda: write(cache, layer, k, v, slots, k_out, v_out), index, stream)
     _int32("layer", layer)
     kp, ks = _rows("k", k, None, kv, hd, index)
-    n = k.shape[0]
+    n = _int32("the number of rows", k.shape[0])
     vp, vs = _rows("v", v, n, kv, hd, index)
     kop = vop = None
     kos = vos = 0

@@ -113,3 +113,33 @@ def test_definition(kind, hd):
     # and d come back to half an fp16 step each, 2^-11 (|m| + levels d) in all, at most three times max |y|
     again = kvq.values(kvq.quantise(y.astype(np.float32), kind), kind, hd)
     assert np.abs(again - y).max() <= np.abs(y).max() * 2.0 ** -9
+
+
+def test_more_rows_than_a_c_int_holds(pkg, monkeypatch):
+    """2^32 + 5 rows would be taken as 5 (tensors without memory: what is not refused fails as a null address)."""
+    from types import SimpleNamespace
+
+    import torch
+    from mini_llama_amd import paged
+
+    def tensor(*shape, dtype=torch.float32):
+        strides = tuple(int(np.prod(shape[i + 1:], dtype=np.int64)) for i in range(len(shape)))
+        return SimpleNamespace(shape=shape, dtype=dtype, device="cuda:0", get_device=lambda: 0, dim=lambda: len(shape), stride=lambda: strides,
+                               is_contiguous=lambda: True, data_ptr=lambda: None)
+    c = SimpleNamespace(index=0, device="cuda:0", head_dim=128, n_kv_heads=4, ref=ctypes.byref(cache(pkg)))
+    r = SimpleNamespace(index=0, head_dim=128, ref=ctypes.byref(pkg.MlqRotary(128, 0, 0, 1.0, 1e-6, None, None, None)))
+    monkeypatch.setattr(paged, "_current_device", lambda: 0)
+    monkeypatch.setattr(paged, "_raw_stream", lambda index: None)
+    for n, error in ((5, pkg.MLQError), ((1 << 32) + 5, ValueError), (1 << 31, ValueError)):
+        x, slots, positions = tensor(n, 4, 128), tensor(n, dtype=torch.int64), tensor(n, dtype=torch.int32)
+        with pytest.raises(error):
+            paged.write(c, 0, x, x, slots)
+        with pytest.raises(error):
+            paged.read(c, 0, slots, x, x)
+        with pytest.raises(error):
+            paged.qk_norm_rope(r, x, x, x, positions, q_out=x, k_out=x)
+    b = SimpleNamespace(max_rows=None, struct=pkg.MlqPagedBatch(1, 1, 0, None, None, None, None, None, None), _bounded={})
+    assert paged.PagedBatch.bounded(b, 5)._obj.max_rows == 5
+    for n in ((1 << 32) + 5, 1 << 31):
+        with pytest.raises(ValueError):
+            paged.PagedBatch.bounded(b, n)
