@@ -517,8 +517,8 @@ enum mlq_kv_type { MLQ_KV_F32 = 0, MLQ_KV_F16 = 1, MLQ_KV_BF16 = 2, MLQ_KV_Q4 = 
  * ties to even), and c the nearest code, upwards from halfway, as exact
  * arithmetic has it; d = 0 gives c = z. A block that holds an element that is
  * not finite, or whose d or m passes fp16's range, reads as NaN: it is stored
- * with d and m NaN. d is never negative (attention over rows from elsewhere that
- * have such d keeps 21 bits of a weight). A row has 2, 4 or 8 blocks (head_dim up
+ * with d and m NaN. d is never negative (attention and mlq_paged_read take rows from
+ * elsewhere that have such d as well). A row has 2, 4 or 8 blocks (head_dim up
  * to 64, 128, 256): unit i * blocks + b (i < 16) holds elements 2i and 2i + 1 of
  * block b (Q4: one byte, 2i in its low half; Q8: two bytes), then come d and m of
  * every block:

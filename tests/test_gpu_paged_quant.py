@@ -827,3 +827,22 @@ def test_large_value_rows_that_are_not_seen(paged, heads, kv, hd, softcap, big, 
         for i, m in enumerate(p.lengths):
             put(p.v, p, i, np.arange(m - 3 - window, m - window), (big * r.standard_normal((3, kv, hd))).astype(np.float32))
         compare_prefill(paged, p, (n, window), window=window, softcap=softcap)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,kv,hd", [(8, 2, 128), (28, 4, 128), (24, 2, 128), (4, 4, 64), (16, 1, 64), (4, 1, 256), (12, 1, 256), (6, 2, 80)])
+def test_steps_below_zero(paged, heads, kv, hd, kind):
+    """Rows from elsewhere may have a negative d: some blocks, or all of them, in keys and values."""
+    for share in (0.02, 0.5, 1.0):
+        p = Problem(paged, kind, [700, 33, 1], heads, kv, hd, 16, seed=81, new=[40, 33, 1])
+        r = np.random.default_rng(7)
+        at = 16 * kvq.blocks(hd) * kvq.KINDS[kind][2]
+        for pool in (p.k, p.v):
+            s = np.ascontiguousarray(pool[..., at:]).view(np.float16)
+            s[..., ::2] *= np.where(r.random(s[..., ::2].shape) < share, -1, 1).astype(np.float16)
+            pool[..., at:] = s.view(np.uint8)
+        p.cache.keys.copy_(dev(p.k))
+        p.cache.values.copy_(dev(p.v))
+        want = p.want(rows=p.some(20))
+        p.compare(paged.attention_decode(p.cache, 0, p.batch, p.qd), {int(s) - 1: want[int(s) - 1] for s in p.start[1:]}, share)
+        p.compare(paged.attention_prefill(p.cache, 0, p.batch, p.qd), want, share)
