@@ -670,9 +670,11 @@ int mlq_paged_attention_workspace(const mlq_paged_cache* c, int n_heads, int n_s
  * the largest weight in each weight; cached fp16 values below the smallest
  * normal number, 6.1e-5, enter with an absolute error of up to 2^-37 (storing
  * them rounds by up to 2^-25). Q4 and Q8: what the codes stand for, not rounded
- * again; q and the weights in two parts of fp16 with the same absolute errors, a
- * weight's times the largest d among the keys; prefill has elements in two parts
- * too, with one of up to 2^-39 of the largest in the key's or value's row.
+ * again; q in two parts of fp16 with the same absolute error, the weights in two
+ * with one of up to 2^-39 of the largest times the largest |d| (2^-14 at least) of the
+ * seen values for each step of a code. In prefill that is 2^-35 of the largest
+ * weight times the largest |m| + z |d| of the seen values, and elements are in two
+ * parts too, with one of up to 2^-39 of |m| + z |d| of the key's or value's row.
  * NaN / inf among the seen keys and values give NaN / inf outputs. ws:
  * 256-byte aligned, scratch, may be NULL when its size is 0; calls that
  * share one (two captured graphs, too) must be ordered. n_heads: up to 2048

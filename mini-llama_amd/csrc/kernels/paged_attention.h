@@ -839,8 +839,10 @@ struct PreTraits<float> : KvTraits<__bf16> {
 // bits, under a power of two for each key's row, whose largest element could
 // otherwise overflow or all of them lose bits to fp16's subnormals. A score is
 // multiplied by its key's power, a weight by its value row's; the weights of a
-// column have another one, which follows the largest value row so far. Three
-// part products then make a product, as of a bf16 cache.
+// column have another one, which follows the largest value row that it has seen
+// so far: a weight is off by up to 2^-35 of the largest at such a row's size (it is lifted
+// to 2^11 there, 4 below fp16's range for a maximum that is 2^kSlack behind, and fp16
+// ends at 2^-25). Three part products then make a product, as of a bf16 cache.
 template <typename Q>
 struct PreTraitsQuantised : KvTraits<_Float16> {
   typedef _Float16 mat;
