@@ -240,7 +240,10 @@ __device__ __forceinline__ void store_kv(void* base, int type, int64_t at, float
 }
 
 // A head's row of 4 or 8 bits from 4 elements a lane (lane l of the head's has
-// dims 4l ..): a block lies in 8 lanes, and a lane's two units in two places.
+// dims 4l ..): a block lies in 8 lanes, and a lane's two units in two places, stored
+// a unit at a time. 8000 rows of 32 heads on 8 of 128 take 69.6 us with a bf16 cache,
+// 76.0 with q4 and 79.8 with q8 (their bytes at a copy's rate: 70), 48 of 28 on 4 3.6,
+// 4.3 and 4.2.
 template <typename Q>
 __device__ __forceinline__ void store_quantised(char* row, int l, int hd, float4 x) {
   const int nb = kv_blocks(hd), b = l >> 3, d = 4 * l;
@@ -513,7 +516,9 @@ __global__ __launch_bounds__(kRowsThreads) void read_rows_quantised_kernel(RowsA
   }
 }
 
-// Caches of 16 and 32 bits: 4 elements a lane.
+// Caches of 16 and 32 bits: 4 elements a lane. 8 heads of 128, one buffer again and
+// again: 8000 rows written, with their values given back, 29.8 us fp32, 25.1 bf16;
+// 16000 read 34.2 and 24.6.
 __device__ __forceinline__ float4 load_kv(const void* base, int type, int64_t at) {
   typedef float v4 __attribute__((ext_vector_type(4)));
   typedef _Float16 hv4 __attribute__((ext_vector_type(4)));

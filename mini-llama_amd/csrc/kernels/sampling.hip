@@ -370,7 +370,10 @@ __device__ int sample_row(const SampleArgs& a, int row, const Ask& s, float top,
 // Of the histograms' kernel: two workgroups a CU, one's loads beside the other's
 // exponentials (64 rows of 152064 logits: 80.0 us, 83.3 with 1024 threads, 85.7 with 256).
 constexpr int kPartThreads = 512, kPartWaves = kPartThreads / 64;
-constexpr int kPartQuads = 10;  // of four logits that a thread of it holds
+// Of four logits that a thread of it holds; longer parts are read again for each
+// pass, out of the caches. 48 rows of 152064 logits, 15208 a part, 62.7 us, read again
+// 64.4; 65 rows, 21724 a part, 83.8, held (11) 83.2, and beyond that the same.
+constexpr int kPartQuads = 10;
 constexpr int kGrid = 1024;     // bins, the last of them everything behind the others
 constexpr int kListed = 4096;
 constexpr int kDirect = kSampleThreads;  // a row is its own list

@@ -22,8 +22,10 @@ takes any mixture, but a workgroup walks all keys of a sequence if the batch has
 rows enough to fill the chip: long contexts belong to attention_decode.
 
 Activations are float32, the cache float32, float16 or bfloat16, or of 4 or 8
-bits ("q4", "q8": 5 and 9 bits an element with their scales). Tensors are
-passed as they are: q, k, v and outputs are [rows, heads, head_dim] with any
+bits ("q4", "q8": 5 and 9 bits an element with their scales for head dims of 64,
+128 and 256; rows of others are as wide as the next one's, quant_row_bytes: up to
+32 and from 72 to 80 and 136 to 152 "q8" saves next to nothing over float16, or
+takes more). Tensors are passed as they are: q, k, v and outputs are [rows, heads, head_dim] with any
 row stride (views of a fused projection), heads contiguous. There is no CPU
 fallback. Tensors of a call live on one device; it need not be the current
 one. Given a `stream`, the call's work is ordered on it and so must be the
