@@ -268,13 +268,15 @@ __global__ __launch_bounds__(kDecThreads, (DecQuant<T, HD>::kPerCu)) void paged_
 #pragma unroll
       for (int e = 0; e < 8; ++e) mx = fmaxf(mx, p[e]);
       mx = fmaxf(m, xor32_max(xor16_max(mx)));
-      // the largest |d|, by its exponent (rows from elsewhere may have a negative one;
-      // NaN counts for nothing, and makes its block NaN by itself)
+      // the largest |d|, by its exponent (rows from elsewhere may have a negative one).
+      // NaN counts for nothing, it makes its block NaN by itself; a signalling one
+      // hides the instruction's other d, which is of the same block, and not the
+      // largest so far, which comes last.
       uint32_t big = 0;
 #pragma unroll
       for (int e = 0; e < 8; e += 2)
 #pragma unroll
-        for (int c = 0; c < BR; ++c) asm("v_max3_f16 %0, %0, |%1|, |%2|" : "+v"(big) : "v"(vs[e][c]), "v"(vs[e + 1][c]));
+        for (int c = 0; c < BR; ++c) asm("v_max3_f16 %0, |%1|, |%2|, %0" : "+v"(big) : "v"(vs[e][c]), "v"(vs[e + 1][c]));
       const float new_lift = fminf(lift, kMostLift - xor32_max(xor16_max((float)(big >> 10 & 31))));
       const float ref = (mx == -INFINITY ? 0.0f : mx) - new_lift;
       const float al = (mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mx)) * __builtin_amdgcn_exp2f(new_lift - lift);

@@ -846,3 +846,32 @@ def test_steps_below_zero(paged, heads, kv, hd, kind):
         want = p.want(rows=p.some(20))
         p.compare(paged.attention_decode(p.cache, 0, p.batch, p.qd), {int(s) - 1: want[int(s) - 1] for s in p.start[1:]}, share)
         p.compare(paged.attention_prefill(p.cache, 0, p.batch, p.qd), want, share)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,kv,hd", [(8, 2, 128), (28, 4, 128), (24, 2, 128), (8, 2, 64), (16, 1, 64), (4, 1, 256)])
+@pytest.mark.parametrize("bits", [0x7c01, 0xfd55, 0x7e00, 0xffff])
+def test_any_nan_stays_in_its_block(paged, heads, kv, hd, bits, kind):
+    """A d that is NaN, quiet or signalling, beside one large value row of its tile among small ones: the other blocks are as
+    they were."""
+    p = Problem(paged, kind, [70, 64, 33], heads, kv, hd, 16, seed=83, new=[1, 40, 33], size=1e-2)
+    r = np.random.default_rng(3)
+    nb = kvq.blocks(hd)
+    at = 16 * nb * kvq.KINDS[kind][2]
+    for large, bad in ((0, 2), (1, 3), (17, 16), (5, 7), (12, 30), (31, 28)):
+        v = p.v.copy()
+        for i in range(3):
+            put(v, p, i, large, (1e3 * r.standard_normal((kv, hd))).astype(np.float32))
+            v[0, p.table[i, bad // 16], :, bad % 16, at + 4:at + 6] = np.array([bits], np.uint16).view(np.uint8)
+        p.cache.values.copy_(dev(v))
+        kept, p.v = p.v, v
+        with np.errstate(invalid="ignore"):
+            want = p.want(rows=p.some(20))
+        p.v = kept
+        for call, rows in ((paged.attention_decode, {int(s) - 1 for s in p.start[1:]}), (paged.attention_prefill, set(want))):
+            out = call(p.cache, 0, p.batch, p.qd).double().cpu().numpy()
+            for row in rows:
+                y, bound = want[row]
+                fine = ~np.isnan(y)
+                assert np.array_equal(np.isnan(out[row]), ~fine), (large, bad, row)
+                assert (np.abs(out[row] - y)[fine] <= bound[fine]).all(), (large, bad, row)
